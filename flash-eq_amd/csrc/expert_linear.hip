@@ -1,0 +1,612 @@
+// The experts' per-degree channel maps on rows sorted by expert.  With rows offsets[e] ..
+// offsets[e + 1] of every plane belonging to expert e, and r(d) the irrep of plane (component) d,
+//   y[d, p, n] = sum_k x[d, p, k] W[e, r(d), n, k]  (+ b[e, n, j] on the plane of the j-th scalar irrep),
+//   grad_x[d, p, k] = sum_n grad_y[d, p, n] W[e, r(d), n, k],
+//   grad_W[e, r, n, k] = sum over the planes d of r and rows p of e of grad_y[d, p, n] x[d, p, k],
+//   grad_b[e, n, j] = sum over the rows p of e of grad_y[d_j, p, n];
+// rows from offsets[X] on (slots without an expert): y and grad_x are 0, and they enter no sum.
+//
+// Products run on the matrix cores: v_mfma_f32_16x16x4_f32 for float32, v_mfma_f32_16x16x32_{f16, bf16}
+// for 16-bit types, float32 accumulators for both, one rounding at the store.  A workgroup of
+// four waves takes a 128-row block of one expert and plane and 64 or 128 output columns; the
+// expert of a block is found by every wave from the offsets (a lane per expert, sums over
+// lanes), so the host never learns the counts and the grid is their upper bound.
+//
+// The weight is the first operand and the rows the second, so a lane's accumulators are
+// columns of one row; the weight rows are dealt to the tiles so that a lane's 16 accumulators are
+// 16 consecutive columns, which leave as 16-byte stores.  The next block of the reduction is
+// loaded to registers while the present one, in LDS, is multiplied.
+#include <algorithm>
+
+#include "elem_types.h"
+#include "feq_internal.h"
+#include "tile_math.h"
+
+namespace feq {
+namespace {
+
+constexpr int kXlMaxPlanes = FEQ_MAX_SLOTS;
+constexpr int kXlMaxReps = FEQ_MAX_IRREPS;
+constexpr int kXlMaxExperts = 1024;
+constexpr int kXlThreads = 256;
+constexpr int kXlBM = 128;          // rows of a block
+constexpr int kXlRowBytes = 128;    // bytes of the reduction staged per row (32 floats, 64 16-bit elements)
+
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef short v4s __attribute__((ext_vector_type(4)));
+typedef short v8s __attribute__((ext_vector_type(8)));
+typedef __attribute__((address_space(3))) v4s lds_v4s;
+
+// Irrep and bias column (-1: none) of every plane; first plane of every irrep.
+struct XlMap {
+    int8_t rep[kXlMaxPlanes];
+    int8_t bcol[kXlMaxPlanes];
+    int16_t first[kXlMaxReps + 1];
+};
+
+// One reduction step of a 16 x 16 tile: KS elements, a lane holding FE of them.
+// Lane (c = l % 16, g = l / 16) holds elements FE g .. FE g + FE - 1 of row (or column) c.
+template <class T>
+struct Mma;
+template <>
+struct Mma<float> {
+    static constexpr int KS = 16, FE = 4;
+    typedef v4f frag;
+    static __device__ __forceinline__ v4f mul(frag a, frag b, v4f c) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = mfma4(a[j], b[j], c);
+        return c;
+    }
+    // element j: row k0 + 4 g + j of a table with `stride` elements a row, column q0 + step (c / 4) + c % 4
+    static __device__ __forceinline__ frag columns(const float* t, int stride, int k0, int g, int c, int q0, int step) {
+        const float* p = t + (k0 + 4 * g) * stride + q0 + step * (c >> 2) + (c & 3);
+        return frag{p[0], p[stride], p[2 * stride], p[3 * stride]};
+    }
+};
+// ds_read_b64_tr_b16: in a group of 16 lanes, lane s points at row s / 4 and the four columns of the group's
+// quad s % 4 and receives, of column s, the four rows.
+template <class T, class F>
+struct MmaHalf {
+    static constexpr int KS = 32, FE = 8;
+    typedef F frag;
+    static __device__ __forceinline__ frag columns(const T* t, int stride, int k0, int g, int c, int q0, int step) {
+        const T* p = t + (k0 + 8 * g + (c >> 2)) * stride + q0 + step * (c & 3);
+        const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
+        const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 4 * stride));
+        const v8s v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        return __builtin_bit_cast(frag, v);
+    }
+};
+template <>
+struct Mma<_Float16> : MmaHalf<_Float16, h8> {
+    static __device__ __forceinline__ v4f mul(h8 a, h8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Mma<__bf16> : MmaHalf<__bf16, b8> {
+    static __device__ __forceinline__ v4f mul(b8 a, b8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+
+// 16 bytes of T at p, of which the first `n` elements exist (n <= 0: none); the others are 0.
+template <class T, bool VEC>
+__device__ __forceinline__ uint4 load16(const T* p, int n) {
+    constexpr int V = 16 / sizeof(T);
+    if constexpr (VEC) {
+        return n > 0 ? *reinterpret_cast<const uint4*>(p) : uint4{0, 0, 0, 0};
+    } else {
+        typename VecOf<T, V>::type v;
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = j < n ? p[j] : static_cast<T>(0.0f);
+        return __builtin_bit_cast(uint4, v);
+    }
+}
+
+struct XlTile {
+    int expert;      // X: rows without an expert; -1: no such block
+    int row0, row1;  // the block's first row, the end of the expert's rows
+    int index;       // the block's index among those of the expert
+    int before;      // blocks of experts before it that have more than one block
+    int count;       // the expert's blocks
+};
+
+// Block `want` of the row blocks (of `bm` rows) of the experts in order, the rows behind them last.  Called
+// by whole waves; the result is the same in every lane.
+__device__ __forceinline__ XlTile find_tile(const int32_t* __restrict__ offsets, int X, int S, int bm, int want) {
+    const int lane = threadIdx.x & 63;
+    int carry = 0, many = 0;
+    for (int e0 = 0; e0 <= X; e0 += 64) {
+        const int e = e0 + lane;
+        int a = 0, z = 0;
+        if (e <= X) {
+            a = offsets[e];
+            z = e < X ? offsets[e + 1] : S;
+        }
+        const int n = (z - a + bm - 1) / bm;
+        int incl = n, multi = (e < X && n > 1) ? n : 0, mincl = multi;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(incl, o, 64), w = __shfl_up(mincl, o, 64);
+            if (lane >= o) {
+                incl += u;
+                mincl += w;
+            }
+        }
+        const uint64_t hit = __ballot(carry + incl > want);
+        if (hit) {
+            const int f = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            const int begin = carry + __shfl(incl - n, f, 64);
+            XlTile t;
+            t.expert = e0 + f;
+            t.index = want - begin;
+            t.row0 = __shfl(a, f, 64) + t.index * bm;
+            t.row1 = __shfl(z, f, 64);
+            t.before = many + __shfl(mincl - multi, f, 64);
+            t.count = __shfl(n, f, 64);
+            return t;
+        }
+        carry += __shfl(incl, 63, 64);
+        many += __shfl(mincl, 63, 64);
+    }
+    return XlTile{-1, 0, 0, 0, 0, 0};
+}
+
+// Blocks of `bm` rows that X experts and the rows behind them can make of S rows.
+inline int64_t tile_bound(int64_t S, int X, int bm) { return S / bm + std::min<int64_t>(S, X + 1); }
+
+// out[d, p, :] = in[d, p, :] B (+ bias), B = W[e, r]^T (TRANS false: in has Cin columns, out Cout) or W[e, r]
+// (TRANS: in has Cout columns, out Cin).  K: columns of in, N: of out; W rows have wld = Cin elements.
+// WR: waves along the output columns (64 each), 4 / WR along the rows.
+template <class T, bool VEC, bool TRANS, int WR>
+__global__ void __launch_bounds__(kXlThreads)
+k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,
+        int N, int nreps, XlMap map, const T* __restrict__ bias, int nbias, T* __restrict__ out) {
+    using M = Mma<T>;
+    constexpr int V = 16 / sizeof(T), BK = kXlRowBytes / sizeof(T), CH = BK / V;   // 8 vectors of a staged row
+    constexpr int BN = 64 * WR, WC = 4 / WR, PT = kXlBM / (16 * WC);
+    constexpr int LD = BK + V;                       // stride of a K-contiguous row: 144 bytes
+    constexpr int LDT = BN + V;                      // stride of a W row staged as it lies (TRANS)
+    constexpr int NIN = kXlBM * CH / kXlThreads;     // vectors a thread stages
+    constexpr int NW = BN * CH / kXlThreads;
+    __shared__ __align__(16) T sIn[kXlBM * LD];
+    __shared__ __align__(16) T sW[TRANS ? BK * LDT : BN * LD];
+    const int d = blockIdx.y;
+    const int nb = (N + BN - 1) / BN;
+    const XlTile t = find_tile(offsets, X, S, kXlBM, blockIdx.x / nb);
+    if (t.expert < 0) return;
+    const int n0 = (blockIdx.x % nb) * BN;
+    const int rows = t.row1 - t.row0 < kXlBM ? t.row1 - t.row0 : kXlBM;
+    T* od = out + (static_cast<int64_t>(d) * S + t.row0) * N;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave % WR, wc = wave / WR;
+    const bool none = t.expert == X;                 // uniform: rows without an expert
+    const T* id = in + (static_cast<int64_t>(d) * S + t.row0) * K;
+    const int64_t wmat = static_cast<int64_t>(TRANS ? K : N) * (TRANS ? N : K);
+    const T* we = W + (static_cast<int64_t>(none ? 0 : t.expert) * nreps + map.rep[d]) * wmat;
+
+    uint4 vin[NIN], vw[NW];
+    auto load = [&](int k0) {
+#pragma unroll
+        for (int i = 0; i < NIN; ++i) {
+            const int q = tid + kXlThreads * i, r = q / CH, k = k0 + (q % CH) * V;
+            vin[i] = load16<T, VEC>(id + static_cast<int64_t>(r) * K + k, r < rows ? K - k : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const int q = tid + kXlThreads * i;
+            if constexpr (TRANS) {                   // W rows are k, columns n
+                const int r = k0 + q / (BN / V), n = n0 + (q % (BN / V)) * V;
+                vw[i] = load16<T, VEC>(we + static_cast<int64_t>(r) * N + n, r < K ? N - n : 0);
+            } else {
+                const int r = n0 + q / CH, k = k0 + (q % CH) * V;
+                vw[i] = load16<T, VEC>(we + static_cast<int64_t>(r) * K + k, r < N ? K - k : 0);
+            }
+        }
+    };
+    auto stage = [&]() {
+#pragma unroll
+        for (int i = 0; i < NIN; ++i) {
+            const int q = tid + kXlThreads * i;
+            *reinterpret_cast<uint4*>(sIn + (q / CH) * LD + (q % CH) * V) = vin[i];
+        }
+#pragma unroll
+        for (int i = 0; i < NW; ++i) {
+            const int q = tid + kXlThreads * i;
+            if constexpr (TRANS) *reinterpret_cast<uint4*>(sW + (q / (BN / V)) * LDT + (q % (BN / V)) * V) = vw[i];
+            else *reinterpret_cast<uint4*>(sW + (q / CH) * LD + (q % CH) * V) = vw[i];
+        }
+    };
+
+    v4f acc[4][PT];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < PT; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    if (!none) {
+        load(0);
+        for (int k0 = 0; k0 < K; k0 += BK) {
+            __syncthreads();
+            stage();
+            __syncthreads();
+            if (k0 + BK < K) load(k0 + BK);
+#pragma unroll
+            for (int ks = 0; ks < BK; ks += M::KS) {
+                typename M::frag a[4], b[PT];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    // row m = c of tile i is column 16 (m / 4) + 4 i + m % 4 of the wave's 64
+                    const int q0 = 64 * wr + 4 * i;
+                    if constexpr (TRANS) {
+                        a[i] = M::columns(sW, LDT, ks, g, c, q0, 16);
+                    } else {
+                        a[i] = *reinterpret_cast<const typename M::frag*>(sW + (q0 + 16 * (c >> 2) + (c & 3)) * LD + ks +
+                                                                          M::FE * g);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < PT; ++j)
+                    b[j] = *reinterpret_cast<const typename M::frag*>(sIn + (16 * (wc * PT + j) + c) * LD + ks + M::FE * g);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < PT; ++j) acc[i][j] = M::mul(a[i], b[j], acc[i][j]);
+            }
+        }
+    }
+    // lane (c, g): row c of row tile j, columns 16 g + 4 i + r of the wave's 64
+    const int nw = n0 + 64 * wr + 16 * g;
+    float bv[16];
+#pragma unroll
+    for (int u = 0; u < 16; ++u) bv[u] = 0.0f;
+    const int bc = map.bcol[d];
+    if (!TRANS && bias && bc >= 0 && !none) {
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            if (nw + u < N) bv[u] = static_cast<float>(bias[(static_cast<int64_t>(t.expert) * N + nw + u) * nbias + bc]);
+    }
+#pragma unroll
+    for (int j = 0; j < PT; ++j) {
+        const int r = 16 * (wc * PT + j) + c;
+        if (r >= rows) continue;
+        T* orow = od + static_cast<int64_t>(r) * N + nw;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int u = 0; u < 16; u += V)
+                if (nw + u < N) {
+                    float o[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) o[v] = acc[(u + v) / 4][j][(u + v) % 4] + bv[u + v];
+                    store_f<T, V>(orow + u, o);
+                }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 16; ++u)
+                if (nw + u < N) orow[u] = static_cast<T>(acc[u / 4][j][u % 4] + bv[u]);
+        }
+    }
+}
+
+// grad_W and grad_b over row chunks of rc rows.  A workgroup takes a chunk of one expert, one irrep r (all its
+// planes), 64 WR columns k of x and 128 columns n of grad_y (tiles of k first).  An expert of one chunk gets its
+// gradient written, one of several a float32 partial per chunk: pw[(r nslots + slot) N K + n K + k],
+// pb[(j nslots + slot) N + n], summed by k_xl_wsum.
+template <class T, bool VEC, int WR>
+__global__ void __launch_bounds__(kXlThreads)
+k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __restrict__ offsets, int X, int S,
+           int ci, int co, int nreps, XlMap map, int rc, int nslots, T* __restrict__ gw, T* __restrict__ gb, int nbias,
+           float* __restrict__ pw, float* __restrict__ pb) {
+    using M = Mma<T>;
+    constexpr int V = 16 / sizeof(T), BP = kXlRowBytes / sizeof(T);   // rows staged at a time
+    constexpr int BK = 64 * WR, BN = 128, WC = 4 / WR, NT = BN / (16 * WC);
+    constexpr int LX = BK + V, LG = BN + V;
+    constexpr int NX = BP * (BK / V) / kXlThreads, NG = BP * (BN / V) / kXlThreads;
+    __shared__ __align__(16) T sX[BP * LX];
+    __shared__ __align__(16) T sG[BP * LG];
+    const int nk = (ci + BK - 1) / BK, nn = (co + BN - 1) / BN;
+    const int tile = blockIdx.x / (nk * nn), sub = blockIdx.x % (nk * nn);
+    const int rep = nreps - 1 - static_cast<int>(blockIdx.y);      // the irreps of most planes first
+    const XlTile t = find_tile(offsets, X, S, rc, tile);
+    if (t.expert < 0 || t.expert == X) return;
+    const int k0 = (sub % nk) * BK, n0 = (sub / nk) * BN;
+    const int rend = t.row1 - t.row0 < rc ? t.row1 : t.row0 + rc;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wr = wave % WR, wc = wave / WR;
+    const int d0 = map.first[rep], d1 = map.first[rep + 1];
+    const int steps = (rend - t.row0 + BP - 1) / BP, total = steps * (d1 - d0);
+    const int bc = map.bcol[d0];
+    const bool sums = gb && bc >= 0 && k0 == 0;                    // uniform
+
+    uint4 vx[NX], vg[NG];
+    auto load = [&](int it) {
+        const int d = d0 + it / steps, r0 = t.row0 + (it % steps) * BP;
+        const int64_t base = static_cast<int64_t>(d) * S;
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+            const int q = tid + kXlThreads * i, r = r0 + q / (BK / V), k = k0 + (q % (BK / V)) * V;
+            vx[i] = load16<T, VEC>(x + (base + r) * ci + k, r < rend ? ci - k : 0);
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int q = tid + kXlThreads * i, r = r0 + q / (BN / V), n = n0 + (q % (BN / V)) * V;
+            vg[i] = load16<T, VEC>(gy + (base + r) * co + n, r < rend ? co - n : 0);
+        }
+    };
+    v4f acc[4][NT];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    float bsum = 0.0f;                                             // thread n < 128: column n0 + n
+    load(0);
+    for (int it = 0; it < total; ++it) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+            const int q = tid + kXlThreads * i;
+            *reinterpret_cast<uint4*>(sX + (q / (BK / V)) * LX + (q % (BK / V)) * V) = vx[i];
+        }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            const int q = tid + kXlThreads * i;
+            *reinterpret_cast<uint4*>(sG + (q / (BN / V)) * LG + (q % (BN / V)) * V) = vg[i];
+        }
+        __syncthreads();
+        if (it + 1 < total) load(it + 1);
+#pragma unroll
+        for (int ks = 0; ks < BP; ks += M::KS) {
+            typename M::frag a[4], b[NT];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int q0 = 64 * wr + 4 * i;                    // as in k_xl_mm: 16 consecutive k a lane
+                a[i] = M::columns(sX, LX, ks, g, c, q0, 16);
+            }
+#pragma unroll
+            for (int j = 0; j < NT; ++j) b[j] = M::columns(sG, LG, ks, g, c, 16 * (wc * NT + j), 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = M::mul(a[i], b[j], acc[i][j]);
+        }
+        if (sums && tid < BN)
+            for (int p = 0; p < BP; ++p) bsum += static_cast<float>(sG[p * LG + tid]);
+    }
+    const bool direct = t.count == 1;
+    const int slot = t.before + t.index;
+    const int kw = k0 + 64 * wr + 16 * g;
+    const int64_t base = direct ? (static_cast<int64_t>(t.expert) * nreps + rep) * co
+                                : (static_cast<int64_t>(rep) * nslots + slot) * co;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int n = n0 + 16 * (wc * NT + j) + c;
+        if (n >= co) continue;
+        if (direct) {
+            T* o = gw + (base + n) * ci + kw;
+#pragma unroll
+            for (int u = 0; u < 16; u += VEC ? V : 1) {
+                if (kw + u >= ci) continue;
+                if constexpr (VEC) {
+                    float f[V];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) f[v] = acc[(u + v) / 4][j][(u + v) % 4];
+                    store_f<T, V>(o + u, f);
+                } else {
+                    o[u] = static_cast<T>(acc[u / 4][j][u % 4]);
+                }
+            }
+        } else {
+            float* o = pw + (base + n) * ci + kw;
+#pragma unroll
+            for (int u = 0; u < 16; u += 4) {
+                if constexpr (VEC) {
+                    if (kw + u < ci) *reinterpret_cast<v4f*>(o + u) = acc[u / 4][j];
+                } else {
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        if (kw + u + v < ci) o[u + v] = acc[u / 4][j][v];
+                }
+            }
+        }
+    }
+    if (sums && tid < BN && n0 + tid < co) {
+        if (direct) gb[(static_cast<int64_t>(t.expert) * co + n0 + tid) * nbias + bc] = static_cast<T>(bsum);
+        else pb[(static_cast<int64_t>(bc) * nslots + slot) * co + n0 + tid] = bsum;
+    }
+}
+
+// The experts' chunk counts and first partials as find_tile numbers them.  Lane-uniform.
+__device__ __forceinline__ void expert_chunks(const int32_t* __restrict__ offsets, int X, int rc, int e, int& first, int& count) {
+    const int lane = threadIdx.x & 63;
+    int s = 0;
+    for (int i = lane; i < e; i += 64) {
+        const int n = (offsets[i + 1] - offsets[i] + rc - 1) / rc;
+        s += n > 1 ? n : 0;
+    }
+    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+    first = s;
+    count = (offsets[e + 1] - offsets[e] + rc - 1) / rc;
+}
+
+// Experts of several chunks: the partials in order; of none: zeros.  blockIdx.y: expert, blockIdx.z: irrep, and
+// behind the irreps the bias columns.
+template <class T>
+__global__ void __launch_bounds__(256)
+k_xl_wsum(const float* __restrict__ pw, const float* __restrict__ pb, const int32_t* __restrict__ offsets, int X, int rc,
+          int64_t wsize, int co, int nreps, int nslots, T* __restrict__ gw, T* __restrict__ gb, int nbias) {
+    const int e = blockIdx.y, z = blockIdx.z;
+    int first, count;
+    expert_chunks(offsets, X, rc, e, first, count);
+    if (count == 1) return;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const bool w = z < nreps;
+    const int64_t size = w ? wsize : co;
+    if (i >= size) return;
+    const float* p = (w ? pw + (static_cast<int64_t>(z) * nslots + first) * wsize
+                        : pb + (static_cast<int64_t>(z - nreps) * nslots + first) * co) + i;
+    float a = 0.0f;
+#pragma unroll 8
+    for (int q = 0; q < count; ++q) a += p[q * size];
+    if (w) gw[(static_cast<int64_t>(e) * nreps + z) * wsize + i] = static_cast<T>(a);
+    else gb[(static_cast<int64_t>(e) * co + i) * nbias + (z - nreps)] = static_cast<T>(a);
+}
+
+int xl_check(const int32_t* lvals, int32_t nreps, int32_t X, int64_t S, int32_t ci, int32_t co, int32_t dtype,
+             const int32_t* bias_cols, int32_t nbias, XlMap* map) {
+    if (!lvals || nreps < 1) return fail(FEQ_ERR_INVALID, "lvals must be non-empty");
+    if (nreps > kXlMaxReps) return fail(FEQ_ERR_UNSUPPORTED, "more than %d irreps", kXlMaxReps);
+    if (X < 1 || S < 0 || ci < 1 || co < 1)
+        return fail(FEQ_ERR_INVALID, "%lld rows of %d experts, %d to %d channels", (long long)S, X, ci, co);
+    if (X > kXlMaxExperts) return fail(FEQ_ERR_UNSUPPORTED, "more than %d experts", kXlMaxExperts);
+    if (S > INT32_MAX / 2) return fail(FEQ_ERR_UNSUPPORTED, "more than 2^30 rows");
+    if (ci > 65536 || co > 65536) return fail(FEQ_ERR_UNSUPPORTED, "more than 65536 channels");
+    if (!dtype_ok(dtype)) return fail(FEQ_ERR_INVALID, "unknown element type %d", dtype);
+    int d = 0;
+    uint32_t used = 0;
+    for (int r = 0; r < nreps; ++r) {
+        if (lvals[r] < 0) return fail(FEQ_ERR_INVALID, "negative degree");
+        const int n = 2 * lvals[r] + 1;
+        if (d + n > kXlMaxPlanes) return fail(FEQ_ERR_UNSUPPORTED, "representation dimension exceeds %d", kXlMaxPlanes);
+        const int bc = bias_cols ? bias_cols[r] : -1;   // at most 32 irreps: columns below 32
+        if (bc >= 0) {
+            if (bc >= nbias || n != 1 || (used >> bc & 1))
+                return fail(FEQ_ERR_INVALID, "bias column %d of irrep %d (degree %d, %d columns)", bc, r, lvals[r], nbias);
+            used |= 1u << bc;
+        }
+        map->first[r] = static_cast<int16_t>(d);
+        for (int i = 0; i < n; ++i, ++d) {
+            map->rep[d] = static_cast<int8_t>(r);
+            map->bcol[d] = static_cast<int8_t>(bc);
+        }
+    }
+    map->first[nreps] = static_cast<int16_t>(d);
+    if (bias_cols && (nbias > nreps || used != (nbias >= 32 ? ~0u : (1u << nbias) - 1u)))
+        return fail(FEQ_ERR_INVALID, "%d bias columns, not each of them a scalar irrep's", nbias);
+    return FEQ_OK;
+}
+
+template <class T>
+bool xl_vec(int ci, int co, std::initializer_list<const void*> ptrs) {
+    constexpr int V = 16 / sizeof(T);
+    if (ci % V || co % V) return false;
+    for (const void* p : ptrs)
+        if (p && !aligned_to(p, 16)) return false;
+    return true;
+}
+
+template <class T, bool TRANS>
+int mm_run(const void* in, const void* W, const int32_t* offsets, int X, int64_t S, int ci, int co, int nreps,
+           const XlMap& map, const void* bias, int nbias, void* out, hipStream_t s) {
+    const int K = TRANS ? co : ci, N = TRANS ? ci : co;
+    const bool vec = xl_vec<T>(ci, co, {in, W, out});
+    auto run = [&](auto v, auto wr) -> int {
+        constexpr int WR = decltype(wr)::value;
+        const int64_t blocks = tile_bound(S, X, kXlBM) * ceil_div(N, 64 * WR);
+        if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
+        auto kern = k_xl_mm<T, decltype(v)::value, TRANS, WR>;
+        FEQ_LAUNCH(TRANS ? "k_xl_mm_t" : "k_xl_mm", kern, dim3(blocks, map.first[nreps]), dim3(kXlThreads), 0, s,
+                   static_cast<const T*>(in), static_cast<const T*>(W), offsets, X, static_cast<int>(S), K, N, nreps, map,
+                   static_cast<const T*>(bias), nbias, static_cast<T*>(out));
+        return FEQ_OK;
+    };
+    auto with_wr = [&](auto v) -> int {
+        return N <= 64 ? run(v, std::integral_constant<int, 1>{}) : run(v, std::integral_constant<int, 2>{});
+    };
+    return vec ? with_wr(std::true_type{}) : with_wr(std::false_type{});
+}
+
+// Rows of a weight-gradient chunk: about 1024 workgroups where the rows allow it.
+int wgrad_chunk(int64_t S, int X, int nreps, int ci, int co) {
+    const int64_t tiles = ceil_div(ci, ci <= 64 ? 64 : 128) * ceil_div(co, 128) * nreps;
+    const int64_t want = std::max<int64_t>(1, 1024 / tiles);
+    int64_t rc = align_up(static_cast<size_t>(ceil_div(std::max<int64_t>(S, 1), want)), 64);
+    return static_cast<int>(std::min<int64_t>(std::max<int64_t>(rc, 128), 8192));
+}
+// Partials: an expert of m > 1 chunks has at most 2 rows / rc of them.
+int64_t wgrad_slots(int64_t S, int rc) { return S > rc ? 2 * S / rc : 0; }
+
+}  // namespace
+}  // namespace feq
+
+using namespace feq;
+
+extern "C" int feq_expert_linear_fwd(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
+                                     int32_t cout, int32_t dtype, const void* x, const void* weight,
+                                     const int32_t* offsets, const void* bias, int32_t nbias, const int32_t* bias_cols,
+                                     void* y, feq_stream_t stream) {
+    XlMap map;
+    if (int rc = xl_check(lvals, nreps, experts, slots, cin, cout, dtype, bias ? bias_cols : nullptr, nbias, &map)) return rc;
+    if (slots == 0) return FEQ_OK;
+    if (!x || !weight || !offsets || !y) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    return with_dtype(dtype, [&](auto t) -> int {
+        return mm_run<decltype(t), false>(x, weight, offsets, experts, slots, cin, cout, nreps, map, bias, nbias, y,
+                                          stream_of(stream));
+    });
+}
+
+extern "C" int feq_expert_linear_bwd_x(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
+                                       int32_t cout, int32_t dtype, const void* grad_y, const void* weight,
+                                       const int32_t* offsets, void* grad_x, feq_stream_t stream) {
+    XlMap map;
+    if (int rc = xl_check(lvals, nreps, experts, slots, cin, cout, dtype, nullptr, 0, &map)) return rc;
+    if (slots == 0) return FEQ_OK;
+    if (!grad_y || !weight || !offsets || !grad_x) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    return with_dtype(dtype, [&](auto t) -> int {
+        return mm_run<decltype(t), true>(grad_y, weight, offsets, experts, slots, cin, cout, nreps, map, nullptr, 0,
+                                         grad_x, stream_of(stream));
+    });
+}
+
+extern "C" size_t feq_expert_linear_bwd_w_workspace(int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
+                                                    int32_t cout, int32_t nbias) {
+    if (nreps < 1 || experts < 1 || slots < 1 || cin < 1 || cout < 1 || nbias < 0) return 0;
+    const int64_t n = wgrad_slots(slots, wgrad_chunk(slots, experts, nreps, cin, cout));
+    Carver c(nullptr);
+    c.take<float>(static_cast<size_t>(n) * nreps * cin * cout);
+    c.take<float>(static_cast<size_t>(n) * nbias * cout);
+    return c.used;
+}
+
+extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
+                                       int32_t cout, int32_t dtype, const void* grad_y, const void* x,
+                                       const int32_t* offsets, int32_t nbias, const int32_t* bias_cols, void* grad_weight,
+                                       void* grad_bias, void* workspace, size_t ws_bytes, feq_stream_t stream) {
+    XlMap map;
+    if (int rc = xl_check(lvals, nreps, experts, slots, cin, cout, dtype, grad_bias ? bias_cols : nullptr, nbias, &map)) return rc;
+    if (!grad_weight || !offsets || (slots && (!grad_y || !x))) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    if (grad_bias && (!bias_cols || nbias < 1)) return fail(FEQ_ERR_INVALID, "a bias gradient needs bias columns");
+    const int nb = grad_bias ? nbias : 0;
+    if (ws_bytes < feq_expert_linear_bwd_w_workspace(nreps, experts, slots, cin, cout, nb))
+        return fail(FEQ_ERR_WORKSPACE, "weight-gradient workspace of %zu bytes, %zu needed", ws_bytes,
+                    feq_expert_linear_bwd_w_workspace(nreps, experts, slots, cin, cout, nb));
+    hipStream_t s = stream_of(stream);
+    const int rc = wgrad_chunk(slots, experts, nreps, cin, cout);
+    const int64_t nslots = wgrad_slots(slots, rc);
+    if (nslots && !workspace) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    Carver c(workspace);
+    float* pw = c.take<float>(static_cast<size_t>(nslots) * nreps * cin * cout);
+    float* pb = c.take<float>(static_cast<size_t>(nslots) * nb * cout);
+    return with_dtype(dtype, [&](auto tt) -> int {
+        using T = decltype(tt);
+        T *gw = static_cast<T*>(grad_weight), *gb = static_cast<T*>(grad_bias);
+        const bool vec = xl_vec<T>(cin, cout, {grad_y, x, grad_weight});
+        auto run = [&](auto v, auto wr) -> int {
+            constexpr int WR = decltype(wr)::value;
+            const int64_t blocks = tile_bound(slots, experts, rc) * ceil_div(cin, 64 * WR) * ceil_div(cout, 128);
+            if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
+            auto kern = k_xl_wgrad<T, decltype(v)::value, WR>;
+            FEQ_LAUNCH("k_xl_wgrad", kern, dim3(blocks, nreps), dim3(kXlThreads), 0, s, static_cast<const T*>(grad_y),
+                       static_cast<const T*>(x), offsets, experts, static_cast<int>(slots), cin, cout, nreps, map, rc,
+                       static_cast<int>(nslots), gw, gb, nb, pw, pb);
+            return FEQ_OK;
+        };
+        auto with_wr = [&](auto v) -> int {
+            return cin <= 64 ? run(v, std::integral_constant<int, 1>{}) : run(v, std::integral_constant<int, 2>{});
+        };
+        if (slots)
+            if (const int err = vec ? with_wr(std::true_type{}) : with_wr(std::false_type{})) return err;
+        const int64_t wsize = static_cast<int64_t>(cin) * cout;
+        auto kern = k_xl_wsum<T>;
+        FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(wsize, 256), experts, nreps + nb), dim3(256), 0, s, pw, pb, offsets,
+                   experts, rc, wsize, cout, nreps, static_cast<int>(nslots), gw, gb, nb);
+        return FEQ_OK;
+    });
+}

@@ -1,0 +1,598 @@
+// The choice of each row's experts (top-k of the logits with softmax weights) and the plan
+// that sorts the chosen (row, expert) slots by expert.
+//
+// Top-k.  For the logits l (rows, X) of a row: e_i = exp(l_i - max l), p = e / sum e; the K
+// experts of the largest logits are chosen (equal logits: the lowest index first; a NaN counts
+// as the largest), an expert whose logit is -inf never (its place holds id -1, weight 0).
+// Weights: e_sel / sum of the chosen e (normalized) or p_sel.  Also mean_i = the mean of p_i
+// over the rows, for a balancing loss.  Gradient, with g the weights' and m the mean's:
+//   normalized:  dl_sel += w (g - sum w g)
+//   otherwise:   dl_i += p_i (gp_i - sum p gp), gp_sel = g, 0 elsewhere
+//   the mean:    dl_i += p_i (m_i - sum p m) / rows.
+// All sums are float32.  A group of G lanes takes a row, each lane NE of its logits in
+// registers: reductions over a row are a few lane exchanges, and the K maxima are K rounds of
+// (value, index) maxima over the lanes.  HBM bounds the largest calls, issue the ordinary ones;
+// a lane keeps the same experts for all rows of its workgroup, so the mean is a register
+// sum per lane, summed over lanes, waves and workgroups in a fixed order.
+//
+// Plan.  A stable counting sort: per 2048-slot tile a histogram (k_plan_hist), per bucket the
+// tiles' exclusive sums (k_plan_scan), then every tile ranks its slots (k_plan_place).  Up to 8192
+// slots one workgroup does all three (k_plan_one).  Lanes with equal keys find each other by one
+// ballot per key bit, so a slot's rank needs no atomics and the order is the slots' own.  Slots
+// whose expert lies outside [0, X) fill a last bucket.  The plan is integer work on 8 bytes
+// per slot: launches and latency bound it.
+#include <algorithm>
+
+#include "elem_types.h"
+#include "feq_internal.h"
+
+namespace feq {
+namespace {
+
+constexpr int kTopkThreads = 256;
+constexpr int kTopkMaxBlocks = 1024;
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxTopk = 64;
+
+constexpr int kPlanTile = 2048;       // slots of a k_plan_hist / k_plan_place workgroup
+constexpr int kPlanOne = 8192;        // slots of k_plan_one
+constexpr int kPlanRounds = 8;        // 64-slot rounds of a wave
+
+// Larger key = earlier choice: order-preserving bits of the logit, NaN above all, -inf zero
+// (never chosen); +0 and -0 are equal.
+__device__ __forceinline__ uint32_t order_key(float v) {
+    if (v != v) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(v + 0.0f);
+    if (u == 0xff800000u) return 0u;
+    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+
+__device__ __forceinline__ float gsum(float v, int g) {
+    for (int o = g >> 1; o; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+__device__ __forceinline__ float gmax(float v, int g) {
+    for (int o = g >> 1; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+
+// Expert of element (chunk c, j) of lane l: chunks of V elements, chunk c of lane l at (c G + l) V.
+template <int V>
+__device__ __forceinline__ int elem_index(int l, int c, int j, int G) { return (c * G + l) * V + j; }
+
+// The row's logits (-inf behind the last expert) and e = exp(l - max); returns sum e.  A row of
+// -inf alone gives e = 0 and the sum 0.
+template <class T, int V, int NC>
+__device__ __forceinline__ float row_exp(const T* row, int X, int l, int G, float (&x)[NC][V], float (&e)[NC][V]) {
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+        const int i0 = elem_index<V>(l, c, 0, G);
+        if (i0 + V <= X) {
+            load_f<T, V>(row + i0, x[c]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[c][j] = -__builtin_inff();
+        }
+#pragma unroll
+        for (int j = 0; j < V; ++j) m = fmaxf(m, x[c][j]);
+    }
+    m = gmax(m, G);
+    float s = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            // masked experts are 0 also in a row of -inf alone, where l - max is no number
+            e[c][j] = x[c][j] == -__builtin_inff() ? 0.0f : expf(x[c][j] - m);
+            s += e[c][j];
+        }
+    return gsum(s, G);
+}
+
+// X is a multiple of V (V = 1 where it is not, or the logits are not aligned for it).
+template <class T, int V, int NC>
+__global__ void __launch_bounds__(kTopkThreads)
+k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normalize, int64_t* __restrict__ ids,
+           float* __restrict__ weights, float* __restrict__ part, int G) {
+    __shared__ float sums[4 * kMaxExperts];
+    const int l = threadIdx.x & (G - 1);
+    const int per = kTopkThreads / G;
+    float mean[NC][V];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j) mean[c][j] = 0.0f;
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / G; r < rows;
+         r += static_cast<int64_t>(gridDim.x) * per) {
+        float x[NC][V], e[NC][V];
+        const float s = row_exp<T, V, NC>(logits + r * X, X, l, G, x, e);
+        const float inv = s == 0.0f ? 0.0f : 1.0f / s;
+        uint32_t key[NC][V];
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                mean[c][j] += e[c][j] * inv;
+                key[c][j] = order_key(x[c][j]);
+            }
+        float total = 0.0f;
+        for (int k = 0; k < K; ++k) {
+            uint32_t best = 0;
+            int at = 0x7fffffff;
+            float ev = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (key[c][j] > best) {
+                        best = key[c][j];
+                        at = elem_index<V>(l, c, j, G);
+                        ev = e[c][j];
+                    }
+            for (int o = G >> 1; o; o >>= 1) {
+                const uint32_t b2 = __shfl_xor(best, o, 64);
+                const int a2 = __shfl_xor(at, o, 64);
+                const float e2 = __shfl_xor(ev, o, 64);
+                if (b2 > best || (b2 == best && a2 < at)) {
+                    best = b2;
+                    at = a2;
+                    ev = e2;
+                }
+            }
+            const bool got = best != 0;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (got && elem_index<V>(l, c, j, G) == at) key[c][j] = 0;
+            total += ev;
+            if (l == 0) {
+                ids[r * K + k] = got ? at : -1;
+                weights[r * K + k] = ev;
+            }
+        }
+        const float den = normalize ? total : s;
+        // a row without a choice has weights 0, not 0 / 0
+        const float scale = den == 0.0f ? 0.0f : 1.0f / den;
+        if (l == 0)
+            for (int k = 0; k < K; ++k) weights[r * K + k] *= scale;
+    }
+    if (!part) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float a = mean[c][j];
+            for (int o = G; o < 64; o <<= 1) a += __shfl_xor(a, o, 64);
+            const int i = elem_index<V>(l, c, j, G);
+            if (lane < G && i < X) sums[wave * X + i] = a;
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < X; i += kTopkThreads)
+        part[static_cast<int64_t>(blockIdx.x) * X + i] =
+            (sums[i] + sums[X + i]) + (sums[2 * X + i] + sums[3 * X + i]);
+}
+
+// mean[i] = (sum of the workgroups' sums) / rows, 16 experts a workgroup.
+__global__ void __launch_bounds__(1024)
+k_topk_mean(const float* __restrict__ part, int groups, int X, float inv_rows, float* __restrict__ mean) {
+    __shared__ float s[64][17];
+    const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4, i = blockIdx.x * 16 + c;
+    float a = 0.0f;
+    if (i < X)
+        for (int r = r0; r < groups; r += 64) a += part[static_cast<int64_t>(r) * X + i];
+    s[r0][c] = a;
+    __syncthreads();
+    for (int o = 32; o; o >>= 1) {
+        if (r0 < o) s[r0][c] += s[r0 + o][c];
+        __syncthreads();
+    }
+    if (r0 == 0 && i < X) mean[i] = s[0][c] * inv_rows;
+}
+
+// gw (rows, K) or NULL, gmean (X) or NULL.
+template <class T, int V, int NC>
+__global__ void __launch_bounds__(kTopkThreads)
+k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const float* __restrict__ weights,
+           const float* __restrict__ gw, const float* __restrict__ gmean, int64_t rows, int X, int K, int normalize,
+           float inv_rows, T* __restrict__ gl, int G) {
+    const int l = threadIdx.x & (G - 1);
+    const int per = kTopkThreads / G;
+    float gm[NC][V];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const int i = elem_index<V>(l, c, j, G);
+            gm[c][j] = (gmean && i < X) ? gmean[i] * inv_rows : 0.0f;
+        }
+    const bool full = gmean || (gw && !normalize);      // uniform: the probabilities enter
+    for (int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / G; r < rows;
+         r += static_cast<int64_t>(gridDim.x) * per) {
+        float gp[NC][V], d[NC][V];
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                gp[c][j] = gm[c][j];
+                d[c][j] = 0.0f;
+            }
+        if (gw) {
+            float dot = 0.0f;
+            if (normalize)
+                for (int k = 0; k < K; ++k) dot += weights[r * K + k] * gw[r * K + k];
+            for (int k = 0; k < K; ++k) {
+                const int64_t id = ids[r * K + k];
+                const float g = gw[r * K + k];
+                const float a = normalize ? weights[r * K + k] * (g - dot) : g;
+#pragma unroll
+                for (int c = 0; c < NC; ++c)
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (elem_index<V>(l, c, j, G) == id) {
+                            if (normalize) d[c][j] += a;
+                            else gp[c][j] += a;
+                        }
+            }
+        }
+        if (full) {
+            float x[NC][V], e[NC][V];
+            const float s = row_exp<T, V, NC>(logits + r * X, X, l, G, x, e);
+            const float inv = s == 0.0f ? 0.0f : 1.0f / s;
+            float dot = 0.0f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    e[c][j] *= inv;
+                    dot += e[c][j] * gp[c][j];
+                }
+            dot = gsum(dot, G);
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < V; ++j) d[c][j] += e[c][j] * (gp[c][j] - dot);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const int i0 = elem_index<V>(l, c, 0, G);
+            if (i0 + V <= X) store_f<T, V>(gl + r * X + i0, d[c]);
+        }
+    }
+}
+
+int topk_check(int64_t rows, int32_t X, int32_t K, int32_t dtype) {
+    if (rows < 0 || X < 1 || K < 1) return fail(FEQ_ERR_INVALID, "top-k of %lld rows: %d of %d experts", (long long)rows, K, X);
+    if (K > X) return fail(FEQ_ERR_INVALID, "top-k chooses %d of %d experts", K, X);
+    if (X > kMaxExperts) return fail(FEQ_ERR_UNSUPPORTED, "more than %d experts", kMaxExperts);
+    if (K > kMaxTopk) return fail(FEQ_ERR_UNSUPPORTED, "more than %d choices a row", kMaxTopk);
+    if (!dtype_ok(dtype)) return fail(FEQ_ERR_INVALID, "unknown element type %d", dtype);
+    return FEQ_OK;
+}
+
+// Lanes of a row: 8 logits a lane up to 512 experts, 16 above.
+int topk_lanes(int X) {
+    int g = 1;
+    while (g < 64 && g * 8 < X) g <<= 1;
+    return g;
+}
+int topk_blocks(int64_t rows, int X) {
+    return static_cast<int>(std::min<int64_t>(ceil_div(rows, kTopkThreads / topk_lanes(X)), kTopkMaxBlocks));
+}
+
+// f(V, NC) for the instance of X experts, vectors where `vec`
+template <class T, class F>
+int with_topk_form(int X, bool vec, F&& f) {
+    constexpr int VV = 16 / sizeof(T);
+    if (X <= 512)
+        return vec ? f(std::integral_constant<int, VV>{}, std::integral_constant<int, 8 / VV>{})
+                   : f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
+    return vec ? f(std::integral_constant<int, VV>{}, std::integral_constant<int, 16 / VV>{})
+               : f(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+}
+
+// ---- plan ------------------------------------------------------------------------
+
+// Bucket of slot i: its expert, X where it has none, X + 1 behind the last slot.
+__device__ __forceinline__ int slot_key(const int64_t* ids, int64_t i, int64_t n, int X) {
+    if (i >= n) return X + 1;
+    const int64_t e = ids[i];
+    return (e >= 0 && e < X) ? static_cast<int>(e) : X;
+}
+
+__device__ __forceinline__ uint64_t lanes_with(int key, int bits) {
+    uint64_t m = ~0ull;
+    for (int b = 0; b < bits; ++b) {
+        const bool on = (key >> b) & 1;
+        const uint64_t v = __ballot(on);
+        m &= on ? v : ~v;
+    }
+    return m;
+}
+
+// A wave's slots [beg, beg + 512) in order: key[i] and rank[i] of this lane's slot of round i among
+// the wave's equal keys; cnt (X + 2 ints, zero) receives the wave's histogram.
+__device__ __forceinline__ void rank_wave(const int64_t* ids, int64_t beg, int64_t n, int X, int bits, int* cnt,
+                                          int (&key)[kPlanRounds], int (&rank)[kPlanRounds]) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < kPlanRounds; ++i) key[i] = slot_key(ids, beg + 64 * i + lane, n, X);
+#pragma unroll
+    for (int i = 0; i < kPlanRounds; ++i) {
+        const uint64_t m = lanes_with(key[i], bits);
+        const int before = __popcll(m & ((1ull << lane) - 1ull));
+        const int base = cnt[key[i]];
+        rank[i] = base + before;
+        // every lane has read before a lane writes, and the write comes before the next round's reads
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (before == 0) cnt[key[i]] = base + static_cast<int>(__popcll(m));
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// Exclusive sums of v[0..X) in place (X <= 1024), the total returned, by a workgroup of NT threads.
+template <int NT>
+__device__ __forceinline__ int scan_buckets(int* v, int X, int* tmp) {
+    constexpr int PER = kMaxExperts / NT;
+    int own[PER], s = 0;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int b = threadIdx.x * PER + i;
+        own[i] = b < X ? v[b] : 0;
+        s += own[i];
+    }
+    int incl = s;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(incl, o, 64);
+        if ((threadIdx.x & 63) >= static_cast<unsigned>(o)) incl += u;
+    }
+    const int wave = threadIdx.x >> 6;
+    if ((threadIdx.x & 63) == 63) tmp[wave] = incl;
+    __syncthreads();
+    int base = 0, total = 0;
+    for (int w = 0; w < NT / 64; ++w) {
+        if (w < wave) base += tmp[w];
+        total += tmp[w];
+    }
+    int run = base + incl - s;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int b = threadIdx.x * PER + i;
+        if (b < X) v[b] = run;
+        run += own[i];
+    }
+    __syncthreads();
+    return total;
+}
+
+// Up to 8192 slots in one workgroup.  LDS: cnt[16][X + 2], base[X + 2].
+__global__ void __launch_bounds__(1024)
+k_plan_one(const int64_t* __restrict__ ids, int n, int X, int bits, int32_t* __restrict__ order,
+           int32_t* __restrict__ positions, int32_t* __restrict__ offsets) {
+    extern __shared__ int lds[];
+    __shared__ int tmp[16];
+    const int nb = X + 2, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int* base = lds + 16 * nb;
+    for (int i = threadIdx.x; i < 16 * nb; i += 1024) lds[i] = 0;
+    __syncthreads();
+    int key[kPlanRounds], rank[kPlanRounds];
+    const int beg = wave * 512;
+    if (beg < n) rank_wave(ids, beg, n, X, bits, lds + wave * nb, key, rank);
+    __syncthreads();
+    for (int b = threadIdx.x; b < nb; b += 1024) {      // the waves' exclusive sums per bucket
+        int run = 0;
+        for (int w = 0; w < 16; ++w) {
+            const int c = lds[w * nb + b];
+            lds[w * nb + b] = run;
+            run += c;
+        }
+        base[b] = run;
+    }
+    __syncthreads();
+    const int total = scan_buckets<1024>(base, X, tmp);
+    if (threadIdx.x == 0) base[X] = total;
+    __syncthreads();
+    for (int b = threadIdx.x; b <= X; b += 1024) offsets[b] = base[b];
+    if (beg < n) {
+#pragma unroll
+        for (int i = 0; i < kPlanRounds; ++i) {
+            const int slot = beg + 64 * i + lane;
+            if (slot < n) {
+                const int p = base[key[i]] + lds[wave * nb + key[i]] + rank[i];
+                order[p] = slot;
+                positions[slot] = p;
+            }
+        }
+    }
+}
+
+// hist[bucket][tile]
+__global__ void __launch_bounds__(256)
+k_plan_hist(const int64_t* __restrict__ ids, int64_t n, int X, int64_t ntiles, int32_t* __restrict__ hist) {
+    __shared__ int cnt[kMaxExperts + 2];
+    for (int i = threadIdx.x; i < X + 2; i += 256) cnt[i] = 0;
+    __syncthreads();
+    const int64_t beg = static_cast<int64_t>(blockIdx.x) * kPlanTile;
+#pragma unroll
+    for (int i = 0; i < kPlanTile / 256; ++i) atomicAdd(&cnt[slot_key(ids, beg + 256 * i + threadIdx.x, n, X)], 1);
+    __syncthreads();
+    for (int i = threadIdx.x; i <= X; i += 256) hist[i * ntiles + blockIdx.x] = cnt[i];
+}
+
+// Exclusive sums over the tiles of each bucket; total[bucket].
+__global__ void __launch_bounds__(256)
+k_plan_scan(int32_t* __restrict__ hist, int64_t ntiles, int32_t* __restrict__ total) {
+    __shared__ int tmp[4];
+    int32_t* h = hist + static_cast<int64_t>(blockIdx.x) * ntiles;
+    int carry = 0;
+    for (int64_t t0 = 0; t0 < ntiles; t0 += 256) {
+        const int64_t t = t0 + threadIdx.x;
+        const int v = t < ntiles ? h[t] : 0;
+        int incl = v;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(incl, o, 64);
+            if ((threadIdx.x & 63) >= static_cast<unsigned>(o)) incl += u;
+        }
+        __syncthreads();
+        if ((threadIdx.x & 63) == 63) tmp[threadIdx.x >> 6] = incl;
+        __syncthreads();
+        int before = carry, all = 0;
+        for (int w = 0; w < 4; ++w) {
+            if (w < static_cast<int>(threadIdx.x >> 6)) before += tmp[w];
+            all += tmp[w];
+        }
+        if (t < ntiles) h[t] = before + incl - v;
+        carry += all;
+    }
+    if (threadIdx.x == 0) total[blockIdx.x] = carry;
+}
+
+__global__ void __launch_bounds__(256)
+k_plan_place(const int64_t* __restrict__ ids, int64_t n, int X, int bits, int64_t ntiles,
+             const int32_t* __restrict__ hist, const int32_t* __restrict__ total, int32_t* __restrict__ order,
+             int32_t* __restrict__ positions, int32_t* __restrict__ offsets) {
+    __shared__ int cnt[4 * (kMaxExperts + 2)];
+    __shared__ int base[kMaxExperts + 2];
+    __shared__ int tmp[4];
+    const int nb = X + 2, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (int i = threadIdx.x; i < 4 * nb; i += 256) cnt[i] = 0;
+    for (int i = threadIdx.x; i < X; i += 256) base[i] = total[i];
+    __syncthreads();
+    const int all = scan_buckets<256>(base, X, tmp);
+    if (threadIdx.x == 0) base[X] = all;
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int b = threadIdx.x; b <= X; b += 256) offsets[b] = base[b];
+    int key[kPlanRounds], rank[kPlanRounds];
+    const int64_t beg = static_cast<int64_t>(blockIdx.x) * kPlanTile + wave * 512;
+    rank_wave(ids, beg, n, X, bits, cnt + wave * nb, key, rank);
+    __syncthreads();
+    for (int b = threadIdx.x; b <= X; b += 256) {
+        int run = base[b] + hist[b * ntiles + blockIdx.x];
+        for (int w = 0; w < 4; ++w) {
+            const int c = cnt[w * nb + b];
+            cnt[w * nb + b] = run;
+            run += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kPlanRounds; ++i) {
+        const int64_t slot = beg + 64 * i + lane;
+        if (slot < n) {
+            const int p = cnt[wave * nb + key[i]] + rank[i];
+            order[p] = static_cast<int32_t>(slot);
+            positions[slot] = p;
+        }
+    }
+}
+
+__global__ void k_plan_empty(int32_t* offsets, int X) {
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    if (i <= X) offsets[i] = 0;
+}
+
+// The one-workgroup form: its 17 (X + 2) counters fit 64 KB.
+bool plan_one(int64_t slots, int X) { return slots <= kPlanOne && 17 * (X + 2) * sizeof(int) <= 64 * 1024; }
+
+}  // namespace
+}  // namespace feq
+
+using namespace feq;
+
+extern "C" size_t feq_expert_topk_workspace(int64_t rows, int32_t experts) {
+    if (rows < 1 || experts < 1 || experts > kMaxExperts) return 0;
+    return sizeof(float) * static_cast<size_t>(experts) * topk_blocks(rows, experts);
+}
+
+extern "C" int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t experts, int32_t dtype, int32_t top_k,
+                                   int32_t normalize, int64_t* ids, float* weights, float* mean, void* workspace,
+                                   size_t ws_bytes, feq_stream_t stream) {
+    if (int rc = topk_check(rows, experts, top_k, dtype)) return rc;
+    if (rows && (!logits || !ids || !weights)) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    if (mean && rows && (!workspace || ws_bytes < feq_expert_topk_workspace(rows, experts)))
+        return fail(FEQ_ERR_WORKSPACE, "top-k workspace of %zu bytes, %zu needed", ws_bytes,
+                    feq_expert_topk_workspace(rows, experts));
+    hipStream_t s = stream_of(stream);
+    const int G = topk_lanes(experts), blocks = rows ? topk_blocks(rows, experts) : 0;
+    float* part = mean ? static_cast<float*>(workspace) : nullptr;
+    if (rows) {
+        const int rc = with_dtype(dtype, [&](auto t) -> int {
+            using T = decltype(t);
+            const bool vec = experts % (16 / sizeof(T)) == 0 && aligned_to(logits, 16);
+            return with_topk_form<T>(experts, vec, [&](auto v, auto nc) -> int {
+                auto kern = k_topk_fwd<T, decltype(v)::value, decltype(nc)::value>;
+                FEQ_LAUNCH("k_topk_fwd", kern, dim3(blocks), dim3(kTopkThreads), 0, s, static_cast<const T*>(logits),
+                           rows, experts, top_k, normalize, ids, weights, part, G);
+                return FEQ_OK;
+            });
+        });
+        if (rc) return rc;
+    }
+    if (mean)     // of no rows: 0
+        FEQ_LAUNCH("k_topk_mean", k_topk_mean, dim3(ceil_div(experts, 16)), dim3(1024), 0, s, part, blocks, experts,
+                   rows ? 1.0f / static_cast<float>(rows) : 0.0f, mean);
+    return FEQ_OK;
+}
+
+extern "C" int feq_expert_topk_bwd(const void* logits, const int64_t* ids, const float* weights, const float* grad_weights,
+                                   const float* grad_mean, int64_t rows, int32_t experts, int32_t dtype, int32_t top_k,
+                                   int32_t normalize, void* grad_logits, feq_stream_t stream) {
+    if (int rc = topk_check(rows, experts, top_k, dtype)) return rc;
+    if (rows == 0) return FEQ_OK;
+    if (!logits || !ids || !weights || !grad_logits) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    hipStream_t s = stream_of(stream);
+    const int G = topk_lanes(experts);
+    const int64_t blocks = std::min<int64_t>(ceil_div(rows, kTopkThreads / G), 8192);
+    return with_dtype(dtype, [&](auto t) -> int {
+        using T = decltype(t);
+        const bool vec = experts % (16 / sizeof(T)) == 0 && aligned_to(logits, 16) && aligned_to(grad_logits, 16);
+        return with_topk_form<T>(experts, vec, [&](auto v, auto nc) -> int {
+            auto kern = k_topk_bwd<T, decltype(v)::value, decltype(nc)::value>;
+            FEQ_LAUNCH("k_topk_bwd", kern, dim3(blocks), dim3(kTopkThreads), 0, s, static_cast<const T*>(logits), ids,
+                       weights, grad_weights, grad_mean, rows, experts, top_k, normalize,
+                       1.0f / static_cast<float>(rows), static_cast<T*>(grad_logits), G);
+            return FEQ_OK;
+        });
+    });
+}
+
+extern "C" size_t feq_expert_plan_workspace(int64_t slots, int32_t experts) {
+    if (slots < 1 || experts < 1 || experts > kMaxExperts || plan_one(slots, experts)) return 0;
+    return sizeof(int32_t) * static_cast<size_t>(experts + 1) * (ceil_div(slots, kPlanTile) + 1);
+}
+
+extern "C" int feq_expert_plan(const int64_t* ids, int64_t slots, int32_t experts, int32_t* order, int32_t* positions,
+                               int32_t* offsets, void* workspace, size_t ws_bytes, feq_stream_t stream) {
+    if (slots < 0 || experts < 1) return fail(FEQ_ERR_INVALID, "plan of %lld slots over %d experts", (long long)slots, experts);
+    if (experts > kMaxExperts) return fail(FEQ_ERR_UNSUPPORTED, "more than %d experts", kMaxExperts);
+    if (slots > INT32_MAX) return fail(FEQ_ERR_UNSUPPORTED, "more than 2^31 - 1 slots");
+    if (!offsets || (slots && (!ids || !order || !positions))) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    hipStream_t s = stream_of(stream);
+    if (slots == 0) {
+        FEQ_LAUNCH("k_plan_empty", k_plan_empty, dim3(ceil_div(experts + 1, 256)), dim3(256), 0, s, offsets, experts);
+        return FEQ_OK;
+    }
+    int bits = 1;
+    while ((1 << bits) < experts + 2) ++bits;
+    if (plan_one(slots, experts)) {
+        FEQ_LAUNCH("k_plan_one", k_plan_one, dim3(1), dim3(1024), 17 * (experts + 2) * sizeof(int), s, ids,
+                   static_cast<int>(slots), experts, bits, order, positions, offsets);
+        return FEQ_OK;
+    }
+    if (!workspace || ws_bytes < feq_expert_plan_workspace(slots, experts))
+        return fail(FEQ_ERR_WORKSPACE, "plan workspace of %zu bytes, %zu needed", ws_bytes,
+                    feq_expert_plan_workspace(slots, experts));
+    const int64_t ntiles = ceil_div(slots, kPlanTile);
+    int32_t* hist = static_cast<int32_t*>(workspace);
+    int32_t* total = hist + (experts + 1) * ntiles;
+    FEQ_LAUNCH("k_plan_hist", k_plan_hist, dim3(ntiles), dim3(256), 0, s, ids, slots, experts, ntiles, hist);
+    FEQ_LAUNCH("k_plan_scan", k_plan_scan, dim3(experts + 1), dim3(256), 0, s, hist, ntiles, total);
+    FEQ_LAUNCH("k_plan_place", k_plan_place, dim3(ntiles), dim3(256), 0, s, ids, slots, experts, bits, ntiles, hist,
+               total, order, positions, offsets);
+    return FEQ_OK;
+}

@@ -9,6 +9,7 @@ runs in hand-written HIP kernels (``libflasheq.so``) reached through a C ABI.
 from .representations import (Irrep, ProductIrrep, Repr, ProductRepr, WignerD, WignerDBasis,
                               random_rotation)
 from .graph import Graph
+from .experts import ExpertPlan, expert_linear, expert_topk
 from .layers.radial import RadialBasisFunctions, RadialMLP, SeparableRadialNet
 from .layers import (
     EquivariantEdgewiseLinear,
@@ -19,6 +20,10 @@ from .layers import (
     EquivariantGating,
     EquivariantLayerNorm,
     SeparableEquivariantLayerNorm,
+    InvariantLayerNorm,
+    ExpertRouter,
+    EquivariantExpertLinear,
+    EquivariantExpertMLP,
     GraphPooling,
     EquivariantTransformerBlock,
     EquivariantTransformer,
@@ -33,6 +38,8 @@ __all__ = [
     "GraphPooling", "EquivariantEdgeAttention",
     "EquivariantTransformerBlock", "EquivariantTransformer",
     "WignerDBasis",
+    "InvariantLayerNorm", "ExpertPlan", "expert_topk", "expert_linear",
+    "ExpertRouter", "EquivariantExpertLinear", "EquivariantExpertMLP",
     "RadialBasisFunctions", "RadialMLP", "SeparableRadialNet",
     "CUDANotAvailableError",
 ]

@@ -20,6 +20,7 @@ FEQ_MAX_BLOCKS = 17
 FEQ_MAX_SLOTS = 128
 FEQ_EW_HALF_ACCURACY = 1          # flags of feq_edgewise_*_ex
 POOL_MAX_HEADS = 16               # heads of feq_edgewise_*_src_pool
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}    # feq_dtype
 
 
 class CUDANotAvailableError(RuntimeError):
@@ -184,6 +185,25 @@ _SIGS = {
     "feq_attn_pool_bwd": ([_P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _P, _P],
                           ctypes.c_int),
     "feq_attn_pool_grad_attn": ([_P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _P], ctypes.c_int),
+    # mixture-of-experts node MLP
+    "feq_layernorm_fwd": ([_P, _I64, _I64, _I64, _I32, _P, _P, _I32, _F, _P, _P, _P, _P], ctypes.c_int),
+    "feq_layernorm_bwd_workspace": ([_I64, _I64], _SZ),
+    "feq_layernorm_bwd": ([_P, _I64, _P, _I64, _I64, _I64, _I32, _P, _I32, _P, _P, _P, _P, _P, _P, _SZ, _P],
+                          ctypes.c_int),
+    "feq_expert_topk_workspace": ([_I64, _I32], _SZ),
+    "feq_expert_topk_fwd": ([_P, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _SZ, _P], ctypes.c_int),
+    "feq_expert_topk_bwd": ([_P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _P], ctypes.c_int),
+    "feq_expert_plan_workspace": ([_I64, _I32], _SZ),
+    "feq_expert_plan": ([_P, _I64, _I32, _P, _P, _P, _P, _SZ, _P], ctypes.c_int),
+    "feq_expert_dispatch": ([_P, _I64, _I64, _I32, _I64, _I32, _P, _P, _P, _P], ctypes.c_int),
+    "feq_expert_combine": ([_P, _I64, _I64, _I32, _I64, _I32, _P, _P, _P, _I32, _P, _P], ctypes.c_int),
+    "feq_expert_combine_bwd": ([_P, _P, _I64, _I64, _I32, _I64, _I32, _P, _P, _P, _I32, _P, _P, _P], ctypes.c_int),
+    "feq_expert_linear_fwd": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I32, _P, _P, _P],
+                              ctypes.c_int),
+    "feq_expert_linear_bwd_x": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P], ctypes.c_int),
+    "feq_expert_linear_bwd_w_workspace": ([_I32, _I32, _I64, _I32, _I32, _I32], _SZ),
+    "feq_expert_linear_bwd_w": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _I32, _P, _P, _P, _P, _SZ, _P],
+                                ctypes.c_int),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGS)

@@ -228,3 +228,34 @@ class SeparableEquivariantLayerNorm(nn.Module):
 
     def extra_repr(self) -> str:
         return f"nscalar={self.nscalar}, nhigher={self.nhigher}"
+
+
+class InvariantLayerNorm(nn.Module):
+    """LayerNorm over the last axis of invariant features (..., width): irrep norms, scalar
+    channels, the input of a router or an invariant head.  (The equivariant norms above
+    normalise the channels of (..., mult, dim) features.)  GPU features in float32, float16 or
+    bfloat16 take the kernels (``csrc/layernorm.hip``) with float32 statistics; other dtypes and
+    devices PyTorch's layer norm."""
+
+    def __init__(self, width: int, epsilon: float = 1e-5, affine: bool = True) -> None:
+        super().__init__()
+        if width < 1:
+            raise ValueError(f"width must be positive, got {width}")
+        self.width = width
+        self.epsilon = epsilon
+        if affine:
+            self.weight = nn.Parameter(torch.ones(width))
+            self.bias = nn.Parameter(torch.zeros(width))
+        else:
+            self.register_parameter("weight", None)
+            self.register_parameter("bias", None)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.shape[-1:] != (self.width,):
+            raise ValueError(f"features must be (..., {self.width}), got {tuple(x.shape)}")
+        if x.is_cuda and x.dtype in ops.N.DTYPES:
+            return ops.layer_norm(x, self.weight, self.bias, self.epsilon)
+        return nn.functional.layer_norm(x, (self.width,), self.weight, self.bias, self.epsilon)
+
+    def extra_repr(self) -> str:
+        return f"{self.width}, epsilon={self.epsilon}, affine={self.weight is not None}"

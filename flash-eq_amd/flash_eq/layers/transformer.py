@@ -14,6 +14,7 @@ from ..graph import Graph
 from ..representations import Repr, WignerDBasis
 from ..ops import FanOutFn, ResidualScaleCmFn, ResidualScaleFn, ScaleFn
 from .attention import EquivariantAttention
+from .experts import EquivariantExpertMLP
 from .gating import EquivariantGating
 from .linear import EquivariantLinear
 from .norm import SeparableEquivariantLayerNorm
@@ -60,7 +61,10 @@ class DropPath(nn.Module):
 
 
 class EquivariantTransformerBlock(nn.Module):
-    """norm -> attention (-> residual when reprs match) -> norm -> gated MLP -> residual."""
+    """norm -> attention (-> residual when reprs match) -> norm -> gated MLP -> residual.
+
+    With ``num_experts`` > 0 the MLP is a mixture of experts (``EquivariantExpertMLP``), each node
+    taking ``experts_per_node`` of them; the reference has no such option."""
 
     def __init__(self, in_repr: Repr, out_repr: Repr, num_heads: int = 1, num_bins: int = 100,
                  rank: int = 4, hidden_dim: int = 64, min_dist: float = 0.0,
@@ -68,7 +72,8 @@ class EquivariantTransformerBlock(nn.Module):
                  dropout: float = 0.0, drop_path: float = 0.0,
                  layer_scale_init: float | None = 1e-4, use_gating: bool = True,
                  use_s2_activation: bool = False, s2_precision: int = 47,
-                 distance_decay_scale: float | None = None) -> None:
+                 distance_decay_scale: float | None = None, num_experts: int = 0,
+                 experts_per_node: int = 2) -> None:
         super().__init__()
         if use_s2_activation:
             raise NotImplementedError(
@@ -84,10 +89,14 @@ class EquivariantTransformerBlock(nn.Module):
             hidden_dim=hidden_dim, min_dist=min_dist, max_dist=max_dist, log_bins=log_bins,
             dropout=dropout, reduce="sum", distance_decay_scale=distance_decay_scale)
         self.norm2 = SeparableEquivariantLayerNorm(out_repr)
-        hidden = Repr(lvals=out_repr.lvals, mult=out_repr.mult * mlp_ratio)
-        self.mlp_up = EquivariantLinear(out_repr, hidden, bias=True)
-        self.mlp_act: nn.Module = EquivariantGating(hidden) if use_gating else nn.Identity()
-        self.mlp_down = EquivariantLinear(hidden, out_repr, bias=True)
+        self.experts: EquivariantExpertMLP | None = None
+        if num_experts > 0:
+            self.experts = EquivariantExpertMLP(out_repr, num_experts, experts_per_node, mlp_ratio, use_gating)
+        else:
+            hidden = Repr(lvals=out_repr.lvals, mult=out_repr.mult * mlp_ratio)
+            self.mlp_up = EquivariantLinear(out_repr, hidden, bias=True)
+            self.mlp_act: nn.Module = EquivariantGating(hidden) if use_gating else nn.Identity()
+            self.mlp_down = EquivariantLinear(hidden, out_repr, bias=True)
         if layer_scale_init is not None and self._use_attn_residual:
             self.layer_scale_attn: nn.Module = LayerScale(layer_scale_init)
         else:
@@ -115,6 +124,9 @@ class EquivariantTransformerBlock(nn.Module):
             x = _residual(nf, attn_out, self.layer_scale_attn, self.drop_path)
         else:
             x = attn_out
+        if self.experts is not None:
+            h, xr = self.norm2.forward_pair(x) if self.norm2.cm_ok(x) else (self.norm2(x), x)
+            return _residual(xr, self.experts(h), self.layer_scale_mlp, self.drop_path)
         if (isinstance(self.mlp_act, EquivariantGating) and self.mlp_act.kernels_ok(x)
                 and self.mlp_up.fused_ok(x) and self.mlp_down.fused_ok(x)):
             # the MLP runs component-major (dim, N, c) from the norm's output to
@@ -140,14 +152,16 @@ class EquivariantTransformerBlock(nn.Module):
 
 
 class EquivariantTransformer(nn.Module):
-    """Stack of blocks: in -> hidden -> ... -> hidden -> out, basis computed from coordinates."""
+    """Stack of blocks: in -> hidden -> ... -> hidden -> out, basis computed from coordinates.
+    ``num_experts`` > 0 makes every block's MLP a mixture of experts."""
 
     def __init__(self, in_repr: Repr, hidden_repr: Repr, out_repr: Repr, num_layers: int = 6,
                  num_heads: int = 1, num_bins: int = 100, rank: int = 4, hidden_dim: int = 64,
                  min_dist: float = 0.0, max_dist: float = 10.0, log_bins: bool = False,
                  mlp_ratio: int = 2, dropout: float = 0.0, drop_path: float = 0.0,
                  layer_scale_init: float | None = 1e-4, use_s2_activation: bool = False,
-                 s2_precision: int = 47, distance_decay_scale: float | None = None) -> None:
+                 s2_precision: int = 47, distance_decay_scale: float | None = None,
+                 num_experts: int = 0, experts_per_node: int = 2) -> None:
         super().__init__()
         self.in_repr = in_repr
         self.hidden_repr = hidden_repr
@@ -166,7 +180,8 @@ class EquivariantTransformer(nn.Module):
                 rank=rank, hidden_dim=hidden_dim, min_dist=min_dist, max_dist=max_dist,
                 log_bins=log_bins, mlp_ratio=mlp_ratio, dropout=dropout, drop_path=rates[i],
                 layer_scale_init=layer_scale_init, use_s2_activation=use_s2_activation,
-                s2_precision=s2_precision, distance_decay_scale=distance_decay_scale))
+                s2_precision=s2_precision, distance_decay_scale=distance_decay_scale,
+                num_experts=num_experts, experts_per_node=experts_per_node))
         self.final_norm = SeparableEquivariantLayerNorm(out_repr)
 
     def forward(self, coordinates: torch.Tensor, node_features: torch.Tensor,

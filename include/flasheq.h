@@ -733,6 +733,91 @@ size_t feq_dot_f64_workspace(void);
 int feq_dot_f64(const float* a, const float* b, int64_t n, float* out, void* workspace,
                 size_t ws_bytes, feq_stream_t stream);
 
+/* ---- mixture-of-experts node MLP -------------------------------------------------
+ * No counterpart in the reference, whose block has one dense MLP for all nodes
+ * (transformer.py:187-206): here a router chooses experts per node from the node's
+ * invariants, the rows are sorted by expert, mapped by the experts' EquivariantLinear
+ * weights and summed back with the router's weights.  Element types are feq_dtype;
+ * sums, statistics and accumulators are float32 and results are rounded once. */
+enum feq_dtype { FEQ_F32 = 0, FEQ_F16 = 1, FEQ_BF16 = 2 };
+
+/* Layer norm over the last axis, y = (x - mean) / sqrt(var + eps) * weight + bias with
+ * the biased variance.  x: rows of `width` elements, ldx apart (ldx >= width); y contiguous;
+ * weight, bias (width) of param_dtype, either may be NULL.  mean, rstd (rows floats): for
+ * the backward, both or neither NULL. */
+int feq_layernorm_fwd(const void* x, int64_t rows, int64_t width, int64_t ldx, int32_t dtype, const void* weight,
+                      const void* bias, int32_t param_dtype, float eps, void* y, float* mean, float* rstd,
+                      feq_stream_t stream);
+/* Its gradients from grad_y (rows ldg apart): grad_x (contiguous), grad_w, grad_b of
+ * param_dtype, any of them NULL.  The parameters' sums over rows run in a fixed order.
+ * rows = 0 writes zero parameter gradients.  Workspace feq_layernorm_bwd_workspace bytes
+ * when a parameter gradient is wanted. */
+size_t feq_layernorm_bwd_workspace(int64_t rows, int64_t width);
+int feq_layernorm_bwd(const void* grad_y, int64_t ldg, const void* x, int64_t rows, int64_t width, int64_t ldx,
+                      int32_t dtype, const void* weight, int32_t param_dtype, const float* mean, const float* rstd,
+                      void* grad_x, void* grad_w, void* grad_b, void* workspace, size_t ws_bytes,
+                      feq_stream_t stream);
+
+/* The top_k largest of each row of logits (rows, experts), equal ones by the lowest
+ * index, a NaN as the largest: ids (rows, top_k) and weights, the softmax over all experts
+ * at the chosen ones, divided by their sum where normalize is set.  A logit of -inf is
+ * never chosen: its place holds id -1 and weight 0.  mean (experts, may be NULL): the mean
+ * over the rows of the softmax (a row of -inf alone counts 0; of no rows: 0); it needs a workspace of
+ * feq_expert_topk_workspace bytes.  experts <= 1024, top_k <= 64. */
+size_t feq_expert_topk_workspace(int64_t rows, int32_t experts);
+int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t experts, int32_t dtype, int32_t top_k,
+                        int32_t normalize, int64_t* ids, float* weights, float* mean, void* workspace,
+                        size_t ws_bytes, feq_stream_t stream);
+/* grad_logits from the gradients of weights and mean (either may be NULL), with the
+ * forward's ids and weights. */
+int feq_expert_topk_bwd(const void* logits, const int64_t* ids, const float* weights, const float* grad_weights,
+                        const float* grad_mean, int64_t rows, int32_t experts, int32_t dtype, int32_t top_k,
+                        int32_t normalize, void* grad_logits, feq_stream_t stream);
+
+/* The slots (row t, choice k) -> t * top_k + k sorted by their expert ids[slot], stably,
+ * those whose id lies outside [0, experts) last: order (slots), the slot at every place;
+ * positions (slots), its inverse; offsets (experts + 1), every expert's first place, the
+ * last one the number of slots with an expert.  experts <= 1024, slots < 2^31. */
+size_t feq_expert_plan_workspace(int64_t slots, int32_t experts);
+int feq_expert_plan(const int64_t* ids, int64_t slots, int32_t experts, int32_t* order, int32_t* positions,
+                    int32_t* offsets, void* workspace, size_t ws_bytes, feq_stream_t stream);
+
+/* Rows into expert order and back.  x, y (planes, rows, width), xs, ys (planes, rows top_k,
+ * width), contiguous; positions (rows, top_k) and placed = &offsets[experts] of a plan.
+ * dispatch: xs[d, positions[t, k]] = x[d, t]; zeros at places without an expert.
+ * combine: y[d, t] = sum_k weights[t, k] ys[d, positions[t, k]] over the slots with an expert;
+ * weights (rows, top_k) of weight_dtype, NULL for 1 (the gradient of dispatch).
+ * combine_bwd: grad_ys (zeros at places without an expert) and grad_weights (0 there), either NULL. */
+int feq_expert_dispatch(const void* x, int64_t planes, int64_t rows, int32_t top_k, int64_t width, int32_t dtype,
+                        const int32_t* positions, const int32_t* placed, void* xs, feq_stream_t stream);
+int feq_expert_combine(const void* ys, int64_t planes, int64_t rows, int32_t top_k, int64_t width, int32_t dtype,
+                       const int32_t* positions, const int32_t* placed, const void* weights, int32_t weight_dtype,
+                       void* y, feq_stream_t stream);
+int feq_expert_combine_bwd(const void* grad_y, const void* ys, int64_t planes, int64_t rows, int32_t top_k,
+                           int64_t width, int32_t dtype, const int32_t* positions, const int32_t* placed,
+                           const void* weights, int32_t weight_dtype, void* grad_ys, void* grad_weights,
+                           feq_stream_t stream);
+
+/* The experts' EquivariantLinear on component-major tables of rows sorted by expert: x (dim, slots,
+ * cin), y (dim, slots, cout), weight (experts, nreps, cout, cin), bias (experts, cout, nbias) or NULL,
+ * all of dtype; offsets of the plan.  Rows offsets[e] .. offsets[e + 1] of the plane of a component of irrep r
+ * are multiplied by weight[e, r]^T; bias column bias_cols[r] (-1: none; each column one scalar irrep's) is added;
+ * rows from offsets[experts] on are 0 and enter no gradient.  experts <= 1024, nreps <= 32, dim <= 128. */
+int feq_expert_linear_fwd(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
+                          int32_t cout, int32_t dtype, const void* x, const void* weight, const int32_t* offsets,
+                          const void* bias, int32_t nbias, const int32_t* bias_cols, void* y, feq_stream_t stream);
+int feq_expert_linear_bwd_x(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
+                            int32_t cout, int32_t dtype, const void* grad_y, const void* weight,
+                            const int32_t* offsets, void* grad_x, feq_stream_t stream);
+/* grad_weight and, unless NULL, grad_bias: sums in a fixed order, zeros for an expert without rows.
+ * Workspace feq_expert_linear_bwd_w_workspace bytes (nbias 0 without grad_bias). */
+size_t feq_expert_linear_bwd_w_workspace(int32_t nreps, int32_t experts, int64_t slots, int32_t cin, int32_t cout,
+                                         int32_t nbias);
+int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
+                            int32_t cout, int32_t dtype, const void* grad_y, const void* x, const int32_t* offsets,
+                            int32_t nbias, const int32_t* bias_cols, void* grad_weight, void* grad_bias,
+                            void* workspace, size_t ws_bytes, feq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -17,6 +17,7 @@ Contents (each function cites the reference ``file:line`` it restates):
                     follows the CUDA kernels' per-edge loops and float32 binning.
 * ``radial``     -- ``SeparableRadialNet`` table formula.
 * ``graphops``   -- sum pooling and the per-destination edge softmax.
+* ``experts``    -- mixture-of-experts routing, the experts' maps, plain layer norm.
 * ``layer``      -- ``EquivariantEdgewiseLinear`` / attention composition.
 
 Pinning status of every function is recorded in its docstring ("pinned by"

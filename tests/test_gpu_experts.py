@@ -1,0 +1,565 @@
+"""Expert routing kernels (csrc/expert_route.hip, expert_rows.hip, expert_linear.hip) against the float64
+oracle on the same inputs.
+
+u = 2^-24 (float32), h(t) half a step of the stored type t.  Whole numbers and moved rows are exact.
+Float32 sums of n terms are off by at most n u of their absolute terms; the matrix cores' sums are
+counted twice (2 n u), for the steps inside an instruction."""
+import pytest
+import torch
+
+import flash_eq as fe
+from oracle import experts as OE
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -133}
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+INF, NAN = float("inf"), float("nan")
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def within(got, want, tol):
+    err = (got.detach().double().cpu() - want).abs()
+    bad = ~(err <= tol + TINY[got.dtype])
+    assert not bad.any(), (float((err - tol).max()), int(bad.sum()), tuple(got.shape))
+
+
+# ---- top-k -----------------------------------------------------------------------------
+
+def check_topk(dev, logits, k, normalize, seed=0):
+    g = gen(seed)
+    rows, experts = logits.shape
+    l64 = logits.double().cpu().requires_grad_()
+    ids = OE.topk_ids(l64.detach(), k)
+    w, mean = OE.topk_weights(l64, ids, normalize)
+    gw, gm = torch.randn(rows, k, generator=g), torch.randn(experts, generator=g)
+    (gl,) = torch.autograd.grad((w * gw.double()).sum() + (mean * gm.double()).sum(), [l64])
+
+    ll = logits.detach().requires_grad_()
+    ids2, w2, mean2 = fe.expert_topk(ll, k, normalize)
+    assert ids2.dtype == torch.int64 and w2.dtype == mean2.dtype == torch.float32
+    assert torch.equal(ids2.cpu(), ids)
+    (gl2,) = torch.autograd.grad([w2, mean2], [ll], [gw.to(dev), gm.to(dev)])
+    # the exponent l - max is off by u |l - max|; exp by 2 u; sums over the experts by 24 u (16 a lane, 6 levels)
+    x = l64.detach()
+    top = x.masked_fill(torch.isinf(x), -1e30).amax(1, keepdim=True)
+    span = (x - top).abs().masked_fill(torch.isinf(x), 0.0).clamp(max=110)    # below, exp is 0 in float32
+    rel = U * (40 + span.amax(1, keepdim=True))
+    floor = 2.0 ** -125           # below the smallest normal number exp may flush to 0
+    within(w2, w.detach(), rel * w.detach() + floor)
+    p = OE.softmax(x)
+    # a lane adds at most rows / 4 values and 1024 workgroups' sums are added by a fixed tree
+    within(mean2, mean.detach(), ((rel + U * (96 + rows / 4)) * p).sum(0) / max(rows, 1) + floor)
+    routed = torch.zeros_like(x)
+    scale = (w.detach() if normalize else p.gather(1, ids.clamp(min=0)) * (ids >= 0))
+    dot = (scale * gw.double().abs()).sum(1, keepdim=True)
+    routed.scatter_add_(1, ids.clamp(min=0), scale * (gw.double().abs() + dot) * (ids >= 0))
+    if not normalize:
+        routed = routed + p * dot
+    gma = gm.double().abs() / max(rows, 1)
+    tol = HALF[logits.dtype] * gl.abs() + (4 * rel + U * 64) * (routed + p * (gma + (p * gma).sum(1, keepdim=True))) + floor
+    within(gl2, gl, tol)
+    with torch.no_grad():
+        for a, b in zip(fe.expert_topk(logits, k, normalize), (ids2, w2, mean2)):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,experts,k", [(1, 1, 1), (5, 2, 1), (9, 7, 7), (100, 8, 2), (64, 16, 4), (33, 64, 8),
+                                            (17, 100, 3), (9, 256, 5), (5, 512, 2), (4, 513, 4), (3, 1000, 64),
+                                            (3, 1024, 1), (3001, 8, 2)])
+def test_topk_sizes(dev, rows, experts, k, dtype):
+    logits = (2 * torch.randn(rows, experts, generator=gen(rows + experts))).to(dev, dtype)
+    for normalize in (True, False):
+        check_topk(dev, logits, k, normalize)
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_topk_masks_and_ties(dev, dtype, normalize):
+    g = gen(1)
+    l = torch.randn(12, 10, generator=g)
+    l[0] = -INF                                  # nothing left
+    l[1, 1:] = -INF                              # less left than chosen
+    l[2, ::2] = -INF
+    l[3] = 0.0                                   # all equal
+    l[4] = torch.tensor([0.0, -0.0] * 5)
+    l[5] = torch.finfo(dtype).min                # masked by the type's lowest value instead
+    l[6, 3:] = torch.finfo(dtype).min
+    l[7, 0], l[7, 9] = torch.finfo(dtype).max, torch.finfo(dtype).min
+    l[8] = torch.round(l[8])                     # some equal
+    l[9] *= 50
+    check_topk(dev, l.to(dev, dtype), 3, normalize)
+    check_topk(dev, l.to(dev, dtype), 10, normalize)
+
+
+def test_topk_nan_and_infinity_stay_in_their_rows(dev):
+    l = torch.randn(40, 24, generator=gen(2)).to(dev)
+    a = l.clone().requires_grad_()
+    ids, w, _ = fe.expert_topk(a, 3)
+    gw = torch.randn(40, 3, generator=gen(3)).to(dev)
+    (ga,) = torch.autograd.grad([w], [a], [gw])
+    b = l.clone()
+    b[4, 20], b[9, 2], b[9, 7], b[30, 5] = NAN, NAN, NAN, INF
+    b.requires_grad_()
+    ids2, w2, _ = fe.expert_topk(b, 3)
+    (gb,) = torch.autograd.grad([w2], [b], [gw])
+    assert ids2[4, 0] == 20 and ids2[9, :2].tolist() == [2, 7] and ids2[30, 0] == 5
+    assert torch.isnan(w2[4]).any() and torch.isnan(w2[9]).any()
+    keep = [r for r in range(40) if r not in (4, 9, 30)]
+    for x, y in ((ids, ids2), (w, w2), (ga, gb)):
+        assert torch.equal(x[keep], y[keep])
+
+
+def test_topk_gradients_one_by_one_shapes_and_no_rows(dev):
+    l = torch.randn(6, 5, 12, generator=gen(4)).to(dev)
+    ids, w, mean = fe.expert_topk(l, 2)
+    ids2, w2, mean2 = fe.expert_topk(l.view(30, 12), 2)
+    assert ids.shape == w.shape == (6, 5, 2)
+    assert torch.equal(ids.view(30, 2), ids2) and torch.equal(w.view(30, 2), w2) and torch.equal(mean, mean2)
+    t = l.view(30, 12).t().contiguous().t()      # not contiguous
+    assert torch.equal(fe.expert_topk(t, 2)[1], w2)
+    for normalize in (True, False):
+        a = l.view(30, 12).clone().requires_grad_()
+        ids, w, mean = fe.expert_topk(a, 2, normalize)
+        gw, gm = torch.randn(30, 2, generator=gen(5)).to(dev), torch.randn(12, generator=gen(6)).to(dev)
+        (both,) = torch.autograd.grad([w, mean], [a], [gw, gm], retain_graph=True)
+        (one,) = torch.autograd.grad([w], [a], [gw], retain_graph=True)
+        (two,) = torch.autograd.grad([mean], [a], [gm])
+        assert (one + two - both).abs().max() < 1e-6 * both.abs().max()
+    e = torch.empty(0, 12, device=dev, requires_grad=True)
+    ids, w, mean = fe.expert_topk(e, 2)
+    assert ids.shape == (0, 2) and not mean.any()
+    (ge,) = torch.autograd.grad([w, mean], [e], [torch.empty(0, 2, device=dev), torch.ones(12, device=dev)])
+    assert ge.shape == (0, 12)
+
+
+def test_topk_gradient_against_differences(dev):
+    l = torch.randn(3, 6, generator=gen(7), dtype=torch.float64)
+    gw = torch.randn(3, 2, generator=gen(8), dtype=torch.float64)
+
+    def loss(v):
+        _, w, mean = fe.expert_topk(v.float().to(dev), 2, False)
+        return (w.double().cpu() * gw).sum() + mean.double().cpu()[0]
+
+    a = l.float().to(dev).requires_grad_()
+    _, w, mean = fe.expert_topk(a, 2, False)
+    ((w * gw.float().to(dev)).sum() + mean[0]).backward()
+    step = 2.0 ** -7
+    for i in range(3):
+        for j in range(6):
+            d = torch.zeros_like(l)
+            d[i, j] = step
+            diff = (loss(l + d) - loss(l - d)) / (2 * step)
+            # third derivatives of a softmax are below 1 per unit of weight; float32 values are off by 2^-22 each
+            assert abs(diff - a.grad[i, j].item()) < step ** 2 * gw.abs().sum() + 2.0 ** -20 / step
+
+
+# ---- plan and rows ---------------------------------------------------------------------
+
+def some_ids(g, rows, k, experts, bad=0.1):
+    """Random experts; a tenth of the slots outside the experts' range, near and far."""
+    ids = torch.randint(0, experts, (rows, k), generator=g)
+    outside = torch.tensor([-1, experts, 2 ** 40, -2 ** 62])[torch.randint(0, 4, (rows, k), generator=g)]
+    return torch.where(torch.rand(rows, k, generator=g) < bad, outside, ids)
+
+
+@pytest.mark.parametrize("rows,k,experts", [(0, 2, 4), (1, 1, 1), (5, 1, 3), (100, 2, 8), (64, 1, 64), (333, 3, 65),
+                                            (4096, 2, 8), (8193, 1, 5), (1000, 64, 9), (3000, 4, 1024), (2049, 8, 100),
+                                            (30011, 2, 16), (700, 2, 1024)])
+def test_plan_is_exact(dev, rows, k, experts):
+    ids = some_ids(gen(rows + k), rows, k, experts)
+    order, positions, offsets = OE.plan(ids, experts)
+    plan = fe.ExpertPlan(ids.to(dev), experts)
+    assert torch.equal(plan.order.cpu().long(), order)
+    assert torch.equal(plan.positions.cpu().long(), positions)
+    assert torch.equal(plan.offsets.cpu().long(), offsets)
+
+
+def test_plan_of_one_expert_none_and_small_integer_types(dev):
+    for value, n in ((3, 5000), (-1, 5000), (7, 20)):
+        plan = fe.ExpertPlan(torch.full((n, 2), value, device=dev), 7)
+        want = 2 * n if 0 <= value < 7 else 0
+        assert plan.offsets[-1].item() == want and torch.equal(plan.order.cpu(), torch.arange(2 * n, dtype=torch.int32))
+    ids = torch.tensor([2, 0, 1, 0])
+    for t in (torch.int32, torch.int16, torch.int8, torch.uint8):
+        plan = fe.ExpertPlan(ids.to(dev, t), 3)
+        assert plan.order.tolist() == [1, 3, 2, 0] and plan.positions.shape == (4, 1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lead,rows,k,width,experts", [
+    ((), 1, 1, 1, 1), ((), 7, 2, 3, 4), ((9,), 50, 2, 64, 8), ((2, 3), 33, 3, 20, 5), ((49,), 20, 4, 128, 16),
+    ((4,), 100, 5, 33, 8), ((), 300, 8, 576, 12), ((1,), 65, 1, 1152, 3), ((3,), 41, 9, 6, 10)])
+def test_rows_and_their_gradients(dev, lead, rows, k, width, experts, dtype):
+    g = gen(rows * k + width)
+    ids = some_ids(g, rows, k, experts)
+    ids[0] = -1                                  # a row without any expert
+    x = torch.randn(*lead, rows, width, generator=g).to(dtype)
+    ys = torch.randn(*lead, rows * k, width, generator=g).to(dtype)
+    w = torch.randn(rows, k, generator=g)
+    gxs, gy = torch.randn(*lead, rows * k, width, generator=g).to(dtype), torch.randn(*lead, rows, width, generator=g).to(dtype)
+    x64, ys64, w64 = (t.double().requires_grad_() for t in (x, ys, w))
+    xs_r = OE.dispatch(x64, ids, experts)
+    y_r = OE.combine(ys64, w64, ids, experts)
+    gx_r, gys_r, gw_r = torch.autograd.grad([xs_r, y_r], [x64, ys64, w64], [gxs.double(), gy.double()])
+
+    plan = fe.ExpertPlan(ids.to(dev), experts)
+    xl, yl, wl = (t.to(dev).requires_grad_() for t in (x, ys, w))
+    xs = plan.dispatch(xl)
+    y = plan.combine(yl, wl)
+    gx, gys, gw = torch.autograd.grad([xs, y], [xl, yl, wl], [gxs.to(dev), gy.to(dev)])
+    assert torch.equal(xs.detach().cpu().double(), xs_r.detach())           # moved, not computed
+    absolute = OE.combine(ys.double().abs(), w.double().abs(), ids, experts)
+    within(y, y_r.detach(), HALF[dtype] * y_r.detach().abs() + U * (k + 1) * absolute)
+    ones = torch.ones(rows, k, dtype=torch.float64)
+    within(gx, gx_r, HALF[dtype] * gx_r.abs() + U * k * OE.combine(gxs.double().abs(), ones, ids, experts))
+    within(gys, gys_r, (HALF[dtype] + U) * gys_r.abs())
+    # a lane's run: its planes times its 8 (16-bit) or 4 elements a vector, one for odd widths, then 6 + 16 more
+    a64, b64 = ys.double().abs().requires_grad_(), torch.ones(rows, k, dtype=torch.float64, requires_grad=True)
+    (mass,) = torch.autograd.grad(OE.combine(a64, b64, ids, experts), [b64], gy.double().abs())
+    planes = x.numel() // (rows * width)
+    within(gw, gw_r, U * (gw_r.abs() + (planes + 8 * (width // 64 + 1) * (planes // 4 + 1) + 32) * mass))
+
+
+def test_rows_strides_weight_types_and_unaligned_views(dev):
+    g = gen(11)
+    ids = some_ids(g, 30, 2, 4).to(dev)
+    plan = fe.ExpertPlan(ids, 4)
+    x = torch.randn(30, 9, 16, generator=g).to(dev).permute(1, 0, 2)        # node-major, seen component-major
+    assert torch.equal(plan.dispatch(x), plan.dispatch(x.contiguous()))
+    flat = torch.randn(9 * 30 * 16 + 1, generator=g).to(dev)[1:].view(9, 30, 16)   # 4-byte aligned
+    assert torch.equal(plan.dispatch(flat), plan.dispatch(flat.clone()))
+    half = torch.randn(30 * 16 + 1, generator=g).to(dev, torch.bfloat16)[1:].view(30, 16)
+    assert torch.equal(plan.dispatch(half), plan.dispatch(half.clone()))
+    ys = torch.randn(9 * 60 * 16 + 1, generator=g).to(dev)[1:].view(9, 60, 16)
+    w = torch.rand(30, 2, generator=g).to(dev)
+    for t in TYPES:
+        wt = w.to(t).requires_grad_()
+        y = plan.combine(ys, wt)
+        assert torch.equal(y, plan.combine(ys.clone(), wt.detach().float()))
+        (gw,) = torch.autograd.grad(y.sum(), [wt])
+        assert gw.dtype == t
+    one = fe.ExpertPlan(ids[:, 0].contiguous(), 4)
+    assert torch.equal(one.combine(ys[0, :30], w[:, 0]), one.combine(ys[0, :30], w[:, :1]))
+
+
+def test_the_same_expert_twice_and_unrouted_garbage(dev):
+    """A row may name an expert twice; what stands in the places without an expert is never read."""
+    ids = torch.tensor([[1, 1], [0, -1], [-1, -1], [2, 0]], device=dev)
+    plan = fe.ExpertPlan(ids, 3)
+    x = torch.randn(4, 5, generator=gen(12)).to(dev)
+    xs = plan.dispatch(x)
+    n = plan.offsets[-1].item()
+    assert n == 5 and not xs[n:].any()
+    w = torch.tensor([[0.25, 0.5], [2.0, NAN], [INF, NAN], [1.0, 1.0]], device=dev)
+    ys = xs.clone()
+    ys[n:] = NAN
+    ys.requires_grad_()
+    wl = w.clone().requires_grad_()
+    y = plan.combine(ys, wl)
+    want = torch.stack([0.75 * x[0], 2 * x[1], 0 * x[2], 2 * x[3]])
+    assert torch.allclose(y, want, atol=1e-6) and not y[2].any()
+    gys, gw = torch.autograd.grad(y, [ys, wl], torch.ones_like(y))
+    assert not gys[n:].any() and torch.isfinite(gys).all()
+    assert gw[1, 1] == 0 and not gw[2].any() and torch.isfinite(gw).all()
+    xl = x.clone().requires_grad_()
+    g = torch.randn(8, 5, generator=gen(13)).to(dev)
+    g[n:] = NAN
+    (gx,) = torch.autograd.grad(plan.dispatch(xl), [xl], g)
+    assert torch.isfinite(gx).all() and not gx[2].any()
+
+
+def test_rows_without_elements(dev):
+    plan = fe.ExpertPlan(torch.empty(0, 2, dtype=torch.int64, device=dev), 3)
+    assert plan.offsets.tolist() == [0] * 4
+    x = torch.empty(4, 0, 8, device=dev, requires_grad=True)
+    w = torch.empty(0, 2, device=dev, requires_grad=True)
+    y = plan.combine(plan.dispatch(x), w)
+    gx, gw = torch.autograd.grad(y, [x, w], torch.empty(4, 0, 8, device=dev))
+    assert y.shape == gx.shape == (4, 0, 8) and gw.shape == (0, 2)
+
+
+# ---- the experts' maps -----------------------------------------------------------------
+
+def check_linear(dev, lvals, counts, unrouted, cin, cout, dtype, bias=True, seed=0):
+    g = gen(seed)
+    experts = len(counts)
+    ids = torch.cat([torch.full((n,), e) for e, n in enumerate(counts)] + [torch.full((unrouted,), -1)]).long()
+    ids = ids[torch.randperm(ids.numel(), generator=g)]
+    slots, dim = ids.numel(), sum(2 * l + 1 for l in lvals)
+    x = torch.randn(dim, slots, cin, generator=g).to(dtype)
+    w = torch.randn(experts, len(lvals), cout, cin, generator=g).to(dtype)
+    ns = sum(l == 0 for l in lvals)
+    b = torch.randn(experts, cout, ns, generator=g).to(dtype) if bias and ns else None
+    gy = torch.randn(dim, slots, cout, generator=g).to(dtype)
+    plan = fe.ExpertPlan(ids.to(dev), experts)
+    n = plan.offsets[-1].item()
+    gyd = gy.clone()
+    x[:, n:], gyd[:, n:] = NAN, NAN              # the rows without an expert are not read
+    xl, wl = x.to(dev).requires_grad_(), w.to(dev).requires_grad_()
+    bl = b.to(dev).requires_grad_() if b is not None else None
+    leaves = [t for t in (xl, wl, bl) if t is not None]
+    y = fe.expert_linear(xl, wl, plan, lvals, bl)
+    got = torch.autograd.grad(y, leaves, gyd.to(dev))
+    with torch.no_grad():
+        assert torch.equal(fe.expert_linear(xl, wl, plan, lvals, bl), y)
+
+    def reference(f):
+        x64, w64 = f(x.nan_to_num().double()).requires_grad_(), f(w.double()).requires_grad_()
+        b64 = f(b.double()).requires_grad_() if b is not None else None
+        y64 = OE.linear(x64, w64, plan.offsets.cpu(), lvals, b64)
+        return (y64.detach(), *torch.autograd.grad(y64, [t for t in (x64, w64, b64) if t is not None], f(gy.double())))
+    want, mass = reference(lambda t: t.clone()), reference(torch.abs)
+    terms = [2 * cin + 2, 2 * cout, None, None]
+    rows = 2 * (max([1, *counts]) * (2 * max(lvals) + 1)) + 64              # terms of a weight's gradient
+    for i, (a, r, m) in enumerate(zip((y, *got), want, mass)):
+        within(a, r, HALF[dtype] * r.abs() + U * (terms[i] or rows) * m)
+    assert not y[:, n:].any() and not got[0][:, n:].any()
+
+
+CHANNELS = [(64, 128), (128, 64), (8, 8), (33, 7), (1, 1), (160, 200), (12, 260), (300, 20)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("cin,cout", CHANNELS)
+def test_linear_channels(dev, cin, cout, dtype):
+    check_linear(dev, (0, 1), [30, 0, 200, 5], 9, cin, cout, dtype, seed=cin + cout)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("lvals", [(0,), (1,), (0, 0), (2, 0, 1, 0), (0, 1, 2, 3, 4, 5, 6)])
+def test_linear_irreps(dev, lvals, dtype):
+    check_linear(dev, lvals, [17, 140], 0, 32, 48, dtype, seed=len(lvals))
+    check_linear(dev, lvals, [17, 140], 3, 32, 48, dtype, bias=False, seed=len(lvals))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("counts,unrouted", [([1], 0), ([0], 0), ([0, 0, 0], 5), ([0, 1], 0), ([128], 0), ([129, 127], 0),
+                                             ([1] * 64, 0), ([3] * 65, 2), ([0] * 100 + [40] + [2] * 99, 1), ([900, 1, 1], 0),
+                                             ([2] * 1024, 0)])
+def test_linear_counts(dev, counts, unrouted, dtype):
+    check_linear(dev, (0, 1), counts, unrouted, 24, 40, dtype, seed=len(counts))
+
+
+def test_linear_many_chunks(dev):
+    """Experts of several weight-gradient chunks beside ones of one and none."""
+    check_linear(dev, (0, 1), [5000, 100, 0, 2000, 129], 50, 16, 24, torch.float32, seed=3)
+    check_linear(dev, (0,), [3000, 64, 1500], 0, 64, 64, torch.bfloat16, seed=4)
+
+
+def test_linear_views_and_two_dimensions(dev):
+    g = gen(5)
+    plan = fe.ExpertPlan(torch.tensor([1, 0, 1, 1], device=dev), 2)
+    x = torch.randn(4, 9, generator=g).to(dev)
+    w = torch.randn(2, 1, 5, 9, generator=g).to(dev)
+    y = fe.expert_linear(x, w, plan)
+    assert y.shape == (4, 5) and torch.equal(y, fe.expert_linear(x[None], w, plan)[0])
+    t = torch.randn(9, 4, generator=g).to(dev).t()          # strided
+    assert torch.equal(fe.expert_linear(t, w, plan), fe.expert_linear(t.contiguous(), w, plan))
+    flat = torch.randn(4 * 16 + 1, generator=g).to(dev)[1:].view(4, 16)     # 4-byte aligned
+    w16 = torch.randn(2, 1, 8, 16, generator=g).to(dev)
+    assert torch.equal(fe.expert_linear(flat, w16, plan), fe.expert_linear(flat.clone(), w16, plan))
+
+
+def test_linear_infinity_stays_in_its_row_and_expert(dev):
+    g = gen(6)
+    ids = torch.arange(300, device=dev) % 3
+    plan = fe.ExpertPlan(ids, 3)
+    x = torch.randn(4, 300, 20, generator=g).to(dev)
+    w = torch.randn(3, 2, 12, 20, generator=g).to(dev)
+    gy = torch.randn(4, 300, 12, generator=g).to(dev)
+
+    def step(x):
+        xl, wl = x.clone().requires_grad_(), w.clone().requires_grad_()
+        y = fe.expert_linear(xl, wl, plan, (0, 1))
+        return (y.detach(), *torch.autograd.grad(y, [xl, wl], gy))
+    y, gx, gw = step(x)
+    x2 = x.clone()
+    x2[1, 150, 3], x2[0, 10, 0] = INF, NAN       # rows of experts 1 and 0
+    y2, gx2, gw2 = step(x2)
+    assert torch.equal(gx, gx2)
+    want = torch.sign(w[1, 1, :, 3]) * INF       # infinity times the weight
+    assert torch.equal(y2[1, 150], want) and torch.isnan(y2[0, 10]).all()
+    y2[1, 150], y2[0, 10] = y[1, 150], y[0, 10]
+    assert torch.equal(y, y2)
+    assert torch.equal(gw[2], gw2[2]) and torch.equal(gw[0, 1], gw2[0, 1]) and torch.equal(gw[1, 0], gw2[1, 0])
+
+
+def test_refusals(dev):
+    x, ids = torch.randn(6, 8, device=dev), torch.zeros(6, 2, dtype=torch.int64, device=dev)
+    with pytest.raises(ValueError, match="top_k must be 1 to 8"):
+        fe.expert_topk(x, 9)
+    with pytest.raises(TypeError, match="float64"):
+        fe.expert_topk(x.double(), 2)
+    with pytest.raises(TypeError, match="ids must be integers"):
+        fe.ExpertPlan(ids.float(), 3)
+    with pytest.raises(ValueError, match="num_experts must be"):
+        fe.ExpertPlan(ids, 0)
+    with pytest.raises(ValueError, match="ids must be"):
+        fe.ExpertPlan(ids[None], 3)
+    plan = fe.ExpertPlan(ids, 3)
+    with pytest.raises(ValueError, match="x must be"):
+        plan.dispatch(x[:5])
+    with pytest.raises(ValueError, match="ys must be"):
+        plan.combine(x, torch.ones(6, 2, device=dev))
+    with pytest.raises(ValueError, match="weights must be"):
+        plan.combine(torch.randn(12, 8, device=dev), torch.ones(6, device=dev))
+    with pytest.raises(fe.CUDANotAvailableError):
+        plan.dispatch(x.cpu())
+    with pytest.raises(TypeError, match="weights"):
+        plan.combine(torch.randn(12, 8, device=dev), torch.ones(6, 2, device=dev, dtype=torch.float64))
+    xs, w = torch.randn(1, 12, 8, device=dev), torch.randn(3, 1, 4, 8, device=dev)
+    for args, text in (((xs, w[:2], plan), "weight must be"), ((xs[:, :11], w, plan), "x must be"),
+                       ((xs, w, plan, (0, 1)), "weight must be"), ((xs, w, plan, (0,), torch.zeros(3, 4, 2, device=dev)), "bias must be"),
+                       ((xs, w, plan, ()), "lvals must be"), ((xs, w[:, :, :0], plan), "no channels")):
+        with pytest.raises(ValueError, match=text):
+            fe.expert_linear(*args)
+    with pytest.raises(TypeError, match="different dtypes"):
+        fe.expert_linear(xs, w.half(), plan)
+
+
+# ---- a run of them together ------------------------------------------------------------
+
+@pytest.mark.parametrize("top_k", [1, 2])
+def test_expert_mlp_matches_the_oracle(dev, top_k):
+    torch.manual_seed(5)
+    rp = fe.Repr([0, 1, 2], 32)
+    mlp = fe.EquivariantExpertMLP(rp, 6, top_k=top_k).to(dev)
+    with torch.no_grad():
+        for b in (mlp.up.bias, mlp.down.bias, mlp.act.linear.bias):
+            b.normal_(generator=torch.Generator(device=dev).manual_seed(1))
+    x = torch.randn(403, 32, 9, generator=gen(6))
+    xl = x.to(dev).requires_grad_()
+    y = mlp(xl)
+    gy = torch.randn(403, 32, 9, generator=gen(7))
+    params = dict(mlp.named_parameters())
+    grads = torch.autograd.grad((y * gy.to(dev)).sum() + mlp.balance, [xl, *params.values()])
+
+    x64 = x.double().requires_grad_()
+    p64 = {k: v.detach().double().cpu().requires_grad_() for k, v in params.items()}
+    inv = torch.stack([(x64[..., a:b] ** 2).sum(-1) for a, b in ((0, 1), (1, 4), (4, 9))], -1) + 1e-8
+    logits = OE.layer_norm(inv.sqrt().flatten(-2), p64["router.lnorm.weight"], p64["router.lnorm.bias"]) \
+        @ p64["router.linear.weight"].t()
+    ids = OE.topk_ids(logits.detach(), top_k)
+    # float32 logits of this size are off by less than 1e-5: no choice lies that close to another
+    top = logits.detach().sort(1, descending=True).values
+    assert (top[:, top_k - 1] - top[:, top_k]).min() > 1e-5
+    w, mean = OE.topk_weights(logits, ids, True)
+    _, _, offsets = OE.plan(ids, 6)
+    balance = 6 * ((offsets[1:] - offsets[:-1]).double() * mean).sum() / ids.numel()
+    names = dict(up_w="up.weight", up_b="up.bias", gate_w="act.linear.weight", gate_b="act.linear.bias",
+                 down_w="down.weight", down_b="down.bias")
+    y64 = OE.expert_mlp(x64, ids, w, {k: p64[v] for k, v in names.items()}, (0, 1, 2), 1e-8)
+    want = torch.autograd.grad((y64 * gy.double()).sum() + balance, [x64, *p64.values()])
+    rel = lambda a, b: ((a.detach().double().cpu() - b).abs().max() / b.abs().max()).item()
+    assert rel(y, y64.detach()) < 1e-5 and rel(mlp.balance, balance.detach()) < 1e-5
+    for name, a, b in zip(["x", *params], grads, want):
+        if top_k == 1 and name.startswith("router"):     # one weight of 1: only the balance is left, tiny
+            assert (a.detach().double().cpu() - b).abs().max() < 1e-5
+        else:
+            assert rel(a, b) < 2e-5, name
+
+
+def test_expert_block_is_equivariant_and_trains(dev):
+    """A transformer with expert MLPs: rotated inputs give the rotated output (the choice reads invariants),
+    and every parameter has a gradient."""
+    torch.manual_seed(2)
+    rp = fe.Repr([0, 1], 16)
+    model = fe.EquivariantTransformer(rp, rp, rp, num_layers=2, num_heads=4, layer_scale_init=0.3, num_experts=4,
+                                      experts_per_node=2).to(dev)
+    g = gen(3)
+    xyz = torch.randn(120, 3, generator=g) * 3
+    d = torch.cdist(xyz, xyz) + torch.eye(120) * 1e9
+    src = d.topk(8, largest=False).indices.reshape(-1)
+    dst = torch.arange(120).repeat_interleave(8)
+    graph = fe.Graph(src.to(dev), dst.to(dev), 120)
+    x = torch.randn(120, 16, 4, generator=g)
+    axis, angle = fe.random_rotation()
+    D = fe.WignerD(rp).rot(axis, angle)
+    R = fe.WignerD(fe.Repr([1])).rot(axis, angle, cartesian=True)
+    y = model(xyz.to(dev), x.to(dev), graph)
+    y2 = model((xyz @ R.t()).to(dev), (x @ D.t()).to(dev), graph)
+    err = ((y2 - y @ D.t().to(dev)).abs().max() / y.abs().max()).item()
+    assert err < 1e-2, err           # the bar of the model's other equivariance tests
+    loss = y.pow(2).mean() + 0.01 * sum(layer.experts.balance for layer in model.layers)
+    loss.backward()
+    missing = [k for k, p in model.named_parameters() if p.grad is None]
+    assert not missing, missing
+    for layer in model.layers:
+        for p in (layer.experts.up.weight, layer.experts.down.weight, layer.experts.router.linear.weight):
+            assert torch.isfinite(p.grad).all() and p.grad.any()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_half_precision_block_and_mlp(dev, dtype):
+    torch.manual_seed(4)
+    rp = fe.Repr([0, 1], 16)
+    mlp = fe.EquivariantExpertMLP(rp, 4, 2).to(dev, dtype)
+    x = torch.randn(50, 16, 4, generator=gen(8)).to(dev, dtype).requires_grad_()
+    y = mlp(x)
+    (gx,) = torch.autograd.grad(y.sum() + mlp.balance, [x])
+    assert y.dtype == gx.dtype == dtype and torch.isfinite(y).all() and torch.isfinite(gx).all()
+    block = fe.EquivariantTransformerBlock(rp, rp, num_heads=2, num_experts=4).to(dev, dtype)
+    graph = fe.Graph.random(50, 300, device=dev)
+    vec = torch.randn(300, 3, generator=gen(9)).to(dev)
+    (P,) = fe.WignerDBasis([rp]).to(dev)(vec)
+    out = block(P.to(dtype), P.to(dtype), x, vec.norm(dim=-1).to(dtype), graph)
+    assert out.dtype == dtype and torch.isfinite(out).all()
+    with pytest.raises(TypeError, match="float64"):
+        fe.EquivariantExpertMLP(rp, 4, 2).to(dev).double()(x.double())
+
+
+def test_captured_training_step(dev):
+    """The whole mixture in a graph: replays on new inputs give the eager step's bits."""
+    from flash_eq.capture import capture_step
+    torch.manual_seed(6)
+    rp = fe.Repr([0, 1], 32)
+    mlp = fe.EquivariantExpertMLP(rp, 8, 2).to(dev)
+    x = torch.randn(5000, 32, 4, generator=gen(1)).to(dev).requires_grad_()      # 10000 slots: the plan's tiled form
+    gy = torch.randn(5000, 32, 4, generator=gen(2)).to(dev)
+    leaves = [x, *mlp.parameters()]
+
+    def step():
+        loss = (mlp(x) * gy).sum((1, 2)).mean() + mlp.balance
+        loss.backward()
+        return loss
+
+    graph, loss = capture_step(step, leaves)
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(5000, 32, 4, generator=gen(30 + k)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.grad.clone() for t in leaves]
+        y = (mlp(x) * gy).sum((1, 2)).mean() + mlp.balance
+        want = torch.autograd.grad(y, leaves)
+        for a, b in zip(got, want):
+            assert torch.allclose(a, b, rtol=1e-5, atol=1e-6 * b.abs().max().item())
+        torch.cuda.synchronize()
+
+
+def test_another_stream_and_the_same_bits(dev):
+    g = gen(9)
+    ids = some_ids(g, 900, 2, 8).to(dev)
+    x = torch.randn(9, 900, 64, generator=g).to(dev)
+    w = torch.randn(8, 3, 64, 64, generator=g).to(dev).requires_grad_()
+    probs = torch.rand(900, 2, generator=g).to(dev).requires_grad_()
+
+    def step():
+        plan = fe.ExpertPlan(ids, 8)
+        y = plan.combine(fe.expert_linear(plan.dispatch(x), w, plan, (0, 1, 2)), probs)
+        return (y.detach(), *torch.autograd.grad(y.square().sum(), [w, probs]))
+    first = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = step()
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b, c in zip(first, other, step()):
+        assert torch.equal(a, b) and torch.equal(a, c)
