@@ -3,14 +3,20 @@
 Every translation unit is compiled to an object under ``_build/`` (git-ignored)
 and linked into one shared library with a plain C ABI (``include/flasheq.h``).
 Packed-FP32 instructions are disabled for all device code.
+
+``_lib/flasheq_torch.so`` is the PyTorch module over that library
+(``csrc/torch_nodes.cpp``): host code only, compiled with g++ against the
+installed PyTorch's headers.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
 import glob
+import importlib.util
 import os
 import subprocess
 import sys
+import sysconfig
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG_DIR)                      # flash-eq_amd/
@@ -20,6 +26,7 @@ INCLUDE = os.path.join(REPO, "include")
 BUILD_DIR = os.path.join(ROOT, "_build")
 LIB_DIR = os.path.join(PKG_DIR, "_lib")
 LIB_PATH = os.path.join(LIB_DIR, "libflasheq.so")
+NODES_PATH = os.path.join(LIB_DIR, "flasheq_torch.so")
 ARCH = os.environ.get("FEQ_OFFLOAD_ARCH", "gfx950")
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -40,13 +47,40 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _compile_nodes() -> str:
+    torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]
+    obj = os.path.join(BUILD_DIR, "torch_nodes.o")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-fPIC", "-std=c++17", "-Wall", "-Wno-sign-compare",
+           "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f"-isystem{torch_dir}/include",
+           f"-isystem{torch_dir}/include/torch/csrc/api/include", "-isystem/opt/rocm/include",
+           f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}", "-c",
+           os.path.join(CSRC, "torch_nodes.cpp"), "-o", obj]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compiling torch_nodes.cpp failed:\n{res.stdout}\n{res.stderr}")
+    return obj
+
+
+def _link_nodes(obj: str) -> None:
+    torch_dir = importlib.util.find_spec("torch").submodule_search_locations[0]
+    tmp = NODES_PATH + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-shared", "-o", tmp, obj, f"-L{torch_dir}/lib", "-ltorch_python", "-ltorch",
+           "-ltorch_cpu", "-lc10", "-lc10_hip", f"-L{LIB_DIR}", "-l:libflasheq.so", "-Wl,-rpath,$ORIGIN"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"linking flasheq_torch.so failed:\n{res.stdout}\n{res.stderr}")
+    os.replace(tmp, NODES_PATH)
+
+
 def build(verbose: bool = False) -> str:
-    """Compile every HIP source and link the shared library; returns its path."""
+    """Compile every source and link the shared library and the PyTorch module; returns the library's path."""
     os.makedirs(BUILD_DIR, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
     with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
+        nodes = ex.submit(_compile_nodes)
         objs = list(ex.map(_compile, srcs))
+        nodes = nodes.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs,
            "-L/opt/rocm/lib", "-Wl,-rpath,/opt/rocm/lib"]
@@ -54,8 +88,9 @@ def build(verbose: bool = False) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB_PATH)
+    _link_nodes(nodes)
     if verbose:
-        print(f"built {LIB_PATH}", file=sys.stderr)
+        print(f"built {LIB_PATH} and {NODES_PATH}", file=sys.stderr)
     return LIB_PATH
 
 

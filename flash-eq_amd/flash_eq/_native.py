@@ -9,18 +9,19 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import importlib.util
 import os
 from typing import Optional, Sequence
 
 import torch
 
-from ._build import LIB_PATH
+from ._build import LIB_PATH, NODES_PATH
 
 FEQ_MAX_BLOCKS = 17
 FEQ_MAX_SLOTS = 128
 FEQ_EW_HALF_ACCURACY = 1          # flags of feq_edgewise_*_ex
 POOL_MAX_HEADS = 16               # heads of feq_edgewise_*_src_pool
-DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}    # feq_dtype
+KERNEL_DTYPES = (torch.float32, torch.float16, torch.bfloat16)     # feq_dtype
 
 
 class CUDANotAvailableError(RuntimeError):
@@ -243,6 +244,27 @@ def lib() -> ctypes.CDLL:
             "torch.cuda.is_available() is False.")
     _gpu_seen = True
     return load_library()
+
+
+_nodes = None
+
+
+def nodes():
+    """The PyTorch module over the library (``csrc/torch_nodes.cpp``), loaded on first use.  It
+    checks its arguments itself (a tensor off the GPU raises ``CUDANotAvailableError``)."""
+    global _nodes
+    if _nodes is None:
+        load_library()
+        if not os.path.exists(NODES_PATH):
+            raise ImportError(
+                f"flash-eq PyTorch module not found at {NODES_PATH}.\n"
+                "Build it with: python -c 'import __graft_entry__ as g; g.build()' "
+                "(or python flash-eq_amd/flash_eq/_build.py)")
+        spec = importlib.util.spec_from_file_location("flasheq_torch", NODES_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _nodes = module
+    return _nodes
 
 
 def check(rc: int, what: str) -> None:

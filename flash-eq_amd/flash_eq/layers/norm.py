@@ -16,6 +16,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from .. import _native as N
 from .. import ops
 from ..representations import Repr
 from ..utils import get_epsilon
@@ -253,7 +254,7 @@ class InvariantLayerNorm(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.shape[-1:] != (self.width,):
             raise ValueError(f"features must be (..., {self.width}), got {tuple(x.shape)}")
-        if x.is_cuda and x.dtype in ops.N.DTYPES:
+        if x.is_cuda and x.dtype in N.KERNEL_DTYPES:
             return ops.layer_norm(x, self.weight, self.bias, self.epsilon)
         return nn.functional.layer_norm(x, (self.width,), self.weight, self.bias, self.epsilon)
 

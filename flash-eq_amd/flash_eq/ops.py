@@ -14,7 +14,6 @@ from functools import lru_cache
 from typing import Optional, Sequence, Tuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as N
 
@@ -1561,96 +1560,10 @@ class SumSquaresFn(torch.autograd.Function):
 
 # ---- layer norm over the last axis (csrc/layernorm.hip) ------------------------------
 
-def element_type(t: torch.Tensor, name: str) -> int:
-    """The feq_dtype of a GPU tensor for the entry points that take several."""
-    N.require_cuda_tensor(t, name)
-    code = N.DTYPES.get(t.dtype)
-    if code is None:
-        raise TypeError(f"{name}: dtype {t.dtype} is not supported (float32, float16 or bfloat16)")
-    return code
-
-
-def _strided_rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """(t or a contiguous copy, the distance of its rows): two-dimensional tables whose
-    rows lie apart (a slice of a wider table) are read where they are."""
-    t = t.detach()
-    if t.is_contiguous():
-        return t, t.shape[-1]
-    if t.dim() == 2 and t.stride(1) == 1 and t.stride(0) >= t.shape[1]:
-        return t, t.stride(0)
-    return t.contiguous(), t.shape[-1]
-
-
-class LayerNormFn(torch.autograd.Function):
-    """y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis
-    (``feq_layernorm_fwd`` / ``_bwd``): float32 statistics and sums, the result in x's type,
-    the parameters' gradients in theirs."""
-
-    @staticmethod
-    def run(x, weight, bias, eps: float, stats: bool):
-        code = element_type(x, "x")
-        width = x.shape[-1]
-        xs, ld = _strided_rows(x)
-        rows = xs.numel() // width
-        dev = x.device
-        y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=dev) if stats else (None, None)
-        w, b = _c(weight), _c(bias)
-        p = w if w is not None else b
-        with N.on_device(dev):
-            rc = N.lib().feq_layernorm_fwd(N.ptr(xs), rows, width, ld, code, N.ptr(w), N.ptr(b),
-                                           N.DTYPES[p.dtype] if p is not None else 0, eps, N.ptr(y), N.ptr(mean),
-                                           N.ptr(rstd), N.stream_ptr(dev))
-        N.check(rc, "feq_layernorm_fwd")
-        return y, xs, w, mean, rstd
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps: float):
-        y, xs, w, mean, rstd = LayerNormFn.run(x, weight, bias, eps, True)
-        ctx.save_for_backward(xs, w, mean, rstd)
-        p = weight if weight is not None else bias
-        ctx.pdtype = p.dtype if p is not None else None
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        xs, w, mean, rstd = ctx.saved_tensors
-        need_x, need_w, need_b, _ = ctx.needs_input_grad
-        dev = xs.device
-        width = xs.shape[-1]
-        rows = xs.numel() // width
-        ldx = xs.stride(0) if xs.dim() == 2 and not xs.is_contiguous() else width
-        g, ldg = _strided_rows(gy)
-        gx = torch.empty(xs.shape, dtype=xs.dtype, device=dev) if need_x else None
-        gw = torch.empty(width, dtype=ctx.pdtype, device=dev) if need_w else None
-        gb = torch.empty(width, dtype=ctx.pdtype, device=dev) if need_b else None
-        lib = N.lib()
-        ws = N.workspace(lib.feq_layernorm_bwd_workspace(rows, width), dev) if need_w or need_b else None
-        with N.on_device(dev):
-            rc = lib.feq_layernorm_bwd(N.ptr(g), ldg, N.ptr(xs), rows, width, ldx, N.DTYPES[xs.dtype], N.ptr(w),
-                                       N.DTYPES[ctx.pdtype] if ctx.pdtype is not None else 0, N.ptr(mean), N.ptr(rstd),
-                                       N.ptr(gx), N.ptr(gw), N.ptr(gb), N.ptr(ws), ws.numel() if ws is not None else 0,
-                                       N.stream_ptr(dev))
-        N.check(rc, "feq_layernorm_bwd")
-        return gx, gw, gb, None
-
-
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                epsilon: float = 1e-5) -> torch.Tensor:
-    """Layer norm of GPU rows over their last axis, float32, float16 or bfloat16; weight and
-    bias (width,) of that type or another of the three (both of one type), or None."""
-    element_type(x, "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"x must have a last axis to normalise, got shape {tuple(x.shape)}")
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is not None:
-            element_type(t, name)
-            if t.shape != x.shape[-1:]:
-                raise ValueError(f"{name} must have shape ({x.shape[-1]},), got {tuple(t.shape)}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"weight and bias of different dtypes: {weight.dtype} and {bias.dtype}")
-    _same_device(x, weight, bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
-        return LayerNormFn.apply(x, weight, bias, epsilon)
-    return LayerNormFn.run(x, weight, bias, epsilon, False)[0]
+    """(x - mean) / sqrt(var + epsilon) * weight + bias over the last axis of GPU rows, float32, float16
+    or bfloat16 with float32 statistics and sums (``feq_layernorm_fwd`` / ``_bwd``); weight and bias
+    (width,) of that type or another of the three (both of one type), or None.  The rows of a
+    two-dimensional slice of a wider table are read in place."""
+    return N.nodes().layer_norm(x, weight, bias, epsilon)
