@@ -30,6 +30,7 @@ constexpr int kXlMaxReps = FEQ_MAX_IRREPS;
 constexpr int kXlMaxExperts = 1024;
 constexpr int kXlThreads = 256;
 constexpr int kXlBM = 128;          // rows of a block
+constexpr int kXlStreamK = 128;     // reduction columns of the streaming kernel
 constexpr int kXlRowBytes = 128;    // bytes of the reduction staged per row (32 floats, 64 16-bit elements)
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
@@ -58,9 +59,18 @@ struct Mma<float> {
         for (int j = 0; j < 4; ++j) c = mfma4(a[j], b[j], c);
         return c;
     }
-    // element j: row k0 + 4 g + j of a table with `stride` elements a row, column q0 + step (c / 4) + c % 4
-    static __device__ __forceinline__ frag columns(const float* t, int stride, int k0, int g, int c, int q0, int step) {
-        const float* p = t + (k0 + 4 * g) * stride + q0 + step * (c >> 2) + (c & 3);
+    // tile by tile within a step, so that no product waits for the one before
+    template <int NT>
+    static __device__ __forceinline__ void mul_all(const frag (&a)[NT], frag b, v4f (&acc)[NT]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) acc[i] = mfma4(a[i][j], b[j], acc[i]);
+    }
+    static constexpr int PAD = 4;      // four rows are 16 banks apart
+    // element j: row k0 + 4 g + j, column c0 + c of a table with `stride` elements a row
+    static __device__ __forceinline__ frag columns(const float* t, int stride, int k0, int g, int c, int c0) {
+        const float* p = t + (k0 + 4 * g) * stride + c0 + c;
         return frag{p[0], p[stride], p[2 * stride], p[3 * stride]};
     }
 };
@@ -69,9 +79,10 @@ struct Mma<float> {
 template <class T, class F>
 struct MmaHalf {
     static constexpr int KS = 32, FE = 8;
+    static constexpr int PAD = 16;     // a row is 8 banks on from the one before
     typedef F frag;
-    static __device__ __forceinline__ frag columns(const T* t, int stride, int k0, int g, int c, int q0, int step) {
-        const T* p = t + (k0 + 8 * g + (c >> 2)) * stride + q0 + step * (c & 3);
+    static __device__ __forceinline__ frag columns(const T* t, int stride, int k0, int g, int c, int c0) {
+        const T* p = t + (k0 + 8 * g + (c >> 2)) * stride + c0 + 4 * (c & 3);
         const v4s x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
         const v4s y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 4 * stride));
         const v8s v = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
@@ -81,10 +92,20 @@ struct MmaHalf {
 template <>
 struct Mma<_Float16> : MmaHalf<_Float16, h8> {
     static __device__ __forceinline__ v4f mul(h8 a, h8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    template <int NT>
+    static __device__ __forceinline__ void mul_all(const frag (&a)[NT], frag b, v4f (&acc)[NT]) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i] = mul(a[i], b, acc[i]);
+    }
 };
 template <>
 struct Mma<__bf16> : MmaHalf<__bf16, b8> {
     static __device__ __forceinline__ v4f mul(b8 a, b8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    template <int NT>
+    static __device__ __forceinline__ void mul_all(const frag (&a)[NT], frag b, v4f (&acc)[NT]) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i] = mul(a[i], b, acc[i]);
+    }
 };
 
 // 16 bytes of T at p, of which the first `n` elements exist (n <= 0: none); the others are 0.
@@ -101,6 +122,49 @@ __device__ __forceinline__ uint4 load16(const T* p, int n) {
     }
 }
 
+// A lane's accumulators are four consecutive columns of a tile: 16 bytes of float32, half of that of a 16-bit type,
+// whose columns are therefore dealt to pairs of tiles: element m of tile i of a pair is column 8 (m / 4) + 4 i +
+// m % 4 of the pair's 32, so the two tiles make one 16-byte store, four lanes' stores 64 bytes of a row (dealt to
+// groups of four, a store instruction touches memory in 16-byte pieces: 116 against 107 us for 40000 x 9 float32
+// rows, 64 to 128 columns).  LDS holds columns (or the rows of a K-contiguous table) in the dealt order, 16 i + m, so the 16 lanes
+// of a read touch neighbours and no bank twice.  Four columns whose first is a multiple of four stay together.
+template <class T>
+constexpr int kDealt = sizeof(T) == 4 ? 1 : 2;     // tiles of a group
+template <class T>
+__device__ __forceinline__ int dealt(int n) {
+    if constexpr (sizeof(T) == 4) return n;
+    const int w = n & 31;
+    return (n - w) + 16 * (w >> 2 & 1) + 4 * (w >> 3) + (w & 3);
+}
+
+// 16 bytes of consecutive columns from `n` (a multiple of V) at their dealt places in the row at `row`.
+template <class T>
+__device__ __forceinline__ void put_dealt(T* row, int n, uint4 v) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<uint4*>(row + n) = v;
+    } else {
+        *reinterpret_cast<uint2*>(row + dealt<T>(n)) = uint2{v.x, v.y};
+        *reinterpret_cast<uint2*>(row + dealt<T>(n + 4)) = uint2{v.z, v.w};
+    }
+}
+
+// A lane's V columns of a tile group (accumulators of tile u at acc[u STEP]) to o, of which `n` exist.
+template <class T, bool VEC, int STEP>
+__device__ __forceinline__ void store_tiles(T* o, int n, const v4f* acc) {
+    constexpr int V = 16 / sizeof(T);
+    if constexpr (VEC) {
+        if (n <= 0) return;
+        float f[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) f[v] = acc[v / 4 * STEP][v % 4];
+        store_f<T, V>(o, f);
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (v < n) o[v] = static_cast<T>(acc[v / 4 * STEP][v % 4]);
+    }
+}
+
 struct XlTile {
     int expert;      // X: rows without an expert; -1: no such block
     int row0, row1;  // the block's first row, the end of the expert's rows
@@ -110,7 +174,8 @@ struct XlTile {
 };
 
 // Block `want` of the row blocks (of `bm` rows) of the experts in order, the rows behind them last.  Called
-// by whole waves; the result is the same in every lane.
+// by whole waves; the result is the same in every lane.  EMPTY: an expert without rows has one block.
+template <bool EMPTY = false>
 __device__ __forceinline__ XlTile find_tile(const int32_t* __restrict__ offsets, int X, int S, int bm, int want) {
     const int lane = threadIdx.x & 63;
     int carry = 0, many = 0;
@@ -121,7 +186,8 @@ __device__ __forceinline__ XlTile find_tile(const int32_t* __restrict__ offsets,
             a = offsets[e];
             z = e < X ? offsets[e + 1] : S;
         }
-        const int n = (z - a + bm - 1) / bm;
+        int n = (z - a + bm - 1) / bm;
+        if (EMPTY && n == 0 && e < X) n = 1;
         int incl = n, multi = (e < X && n > 1) ? n : 0, mincl = multi;
         for (int o = 1; o < 64; o <<= 1) {
             const int u = __shfl_up(incl, o, 64), w = __shfl_up(mincl, o, 64);
@@ -163,7 +229,7 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
     constexpr int V = 16 / sizeof(T), BK = kXlRowBytes / sizeof(T), CH = BK / V;   // 8 vectors of a staged row
     constexpr int BN = 64 * WR, WC = 4 / WR, PT = kXlBM / (16 * WC);
     constexpr int LD = BK + V;                       // stride of a K-contiguous row: 144 bytes
-    constexpr int LDT = BN + V;                      // stride of a W row staged as it lies (TRANS)
+    constexpr int LDT = BN + M::PAD;                 // stride of a W row staged as it lies (TRANS)
     constexpr int NIN = kXlBM * CH / kXlThreads;     // vectors a thread stages
     constexpr int NW = BN * CH / kXlThreads;
     __shared__ __align__(16) T sIn[kXlBM * LD];
@@ -211,8 +277,8 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             const int q = tid + kXlThreads * i;
-            if constexpr (TRANS) *reinterpret_cast<uint4*>(sW + (q / (BN / V)) * LDT + (q % (BN / V)) * V) = vw[i];
-            else *reinterpret_cast<uint4*>(sW + (q / CH) * LD + (q % CH) * V) = vw[i];
+            if constexpr (TRANS) put_dealt<T>(sW + (q / (BN / V)) * LDT, (q % (BN / V)) * V, vw[i]);
+            else *reinterpret_cast<uint4*>(sW + dealt<T>(q / CH) * LD + (q % CH) * V) = vw[i];
         }
     };
 
@@ -233,14 +299,9 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
                 typename M::frag a[4], b[PT];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    // row m = c of tile i is column 16 (m / 4) + 4 i + m % 4 of the wave's 64
-                    const int q0 = 64 * wr + 4 * i;
-                    if constexpr (TRANS) {
-                        a[i] = M::columns(sW, LDT, ks, g, c, q0, 16);
-                    } else {
-                        a[i] = *reinterpret_cast<const typename M::frag*>(sW + (q0 + 16 * (c >> 2) + (c & 3)) * LD + ks +
-                                                                          M::FE * g);
-                    }
+                    const int q0 = 64 * wr + 16 * i;
+                    if constexpr (TRANS) a[i] = M::columns(sW, LDT, ks, g, c, q0);
+                    else a[i] = *reinterpret_cast<const typename M::frag*>(sW + (q0 + c) * LD + ks + M::FE * g);
                 }
 #pragma unroll
                 for (int j = 0; j < PT; ++j)
@@ -252,43 +313,148 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
             }
         }
     }
-    // lane (c, g): row c of row tile j, columns 16 g + 4 i + r of the wave's 64
-    const int nw = n0 + 64 * wr + 16 * g;
-    float bv[16];
-#pragma unroll
-    for (int u = 0; u < 16; ++u) bv[u] = 0.0f;
+    // lane (c, g): row c of row tile j, columns 16 i + V g + 0 .. V - 1 of the wave's 64 for tile group i
+    const int nw = n0 + 64 * wr + V * g;
     const int bc = map.bcol[d];
-    if (!TRANS && bias && bc >= 0 && !none) {
+    const bool biased = !TRANS && bias && bc >= 0 && !none;
 #pragma unroll
-        for (int u = 0; u < 16; ++u)
-            if (nw + u < N) bv[u] = static_cast<float>(bias[(static_cast<int64_t>(t.expert) * N + nw + u) * nbias + bc]);
+    for (int i = 0; i < 4; i += kDealt<T>) {
+        const int n = nw + 16 * i;
+        if (biased) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float bv = n + v < N ? static_cast<float>(bias[(static_cast<int64_t>(t.expert) * N + n + v) * nbias + bc]) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < PT; ++j) acc[i + v / 4][j][v % 4] += bv;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < PT; ++j) {
+            const int r = 16 * (wc * PT + j) + c;
+            if (r < rows) store_tiles<T, VEC, PT>(od + static_cast<int64_t>(r) * N + n, N - n, &acc[i][j]);
+        }
     }
+}
+
+// 16-row blocks of the experts' rows and of the rows behind them, in one plane.  Called by whole waves.
+__device__ __forceinline__ int count_blocks(const int32_t* __restrict__ offsets, int X, int S) {
+    int n = 0;
+    for (int e = threadIdx.x & 63; e <= X; e += 64) n += ((e < X ? offsets[e + 1] : S) - offsets[e] + 15) / 16;
+    for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o, 64);
+    return n;
+}
+
+// The same product for a reduction of at most 128 columns: a block of the weight stays in LDS, the rows stream.  The
+// 16-row blocks of all planes (and, for wide outputs, of their groups of NB columns) lie in one line; every
+// workgroup takes an equal run of it, as many workgroups as fit the chip at once, and stages the weight again
+// where its run comes to another expert or plane.  Its waves take the run's blocks in turn, straight from memory
+// in the matrix cores' layout (lane (c, g): FE elements of row c), the next block's rows in flight during this
+// one's products.  Nothing but the weight passes through LDS and no barrier stands between blocks of an
+// expert.  NS: reduction steps held (K <= NS KS).
+template <class T, bool VEC, bool TRANS, int NB, int NS>
+__global__ void __launch_bounds__(kXlThreads)
+k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,
+            int N, int nreps, XlMap map, int dim, const T* __restrict__ bias, int nbias, T* __restrict__ out) {
+    using M = Mma<T>;
+    typedef typename M::frag frag;
+    constexpr int V = 16 / sizeof(T), KM = NS * M::KS;
+    constexpr int NT = NB / 16;
+    constexpr int LD = KM + V, LDT = NB + M::PAD;
+    __shared__ __align__(16) T sW[TRANS ? KM * LDT : NB * LD];
+    __shared__ __align__(16) float sBias[NB];
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int nb = (N + NB - 1) / NB;
+    const int per_plane = __builtin_amdgcn_readfirstlane(count_blocks(offsets, X, S));
+    const int64_t total = static_cast<int64_t>(per_plane) * dim * nb;
+    const int64_t share = total / gridDim.x, more = total % gridDim.x;
+    int64_t at = blockIdx.x * share + (blockIdx.x < more ? blockIdx.x : more);
+    const int64_t end = at + share + (blockIdx.x < more ? 1 : 0);
+    while (at < end) {
+        const int line = static_cast<int>(at / per_plane), d = line / nb, n0 = line % nb * NB;
+        const XlTile t = find_tile(offsets, X, S, 16, static_cast<int>(at % per_plane));
+        const int expert = __builtin_amdgcn_readfirstlane(t.expert), row0 = __builtin_amdgcn_readfirstlane(t.row0);
+        const int rows = __builtin_amdgcn_readfirstlane(t.row1) - row0;
+        const int left = __builtin_amdgcn_readfirstlane(t.count - t.index);
+        const int nblocks = static_cast<int>(end - at < left ? end - at : left);
+        at += nblocks;
+        const T* id = in + (static_cast<int64_t>(d) * S + row0) * K;
+        T* od = out + (static_cast<int64_t>(d) * S + row0) * N + n0;
+
+        auto load = [&](int blk, frag (&b)[NS]) {
+            const int r = 16 * blk + c;
+            const T* p = id + static_cast<int64_t>(r < rows ? r : rows - 1) * K + M::FE * g;
 #pragma unroll
-    for (int j = 0; j < PT; ++j) {
-        const int r = 16 * (wc * PT + j) + c;
-        if (r >= rows) continue;
-        T* orow = od + static_cast<int64_t>(r) * N + nw;
-        if constexpr (VEC) {
+            for (int ks = 0; ks < NS; ++ks)
+                b[ks] = __builtin_bit_cast(frag, load16<T, VEC>(p + ks * M::KS, K - ks * M::KS - M::FE * g));
+        };
+        auto store = [&](int blk, const v4f (&acc)[NT]) {
+            const int r = 16 * blk + c;
+            if (r >= rows) return;
+            T* o = od + static_cast<int64_t>(r) * N;
 #pragma unroll
-            for (int u = 0; u < 16; u += V)
-                if (nw + u < N) {
-                    float o[V];
+            for (int i = 0; i < NT; i += kDealt<T>) {
+                const int n = 16 * i + V * g;
+                store_tiles<T, VEC, 1>(o + n, N - n0 - n, &acc[i]);
+            }
+        };
+        if (expert == X) {                           // rows without an expert
+            v4f zero[NT];
 #pragma unroll
-                    for (int v = 0; v < V; ++v) o[v] = acc[(u + v) / 4][j][(u + v) % 4] + bv[u + v];
-                    store_f<T, V>(orow + u, o);
-                }
+            for (int i = 0; i < NT; ++i) zero[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int blk = wave; blk < nblocks; blk += 4) store(blk, zero);
+            continue;
+        }
+        frag b0[NS], b1[NS];
+        if (wave < nblocks) load(wave, b0);
+        __syncthreads();                             // the last expert's weight has been read
+        const T* we = W + (static_cast<int64_t>(expert) * nreps + map.rep[d]) * K * N;
+        if constexpr (TRANS) {
+            for (int q = tid; q < KM * (NB / V); q += kXlThreads) {
+                const int k = q / (NB / V), n = (q % (NB / V)) * V;
+                put_dealt<T>(sW + k * LDT, n, load16<T, VEC>(we + static_cast<int64_t>(k) * N + n0 + n, k < K ? N - n0 - n : 0));
+            }
         } else {
+            for (int q = tid; q < NB * (KM / V); q += kXlThreads) {
+                const int n = q / (KM / V), k = (q % (KM / V)) * V;
+                *reinterpret_cast<uint4*>(sW + dealt<T>(n) * LD + k) =
+                    load16<T, VEC>(we + static_cast<int64_t>(n0 + n) * K + k, n0 + n < N ? K - k : 0);
+            }
+        }
+        const int bc = map.bcol[d];
+        if (tid < NB)
+            sBias[tid] = (!TRANS && bias && bc >= 0 && n0 + tid < N)
+                             ? static_cast<float>(bias[(static_cast<int64_t>(expert) * N + n0 + tid) * nbias + bc]) : 0.0f;
+        __syncthreads();
+        for (int blk = wave; blk < nblocks; blk += 4) {
+            load(blk + 4 < nblocks ? blk + 4 : blk, b1);
+            // the weight is read from LDS for every block: kept in registers it would take them from the rows in flight
+            asm volatile("" ::: "memory");
+            v4f acc[NT];
 #pragma unroll
-            for (int u = 0; u < 16; ++u)
-                if (nw + u < N) orow[u] = static_cast<T>(acc[u / 4][j][u % 4] + bv[u]);
+            for (int i = 0; i < NT; ++i)
+                acc[i] = *reinterpret_cast<const v4f*>(sBias + 16 * (i - i % kDealt<T>) + V * g + 4 * (i % kDealt<T>));
+#pragma unroll
+            for (int ks = 0; ks < NS; ++ks) {
+                frag a[NT];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    if constexpr (TRANS) a[i] = M::columns(sW, LDT, ks * M::KS, g, c, 16 * i);
+                    else a[i] = *reinterpret_cast<const frag*>(sW + (16 * i + c) * LD + ks * M::KS + M::FE * g);
+                }
+                M::template mul_all<NT>(a, b0[ks], acc);
+            }
+            store(blk, acc);
+#pragma unroll
+            for (int ks = 0; ks < NS; ++ks) b0[ks] = b1[ks];
         }
     }
 }
 
 // grad_W and grad_b over row chunks of rc rows.  A workgroup takes a chunk of one expert, one irrep r (all its
 // planes), 64 WR columns k of x and 128 columns n of grad_y (tiles of k first).  An expert of one chunk gets its
-// gradient written, one of several a float32 partial per chunk: pw[(r nslots + slot) N K + n K + k],
-// pb[(j nslots + slot) N + n], summed by k_xl_wsum.
+// gradient written (zeros without rows), one of several a float32 partial per chunk:
+// pw[(r nslots + slot) N K + n K + k], pb[(j nslots + slot) N + n], summed by k_xl_wsum.
 template <class T, bool VEC, int WR>
 __global__ void __launch_bounds__(kXlThreads)
 k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __restrict__ offsets, int X, int S,
@@ -297,14 +463,14 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
     using M = Mma<T>;
     constexpr int V = 16 / sizeof(T), BP = kXlRowBytes / sizeof(T);   // rows staged at a time
     constexpr int BK = 64 * WR, BN = 128, WC = 4 / WR, NT = BN / (16 * WC);
-    constexpr int LX = BK + V, LG = BN + V;
+    constexpr int LX = BK + M::PAD, LG = BN + M::PAD;
     constexpr int NX = BP * (BK / V) / kXlThreads, NG = BP * (BN / V) / kXlThreads;
     __shared__ __align__(16) T sX[BP * LX];
     __shared__ __align__(16) T sG[BP * LG];
     const int nk = (ci + BK - 1) / BK, nn = (co + BN - 1) / BN;
     const int tile = blockIdx.x / (nk * nn), sub = blockIdx.x % (nk * nn);
     const int rep = nreps - 1 - static_cast<int>(blockIdx.y);      // the irreps of most planes first
-    const XlTile t = find_tile(offsets, X, S, rc, tile);
+    const XlTile t = find_tile<true>(offsets, X, S, rc, tile);
     if (t.expert < 0 || t.expert == X) return;
     const int k0 = (sub % nk) * BK, n0 = (sub / nk) * BN;
     const int rend = t.row1 - t.row0 < rc ? t.row1 : t.row0 + rc;
@@ -337,13 +503,13 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     float bsum = 0.0f;                                             // thread n < 128: column n0 + n
-    load(0);
+    if (total) load(0);
     for (int it = 0; it < total; ++it) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
             const int q = tid + kXlThreads * i;
-            *reinterpret_cast<uint4*>(sX + (q / (BK / V)) * LX + (q % (BK / V)) * V) = vx[i];
+            put_dealt<T>(sX + (q / (BK / V)) * LX, (q % (BK / V)) * V, vx[i]);
         }
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
@@ -356,12 +522,9 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
         for (int ks = 0; ks < BP; ks += M::KS) {
             typename M::frag a[4], b[NT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int q0 = 64 * wr + 4 * i;                    // as in k_xl_mm: 16 consecutive k a lane
-                a[i] = M::columns(sX, LX, ks, g, c, q0, 16);
-            }
+            for (int i = 0; i < 4; ++i) a[i] = M::columns(sX, LX, ks, g, c, 64 * wr + 16 * i);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) b[j] = M::columns(sG, LG, ks, g, c, 16 * (wc * NT + j), 4);
+            for (int j = 0; j < NT; ++j) b[j] = M::columns(sG, LG, ks, g, c, 16 * (wc * NT + j));
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -372,38 +535,22 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
     }
     const bool direct = t.count == 1;
     const int slot = t.before + t.index;
-    const int kw = k0 + 64 * wr + 16 * g;
+    const int kw = k0 + 64 * wr + V * g;
     const int64_t base = direct ? (static_cast<int64_t>(t.expert) * nreps + rep) * co
                                 : (static_cast<int64_t>(rep) * nslots + slot) * co;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const int n = n0 + 16 * (wc * NT + j) + c;
         if (n >= co) continue;
-        if (direct) {
-            T* o = gw + (base + n) * ci + kw;
 #pragma unroll
-            for (int u = 0; u < 16; u += VEC ? V : 1) {
-                if (kw + u >= ci) continue;
-                if constexpr (VEC) {
-                    float f[V];
+        for (int i = 0; i < 4; i += kDealt<T>) {
+            const int k = kw + 16 * i;
+            if (direct) {
+                store_tiles<T, VEC, NT>(gw + (base + n) * ci + k, ci - k, &acc[i][j]);
+            } else {
+                float* o = pw + (base + n) * ci + k;
 #pragma unroll
-                    for (int v = 0; v < V; ++v) f[v] = acc[(u + v) / 4][j][(u + v) % 4];
-                    store_f<T, V>(o + u, f);
-                } else {
-                    o[u] = static_cast<T>(acc[u / 4][j][u % 4]);
-                }
-            }
-        } else {
-            float* o = pw + (base + n) * ci + kw;
-#pragma unroll
-            for (int u = 0; u < 16; u += 4) {
-                if constexpr (VEC) {
-                    if (kw + u < ci) *reinterpret_cast<v4f*>(o + u) = acc[u / 4][j];
-                } else {
-#pragma unroll
-                    for (int v = 0; v < 4; ++v)
-                        if (kw + u + v < ci) o[u + v] = acc[u / 4][j][v];
-                }
+                for (int u = 0; u < kDealt<T>; ++u) store_tiles<float, VEC, 1>(o + 4 * u, ci - k - 4 * u, &acc[i + u][j]);
             }
         }
     }
@@ -413,40 +560,58 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
     }
 }
 
-// The experts' chunk counts and first partials as find_tile numbers them.  Lane-uniform.
-__device__ __forceinline__ void expert_chunks(const int32_t* __restrict__ offsets, int X, int rc, int e, int& first, int& count) {
-    const int lane = threadIdx.x & 63;
-    int s = 0;
-    for (int i = lane; i < e; i += 64) {
-        const int n = (offsets[i + 1] - offsets[i] + rc - 1) / rc;
-        s += n > 1 ? n : 0;
-    }
-    for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
-    first = s;
-    count = (offsets[e + 1] - offsets[e] + rc - 1) / rc;
-}
-
-// Experts of several chunks: the partials in order; of none: zeros.  blockIdx.y: expert, blockIdx.z: irrep, and
-// behind the irreps the bias columns.
-template <class T>
+// The gradients of the experts of several chunks: their partials in order.  blockIdx.y: the expert's number among
+// these, blockIdx.z: the irrep, and behind the irreps the bias columns.
+template <class T, int V>
 __global__ void __launch_bounds__(256)
 k_xl_wsum(const float* __restrict__ pw, const float* __restrict__ pb, const int32_t* __restrict__ offsets, int X, int rc,
           int64_t wsize, int co, int nreps, int nslots, T* __restrict__ gw, T* __restrict__ gb, int nbias) {
-    const int e = blockIdx.y, z = blockIdx.z;
-    int first, count;
-    expert_chunks(offsets, X, rc, e, first, count);
-    if (count == 1) return;
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int z = blockIdx.z, lane = threadIdx.x & 63, want = blockIdx.y;
+    int expert = -1, first = 0, count = 0, carry = 0, slots = 0;
+    for (int e0 = 0; e0 < X; e0 += 64) {
+        const int e = e0 + lane;
+        const int n = e < X ? (offsets[e + 1] - offsets[e] + rc - 1) / rc : 0;
+        const int m = n > 1 ? n : 0;
+        const uint64_t many = __ballot(n > 1);
+        int incl = m;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(incl, o, 64);
+            if (lane >= o) incl += u;
+        }
+        const uint64_t hit = __ballot(n > 1 && carry + static_cast<int>(__popcll(many & ((1ull << lane) - 1ull))) == want);
+        if (hit) {
+            const int f = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            expert = e0 + f;
+            first = slots + __shfl(incl - m, f, 64);
+            count = __shfl(n, f, 64);
+            break;
+        }
+        carry += static_cast<int>(__popcll(many));
+        slots += __shfl(incl, 63, 64);
+    }
+    if (expert < 0) return;
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * V;
     const bool w = z < nreps;
     const int64_t size = w ? wsize : co;
     if (i >= size) return;
     const float* p = (w ? pw + (static_cast<int64_t>(z) * nslots + first) * wsize
                         : pb + (static_cast<int64_t>(z - nreps) * nslots + first) * co) + i;
-    float a = 0.0f;
+    float a[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) a[v] = 0.0f;
 #pragma unroll 8
-    for (int q = 0; q < count; ++q) a += p[q * size];
-    if (w) gw[(static_cast<int64_t>(e) * nreps + z) * wsize + i] = static_cast<T>(a);
-    else gb[(static_cast<int64_t>(e) * co + i) * nbias + (z - nreps)] = static_cast<T>(a);
+    for (int q = 0; q < count; ++q) {
+        float f[V];
+        load_f<float, V>(p + q * size, f);
+#pragma unroll
+        for (int v = 0; v < V; ++v) a[v] += f[v];
+    }
+    if (w) {
+        store_f<T, V>(gw + (static_cast<int64_t>(expert) * nreps + z) * wsize + i, a);
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) gb[(static_cast<int64_t>(expert) * co + i + v) * nbias + (z - nreps)] = static_cast<T>(a[v]);
+    }
 }
 
 int xl_check(const int32_t* lvals, int32_t nreps, int32_t X, int64_t S, int32_t ci, int32_t co, int32_t dtype,
@@ -492,11 +657,40 @@ bool xl_vec(int ci, int co, std::initializer_list<const void*> ptrs) {
     return true;
 }
 
+// Workgroups of a kernel that the chip holds at once (256 CUs).
+int resident_blocks(const void* kern, int threads) {
+    int n = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != hipSuccess || n < 1) n = 2;
+    return 256 * n;
+}
+
 template <class T, bool TRANS>
 int mm_run(const void* in, const void* W, const int32_t* offsets, int X, int64_t S, int ci, int co, int nreps,
            const XlMap& map, const void* bias, int nbias, void* out, hipStream_t s) {
     const int K = TRANS ? co : ci, N = TRANS ? ci : co;
     const bool vec = xl_vec<T>(ci, co, {in, W, out});
+    if (K <= kXlStreamK) {
+        const int dim = map.first[nreps];
+        auto go = [&](auto v, auto nn, auto ns) -> int {
+            constexpr int NB = decltype(nn)::value;
+            auto kern = k_xl_stream<T, decltype(v)::value, TRANS, NB, decltype(ns)::value>;
+            // as many workgroups as run at once
+            static const int resident = resident_blocks(reinterpret_cast<const void*>(kern), kXlThreads);
+            const int64_t blocks = std::min<int64_t>(resident, tile_bound(S, X, 16) * dim * ceil_div(N, NB));
+            FEQ_LAUNCH(TRANS ? "k_xl_stream_t" : "k_xl_stream", kern, dim3(blocks), dim3(kXlThreads), 0, s,
+                       static_cast<const T*>(in), static_cast<const T*>(W), offsets, X, static_cast<int>(S), K, N, nreps, map,
+                       dim, static_cast<const T*>(bias), nbias, static_cast<T*>(out));
+            return FEQ_OK;
+        };
+        constexpr int H = 64 / Mma<T>::KS;           // steps of 64 columns
+        auto with_ns = [&](auto v, auto nn) -> int {
+            return K <= 64 ? go(v, nn, std::integral_constant<int, H>{}) : go(v, nn, std::integral_constant<int, 2 * H>{});
+        };
+        if (!vec) return with_ns(std::false_type{}, std::integral_constant<int, 128>{});
+        if (N <= 32) return with_ns(std::true_type{}, std::integral_constant<int, 32>{});
+        if (N <= 64) return with_ns(std::true_type{}, std::integral_constant<int, 64>{});
+        return with_ns(std::true_type{}, std::integral_constant<int, 128>{});
+    }
     auto run = [&](auto v, auto wr) -> int {
         constexpr int WR = decltype(wr)::value;
         const int64_t blocks = tile_bound(S, X, kXlBM) * ceil_div(N, 64 * WR);
@@ -513,11 +707,14 @@ int mm_run(const void* in, const void* W, const int32_t* offsets, int X, int64_t
     return vec ? with_wr(std::true_type{}) : with_wr(std::false_type{});
 }
 
-// Rows of a weight-gradient chunk: about 1024 workgroups where the rows allow it.
+// Rows of a weight-gradient chunk.  Few experts and small weights: about 1024 workgroups, whose partials cost
+// little beside the rows.  Where the experts' weights alone make half of that (64 experts, 512 to 1024 channels:
+// 2048), chunks four times as long: a chunk's partial is written and read at 8 bytes an element, which 1024 rows
+// are worth and 256 are not (8191 bfloat16 rows: the sums took 166 us beside 44 of products).
 int wgrad_chunk(int64_t S, int X, int nreps, int ci, int co) {
     const int64_t tiles = ceil_div(ci, ci <= 64 ? 64 : 128) * ceil_div(co, 128) * nreps;
-    const int64_t want = std::max<int64_t>(1, 1024 / tiles);
-    int64_t rc = align_up(static_cast<size_t>(ceil_div(std::max<int64_t>(S, 1), want)), 64);
+    const int64_t want = tiles * X >= 512 ? 256 : 1024;
+    const int64_t rc = ceil_div(ceil_div(std::max<int64_t>(S, 1) * tiles, want), 64) * 64;
     return static_cast<int>(std::min<int64_t>(std::max<int64_t>(rc, 128), 8192));
 }
 // Partials: an expert of m > 1 chunks has at most 2 rows / rc of them.
@@ -590,7 +787,7 @@ extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int3
         const bool vec = xl_vec<T>(cin, cout, {grad_y, x, grad_weight});
         auto run = [&](auto v, auto wr) -> int {
             constexpr int WR = decltype(wr)::value;
-            const int64_t blocks = tile_bound(slots, experts, rc) * ceil_div(cin, 64 * WR) * ceil_div(cout, 128);
+            const int64_t blocks = (slots / rc + experts) * ceil_div(cin, 64 * WR) * ceil_div(cout, 128);
             if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
             auto kern = k_xl_wgrad<T, decltype(v)::value, WR>;
             FEQ_LAUNCH("k_xl_wgrad", kern, dim3(blocks, nreps), dim3(kXlThreads), 0, s, static_cast<const T*>(grad_y),
@@ -601,12 +798,17 @@ extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int3
         auto with_wr = [&](auto v) -> int {
             return cin <= 64 ? run(v, std::integral_constant<int, 1>{}) : run(v, std::integral_constant<int, 2>{});
         };
-        if (slots)
-            if (const int err = vec ? with_wr(std::true_type{}) : with_wr(std::false_type{})) return err;
+        if (const int err = vec ? with_wr(std::true_type{}) : with_wr(std::false_type{})) return err;
+        if (nslots == 0) return FEQ_OK;               // every expert in one chunk
         const int64_t wsize = static_cast<int64_t>(cin) * cout;
-        auto kern = k_xl_wsum<T>;
-        FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(wsize, 256), experts, nreps + nb), dim3(256), 0, s, pw, pb, offsets,
-                   experts, rc, wsize, cout, nreps, static_cast<int>(nslots), gw, gb, nb);
-        return FEQ_OK;
+        const int64_t many = std::min<int64_t>(experts, slots / rc);     // experts of several chunks, at most
+        auto sum = [&](auto vv) -> int {
+            constexpr int V = decltype(vv)::value;
+            auto kern = k_xl_wsum<T, V>;
+            FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(std::max<int64_t>(wsize, cout), 256 * V), many, nreps + nb), dim3(256),
+                       0, s, pw, pb, offsets, experts, rc, wsize, cout, nreps, static_cast<int>(nslots), gw, gb, nb);
+            return FEQ_OK;
+        };
+        return vec ? sum(std::integral_constant<int, 4>{}) : sum(std::integral_constant<int, 1>{});
     });
 }
