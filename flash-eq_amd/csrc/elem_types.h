@@ -51,6 +51,25 @@ __device__ __forceinline__ float load_any(const void* p, int dt, int64_t i) {
     if (dt == FEQ_F16) return static_cast<float>(static_cast<const _Float16*>(p)[i]);
     return static_cast<float>(static_cast<const __bf16*>(p)[i]);
 }
+// V elements from i, a multiple of V, of an array aligned to 16 bytes.
+template <int V>
+__device__ __forceinline__ void load_any_v(const void* p, int dt, int64_t i, float (&o)[V]) {
+    if constexpr (V == 1) {
+        o[0] = load_any(p, dt, i);
+    } else if (dt == FEQ_F32) {
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            float f[4];
+            load_f<float, 4>(static_cast<const float*>(p) + i + j, f);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) o[j + u] = f[u];
+        }
+    } else if (dt == FEQ_F16) {
+        load_f<_Float16, V>(static_cast<const _Float16*>(p) + i, o);
+    } else {
+        load_f<__bf16, V>(static_cast<const __bf16*>(p) + i, o);
+    }
+}
 __device__ __forceinline__ void store_any(void* p, int dt, int64_t i, float v) {
     if (dt == FEQ_F32) static_cast<float*>(p)[i] = v;
     else if (dt == FEQ_F16) static_cast<_Float16*>(p)[i] = static_cast<_Float16>(v);

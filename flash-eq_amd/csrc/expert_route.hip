@@ -25,6 +25,7 @@
 
 #include "elem_types.h"
 #include "feq_internal.h"
+#include "lane_math.h"
 
 namespace feq {
 namespace {
@@ -38,33 +39,26 @@ constexpr int kPlanTile = 2048;       // slots of a k_plan_hist / k_plan_place w
 constexpr int kPlanOne = 8192;        // slots of k_plan_one
 constexpr int kPlanRounds = 8;        // 64-slot rounds of a wave
 
-// Larger key = earlier choice: order-preserving bits of the logit, NaN above all, -inf zero
-// (never chosen); +0 and -0 are equal.
+// Larger key = earlier choice: bits of the logit in an order-preserving form, a NaN above all, +0 and -0 equal.
+// Keys up to kNever (that of -inf) are never chosen; 0 marks what has been.
+constexpr uint32_t kNever = 0x007fffffu;
 __device__ __forceinline__ uint32_t order_key(float v) {
-    if (v != v) return 0xffffffffu;
     const uint32_t u = __float_as_uint(v + 0.0f);
-    if (u == 0xff800000u) return 0u;
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    const uint32_t k = u ^ (static_cast<uint32_t>(static_cast<int32_t>(u) >> 31) | 0x80000000u);
+    return v != v ? 0xffffffffu : k;
 }
-
-__device__ __forceinline__ float gsum(float v, int g) {
-    for (int o = g >> 1; o; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
-__device__ __forceinline__ float gmax(float v, int g) {
-    for (int o = g >> 1; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+// The logit of a key (any NaN for a NaN's).
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
 
 // Expert of element (chunk c, j) of lane l: chunks of V elements, chunk c of lane l at (c G + l) V.
 template <int V>
 __device__ __forceinline__ int elem_index(int l, int c, int j, int G) { return (c * G + l) * V + j; }
 
-// The row's logits (-inf behind the last expert) and e = exp(l - max); returns sum e.  A row of
-// -inf alone gives e = 0 and the sum 0.
+// The row's logits, -inf behind the last expert.
 template <class T, int V, int NC>
-__device__ __forceinline__ float row_exp(const T* row, int X, int l, int G, float (&x)[NC][V], float (&e)[NC][V]) {
-    float m = -__builtin_inff();
+__device__ __forceinline__ void load_row(const T* row, int X, int l, int G, float (&x)[NC][V]) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
         const int i0 = elem_index<V>(l, c, 0, G);
@@ -74,24 +68,36 @@ __device__ __forceinline__ float row_exp(const T* row, int X, int l, int G, floa
 #pragma unroll
             for (int j = 0; j < V; ++j) x[c][j] = -__builtin_inff();
         }
+    }
+}
+
+// e = exp(l - max) of the row; returns sum e.  A row of -inf alone gives e = 0 and the sum 0.  The exponential
+// is 2^((l - max) log2 e): rounding that product costs |l - max| steps of the result, no more than rounding l - max
+// itself has.
+__device__ __forceinline__ float exp_below(float v, float m) { return __builtin_amdgcn_exp2f((v - m) * 1.44269504f); }
+template <int V, int NC>
+__device__ __forceinline__ float row_exp(const float (&x)[NC][V], int G, float (&e)[NC][V], float& m) {
+    m = -__builtin_inff();
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int j = 0; j < V; ++j) m = fmaxf(m, x[c][j]);
-    }
-    m = gmax(m, G);
+    m = group_max(m, G);
+    m = m == -__builtin_inff() ? 0.0f : m;       // nothing left: e = exp(-inf) = 0, not exp(-inf + inf)
     float s = 0.0f;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            // masked experts are 0 also in a row of -inf alone, where l - max is no number
-            e[c][j] = x[c][j] == -__builtin_inff() ? 0.0f : expf(x[c][j] - m);
+            e[c][j] = exp_below(x[c][j], m);
             s += e[c][j];
         }
-    return gsum(s, G);
+    return group_sum(s, G);
 }
 
-// X is a multiple of V (V = 1 where it is not, or the logits are not aligned for it).
-template <class T, int V, int NC>
+// X is a multiple of V (V = 1 where it is not, or the logits are not aligned for it).  KMAX: the choices are kept
+// in registers until the weights' sum is known (K <= KMAX); 0: they wait in memory.
+template <class T, int V, int NC, int KMAX>
 __global__ void __launch_bounds__(kTopkThreads)
 k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normalize, int64_t* __restrict__ ids,
            float* __restrict__ weights, float* __restrict__ part, int G) {
@@ -103,10 +109,14 @@ k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normali
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int j = 0; j < V; ++j) mean[c][j] = 0.0f;
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / G; r < rows;
-         r += static_cast<int64_t>(gridDim.x) * per) {
-        float x[NC][V], e[NC][V];
-        const float s = row_exp<T, V, NC>(logits + r * X, X, l, G, x, e);
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * per;
+    int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / G;
+    float x[NC][V], next[NC][V], e[NC][V];
+    if (r < rows) load_row<T, V, NC>(logits + r * X, X, l, G, x);
+    for (; r < rows; r += stride) {
+        if (r + stride < rows) load_row<T, V, NC>(logits + (r + stride) * X, X, l, G, next);   // in flight meanwhile
+        float m;
+        const float s = row_exp<V, NC>(x, G, e, m);
         const float inv = s == 0.0f ? 0.0f : 1.0f / s;
         uint32_t key[NC][V];
 #pragma unroll
@@ -116,47 +126,69 @@ k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normali
                 mean[c][j] += e[c][j] * inv;
                 key[c][j] = order_key(x[c][j]);
             }
-        float total = 0.0f;
-        for (int k = 0; k < K; ++k) {
+        // the next choice: its expert (none: -1) and e, the same in the group's lanes
+        auto choose = [&](int& id, float& ek) {
             uint32_t best = 0;
-            int at = 0x7fffffff;
-            float ev = 0.0f;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (key[c][j] > best) {
-                        best = key[c][j];
-                        at = elem_index<V>(l, c, j, G);
-                        ev = e[c][j];
-                    }
-            for (int o = G >> 1; o; o >>= 1) {
-                const uint32_t b2 = __shfl_xor(best, o, 64);
-                const int a2 = __shfl_xor(at, o, 64);
-                const float e2 = __shfl_xor(ev, o, 64);
-                if (b2 > best || (b2 == best && a2 < at)) {
-                    best = b2;
-                    at = a2;
-                    ev = e2;
+                for (int j = 0; j < V; ++j) best = key[c][j] > best ? key[c][j] : best;
+            best = group_max_u(best, G);
+            // its lowest index: the lane's first element that holds it, then the lowest over the lanes
+            int mine = NC * V;
+#pragma unroll
+            for (int c = NC - 1; c >= 0; --c)
+#pragma unroll
+                for (int j = V - 1; j >= 0; --j) mine = key[c][j] == best ? c * V + j : mine;
+            const uint32_t at = mine < NC * V ? elem_index<V>(l, mine / V, mine % V, G) : 0xffffffffu;
+            const uint32_t first = group_min_u(at, G);
+            const bool got = best > kNever;
+            mine = at == first ? mine : NC * V;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int j = 0; j < V; ++j) key[c][j] = mine == c * V + j ? 0u : key[c][j];
+            ek = got ? exp_below(key_value(best), m) : 0.0f;
+            id = got ? static_cast<int>(first) : -1;
+        };
+        float total = 0.0f;
+        // a row without a choice has weights 0, not 0 / 0
+        auto inverse = [](float den) { return den == 0.0f ? 0.0f : 1.0f / den; };
+        if constexpr (KMAX > 0) {
+            int id[KMAX];
+            float ek[KMAX];
+#pragma unroll
+            for (int k = 0; k < KMAX; ++k)
+                if (k < K) {
+                    choose(id[k], ek[k]);
+                    total += ek[k];
+                }
+            const float scale = inverse(normalize ? total : s);
+#pragma unroll
+            for (int k = 0; k < KMAX; ++k)
+                if (k < K && l == (k & (G - 1))) {
+                    ids[r * K + k] = id[k];
+                    weights[r * K + k] = ek[k] * scale;
+                }
+        } else {
+            for (int k = 0; k < K; ++k) {
+                int id;
+                float ek;
+                choose(id, ek);
+                total += ek;
+                if (l == 0) {
+                    ids[r * K + k] = id;
+                    weights[r * K + k] = ek;
                 }
             }
-            const bool got = best != 0;
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (got && elem_index<V>(l, c, j, G) == at) key[c][j] = 0;
-            total += ev;
-            if (l == 0) {
-                ids[r * K + k] = got ? at : -1;
-                weights[r * K + k] = ev;
-            }
+            const float scale = inverse(normalize ? total : s);
+            if (l == 0)
+                for (int k = 0; k < K; ++k) weights[r * K + k] *= scale;
         }
-        const float den = normalize ? total : s;
-        // a row without a choice has weights 0, not 0 / 0
-        const float scale = den == 0.0f ? 0.0f : 1.0f / den;
-        if (l == 0)
-            for (int k = 0; k < K; ++k) weights[r * K + k] *= scale;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[c][j] = next[c][j];
     }
     if (!part) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -182,6 +214,7 @@ k_topk_mean(const float* __restrict__ part, int groups, int X, float inv_rows, f
     const int c = threadIdx.x & 15, r0 = threadIdx.x >> 4, i = blockIdx.x * 16 + c;
     float a = 0.0f;
     if (i < X)
+#pragma unroll 8
         for (int r = r0; r < groups; r += 64) a += part[static_cast<int64_t>(r) * X + i];
     s[r0][c] = a;
     __syncthreads();
@@ -219,27 +252,32 @@ k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const 
                 gp[c][j] = gm[c][j];
                 d[c][j] = 0.0f;
             }
+        float x[NC][V];
+        if (full) load_row<T, V, NC>(logits + r * X, X, l, G, x);
         if (gw) {
             float dot = 0.0f;
             if (normalize)
+#pragma unroll 4
                 for (int k = 0; k < K; ++k) dot += weights[r * K + k] * gw[r * K + k];
+#pragma unroll 4
             for (int k = 0; k < K; ++k) {
-                const int64_t id = ids[r * K + k];
+                const int id = static_cast<int>(ids[r * K + k]);
                 const float g = gw[r * K + k];
                 const float a = normalize ? weights[r * K + k] * (g - dot) : g;
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
 #pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        if (elem_index<V>(l, c, j, G) == id) {
-                            if (normalize) d[c][j] += a;
-                            else gp[c][j] += a;
-                        }
+                    for (int j = 0; j < V; ++j) {
+                        const bool here = elem_index<V>(l, c, j, G) == id;
+                        if (normalize) d[c][j] += here ? a : 0.0f;
+                        else gp[c][j] += here ? a : 0.0f;
+                    }
             }
         }
         if (full) {
-            float x[NC][V], e[NC][V];
-            const float s = row_exp<T, V, NC>(logits + r * X, X, l, G, x, e);
+            float e[NC][V];
+            float m;
+            const float s = row_exp<V, NC>(x, G, e, m);
             const float inv = s == 0.0f ? 0.0f : 1.0f / s;
             float dot = 0.0f;
 #pragma unroll
@@ -249,7 +287,7 @@ k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const 
                     e[c][j] *= inv;
                     dot += e[c][j] * gp[c][j];
                 }
-            dot = gsum(dot, G);
+            dot = group_sum(dot, G);
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -525,10 +563,15 @@ extern "C" int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t exp
             using T = decltype(t);
             const bool vec = experts % (16 / sizeof(T)) == 0 && aligned_to(logits, 16);
             return with_topk_form<T>(experts, vec, [&](auto v, auto nc) -> int {
-                auto kern = k_topk_fwd<T, decltype(v)::value, decltype(nc)::value>;
-                FEQ_LAUNCH("k_topk_fwd", kern, dim3(blocks), dim3(kTopkThreads), 0, s, static_cast<const T*>(logits),
-                           rows, experts, top_k, normalize, ids, weights, part, G);
-                return FEQ_OK;
+                auto run = [&](auto km) -> int {
+                    auto kern = k_topk_fwd<T, decltype(v)::value, decltype(nc)::value, decltype(km)::value>;
+                    FEQ_LAUNCH("k_topk_fwd", kern, dim3(blocks), dim3(kTopkThreads), 0, s, static_cast<const T*>(logits),
+                               rows, experts, top_k, normalize, ids, weights, part, G);
+                    return FEQ_OK;
+                };
+                if (top_k <= 2) return run(std::integral_constant<int, 2>{});
+                if (top_k <= 8) return run(std::integral_constant<int, 8>{});
+                return run(std::integral_constant<int, 0>{});
             });
         });
         if (rc) return rc;

@@ -20,6 +20,7 @@
 // for each pass, from L2 (the _wide kernels).
 #include "elem_types.h"
 #include "feq_internal.h"
+#include "lane_math.h"
 
 namespace feq {
 namespace {
@@ -27,25 +28,15 @@ namespace {
 constexpr int kLnThreads = 256;
 constexpr int kLnWaveElems = 16;    // elements a lane holds in the lane-group form
 constexpr int kLnBlockElems = 32;   // and in the workgroup form
+constexpr int kLnFwdBlocks = 2048;   // workgroups of the forward: what the chip holds, each over many rows
 constexpr int kLnMaxBlocks = 1024;  // workgroups of the backward, and weight-gradient partials
 constexpr int kLnWide = 1024;       // threads of the _wide kernels
-
-// Sum of a (and b) over the lane's group of g lanes (a power of two up to 64).
-__device__ __forceinline__ void group_sum2(float& a, float& b, int g) {
-    for (int o = g >> 1; o; o >>= 1) {
-        a += __shfl_xor(a, o, 64);
-        b += __shfl_xor(b, o, 64);
-    }
-}
-__device__ __forceinline__ float group_sum(float a, int g) {
-    for (int o = g >> 1; o; o >>= 1) a += __shfl_xor(a, o, 64);
-    return a;
-}
 
 // Sum over the workgroup of NW waves; red holds 2 NW floats, one use per call.
 template <int NW>
 __device__ __forceinline__ void block_sum2(float& a, float& b, float* red) {
-    group_sum2(a, b, 64);
+    a = group_sum(a, 64);
+    b = group_sum(b, 64);
     const int wave = threadIdx.x >> 6;
     __syncthreads();          // the previous call's readers are done
     if ((threadIdx.x & 63) == 0) {
@@ -76,29 +67,39 @@ k_ln_fwd(const T* __restrict__ x, int64_t rows, int width, int64_t ldx, const vo
     const float inv = 1.0f / static_cast<float>(width);
     float wv[NV][V], bv[NV][V];
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+        const int q = l + v * L;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (l + v * L) * V + j;
-            wv[v][j] = (w && c < width) ? load_any(w, pdt, c) : 1.0f;
-            bv[v][j] = (b && c < width) ? load_any(b, pdt, c) : 0.0f;
+            wv[v][j] = 1.0f;
+            bv[v][j] = 0.0f;
         }
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / L; r < rows; r += stride) {
+        if (w && q < nvec) load_any_v<V>(w, pdt, static_cast<int64_t>(q) * V, wv[v]);
+        if (b && q < nvec) load_any_v<V>(b, pdt, static_cast<int64_t>(q) * V, bv[v]);
+    }
+    float xv[NV][V], xn[NV][V];
+    auto load = [&](int64_t r, float (&o)[NV][V]) {
         const T* xr = x + r * ldx;
-        float xv[NV][V];
-        float s = 0.0f, z = 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
             const int q = l + v * L;
             if (q < nvec) {
-                load_f<T, V>(xr + static_cast<int64_t>(q) * V, xv[v]);
+                load_f<T, V>(xr + static_cast<int64_t>(q) * V, o[v]);
             } else {
 #pragma unroll
-                for (int j = 0; j < V; ++j) xv[v][j] = 0.0f;
+                for (int j = 0; j < V; ++j) o[v][j] = 0.0f;
             }
+        }
+    };
+    int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / L;
+    if (r < rows) load(r, xv);
+    for (; r < rows; r += stride) {
+        if (r + stride < rows) load(r + stride, xn);      // the next row, in flight during this one's sums
+        float s = 0.0f, z = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int j = 0; j < V; ++j) s += xv[v][j];
-        }
         if constexpr (BLK) block_sum2<4>(s, z, red);
         else s = group_sum(s, G);
         const float mu = s * inv;
@@ -130,6 +131,10 @@ k_ln_fwd(const T* __restrict__ x, int64_t rows, int width, int64_t ldx, const vo
             mean[r] = mu;
             rstd[r] = rs;
         }
+#pragma unroll
+        for (int v = 0; v < NV; ++v)
+#pragma unroll
+            for (int j = 0; j < V; ++j) xv[v][j] = xn[v][j];
     }
 }
 
@@ -151,13 +156,15 @@ k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t
     const float inv = 1.0f / static_cast<float>(width);
     float wv[NV][V], dw[NV][V], db[NV][V];
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 0; v < NV; ++v) {
+        const int q = l + v * L;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            const int c = (l + v * L) * V + j;
-            wv[v][j] = (w && c < width) ? load_any(w, pdt, c) : 1.0f;
+            wv[v][j] = 1.0f;
             dw[v][j] = db[v][j] = 0.0f;
         }
+        if (w && q < nvec) load_any_v<V>(w, pdt, static_cast<int64_t>(q) * V, wv[v]);
+    }
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / L; r < rows; r += stride) {
         const T* xr = x + r * ldx;
         const T* gr = gy + r * ldg;
@@ -191,7 +198,10 @@ k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t
             }
         if (gx) {
             if constexpr (BLK) block_sum2<4>(s1, s2, red);
-            else group_sum2(s1, s2, G);
+            else {
+                s1 = group_sum(s1, G);
+                s2 = group_sum(s2, G);
+            }
             s1 *= inv;
             s2 *= inv;
             T* dr = gx + r * width;
@@ -418,7 +428,7 @@ template <class T, int V>
 int ln_fwd_run(const T* x, int64_t rows, int width, int64_t ldx, const void* w, const void* b, int pdt, float eps,
                T* y, float* mean, float* rstd, const LnForm& f, hipStream_t s) {
     const int per = f.blk ? 1 : kLnThreads / f.G;
-    const int64_t blocks = std::min<int64_t>(ceil_div(rows, per), 8192);
+    const int64_t blocks = std::min<int64_t>(ceil_div(rows, per), kLnFwdBlocks);
     return ln_with_nv<V>(f.NV, [&](auto nv) -> int {
         constexpr int NV = decltype(nv)::value;
         if (f.blk) {
@@ -486,7 +496,7 @@ extern "C" int feq_layernorm_fwd(const void* x, int64_t rows, int64_t width, int
         constexpr int VV = 16 / sizeof(T);
         const T* xt = static_cast<const T*>(x);
         T* yt = static_cast<T*>(y);
-        const bool vec = ln_vec_ok<T>(width, {ldx}, {x, y});
+        const bool vec = ln_vec_ok<T>(width, {ldx}, {x, y, weight, bias});
         const LnForm f = ln_form(width, vec ? VV : 1);
         if (f.wide) {
             auto kern = k_ln_fwd_wide<T>;
@@ -528,7 +538,7 @@ extern "C" int feq_layernorm_bwd(const void* grad_y, int64_t ldg, const void* x,
             constexpr int VV = 16 / sizeof(T);
             const T *gt = static_cast<const T*>(grad_y), *xt = static_cast<const T*>(x);
             T* dt = static_cast<T*>(grad_x);
-            const bool vec = ln_vec_ok<T>(width, {ldx, ldg}, {x, grad_y, grad_x});
+            const bool vec = ln_vec_ok<T>(width, {ldx, ldg}, {x, grad_y, grad_x, weight});
             const LnForm f = ln_form(width, vec ? VV : 1);
             if (f.wide) {
                 if (dt) {
