@@ -109,10 +109,14 @@ struct Mma<__bf16> : MmaHalf<__bf16, b8> {
 };
 
 // 16 bytes of T at p, of which the first `n` elements exist (n <= 0: none); the others are 0.
-template <class T, bool VEC>
+// ONCE: read past the caches.
+template <class T, bool VEC, bool ONCE = false>
 __device__ __forceinline__ uint4 load16(const T* p, int n) {
     constexpr int V = 16 / sizeof(T);
-    if constexpr (VEC) {
+    if constexpr (VEC && ONCE) {
+        typedef unsigned u4 __attribute__((ext_vector_type(4)));
+        return n > 0 ? __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u4*>(p))) : uint4{0, 0, 0, 0};
+    } else if constexpr (VEC) {
         return n > 0 ? *reinterpret_cast<const uint4*>(p) : uint4{0, 0, 0, 0};
     } else {
         typename VecOf<T, V>::type v;
@@ -455,7 +459,10 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
 // planes), 64 WR columns k of x and 128 columns n of grad_y (tiles of k first).  An expert of one chunk gets its
 // gradient written (zeros without rows), one of several a float32 partial per chunk:
 // pw[(r nslots + slot) N K + n K + k], pb[(j nslots + slot) N + n], summed by k_xl_wsum.
-template <class T, bool VEC, int WR>
+// ONCE: one tile covers the weight, so every row is read once; the rows then go past the caches, which leaves them to
+// the kernels around (20011 x 49 bfloat16 rows, 128 x 128: 137 -> 97 us, and with both maps a pass 376 -> 353).  Rows
+// that several tiles read lose by it (42 -> 52 us for 512 x 1024).
+template <class T, bool VEC, int WR, bool ONCE>
 __global__ void __launch_bounds__(kXlThreads)
 k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __restrict__ offsets, int X, int S,
            int ci, int co, int nreps, XlMap map, int rc, int nslots, T* __restrict__ gw, T* __restrict__ gb, int nbias,
@@ -489,12 +496,12 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
             const int q = tid + kXlThreads * i, r = r0 + q / (BK / V), k = k0 + (q % (BK / V)) * V;
-            vx[i] = load16<T, VEC>(x + (base + r) * ci + k, r < rend ? ci - k : 0);
+            vx[i] = load16<T, VEC, ONCE>(x + (base + r) * ci + k, r < rend ? ci - k : 0);
         }
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
             const int q = tid + kXlThreads * i, r = r0 + q / (BN / V), n = n0 + (q % (BN / V)) * V;
-            vg[i] = load16<T, VEC>(gy + (base + r) * co + n, r < rend ? co - n : 0);
+            vg[i] = load16<T, VEC, ONCE>(gy + (base + r) * co + n, r < rend ? co - n : 0);
         }
     };
     v4f acc[4][NT];
@@ -789,11 +796,17 @@ extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int3
             constexpr int WR = decltype(wr)::value;
             const int64_t blocks = (slots / rc + experts) * ceil_div(cin, 64 * WR) * ceil_div(cout, 128);
             if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
-            auto kern = k_xl_wgrad<T, decltype(v)::value, WR>;
-            FEQ_LAUNCH("k_xl_wgrad", kern, dim3(blocks, nreps), dim3(kXlThreads), 0, s, static_cast<const T*>(grad_y),
-                       static_cast<const T*>(x), offsets, experts, static_cast<int>(slots), cin, cout, nreps, map, rc,
-                       static_cast<int>(nslots), gw, gb, nb, pw, pb);
-            return FEQ_OK;
+            auto go = [&](auto once) -> int {
+                auto kern = k_xl_wgrad<T, decltype(v)::value, WR, decltype(once)::value>;
+                FEQ_LAUNCH("k_xl_wgrad", kern, dim3(blocks, nreps), dim3(kXlThreads), 0, s, static_cast<const T*>(grad_y),
+                           static_cast<const T*>(x), offsets, experts, static_cast<int>(slots), cin, cout, nreps, map, rc,
+                           static_cast<int>(nslots), gw, gb, nb, pw, pb);
+                return FEQ_OK;
+            };
+            if constexpr (decltype(v)::value) {
+                if (cin <= 64 * WR && cout <= 128) return go(std::true_type{});
+            }
+            return go(std::false_type{});
         };
         auto with_wr = [&](auto v) -> int {
             return cin <= 64 ? run(v, std::integral_constant<int, 1>{}) : run(v, std::integral_constant<int, 2>{});

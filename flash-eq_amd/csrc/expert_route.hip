@@ -16,8 +16,8 @@
 // sum per lane, summed over lanes, waves and workgroups in a fixed order.
 //
 // Plan.  A stable counting sort: per 2048-slot tile a histogram (k_plan_hist), per bucket the
-// tiles' exclusive sums (k_plan_scan), then every tile ranks its slots (k_plan_place).  Up to 8192
-// slots one workgroup does all three (k_plan_one).  Lanes with equal keys find each other by one
+// tiles' exclusive sums (k_plan_scan; up to 64 tiles sum them themselves), then every tile ranks its
+// slots (k_plan_place).  Up to 8192 slots one workgroup does all three (k_plan_one).  Lanes with equal keys find each other by one
 // ballot per key bit, so a slot's rank needs no atomics and the order is the slots' own.  Slots
 // whose expert lies outside [0, X) fill a last bucket.  The plan is integer work on 8 bytes
 // per slot: launches and latency bound it.
@@ -38,6 +38,7 @@ constexpr int kMaxTopk = 64;
 constexpr int kPlanTile = 2048;       // slots of a k_plan_hist / k_plan_place workgroup
 constexpr int kPlanOne = 8192;        // slots of k_plan_one
 constexpr int kPlanRounds = 8;        // 64-slot rounds of a wave
+constexpr int kPlanOwnSums = 64;      // tiles up to which every tile sums the others' histograms itself (a launch less)
 
 // Larger key = earlier choice: bits of the logit in an order-preserving form, a NaN above all, +0 and -0 equal.
 // Keys up to kNever (that of -inf) are never chosen; 0 marks what has been.
@@ -491,14 +492,29 @@ k_plan_scan(int32_t* __restrict__ hist, int64_t ntiles, int32_t* __restrict__ to
 
 __global__ void __launch_bounds__(256)
 k_plan_place(const int64_t* __restrict__ ids, int64_t n, int X, int bits, int64_t ntiles,
-             const int32_t* __restrict__ hist, const int32_t* __restrict__ total, int32_t* __restrict__ order,
+             const int32_t* __restrict__ hist, const int32_t* __restrict__ total, int scanned, int32_t* __restrict__ order,
              int32_t* __restrict__ positions, int32_t* __restrict__ offsets) {
     __shared__ int cnt[4 * (kMaxExperts + 2)];
-    __shared__ int base[kMaxExperts + 2];
+    __shared__ int base[kMaxExperts + 2], before[kMaxExperts + 2];
     __shared__ int tmp[4];
     const int nb = X + 2, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     for (int i = threadIdx.x; i < 4 * nb; i += 256) cnt[i] = 0;
-    for (int i = threadIdx.x; i < X; i += 256) base[i] = total[i];
+    for (int i = threadIdx.x; i <= X; i += 256) {
+        int all = 0, mine = 0;                // slots of the bucket, and those in the tiles before
+        if (scanned) {
+            all = total[i];
+            mine = hist[i * ntiles + blockIdx.x];
+        } else {
+#pragma unroll 8
+            for (int t = 0; t < ntiles; ++t) {
+                const int h = hist[i * ntiles + t];
+                all += h;
+                mine += t < static_cast<int>(blockIdx.x) ? h : 0;
+            }
+        }
+        base[i] = all;
+        before[i] = mine;
+    }
     __syncthreads();
     const int all = scan_buckets<256>(base, X, tmp);
     if (threadIdx.x == 0) base[X] = all;
@@ -510,7 +526,7 @@ k_plan_place(const int64_t* __restrict__ ids, int64_t n, int X, int bits, int64_
     rank_wave(ids, beg, n, X, bits, cnt + wave * nb, key, rank);
     __syncthreads();
     for (int b = threadIdx.x; b <= X; b += 256) {
-        int run = base[b] + hist[b * ntiles + blockIdx.x];
+        int run = base[b] + before[b];
         for (int w = 0; w < 4; ++w) {
             const int c = cnt[w * nb + b];
             cnt[w * nb + b] = run;
@@ -634,8 +650,9 @@ extern "C" int feq_expert_plan(const int64_t* ids, int64_t slots, int32_t expert
     int32_t* hist = static_cast<int32_t*>(workspace);
     int32_t* total = hist + (experts + 1) * ntiles;
     FEQ_LAUNCH("k_plan_hist", k_plan_hist, dim3(ntiles), dim3(256), 0, s, ids, slots, experts, ntiles, hist);
-    FEQ_LAUNCH("k_plan_scan", k_plan_scan, dim3(experts + 1), dim3(256), 0, s, hist, ntiles, total);
+    const bool scan = ntiles > kPlanOwnSums;
+    if (scan) FEQ_LAUNCH("k_plan_scan", k_plan_scan, dim3(experts + 1), dim3(256), 0, s, hist, ntiles, total);
     FEQ_LAUNCH("k_plan_place", k_plan_place, dim3(ntiles), dim3(256), 0, s, ids, slots, experts, bits, ntiles, hist,
-               total, order, positions, offsets);
+               total, scan, order, positions, offsets);
     return FEQ_OK;
 }

@@ -256,8 +256,10 @@ extern "C" int feq_expert_combine_bwd(const void* grad_y, const void* ys, int64_
         auto run = [&](auto v, auto kb) -> int {
             constexpr int V = decltype(v)::value, KB = decltype(kb)::value;
             const int GL = row_lanes(width / V);
-            int PS = 1;     // groups of a row, up to one per plane
-            while (PS < planes && GL * PS * 2 <= kRowThreads) PS <<= 1;
+            // groups of a row: as many as fill the chip (eight waves a SIMD), no more than planes.  20000 rows of 9
+            // planes, 64 float32 columns: one group 43 us, sixteen (seven of them idle) 83
+            int PS = 1;
+            while (PS * 2 <= planes && GL * PS * 2 <= kRowThreads && rows * GL * PS < 64 * 8192) PS <<= 1;
             auto kern = k_rows_combine_bwd<T, V, KB>;
             FEQ_LAUNCH("k_rows_combine_bwd", kern, dim3(std::min(ceil_div(rows, kRowThreads / (GL * PS)), kMaxRowBlocks)), dim3(kRowThreads), 0,
                        s, static_cast<const T*>(grad_y), static_cast<const T*>(ys), rows, top_k, width,
