@@ -14,8 +14,7 @@
 //
 // The weight is the first operand and the rows the second, so a lane's accumulators are
 // columns of one row; the weight rows are dealt to the tiles so that a lane's 16 accumulators are
-// 16 consecutive columns, which leave as 16-byte stores.  The next block of the reduction is
-// loaded to registers while the present one, in LDS, is multiplied.
+// XXX
 #include <algorithm>
 
 #include "elem_types.h"
@@ -61,7 +60,7 @@ struct Mma<float> {
     }
     // tile by tile within a step, so that no product waits for the one before
     template <int NT>
-    static __device__ __forceinline__ void mul_all(const frag (&a)[NT], frag b, v4f (&acc)[NT]) {
+    static __device__ __forceinline__ void mul_all(const frag (&a)[NT], frag b, v4f* acc) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
@@ -93,7 +92,7 @@ template <>
 struct Mma<_Float16> : MmaHalf<_Float16, h8> {
     static __device__ __forceinline__ v4f mul(h8 a, h8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
     template <int NT>
-    static __device__ __forceinline__ void mul_all(const frag (&a)[NT], frag b, v4f (&acc)[NT]) {
+    static __device__ __forceinline__ void mul_all(const frag (&a)[NT], frag b, v4f* acc) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] = mul(a[i], b, acc[i]);
     }
@@ -102,28 +101,50 @@ template <>
 struct Mma<__bf16> : MmaHalf<__bf16, b8> {
     static __device__ __forceinline__ v4f mul(b8 a, b8 b, v4f c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
     template <int NT>
-    static __device__ __forceinline__ void mul_all(const frag (&a)[NT], frag b, v4f (&acc)[NT]) {
+    static __device__ __forceinline__ void mul_all(const frag (&a)[NT], frag b, v4f* acc) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) acc[i] = mul(a[i], b, acc[i]);
     }
 };
 
-// 16 bytes of T at p, of which the first `n` elements exist (n <= 0: none); the others are 0.
-// ONCE: read past the caches.
+// A table read by buffer loads: an offset past its end gives zeros, so absent rows and columns cost no branch.  (A
+// branch around a load makes the compiler wait for every load in flight at the next use: with branches the products of
+// 8191 bfloat16 rows, 512 to 1024 columns, took 36 us whatever was prefetched.)  Base and size are uniform.
+typedef __amdgpu_buffer_rsrc_t Table;
+constexpr uint32_t kTableBytes = 0x7ffffff0u, kOutside = 0x80000000u;
+__device__ __forceinline__ Table table(const void* p, bool there = true) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, there ? kTableBytes : 0u, 0x00020000);
+}
+
+// 16 bytes of T at byte offset `at` (below 2^31) of the table, of which the first `n` elements exist (n <= 0: none);
+// the others are 0.  VEC: n is a multiple of the 16 bytes.  ONCE: read past the caches.
 template <class T, bool VEC, bool ONCE = false>
-__device__ __forceinline__ uint4 load16(const T* p, int n) {
-    constexpr int V = 16 / sizeof(T);
-    if constexpr (VEC && ONCE) {
-        typedef unsigned u4 __attribute__((ext_vector_type(4)));
-        return n > 0 ? __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u4*>(p))) : uint4{0, 0, 0, 0};
-    } else if constexpr (VEC) {
-        return n > 0 ? *reinterpret_cast<const uint4*>(p) : uint4{0, 0, 0, 0};
+__device__ __forceinline__ uint4 load16(Table t, uint32_t at, int n) {
+    constexpr int V = 16 / sizeof(T), kPast = ONCE ? 2 : 0;
+    if constexpr (VEC) {
+        return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(t, n > 0 ? at : kOutside, 0, kPast));
+    } else if constexpr (sizeof(T) == 4) {
+        uint4 v;
+        v.x = __builtin_amdgcn_raw_buffer_load_b32(t, n > 0 ? at : kOutside, 0, kPast);
+        v.y = __builtin_amdgcn_raw_buffer_load_b32(t, n > 1 ? at + 4 : kOutside, 0, kPast);
+        v.z = __builtin_amdgcn_raw_buffer_load_b32(t, n > 2 ? at + 8 : kOutside, 0, kPast);
+        v.w = __builtin_amdgcn_raw_buffer_load_b32(t, n > 3 ? at + 12 : kOutside, 0, kPast);
+        return v;
     } else {
-        typename VecOf<T, V>::type v;
+        typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+        us8 v;
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = j < n ? p[j] : static_cast<T>(0.0f);
+        for (int j = 0; j < V; ++j) v[j] = __builtin_amdgcn_raw_buffer_load_b16(t, n > j ? at + 2 * j : kOutside, 0, kPast);
         return __builtin_bit_cast(uint4, v);
     }
+}
+
+// One element as float32, 0 where it does not exist.
+template <class T>
+__device__ __forceinline__ float load1(Table t, uint32_t at, bool there) {
+    const uint32_t o = there ? at : kOutside;
+    if constexpr (sizeof(T) == 4) return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(t, o, 0, 0));
+    else return static_cast<float>(__builtin_bit_cast(T, static_cast<unsigned short>(__builtin_amdgcn_raw_buffer_load_b16(t, o, 0, 0))));
 }
 
 // A lane's accumulators are four consecutive columns of a tile: 16 bytes of float32, half of that of a 16-bit type,
@@ -178,7 +199,7 @@ struct XlTile {
 };
 
 // Block `want` of the row blocks (of `bm` rows) of the experts in order, the rows behind them last.  Called
-// by whole waves; the result is the same in every lane.  EMPTY: an expert without rows has one block.
+// by whole waves; the result is uniform.  EMPTY: an expert without rows has one block.
 template <bool EMPTY = false>
 __device__ __forceinline__ XlTile find_tile(const int32_t* __restrict__ offsets, int X, int S, int bm, int want) {
     const int lane = threadIdx.x & 63;
@@ -203,18 +224,18 @@ __device__ __forceinline__ XlTile find_tile(const int32_t* __restrict__ offsets,
         const uint64_t hit = __ballot(carry + incl > want);
         if (hit) {
             const int f = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-            const int begin = carry + __shfl(incl - n, f, 64);
+            const int begin = carry + __builtin_amdgcn_readlane(incl - n, f);
             XlTile t;
             t.expert = e0 + f;
             t.index = want - begin;
-            t.row0 = __shfl(a, f, 64) + t.index * bm;
-            t.row1 = __shfl(z, f, 64);
-            t.before = many + __shfl(mincl - multi, f, 64);
-            t.count = __shfl(n, f, 64);
+            t.row0 = __builtin_amdgcn_readlane(a, f) + t.index * bm;
+            t.row1 = __builtin_amdgcn_readlane(z, f);
+            t.before = many + __builtin_amdgcn_readlane(mincl - multi, f);
+            t.count = __builtin_amdgcn_readlane(n, f);
             return t;
         }
-        carry += __shfl(incl, 63, 64);
-        many += __shfl(mincl, 63, 64);
+        carry += __builtin_amdgcn_readlane(incl, 63);
+        many += __builtin_amdgcn_readlane(mincl, 63);
     }
     return XlTile{-1, 0, 0, 0, 0, 0};
 }
@@ -222,11 +243,32 @@ __device__ __forceinline__ XlTile find_tile(const int32_t* __restrict__ offsets,
 // Blocks of `bm` rows that X experts and the rows behind them can make of S rows.
 inline int64_t tile_bound(int64_t S, int X, int bm) { return S / bm + std::min<int64_t>(S, X + 1); }
 
+// The blocks (of `bm` rows) that find_tile numbers.  Called by whole waves.
+__device__ __forceinline__ int count_tiles(const int32_t* __restrict__ offsets, int X, int S, int bm) {
+    int n = 0;
+    for (int e = threadIdx.x & 63; e <= X; e += 64) {
+        n += ((e < X ? offsets[e + 1] : S) - offsets[e] + bm - 1) / bm;
+    }
+    for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o, 64);
+    return __builtin_amdgcn_readfirstlane(n);
+}
+
+// The row block of a workgroup of a grid of 8 ceil(bound / 8) subs workgroups (a plane's), -1: none; `sub` its column
+// block.  Workgroups go to the 8 XCDs in turn.  An XCD takes neighbouring row blocks, whole: an expert's weight and
+// rows then pass to one L2 and once, where column blocks dealt to the XCDs would bring the rows to all of them.
+__device__ __forceinline__ int xcd_tile(int block, int subs, int tiles, int& sub) {
+    const int i = block / 8, chunk = (tiles + 7) / 8;
+    sub = i % subs;
+    const int t = i / subs;
+    return t < chunk && block % 8 * chunk + t < tiles ? block % 8 * chunk + t : -1;
+}
+inline int64_t xcd_grid(int64_t bound, int64_t subs) { return 8 * ceil_div(bound, 8) * subs; }
+
 // out[d, p, :] = in[d, p, :] B (+ bias), B = W[e, r]^T (TRANS false: in has Cin columns, out Cout) or W[e, r]
 // (TRANS: in has Cout columns, out Cin).  K: columns of in, N: of out; W rows have wld = Cin elements.
 // WR: waves along the output columns (64 each), 4 / WR along the rows.
 template <class T, bool VEC, bool TRANS, int WR>
-__global__ void __launch_bounds__(kXlThreads)
+__global__ void __launch_bounds__(kXlThreads, 2)
 k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,
         int N, int nreps, XlMap map, const T* __restrict__ bias, int nbias, T* __restrict__ out) {
     using M = Mma<T>;
@@ -236,116 +278,118 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
     constexpr int LDT = BN + M::PAD;                 // stride of a W row staged as it lies (TRANS)
     constexpr int NIN = kXlBM * CH / kXlThreads;     // vectors a thread stages
     constexpr int NW = BN * CH / kXlThreads;
-    __shared__ __align__(16) T sIn[kXlBM * LD];
-    __shared__ __align__(16) T sW[TRANS ? BK * LDT : BN * LD];
+    __shared__ __align__(16) T sIn[2][kXlBM * LD];
+    __shared__ __align__(16) T sW[2][TRANS ? BK * LDT : BN * LD];
     const int d = blockIdx.y;
-    const int nb = (N + BN - 1) / BN;
-    const XlTile t = find_tile(offsets, X, S, kXlBM, blockIdx.x / nb);
-    if (t.expert < 0) return;
-    const int n0 = (blockIdx.x % nb) * BN;
+    int sub;
+    const int tile = xcd_tile(blockIdx.x, (N + BN - 1) / BN, count_tiles(offsets, X, S, kXlBM), sub);
+    if (tile < 0) return;
+    const XlTile t = find_tile(offsets, X, S, kXlBM, tile);
+    const int n0 = sub * BN;
     const int rows = t.row1 - t.row0 < kXlBM ? t.row1 - t.row0 : kXlBM;
     T* od = out + (static_cast<int64_t>(d) * S + t.row0) * N;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wc = wave / WR;
     const bool none = t.expert == X;                 // uniform: rows without an expert
-    const T* id = in + (static_cast<int64_t>(d) * S + t.row0) * K;
-    const int64_t wmat = static_cast<int64_t>(TRANS ? K : N) * (TRANS ? N : K);
-    const T* we = W + (static_cast<int64_t>(none ? 0 : t.expert) * nreps + map.rep[d]) * wmat;
+    const Table rows_in = table(in + (static_cast<int64_t>(d) * S + t.row0) * K);
+    const T* we = W + (static_cast<int64_t>(none ? 0 : t.expert) * nreps + __builtin_amdgcn_readfirstlane(map.rep[d])) * K * N;
 
-    uint4 vin[NIN], vw[NW];
-    auto load = [&](int k0) {
+    auto load = [&](int k0, uint4 (&vin)[NIN], uint4 (&vw)[NW]) {
 #pragma unroll
         for (int i = 0; i < NIN; ++i) {
             const int q = tid + kXlThreads * i, r = q / CH, k = k0 + (q % CH) * V;
-            vin[i] = load16<T, VEC>(id + static_cast<int64_t>(r) * K + k, r < rows ? K - k : 0);
+            vin[i] = load16<T, VEC>(rows_in, (r * K + k) * sizeof(T), r < rows ? K - k : 0);
         }
+        const Table w = table(TRANS ? we + static_cast<int64_t>(k0) * N + n0 : we + static_cast<int64_t>(n0) * K);
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             const int q = tid + kXlThreads * i;
             if constexpr (TRANS) {                   // W rows are k, columns n
-                const int r = k0 + q / (BN / V), n = n0 + (q % (BN / V)) * V;
-                vw[i] = load16<T, VEC>(we + static_cast<int64_t>(r) * N + n, r < K ? N - n : 0);
+                const int r = q / (BN / V), n = (q % (BN / V)) * V;
+                vw[i] = load16<T, VEC>(w, (r * N + n) * sizeof(T), k0 + r < K ? N - n0 - n : 0);
             } else {
-                const int r = n0 + q / CH, k = k0 + (q % CH) * V;
-                vw[i] = load16<T, VEC>(we + static_cast<int64_t>(r) * K + k, r < N ? K - k : 0);
+                const int r = q / CH, k = k0 + (q % CH) * V;
+                vw[i] = load16<T, VEC>(w, (r * K + k) * sizeof(T), n0 + r < N ? K - k : 0);
             }
         }
     };
-    auto stage = [&]() {
+    auto stage = [&](int u, const uint4 (&vin)[NIN], const uint4 (&vw)[NW]) {
 #pragma unroll
         for (int i = 0; i < NIN; ++i) {
             const int q = tid + kXlThreads * i;
-            *reinterpret_cast<uint4*>(sIn + (q / CH) * LD + (q % CH) * V) = vin[i];
+            *reinterpret_cast<uint4*>(sIn[u] + (q / CH) * LD + (q % CH) * V) = vin[i];
         }
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             const int q = tid + kXlThreads * i;
-            if constexpr (TRANS) put_dealt<T>(sW + (q / (BN / V)) * LDT, (q % (BN / V)) * V, vw[i]);
-            else *reinterpret_cast<uint4*>(sW + dealt<T>(q / CH) * LD + (q % CH) * V) = vw[i];
+            if constexpr (TRANS) put_dealt<T>(sW[u] + (q / (BN / V)) * LDT, (q % (BN / V)) * V, vw[i]);
+            else *reinterpret_cast<uint4*>(sW[u] + dealt<T>(q / CH) * LD + (q % CH) * V) = vw[i];
         }
     };
 
+    // lane (c, g): row c of row tile j, columns 16 i + V g + 0 .. V - 1 of the wave's 64 for tile group i; the sums
+    // begin with the bias
+    const int nw = n0 + 64 * wr + V * g;
+    const int bc = __builtin_amdgcn_readfirstlane(map.bcol[d]);
+    const bool biased = !TRANS && bias && bc >= 0 && !none;
+    const Table be = table(biased ? bias + static_cast<int64_t>(t.expert) * N * nbias : nullptr, biased);
     v4f acc[4][PT];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < PT; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    if (!none) {
-        load(0);
-        for (int k0 = 0; k0 < K; k0 += BK) {
-            __syncthreads();
-            stage();
-            __syncthreads();
-            if (k0 + BK < K) load(k0 + BK);
+        for (int r = 0; r < 4; ++r) {
+            const int n = nw + 16 * (i - i % kDealt<T>) + 4 * (i % kDealt<T>) + r;
+            const float bv = load1<T>(be, (n * nbias + bc) * sizeof(T), n < N);
 #pragma unroll
-            for (int ks = 0; ks < BK; ks += M::KS) {
-                typename M::frag a[4], b[PT];
+            for (int j = 0; j < PT; ++j) acc[i][j][r] = bv;
+        }
+    // step k0 from LDS buffer u: meanwhile the next step goes to the other buffer and the registers take the one
+    // after it
+    auto step = [&](int k0, int u, uint4 (&vin)[NIN], uint4 (&vw)[NW]) {
+        stage(u ^ 1, vin, vw);
+        load(k0 + 3 * BK, vin, vw);                  // nothing behind K
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int q0 = 64 * wr + 16 * i;
-                    if constexpr (TRANS) a[i] = M::columns(sW, LDT, ks, g, c, q0);
-                    else a[i] = *reinterpret_cast<const typename M::frag*>(sW + (q0 + c) * LD + ks + M::FE * g);
-                }
+        for (int ks = 0; ks < BK; ks += M::KS) {
+            typename M::frag a[4], b[PT];
 #pragma unroll
-                for (int j = 0; j < PT; ++j)
-                    b[j] = *reinterpret_cast<const typename M::frag*>(sIn + (16 * (wc * PT + j) + c) * LD + ks + M::FE * g);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < PT; ++j) acc[i][j] = M::mul(a[i], b[j], acc[i][j]);
+            for (int i = 0; i < 4; ++i) {
+                const int q0 = 64 * wr + 16 * i;
+                if constexpr (TRANS) a[i] = M::columns(sW[u], LDT, ks, g, c, q0);
+                else a[i] = *reinterpret_cast<const typename M::frag*>(sW[u] + (q0 + c) * LD + ks + M::FE * g);
             }
+#pragma unroll
+            for (int j = 0; j < PT; ++j)
+                b[j] = *reinterpret_cast<const typename M::frag*>(sIn[u] + (16 * (wc * PT + j) + c) * LD + ks + M::FE * g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < PT; ++j) acc[i][j] = M::mul(a[i], b[j], acc[i][j]);
+        }
+        __syncthreads();
+    };
+    if (!none) {
+        uint4 in0[NIN], w0[NW], in1[NIN], w1[NW];
+        load(0, in0, w0);
+        load(BK, in1, w1);
+        stage(0, in0, w0);
+        load(2 * BK, in0, w0);
+        __syncthreads();
+        for (int k0 = 0; k0 < K; k0 += 2 * BK) {
+            step(k0, 0, in1, w1);
+            if (k0 + BK >= K) break;
+            step(k0 + BK, 1, in0, w0);
         }
     }
-    // lane (c, g): row c of row tile j, columns 16 i + V g + 0 .. V - 1 of the wave's 64 for tile group i
-    const int nw = n0 + 64 * wr + V * g;
-    const int bc = map.bcol[d];
-    const bool biased = !TRANS && bias && bc >= 0 && !none;
 #pragma unroll
     for (int i = 0; i < 4; i += kDealt<T>) {
         const int n = nw + 16 * i;
-        if (biased) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float bv = n + v < N ? static_cast<float>(bias[(static_cast<int64_t>(t.expert) * N + n + v) * nbias + bc]) : 0.0f;
-#pragma unroll
-                for (int j = 0; j < PT; ++j) acc[i + v / 4][j][v % 4] += bv;
-            }
-        }
 #pragma unroll
         for (int j = 0; j < PT; ++j) {
             const int r = 16 * (wc * PT + j) + c;
             if (r < rows) store_tiles<T, VEC, PT>(od + static_cast<int64_t>(r) * N + n, N - n, &acc[i][j]);
         }
     }
-}
-
-// 16-row blocks of the experts' rows and of the rows behind them, in one plane.  Called by whole waves.
-__device__ __forceinline__ int count_blocks(const int32_t* __restrict__ offsets, int X, int S) {
-    int n = 0;
-    for (int e = threadIdx.x & 63; e <= X; e += 64) n += ((e < X ? offsets[e + 1] : S) - offsets[e] + 15) / 16;
-    for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o, 64);
-    return n;
 }
 
 // The same product for a reduction of at most 128 columns: a block of the weight stays in LDS, the rows stream.  The
@@ -356,20 +400,20 @@ __device__ __forceinline__ int count_blocks(const int32_t* __restrict__ offsets,
 // one's products.  Nothing but the weight passes through LDS and no barrier stands between blocks of an
 // expert.  NS: reduction steps held (K <= NS KS).
 template <class T, bool VEC, bool TRANS, int NB, int NS>
-__global__ void __launch_bounds__(kXlThreads)
+__global__ void __launch_bounds__(kXlThreads, NB * NS * Mma<T>::KS * sizeof(T) > 40000 ? 2 : 4)
 k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,
             int N, int nreps, XlMap map, int dim, const T* __restrict__ bias, int nbias, T* __restrict__ out) {
     using M = Mma<T>;
     typedef typename M::frag frag;
     constexpr int V = 16 / sizeof(T), KM = NS * M::KS;
-    constexpr int NT = NB / 16;
+    constexpr int NT = NB / 16, NA = NT < 4 ? NT : 4;   // tiles; those whose weight fragments are held at a time
     constexpr int LD = KM + V, LDT = NB + M::PAD;
     __shared__ __align__(16) T sW[TRANS ? KM * LDT : NB * LD];
     __shared__ __align__(16) float sBias[NB];
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nb = (N + NB - 1) / NB;
-    const int per_plane = __builtin_amdgcn_readfirstlane(count_blocks(offsets, X, S));
+    const int per_plane = count_tiles(offsets, X, S, 16);
     const int64_t total = static_cast<int64_t>(per_plane) * dim * nb;
     const int64_t share = total / gridDim.x, more = total % gridDim.x;
     int64_t at = blockIdx.x * share + (blockIdx.x < more ? blockIdx.x : more);
@@ -377,20 +421,20 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
     while (at < end) {
         const int line = static_cast<int>(at / per_plane), d = line / nb, n0 = line % nb * NB;
         const XlTile t = find_tile(offsets, X, S, 16, static_cast<int>(at % per_plane));
-        const int expert = __builtin_amdgcn_readfirstlane(t.expert), row0 = __builtin_amdgcn_readfirstlane(t.row0);
-        const int rows = __builtin_amdgcn_readfirstlane(t.row1) - row0;
-        const int left = __builtin_amdgcn_readfirstlane(t.count - t.index);
+        const int expert = t.expert, row0 = t.row0, rows = t.row1 - t.row0, left = t.count - t.index;
         const int nblocks = static_cast<int>(end - at < left ? end - at : left);
         at += nblocks;
         const T* id = in + (static_cast<int64_t>(d) * S + row0) * K;
         T* od = out + (static_cast<int64_t>(d) * S + row0) * N + n0;
 
         auto load = [&](int blk, frag (&b)[NS]) {
-            const int r = 16 * blk + c;
-            const T* p = id + static_cast<int64_t>(r < rows ? r : rows - 1) * K + M::FE * g;
+            const Table p = table(id + static_cast<int64_t>(16 * blk) * K);
+            const bool there = 16 * blk + c < rows;
 #pragma unroll
-            for (int ks = 0; ks < NS; ++ks)
-                b[ks] = __builtin_bit_cast(frag, load16<T, VEC>(p + ks * M::KS, K - ks * M::KS - M::FE * g));
+            for (int ks = 0; ks < NS; ++ks) {
+                const int k = ks * M::KS + M::FE * g;
+                b[ks] = __builtin_bit_cast(frag, load16<T, VEC>(p, (c * K + k) * sizeof(T), there ? K - k : 0));
+            }
         };
         auto store = [&](int blk, const v4f (&acc)[NT]) {
             const int r = 16 * blk + c;
@@ -410,28 +454,30 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
             continue;
         }
         frag b0[NS], b1[NS];
-        if (wave < nblocks) load(wave, b0);
+        load(wave, b0);                              // nothing behind the last row
         __syncthreads();                             // the last expert's weight has been read
-        const T* we = W + (static_cast<int64_t>(expert) * nreps + map.rep[d]) * K * N;
-        if constexpr (TRANS) {
-            for (int q = tid; q < KM * (NB / V); q += kXlThreads) {
+        const T* wm = W + (static_cast<int64_t>(expert) * nreps + __builtin_amdgcn_readfirstlane(map.rep[d])) * K * N;
+        const Table we = table(TRANS ? wm + n0 : wm + static_cast<int64_t>(n0) * K);
+#pragma unroll
+        for (int i = 0; i < KM * NB / V / kXlThreads; ++i) {
+            const int q = tid + kXlThreads * i;
+            if constexpr (TRANS) {
                 const int k = q / (NB / V), n = (q % (NB / V)) * V;
-                put_dealt<T>(sW + k * LDT, n, load16<T, VEC>(we + static_cast<int64_t>(k) * N + n0 + n, k < K ? N - n0 - n : 0));
-            }
-        } else {
-            for (int q = tid; q < NB * (KM / V); q += kXlThreads) {
+                put_dealt<T>(sW + k * LDT, n, load16<T, VEC>(we, (k * N + n) * sizeof(T), k < K ? N - n0 - n : 0));
+            } else {
                 const int n = q / (KM / V), k = (q % (KM / V)) * V;
                 *reinterpret_cast<uint4*>(sW + dealt<T>(n) * LD + k) =
-                    load16<T, VEC>(we + static_cast<int64_t>(n0 + n) * K + k, n0 + n < N ? K - k : 0);
+                    load16<T, VEC>(we, (n * K + k) * sizeof(T), n0 + n < N ? K - k : 0);
             }
         }
-        const int bc = map.bcol[d];
+        const int bc = __builtin_amdgcn_readfirstlane(map.bcol[d]);
+        const bool biased = !TRANS && bias && bc >= 0;
         if (tid < NB)
-            sBias[tid] = (!TRANS && bias && bc >= 0 && n0 + tid < N)
-                             ? static_cast<float>(bias[(static_cast<int64_t>(expert) * N + n0 + tid) * nbias + bc]) : 0.0f;
+            sBias[tid] = load1<T>(table(biased ? bias + static_cast<int64_t>(expert) * N * nbias : nullptr, biased),
+                                  ((n0 + tid) * nbias + bc) * sizeof(T), n0 + tid < N);
         __syncthreads();
         for (int blk = wave; blk < nblocks; blk += 4) {
-            load(blk + 4 < nblocks ? blk + 4 : blk, b1);
+            load(blk + 4, b1);                       // nothing behind the last row
             // the weight is read from LDS for every block: kept in registers it would take them from the rows in flight
             asm volatile("" ::: "memory");
             v4f acc[NT];
@@ -440,13 +486,16 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
                 acc[i] = *reinterpret_cast<const v4f*>(sBias + 16 * (i - i % kDealt<T>) + V * g + 4 * (i % kDealt<T>));
 #pragma unroll
             for (int ks = 0; ks < NS; ++ks) {
-                frag a[NT];
 #pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    if constexpr (TRANS) a[i] = M::columns(sW, LDT, ks * M::KS, g, c, 16 * i);
-                    else a[i] = *reinterpret_cast<const frag*>(sW + (16 * i + c) * LD + ks * M::KS + M::FE * g);
+                for (int i0 = 0; i0 < NT; i0 += NA) {
+                    frag a[NA];
+#pragma unroll
+                    for (int i = 0; i < NA; ++i) {
+                        if constexpr (TRANS) a[i] = M::columns(sW, LDT, ks * M::KS, g, c, 16 * (i0 + i));
+                        else a[i] = *reinterpret_cast<const frag*>(sW + (16 * (i0 + i) + c) * LD + ks * M::KS + M::FE * g);
+                    }
+                    M::template mul_all<NA>(a, b0[ks], acc + i0);
                 }
-                M::template mul_all<NT>(a, b0[ks], acc);
             }
             store(blk, acc);
 #pragma unroll
@@ -484,24 +533,26 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wc = wave / WR;
-    const int d0 = map.first[rep], d1 = map.first[rep + 1];
+    const int d0 = __builtin_amdgcn_readfirstlane(map.first[rep]), d1 = __builtin_amdgcn_readfirstlane(map.first[rep + 1]);
     const int steps = (rend - t.row0 + BP - 1) / BP, total = steps * (d1 - d0);
-    const int bc = map.bcol[d0];
+    const int bc = __builtin_amdgcn_readfirstlane(map.bcol[d0]);
     const bool sums = gb && bc >= 0 && k0 == 0;                    // uniform
 
     uint4 vx[NX], vg[NG];
     auto load = [&](int it) {
-        const int d = d0 + it / steps, r0 = t.row0 + (it % steps) * BP;
-        const int64_t base = static_cast<int64_t>(d) * S;
+        const int d = it < total ? d0 + it / steps : d0, r0 = t.row0 + (it % steps) * BP;
+        const int64_t base = static_cast<int64_t>(d) * S + r0;
+        const Table tx = table(x + base * ci + k0), tg = table(gy + base * co + n0);
+        const int there = it < total ? rend - r0 : 0;
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
-            const int q = tid + kXlThreads * i, r = r0 + q / (BK / V), k = k0 + (q % (BK / V)) * V;
-            vx[i] = load16<T, VEC, ONCE>(x + (base + r) * ci + k, r < rend ? ci - k : 0);
+            const int q = tid + kXlThreads * i, r = q / (BK / V), k = (q % (BK / V)) * V;
+            vx[i] = load16<T, VEC, ONCE>(tx, (r * ci + k) * sizeof(T), r < there ? ci - k0 - k : 0);
         }
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-            const int q = tid + kXlThreads * i, r = r0 + q / (BN / V), n = n0 + (q % (BN / V)) * V;
-            vg[i] = load16<T, VEC, ONCE>(gy + (base + r) * co + n, r < rend ? co - n : 0);
+            const int q = tid + kXlThreads * i, r = q / (BN / V), n = (q % (BN / V)) * V;
+            vg[i] = load16<T, VEC, ONCE>(tg, (r * co + n) * sizeof(T), r < there ? co - n0 - n : 0);
         }
     };
     v4f acc[4][NT];
@@ -524,7 +575,7 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
             *reinterpret_cast<uint4*>(sG + (q / (BN / V)) * LG + (q % (BN / V)) * V) = vg[i];
         }
         __syncthreads();
-        if (it + 1 < total) load(it + 1);
+        load(it + 1);
 #pragma unroll
         for (int ks = 0; ks < BP; ks += M::KS) {
             typename M::frag a[4], b[NT];
@@ -700,7 +751,7 @@ int mm_run(const void* in, const void* W, const int32_t* offsets, int X, int64_t
     }
     auto run = [&](auto v, auto wr) -> int {
         constexpr int WR = decltype(wr)::value;
-        const int64_t blocks = tile_bound(S, X, kXlBM) * ceil_div(N, 64 * WR);
+        const int64_t blocks = xcd_grid(tile_bound(S, X, kXlBM), ceil_div(N, 64 * WR));
         if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
         auto kern = k_xl_mm<T, decltype(v)::value, TRANS, WR>;
         FEQ_LAUNCH(TRANS ? "k_xl_mm_t" : "k_xl_mm", kern, dim3(blocks, map.first[nreps]), dim3(kXlThreads), 0, s,
