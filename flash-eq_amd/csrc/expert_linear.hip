@@ -346,9 +346,10 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
         }
     // step k0 from LDS buffer u: meanwhile the next step goes to the other buffer and the registers take the one
     // after it
-    auto step = [&](int k0, int u, uint4 (&vin)[NIN], uint4 (&vw)[NW]) {
+    uint4 vin[NIN], vw[NW];
+    auto step = [&](int k0, int u) {
         stage(u ^ 1, vin, vw);
-        load(k0 + 3 * BK, vin, vw);                  // nothing behind K
+        load(k0 + 2 * BK, vin, vw);                  // nothing behind K
 #pragma unroll
         for (int ks = 0; ks < BK; ks += M::KS) {
             typename M::frag a[4], b[PT];
@@ -369,16 +370,14 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
         __syncthreads();
     };
     if (!none) {
-        uint4 in0[NIN], w0[NW], in1[NIN], w1[NW];
-        load(0, in0, w0);
-        load(BK, in1, w1);
-        stage(0, in0, w0);
-        load(2 * BK, in0, w0);
+        load(0, vin, vw);
+        stage(0, vin, vw);
+        load(BK, vin, vw);
         __syncthreads();
         for (int k0 = 0; k0 < K; k0 += 2 * BK) {
-            step(k0, 0, in1, w1);
+            step(k0, 0);
             if (k0 + BK >= K) break;
-            step(k0 + BK, 1, in0, w0);
+            step(k0 + BK, 1);
         }
     }
 #pragma unroll
