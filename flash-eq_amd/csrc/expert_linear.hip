@@ -45,6 +45,15 @@ struct XlMap {
     int16_t first[kXlMaxReps + 1];
 };
 
+// Weight-gradient chunks, which the irreps of many planes have shorter: rows of a chunk, first workgroup row block
+// (irreps in descending order, as launched) and first partial of every irrep; irrep of every bias column.
+struct XlChunks {
+    int32_t rows[kXlMaxReps];
+    int32_t tile0[kXlMaxReps + 1];
+    int32_t slot0[kXlMaxReps + 1];
+    int8_t brep[kXlMaxReps];
+};
+
 // One reduction step of a 16 x 16 tile: KS elements, a lane holding FE of them.
 // Lane (c = l % 16, g = l / 16) holds elements FE g .. FE g + FE - 1 of row (or column) c.
 template <class T>
@@ -399,7 +408,7 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
 // one's products.  Nothing but the weight passes through LDS and no barrier stands between blocks of an
 // expert.  NS: reduction steps held (K <= NS KS).
 template <class T, bool VEC, bool TRANS, int NB, int NS>
-__global__ void __launch_bounds__(kXlThreads, NB * NS * Mma<T>::KS * sizeof(T) > 40000 ? 2 : 4)
+__global__ void __launch_bounds__(kXlThreads, NB * NS * Mma<T>::KS * sizeof(T) > 40000 ? 2 : NS == 8 ? 3 : 4)
 k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,
             int N, int nreps, XlMap map, int dim, const T* __restrict__ bias, int nbias, T* __restrict__ out) {
     using M = Mma<T>;
@@ -503,17 +512,17 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
     }
 }
 
-// grad_W and grad_b over row chunks of rc rows.  A workgroup takes a chunk of one expert, one irrep r (all its
+// grad_W and grad_b over row chunks.  A workgroup takes a chunk of one expert, one irrep r (all its
 // planes), 64 WR columns k of x and 128 columns n of grad_y (tiles of k first).  An expert of one chunk gets its
-// gradient written (zeros without rows), one of several a float32 partial per chunk:
-// pw[(r nslots + slot) N K + n K + k], pb[(j nslots + slot) N + n], summed by k_xl_wsum.
+// gradient written (zeros without rows), one of several a float32 partial per chunk: pw[slot N K + n K + k],
+// pb[slot N + n], summed by k_xl_wsum.
 // ONCE: one tile covers the weight, so every row is read once; the rows then go past the caches, which leaves them to
 // the kernels around (20011 x 49 bfloat16 rows, 128 x 128: 137 -> 97 us, and with both maps a pass 376 -> 353).  Rows
 // that several tiles read lose by it (42 -> 52 us for 512 x 1024).
 template <class T, bool VEC, int WR, bool ONCE>
 __global__ void __launch_bounds__(kXlThreads)
 k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __restrict__ offsets, int X, int S,
-           int ci, int co, int nreps, XlMap map, int rc, int nslots, T* __restrict__ gw, T* __restrict__ gb, int nbias,
+           int ci, int co, int nreps, XlMap map, XlChunks ch, T* __restrict__ gw, T* __restrict__ gb, int nbias,
            float* __restrict__ pw, float* __restrict__ pb) {
     using M = Mma<T>;
     constexpr int V = 16 / sizeof(T), BP = kXlRowBytes / sizeof(T);   // rows staged at a time
@@ -523,9 +532,11 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
     __shared__ __align__(16) T sX[BP * LX];
     __shared__ __align__(16) T sG[BP * LG];
     const int nk = (ci + BK - 1) / BK, nn = (co + BN - 1) / BN;
-    const int tile = blockIdx.x / (nk * nn), sub = blockIdx.x % (nk * nn);
-    const int rep = nreps - 1 - static_cast<int>(blockIdx.y);      // the irreps of most planes first
-    const XlTile t = find_tile<true>(offsets, X, S, rc, tile);
+    const int block = blockIdx.x / (nk * nn), sub = blockIdx.x % (nk * nn);
+    int rep = nreps - 1;                             // the irreps of most planes first
+    while (rep > 0 && block >= ch.tile0[rep - 1]) --rep;
+    const int rc = ch.rows[rep];
+    const XlTile t = find_tile<true>(offsets, X, S, rc, block - ch.tile0[rep]);
     if (t.expert < 0 || t.expert == X) return;
     const int k0 = (sub % nk) * BK, n0 = (sub / nk) * BN;
     const int rend = t.row1 - t.row0 < rc ? t.row1 : t.row0 + rc;
@@ -591,10 +602,10 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
             for (int p = 0; p < BP; ++p) bsum += static_cast<float>(sG[p * LG + tid]);
     }
     const bool direct = t.count == 1;
-    const int slot = t.before + t.index;
+    const int64_t slot = ch.slot0[rep] + t.before + t.index;
     const int kw = k0 + 64 * wr + V * g;
     const int64_t base = direct ? (static_cast<int64_t>(t.expert) * nreps + rep) * co
-                                : (static_cast<int64_t>(rep) * nslots + slot) * co;
+                                : slot * co;
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const int n = n0 + 16 * (wc * NT + j) + c;
@@ -613,7 +624,7 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
     }
     if (sums && tid < BN && n0 + tid < co) {
         if (direct) gb[(static_cast<int64_t>(t.expert) * co + n0 + tid) * nbias + bc] = static_cast<T>(bsum);
-        else pb[(static_cast<int64_t>(bc) * nslots + slot) * co + n0 + tid] = bsum;
+        else pb[slot * co + n0 + tid] = bsum;
     }
 }
 
@@ -621,9 +632,10 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
 // these, blockIdx.z: the irrep, and behind the irreps the bias columns.
 template <class T, int V>
 __global__ void __launch_bounds__(256)
-k_xl_wsum(const float* __restrict__ pw, const float* __restrict__ pb, const int32_t* __restrict__ offsets, int X, int rc,
-          int64_t wsize, int co, int nreps, int nslots, T* __restrict__ gw, T* __restrict__ gb, int nbias) {
+k_xl_wsum(const float* __restrict__ pw, const float* __restrict__ pb, const int32_t* __restrict__ offsets, int X,
+          XlChunks ch, int64_t wsize, int co, int nreps, T* __restrict__ gw, T* __restrict__ gb, int nbias) {
     const int z = blockIdx.z, lane = threadIdx.x & 63, want = blockIdx.y;
+    const int rep = z < nreps ? z : ch.brep[z - nreps], rc = ch.rows[rep];
     int expert = -1, first = 0, count = 0, carry = 0, slots = 0;
     for (int e0 = 0; e0 < X; e0 += 64) {
         const int e = e0 + lane;
@@ -651,8 +663,7 @@ k_xl_wsum(const float* __restrict__ pw, const float* __restrict__ pb, const int3
     const bool w = z < nreps;
     const int64_t size = w ? wsize : co;
     if (i >= size) return;
-    const float* p = (w ? pw + (static_cast<int64_t>(z) * nslots + first) * wsize
-                        : pb + (static_cast<int64_t>(z - nreps) * nslots + first) * co) + i;
+    const float* p = (w ? pw : pb) + static_cast<int64_t>(ch.slot0[rep] + first) * size + i;
     float a[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) a[v] = 0.0f;
@@ -764,18 +775,30 @@ int mm_run(const void* in, const void* W, const int32_t* offsets, int X, int64_t
     return vec ? with_wr(std::true_type{}) : with_wr(std::false_type{});
 }
 
-// Rows of a weight-gradient chunk.  Few experts and small weights: about 1024 workgroups, whose partials cost
-// little beside the rows.  Where the experts' weights alone make half of that (64 experts, 512 to 1024 channels:
-// 2048), chunks four times as long: a chunk's partial is written and read at 8 bytes an element, which 1024 rows
-// are worth and 256 are not (8191 bfloat16 rows: the sums took 166 us beside 44 of products).
-int wgrad_chunk(int64_t S, int X, int nreps, int ci, int co) {
-    const int64_t tiles = ceil_div(ci, ci <= 64 ? 64 : 128) * ceil_div(co, 128) * nreps;
-    const int64_t want = tiles * X >= 512 ? 256 : 1024;
-    const int64_t rc = ceil_div(ceil_div(std::max<int64_t>(S, 1) * tiles, want), 64) * 64;
-    return static_cast<int>(std::min<int64_t>(std::max<int64_t>(rc, 128), 8192));
+// Weight-gradient chunks: all of about as many row-planes, for about 1024 workgroups, whose partials cost little
+// beside the rows.  Where the experts' weights alone make half of that (64 experts, 512 to 1024 channels: 2048),
+// chunks four times as long: a chunk's partial is written and read at 8 bytes an element, which 1024 rows are
+// worth and 256 are not (8191 bfloat16 rows: the sums took 166 us beside 44 of products).  A partial is needed for
+// an expert of several chunks; those have at most 2 S / rows.  Returns the number of partials.
+int64_t wgrad_chunks(int64_t S, int X, const int32_t* lvals, int nreps, int ci, int co, XlChunks* ch) {
+    const int64_t sub = ceil_div(ci, ci <= 64 ? 64 : 128) * ceil_div(co, 128);
+    int64_t dim = 0;
+    for (int r = 0; r < nreps; ++r) dim += 2 * lvals[r] + 1;
+    const int64_t want = sub * nreps * X >= 512 ? 256 : 1024;
+    const int64_t unit = ceil_div(std::max<int64_t>(S, 1) * dim * sub, want);
+    int64_t tiles = 0, slots = 0;
+    for (int r = nreps - 1; r >= 0; --r) {
+        const int64_t rows = std::min<int64_t>(ceil_div(ceil_div(unit, 2 * lvals[r] + 1), 64) * 64, 8192);
+        ch->rows[r] = static_cast<int32_t>(rows);
+        ch->tile0[r] = static_cast<int32_t>(tiles);
+        ch->slot0[r] = static_cast<int32_t>(slots);
+        tiles += S / rows + X;
+        slots += S > rows ? 2 * S / rows : 0;
+    }
+    ch->tile0[nreps] = static_cast<int32_t>(tiles);      // all
+    ch->slot0[nreps] = static_cast<int32_t>(slots);
+    return slots;
 }
-// Partials: an expert of m > 1 chunks has at most 2 rows / rc of them.
-int64_t wgrad_slots(int64_t S, int rc) { return S > rc ? 2 * S / rc : 0; }
 
 }  // namespace
 }  // namespace feq
@@ -809,13 +832,16 @@ extern "C" int feq_expert_linear_bwd_x(const int32_t* lvals, int32_t nreps, int3
     });
 }
 
-extern "C" size_t feq_expert_linear_bwd_w_workspace(int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
-                                                    int32_t cout, int32_t nbias) {
-    if (nreps < 1 || experts < 1 || slots < 1 || cin < 1 || cout < 1 || nbias < 0) return 0;
-    const int64_t n = wgrad_slots(slots, wgrad_chunk(slots, experts, nreps, cin, cout));
+extern "C" size_t feq_expert_linear_bwd_w_workspace(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots,
+                                                    int32_t cin, int32_t cout, int32_t nbias) {
+    if (!lvals || nreps < 1 || nreps > kXlMaxReps || experts < 1 || slots < 1 || cin < 1 || cout < 1 || nbias < 0) return 0;
+    for (int r = 0; r < nreps; ++r)
+        if (lvals[r] < 0 || lvals[r] > kXlMaxPlanes) return 0;
+    XlChunks ch;
+    const int64_t n = wgrad_chunks(slots, experts, lvals, nreps, cin, cout, &ch);
     Carver c(nullptr);
-    c.take<float>(static_cast<size_t>(n) * nreps * cin * cout);
-    c.take<float>(static_cast<size_t>(n) * nbias * cout);
+    c.take<float>(static_cast<size_t>(n) * cin * cout);
+    c.take<float>(nbias ? static_cast<size_t>(n) * cout : 0);
     return c.used;
 }
 
@@ -828,29 +854,30 @@ extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int3
     if (!grad_weight || !offsets || (slots && (!grad_y || !x))) return fail(FEQ_ERR_INVALID, "NULL pointer");
     if (grad_bias && (!bias_cols || nbias < 1)) return fail(FEQ_ERR_INVALID, "a bias gradient needs bias columns");
     const int nb = grad_bias ? nbias : 0;
-    if (ws_bytes < feq_expert_linear_bwd_w_workspace(nreps, experts, slots, cin, cout, nb))
-        return fail(FEQ_ERR_WORKSPACE, "weight-gradient workspace of %zu bytes, %zu needed", ws_bytes,
-                    feq_expert_linear_bwd_w_workspace(nreps, experts, slots, cin, cout, nb));
+    const size_t need = feq_expert_linear_bwd_w_workspace(lvals, nreps, experts, slots, cin, cout, nb);
+    if (ws_bytes < need) return fail(FEQ_ERR_WORKSPACE, "weight-gradient workspace of %zu bytes, %zu needed", ws_bytes, need);
+    if (need && !workspace) return fail(FEQ_ERR_INVALID, "NULL pointer");
     hipStream_t s = stream_of(stream);
-    const int rc = wgrad_chunk(slots, experts, nreps, cin, cout);
-    const int64_t nslots = wgrad_slots(slots, rc);
-    if (nslots && !workspace) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    XlChunks ch;
+    const int64_t nslots = wgrad_chunks(slots, experts, lvals, nreps, cin, cout, &ch);
+    for (int r = 0; r < nreps; ++r)
+        if (nb && bias_cols[r] >= 0) ch.brep[bias_cols[r]] = static_cast<int8_t>(r);
     Carver c(workspace);
-    float* pw = c.take<float>(static_cast<size_t>(nslots) * nreps * cin * cout);
-    float* pb = c.take<float>(static_cast<size_t>(nslots) * nb * cout);
+    float* pw = c.take<float>(static_cast<size_t>(nslots) * cin * cout);
+    float* pb = c.take<float>(nb ? static_cast<size_t>(nslots) * cout : 0);
     return with_dtype(dtype, [&](auto tt) -> int {
         using T = decltype(tt);
         T *gw = static_cast<T*>(grad_weight), *gb = static_cast<T*>(grad_bias);
         const bool vec = xl_vec<T>(cin, cout, {grad_y, x, grad_weight});
         auto run = [&](auto v, auto wr) -> int {
             constexpr int WR = decltype(wr)::value;
-            const int64_t blocks = (slots / rc + experts) * ceil_div(cin, 64 * WR) * ceil_div(cout, 128);
+            const int64_t blocks = ch.tile0[nreps] * ceil_div(cin, 64 * WR) * ceil_div(cout, 128);
             if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
             auto go = [&](auto once) -> int {
                 auto kern = k_xl_wgrad<T, decltype(v)::value, WR, decltype(once)::value>;
-                FEQ_LAUNCH("k_xl_wgrad", kern, dim3(blocks, nreps), dim3(kXlThreads), 0, s, static_cast<const T*>(grad_y),
-                           static_cast<const T*>(x), offsets, experts, static_cast<int>(slots), cin, cout, nreps, map, rc,
-                           static_cast<int>(nslots), gw, gb, nb, pw, pb);
+                FEQ_LAUNCH("k_xl_wgrad", kern, dim3(blocks), dim3(kXlThreads), 0, s, static_cast<const T*>(grad_y),
+                           static_cast<const T*>(x), offsets, experts, static_cast<int>(slots), cin, cout, nreps, map, ch, gw,
+                           gb, nb, pw, pb);
                 return FEQ_OK;
             };
             if constexpr (decltype(v)::value) {
@@ -864,12 +891,14 @@ extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int3
         if (const int err = vec ? with_wr(std::true_type{}) : with_wr(std::false_type{})) return err;
         if (nslots == 0) return FEQ_OK;               // every expert in one chunk
         const int64_t wsize = static_cast<int64_t>(cin) * cout;
-        const int64_t many = std::min<int64_t>(experts, slots / rc);     // experts of several chunks, at most
+        int least = ch.rows[0];
+        for (int r = 1; r < nreps; ++r) least = std::min(least, static_cast<int>(ch.rows[r]));
+        const int64_t many = std::min<int64_t>(experts, slots / least);  // experts of several chunks, at most
         auto sum = [&](auto vv) -> int {
             constexpr int V = decltype(vv)::value;
             auto kern = k_xl_wsum<T, V>;
             FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(std::max<int64_t>(wsize, cout), 256 * V), many, nreps + nb), dim3(256),
-                       0, s, pw, pb, offsets, experts, rc, wsize, cout, nreps, static_cast<int>(nslots), gw, gb, nb);
+                       0, s, pw, pb, offsets, experts, ch, wsize, cout, nreps, gw, gb, nb);
             return FEQ_OK;
         };
         return vec ? sum(std::integral_constant<int, 4>{}) : sum(std::integral_constant<int, 1>{});

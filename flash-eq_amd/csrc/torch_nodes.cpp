@@ -489,7 +489,7 @@ struct ExpertLinearNode final : OnceNode {
             const int32_t nb = need(2) ? static_cast<int32_t>(nbias) : 0;
             Tensor gw = make(w.sizes(), w, w.scalar_type()), gb;
             if (nb) gb = make({experts, co, nbias}, w, w.scalar_type());
-            const Tensor ws = scratch(feq_expert_linear_bwd_w_workspace(irreps.n(), experts, slots, ci, co, nb), xs);
+            const Tensor ws = scratch(feq_expert_linear_bwd_w_workspace(irreps.lvals.data(), irreps.n(), experts, slots, ci, co, nb), xs);
             done(feq_expert_linear_bwd_w(irreps.lvals.data(), irreps.n(), experts, slots, ci, co, code, ptr(g), ptr(xs),
                                          ptr_as<int32_t>(offsets), nb, irreps.cols.data(), ptr(gw), ptr(gb), ptr(ws),
                                          bytes_of(ws), on.stream),

@@ -811,8 +811,8 @@ int feq_expert_linear_bwd_x(const int32_t* lvals, int32_t nreps, int32_t experts
                             const int32_t* offsets, void* grad_x, feq_stream_t stream);
 /* grad_weight and, unless NULL, grad_bias: sums in a fixed order, zeros for an expert without rows.
  * Workspace feq_expert_linear_bwd_w_workspace bytes (nbias 0 without grad_bias). */
-size_t feq_expert_linear_bwd_w_workspace(int32_t nreps, int32_t experts, int64_t slots, int32_t cin, int32_t cout,
-                                         int32_t nbias);
+size_t feq_expert_linear_bwd_w_workspace(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots,
+                                         int32_t cin, int32_t cout, int32_t nbias);
 int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
                             int32_t cout, int32_t dtype, const void* grad_y, const void* x, const int32_t* offsets,
                             int32_t nbias, const int32_t* bias_cols, void* grad_weight, void* grad_bias,
