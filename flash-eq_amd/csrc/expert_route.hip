@@ -351,15 +351,16 @@ __device__ __forceinline__ uint64_t lanes_with(int key, int bits) {
     return m;
 }
 
-// A wave's slots [beg, beg + 512) in order: key[i] and rank[i] of this lane's slot of round i among
-// the wave's equal keys; cnt (X + 2 ints, zero) receives the wave's histogram.
-__device__ __forceinline__ void rank_wave(const int64_t* ids, int64_t beg, int64_t n, int X, int bits, int* cnt,
+// A wave's slots [beg, beg + 64 rounds) in order: key[i] and rank[i] of this lane's slot of round i among
+// the wave's equal keys; cnt (X + 2 ints, zero) receives the wave's histogram.  rounds is uniform, at most 8.
+__device__ __forceinline__ void rank_wave(const int64_t* ids, int64_t beg, int rounds, int64_t n, int X, int bits, int* cnt,
                                           int (&key)[kPlanRounds], int (&rank)[kPlanRounds]) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int i = 0; i < kPlanRounds; ++i) key[i] = slot_key(ids, beg + 64 * i + lane, n, X);
+    for (int i = 0; i < kPlanRounds; ++i) key[i] = slot_key(ids, i < rounds ? beg + 64 * i + lane : n, n, X);
 #pragma unroll
     for (int i = 0; i < kPlanRounds; ++i) {
+        if (i >= rounds) break;
         const uint64_t m = lanes_with(key[i], bits);
         const int before = __popcll(m & ((1ull << lane) - 1ull));
         const int base = cnt[key[i]];
@@ -419,8 +420,8 @@ k_plan_one(const int64_t* __restrict__ ids, int n, int X, int bits, int32_t* __r
     for (int i = threadIdx.x; i < 16 * nb; i += 1024) lds[i] = 0;
     __syncthreads();
     int key[kPlanRounds], rank[kPlanRounds];
-    const int beg = wave * 512;
-    if (beg < n) rank_wave(ids, beg, n, X, bits, lds + wave * nb, key, rank);
+    const int rounds = (n + 1023) / 1024, beg = wave * 64 * rounds;      // the slots spread over the waves
+    if (beg < n) rank_wave(ids, beg, rounds, n, X, bits, lds + wave * nb, key, rank);
     __syncthreads();
     for (int b = threadIdx.x; b < nb; b += 1024) {      // the waves' exclusive sums per bucket
         int run = 0;
@@ -440,7 +441,7 @@ k_plan_one(const int64_t* __restrict__ ids, int n, int X, int bits, int32_t* __r
 #pragma unroll
         for (int i = 0; i < kPlanRounds; ++i) {
             const int slot = beg + 64 * i + lane;
-            if (slot < n) {
+            if (i < rounds && slot < n) {
                 const int p = base[key[i]] + lds[wave * nb + key[i]] + rank[i];
                 order[p] = slot;
                 positions[slot] = p;
@@ -523,7 +524,7 @@ k_plan_place(const int64_t* __restrict__ ids, int64_t n, int X, int bits, int64_
         for (int b = threadIdx.x; b <= X; b += 256) offsets[b] = base[b];
     int key[kPlanRounds], rank[kPlanRounds];
     const int64_t beg = static_cast<int64_t>(blockIdx.x) * kPlanTile + wave * 512;
-    rank_wave(ids, beg, n, X, bits, cnt + wave * nb, key, rank);
+    rank_wave(ids, beg, kPlanRounds, n, X, bits, cnt + wave * nb, key, rank);
     __syncthreads();
     for (int b = threadIdx.x; b <= X; b += 256) {
         int run = base[b] + before[b];
