@@ -14,19 +14,33 @@ namespace {
 template <class T, int V>
 struct VecOf {
     typedef T type __attribute__((ext_vector_type(V)));
+    typedef type any __attribute__((aligned(sizeof(T))));      // the same in memory, aligned as an element
 };
 template <class T>
 struct VecOf<T, 1> {
     typedef T type;
+    typedef T any;
 };
 
-// V elements at p, aligned to V sizeof(T) bytes, as float32 (exact).
+// Rows whose width is no multiple of a vector, or that begin at an address that is none, are read and written in
+// vectors all the same (gfx950 takes a vector at any element): the last one begins V before the row's end and
+// shares its first elements with the one before.  Vector q of a row of `width` >= V elements:
+template <int V>
+__device__ __forceinline__ int vec_begin(int q, int width) { return q * V < width - V ? q * V : width - V; }
+// and the number of its first elements that belong to the vector before it (V: the row has no vector q).
+template <int V>
+__device__ __forceinline__ int vec_shared(int q, int width) {
+    const int s = q * V - (width - V);
+    return s < 0 ? 0 : s < V ? s : V;
+}
+
+// V elements at p as float32 (exact).
 template <class T, int V>
 __device__ __forceinline__ void load_f(const T* __restrict__ p, float (&o)[V]) {
     if constexpr (V == 1) {
         o[0] = static_cast<float>(p[0]);
     } else {
-        const auto u = *reinterpret_cast<const typename VecOf<T, V>::type*>(p);
+        const typename VecOf<T, V>::type u = *reinterpret_cast<const typename VecOf<T, V>::any*>(p);
 #pragma unroll
         for (int j = 0; j < V; ++j) o[j] = static_cast<float>(u[j]);
     }
@@ -41,7 +55,7 @@ __device__ __forceinline__ void store_f(T* __restrict__ p, const float (&o)[V]) 
         typename VecOf<T, V>::type u;
 #pragma unroll
         for (int j = 0; j < V; ++j) u[j] = static_cast<T>(o[j]);
-        *reinterpret_cast<typename VecOf<T, V>::type*>(p) = u;
+        *reinterpret_cast<typename VecOf<T, V>::any*>(p) = u;
     }
 }
 
@@ -51,7 +65,7 @@ __device__ __forceinline__ float load_any(const void* p, int dt, int64_t i) {
     if (dt == FEQ_F16) return static_cast<float>(static_cast<const _Float16*>(p)[i]);
     return static_cast<float>(static_cast<const __bf16*>(p)[i]);
 }
-// V elements from i, a multiple of V, of an array aligned to 16 bytes.
+// V elements from i of an array of feq_dtype dt.
 template <int V>
 __device__ __forceinline__ void load_any_v(const void* p, int dt, int64_t i, float (&o)[V]) {
     if constexpr (V == 1) {

@@ -53,22 +53,25 @@ __device__ __forceinline__ float key_value(uint32_t k) {
     return __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
 }
 
-// Expert of element (chunk c, j) of lane l: chunks of V elements, chunk c of lane l at (c G + l) V.
-template <int V>
-__device__ __forceinline__ int elem_index(int l, int c, int j, int G) { return (c * G + l) * V + j; }
-
-// The row's logits, -inf behind the last expert.
-template <class T, int V, int NC>
-__device__ __forceinline__ void load_row(const T* row, int X, int l, int G, float (&x)[NC][V]) {
+// A lane's logits: NC vectors of V, vector c of lane l at expert at[c] (vec_begin), the first sh[c] of them another
+// lane's (vec_shared).
+template <int V, int NC>
+__device__ __forceinline__ void lane_vectors(int l, int G, int X, int (&at)[NC], int (&sh)[NC]) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-        const int i0 = elem_index<V>(l, c, 0, G);
-        if (i0 + V <= X) {
-            load_f<T, V>(row + i0, x[c]);
-        } else {
+        at[c] = vec_begin<V>(c * G + l, X);
+        sh[c] = vec_shared<V>(c * G + l, X);
+    }
+}
+
+// The row's logits, -inf for those that are not the lane's.
+template <class T, int V, int NC>
+__device__ __forceinline__ void load_row(const T* row, const int (&at)[NC], const int (&sh)[NC], float (&x)[NC][V]) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) x[c][j] = -__builtin_inff();
-        }
+    for (int c = 0; c < NC; ++c) {
+        load_f<T, V>(row + at[c], x[c]);         // at[c] is a vector of the row in every lane
+#pragma unroll
+        for (int j = 0; j < V; ++j) x[c][j] = j >= sh[c] ? x[c][j] : -__builtin_inff();
     }
 }
 
@@ -96,7 +99,7 @@ __device__ __forceinline__ float row_exp(const float (&x)[NC][V], int G, float (
     return group_sum(s, G);
 }
 
-// X is a multiple of V (V = 1 where it is not, or the logits are not aligned for it).  KMAX: the choices are kept
+// X >= V.  KMAX: the choices are kept
 // in registers until the weights' sum is known (K <= KMAX); 0: they wait in memory.
 template <class T, int V, int NC, int KMAX>
 __global__ void __launch_bounds__(kTopkThreads)
@@ -105,6 +108,8 @@ k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normali
     __shared__ float sums[4 * kMaxExperts];
     const int l = threadIdx.x & (G - 1);
     const int per = kTopkThreads / G;
+    int at[NC], sh[NC];
+    lane_vectors<V, NC>(l, G, X, at, sh);
     float mean[NC][V];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -113,9 +118,9 @@ k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normali
     const int64_t stride = static_cast<int64_t>(gridDim.x) * per;
     int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / G;
     float x[NC][V], next[NC][V], e[NC][V];
-    if (r < rows) load_row<T, V, NC>(logits + r * X, X, l, G, x);
+    if (r < rows) load_row<T, V, NC>(logits + r * X, at, sh, x);
     for (; r < rows; r += stride) {
-        if (r + stride < rows) load_row<T, V, NC>(logits + (r + stride) * X, X, l, G, next);   // in flight meanwhile
+        load_row<T, V, NC>(logits + (r + stride < rows ? r + stride : r) * X, at, sh, next);   // in flight meanwhile
         float m;
         const float s = row_exp<V, NC>(x, G, e, m);
         const float inv = s == 0.0f ? 0.0f : 1.0f / s;
@@ -141,10 +146,13 @@ k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normali
             for (int c = NC - 1; c >= 0; --c)
 #pragma unroll
                 for (int j = V - 1; j >= 0; --j) mine = key[c][j] == best ? c * V + j : mine;
-            const uint32_t at = mine < NC * V ? elem_index<V>(l, mine / V, mine % V, G) : 0xffffffffu;
-            const uint32_t first = group_min_u(at, G);
+            uint32_t index = 0xffffffffu;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                if (mine / V == c) index = at[c] + mine % V;
+            const uint32_t first = group_min_u(index, G);
             const bool got = best > kNever;
-            mine = at == first ? mine : NC * V;
+            mine = index == first ? mine : NC * V;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -199,8 +207,7 @@ k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normali
         for (int j = 0; j < V; ++j) {
             float a = mean[c][j];
             for (int o = G; o < 64; o <<= 1) a += __shfl_xor(a, o, 64);
-            const int i = elem_index<V>(l, c, j, G);
-            if (lane < G && i < X) sums[wave * X + i] = a;
+            if (lane < G && j >= sh[c]) sums[wave * X + at[c] + j] = a;
         }
     __syncthreads();
     for (int i = threadIdx.x; i < X; i += kTopkThreads)
@@ -234,14 +241,13 @@ k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const 
            float inv_rows, T* __restrict__ gl, int G) {
     const int l = threadIdx.x & (G - 1);
     const int per = kTopkThreads / G;
+    int at[NC], sh[NC];
+    lane_vectors<V, NC>(l, G, X, at, sh);
     float gm[NC][V];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int i = elem_index<V>(l, c, j, G);
-            gm[c][j] = (gmean && i < X) ? gmean[i] * inv_rows : 0.0f;
-        }
+        for (int j = 0; j < V; ++j) gm[c][j] = (gmean && j >= sh[c]) ? gmean[at[c] + j] * inv_rows : 0.0f;
     const bool full = gmean || (gw && !normalize);      // uniform: the probabilities enter
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / G; r < rows;
          r += static_cast<int64_t>(gridDim.x) * per) {
@@ -254,7 +260,7 @@ k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const 
                 d[c][j] = 0.0f;
             }
         float x[NC][V];
-        if (full) load_row<T, V, NC>(logits + r * X, X, l, G, x);
+        if (full) load_row<T, V, NC>(logits + r * X, at, sh, x);
         if (gw) {
             float dot = 0.0f;
             if (normalize)
@@ -269,7 +275,7 @@ k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const 
                 for (int c = 0; c < NC; ++c)
 #pragma unroll
                     for (int j = 0; j < V; ++j) {
-                        const bool here = elem_index<V>(l, c, j, G) == id;
+                        const bool here = at[c] + j == id && j >= sh[c];
                         if (normalize) d[c][j] += here ? a : 0.0f;
                         else gp[c][j] += here ? a : 0.0f;
                     }
@@ -296,8 +302,14 @@ k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const 
         }
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
-            const int i0 = elem_index<V>(l, c, 0, G);
-            if (i0 + V <= X) store_f<T, V>(gl + r * X + i0, d[c]);
+            T* o = gl + r * X + at[c];
+            if (sh[c] == 0) {
+                store_f<T, V>(o, d[c]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (j >= sh[c]) o[j] = static_cast<T>(d[c][j]);
+            }
         }
     }
 }
@@ -325,11 +337,9 @@ int topk_blocks(int64_t rows, int X) {
 template <class T, class F>
 int with_topk_form(int X, bool vec, F&& f) {
     constexpr int VV = 16 / sizeof(T);
-    if (X <= 512)
-        return vec ? f(std::integral_constant<int, VV>{}, std::integral_constant<int, 8 / VV>{})
-                   : f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});
-    return vec ? f(std::integral_constant<int, VV>{}, std::integral_constant<int, 16 / VV>{})
-               : f(std::integral_constant<int, 1>{}, std::integral_constant<int, 16>{});
+    if (!vec) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});     // fewer experts than a vector
+    return X <= 512 ? f(std::integral_constant<int, VV>{}, std::integral_constant<int, 8 / VV>{})
+                    : f(std::integral_constant<int, VV>{}, std::integral_constant<int, 16 / VV>{});
 }
 
 // ---- plan ------------------------------------------------------------------------
@@ -578,7 +588,7 @@ extern "C" int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t exp
     if (rows) {
         const int rc = with_dtype(dtype, [&](auto t) -> int {
             using T = decltype(t);
-            const bool vec = experts % (16 / sizeof(T)) == 0 && aligned_to(logits, 16);
+            const bool vec = experts >= static_cast<int>(16 / sizeof(T));
             return with_topk_form<T>(experts, vec, [&](auto v, auto nc) -> int {
                 auto run = [&](auto km) -> int {
                     auto kern = k_topk_fwd<T, decltype(v)::value, decltype(nc)::value, decltype(km)::value>;
@@ -610,7 +620,7 @@ extern "C" int feq_expert_topk_bwd(const void* logits, const int64_t* ids, const
     const int64_t blocks = std::min<int64_t>(ceil_div(rows, kTopkThreads / G), 8192);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const bool vec = experts % (16 / sizeof(T)) == 0 && aligned_to(logits, 16) && aligned_to(grad_logits, 16);
+        const bool vec = experts >= static_cast<int>(16 / sizeof(T));
         return with_topk_form<T>(experts, vec, [&](auto v, auto nc) -> int {
             auto kern = k_topk_bwd<T, decltype(v)::value, decltype(nc)::value>;
             FEQ_LAUNCH("k_topk_bwd", kern, dim3(blocks), dim3(kTopkThreads), 0, s, static_cast<const T*>(logits), ids,

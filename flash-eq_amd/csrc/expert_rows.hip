@@ -9,7 +9,8 @@
 //
 // HBM bounds all three.  A group of lanes takes a row t: it reads the row once and writes its K
 // places (or reads K places and writes the row once), where a pass over the slots would read
-// the row K times.  Lanes hold 16-byte vectors, narrower where the width or an address asks for it.
+// the row K times.  Lanes hold 16-byte vectors, of rows of any width and alignment (vec_begin; what two vectors
+// share is written twice, the same); rows shorter than one take narrower ones.
 // Sums over k and over the row are float32 in a fixed order; the result is rounded once.
 #include <algorithm>
 
@@ -30,23 +31,27 @@ int row_lanes(int64_t chunks) {
     return g;
 }
 
-// U: the unit moved (16, 8, 4 or 2 bytes).
-template <class U>
+// V: elements (of 16 bits) moved at a time, at most the width.
+template <int V>
 __global__ void __launch_bounds__(kRowThreads)
-k_rows_dispatch(const U* __restrict__ x, int64_t rows, int K, int64_t chunks, const int32_t* __restrict__ positions,
-                const int32_t* __restrict__ placed, U* __restrict__ xs, int GL) {
+k_rows_dispatch(const uint16_t* __restrict__ x, int64_t rows, int K, int width, const int32_t* __restrict__ positions,
+                const int32_t* __restrict__ placed, uint16_t* __restrict__ xs, int GL) {
+    typedef typename VecOf<uint16_t, V>::type U;
+    typedef typename VecOf<uint16_t, V>::any UA;
+    const int chunks = (width + V - 1) / V;
     const int l = threadIdx.x & (GL - 1);
     const int n = placed[0], per = kRowThreads / GL;
     const int64_t d = blockIdx.y, slots = rows * K;
-    U* out = xs + d * slots * chunks;
+    uint16_t* out = xs + d * slots * width;
     for (int64_t t = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / GL; t < rows;
          t += static_cast<int64_t>(gridDim.x) * per) {
-        const U* xr = x + (d * rows + t) * chunks;
-        for (int64_t c = l; c < chunks; c += GL) {
-            const U v = xr[c];
+        const uint16_t* xr = x + (d * rows + t) * width;
+        for (int q = l; q < chunks; q += GL) {
+            const int c = vec_begin<V>(q, width);
+            const U v = *reinterpret_cast<const UA*>(xr + c);
             for (int k = 0; k < K; ++k) {
                 const int p = positions[t * K + k];
-                out[p * chunks + c] = p < n ? v : U{};
+                *reinterpret_cast<UA*>(out + static_cast<int64_t>(p) * width + c) = p < n ? v : U{};
             }
         }
     }
@@ -55,16 +60,18 @@ k_rows_dispatch(const U* __restrict__ x, int64_t rows, int K, int64_t chunks, co
 // KB: slots whose loads are issued together.
 template <class T, int V, int KB>
 __global__ void __launch_bounds__(kRowThreads)
-k_rows_combine(const T* __restrict__ ys, int64_t rows, int K, int64_t width, const int32_t* __restrict__ positions,
+k_rows_combine(const T* __restrict__ ys, int64_t rows, int K, int width, const int32_t* __restrict__ positions,
                const int32_t* __restrict__ placed, const void* __restrict__ w, int wdt, T* __restrict__ y, int GL) {
     const int l = threadIdx.x & (GL - 1);
     const int n = placed[0], per = kRowThreads / GL;
-    const int64_t d = blockIdx.y, chunks = width / V;
+    const int64_t d = blockIdx.y;
+    const int chunks = (width + V - 1) / V;
     const T* in = ys + d * rows * K * width;
     for (int64_t t = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / GL; t < rows;
          t += static_cast<int64_t>(gridDim.x) * per) {
         T* yr = y + (d * rows + t) * width;
-        for (int64_t c = l; c < chunks; c += GL) {
+        for (int q = l; q < chunks; q += GL) {
+            const int c = vec_begin<V>(q, width);
             float acc[V];
 #pragma unroll
             for (int j = 0; j < V; ++j) acc[j] = 0.0f;
@@ -77,7 +84,7 @@ k_rows_combine(const T* __restrict__ ys, int64_t rows, int K, int64_t width, con
                     const int p = k < K ? positions[t * K + k] : n;
                     on[i] = p < n;
                     wk[i] = (on[i] && w) ? load_any(w, wdt, t * K + k) : 1.0f;
-                    if (on[i]) load_f<T, V>(in + p * width + c * V, v[i]);
+                    if (on[i]) load_f<T, V>(in + static_cast<int64_t>(p) * width + c, v[i]);
                 }
 #pragma unroll
                 for (int i = 0; i < KB; ++i)
@@ -85,7 +92,7 @@ k_rows_combine(const T* __restrict__ ys, int64_t rows, int K, int64_t width, con
 #pragma unroll
                         for (int j = 0; j < V; ++j) acc[j] += wk[i] * v[i][j];
             }
-            store_f<T, V>(yr + c * V, acc);
+            store_f<T, V>(yr + c, acc);
         }
     }
 }
@@ -94,14 +101,15 @@ k_rows_combine(const T* __restrict__ ys, int64_t rows, int K, int64_t width, con
 // q + PS, ...  gys and gw may be NULL (not both).
 template <class T, int V, int KB>
 __global__ void __launch_bounds__(kRowThreads)
-k_rows_combine_bwd(const T* __restrict__ gy, const T* __restrict__ ys, int64_t rows, int K, int64_t width, int planes,
+k_rows_combine_bwd(const T* __restrict__ gy, const T* __restrict__ ys, int64_t rows, int K, int width, int planes,
                    const int32_t* __restrict__ positions, const int32_t* __restrict__ placed,
                    const void* __restrict__ w, int wdt, T* __restrict__ gys, void* __restrict__ gw, int GL, int PS) {
     __shared__ float red[KB][kRowThreads];
     const int l = threadIdx.x & (GL - 1);
     const int group = threadIdx.x / GL, q = group % PS;
     const int n = placed[0], per = kRowThreads / (GL * PS);
-    const int64_t chunks = width / V, slots = rows * K;
+    const int chunks = (width + V - 1) / V;
+    const int64_t slots = rows * K;
     for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * per; t0 < rows; t0 += static_cast<int64_t>(gridDim.x) * per)
     for (int k0 = 0; k0 < K; k0 += KB) {
         const int64_t t = t0 + group / PS;
@@ -120,19 +128,20 @@ k_rows_combine_bwd(const T* __restrict__ gy, const T* __restrict__ ys, int64_t r
                 const T* gr = gy + (d * rows + t) * width;
                 const T* in = ys + d * slots * width;
                 T* out = gys + d * slots * width;
-                for (int64_t c = l; c < chunks; c += GL) {
+                for (int q2 = l; q2 < chunks; q2 += GL) {
+                    const int c = vec_begin<V>(q2, width), shared = vec_shared<V>(q2, width);
                     float g[V];
-                    load_f<T, V>(gr + c * V, g);
+                    load_f<T, V>(gr + c, g);
 #pragma unroll
                     for (int i = 0; i < KB; ++i) {
                         if (p[i] < 0) continue;
-                        const int64_t at = p[i] * width + c * V;
+                        const int64_t at = static_cast<int64_t>(p[i]) * width + c;
                         const bool on = p[i] < n;
                         if (gw && on) {
                             float v[V];
                             load_f<T, V>(in + at, v);
 #pragma unroll
-                            for (int j = 0; j < V; ++j) dot[i] += g[j] * v[j];
+                            for (int j = 0; j < V; ++j) dot[i] += j >= shared ? g[j] * v[j] : 0.0f;
                         }
                         if (gys) {
                             float o[V];
@@ -167,30 +176,23 @@ int rows_check(int64_t planes, int64_t rows, int32_t K, int64_t width, int32_t d
         return fail(FEQ_ERR_INVALID, "%lld planes of %lld rows, %d slots a row, width %lld", (long long)planes,
                     (long long)rows, K, (long long)width);
     if (planes > 65535) return fail(FEQ_ERR_UNSUPPORTED, "more than 65535 planes");
+    if (width > (1 << 29)) return fail(FEQ_ERR_UNSUPPORTED, "rows wider than 2^29");
     if (K > kMaxRowK) return fail(FEQ_ERR_UNSUPPORTED, "more than %d slots a row", kMaxRowK);
     if (rows * K > INT32_MAX) return fail(FEQ_ERR_UNSUPPORTED, "more than 2^31 - 1 slots");
     if (!dtype_ok(dtype)) return fail(FEQ_ERR_INVALID, "unknown element type %d", dtype);
     return FEQ_OK;
 }
 
-// Elements of a vector: 16 bytes where the width and every address allow it, else 1.
-template <class T>
-bool rows_vec_ok(int64_t width, std::initializer_list<const void*> ptrs) {
-    if (width % static_cast<int64_t>(16 / sizeof(T))) return false;
-    for (const void* p : ptrs)
-        if (p && !aligned_to(p, 16)) return false;
-    return true;
-}
-
-template <class U>
-int dispatch_run(const void* x, int64_t planes, int64_t rows, int K, int64_t bytes, const int32_t* positions,
-                 const int32_t* placed, void* xs, hipStream_t s) {
-    const int64_t chunks = bytes / static_cast<int64_t>(sizeof(U));
-    const int GL = row_lanes(chunks);
-    auto kern = k_rows_dispatch<U>;
-    FEQ_LAUNCH("k_rows_dispatch", kern, dim3(std::min(ceil_div(rows, kRowThreads / GL), kMaxRowBlocks), planes), dim3(kRowThreads), 0, s,
-               static_cast<const U*>(x), rows, K, chunks, positions, placed, static_cast<U*>(xs), GL);
-    return FEQ_OK;
+// f(V) for the vector of a row of `width` elements: 16 bytes, less where the row has less.
+template <class T, class F>
+int with_row_vec(int64_t width, F&& f) {
+    constexpr int VV = 16 / sizeof(T);
+    if (width >= VV) return f(std::integral_constant<int, VV>{});
+    if constexpr (VV == 8) {
+        if (width >= 4) return f(std::integral_constant<int, 4>{});
+    }
+    if (width >= 2) return f(std::integral_constant<int, 2>{});
+    return f(std::integral_constant<int, 1>{});
 }
 
 }  // namespace
@@ -205,12 +207,17 @@ extern "C" int feq_expert_dispatch(const void* x, int64_t planes, int64_t rows, 
     if (rows == 0) return FEQ_OK;
     if (!x || !positions || !placed || !xs) return fail(FEQ_ERR_INVALID, "NULL pointer");
     hipStream_t s = stream_of(stream);
-    const int64_t bytes = width * elem_size(dtype);
-    auto fits = [&](int64_t u) { return bytes % u == 0 && aligned_to(x, u) && aligned_to(xs, u); };
-    if (fits(16)) return dispatch_run<uint4>(x, planes, rows, top_k, bytes, positions, placed, xs, s);
-    if (fits(8)) return dispatch_run<uint2>(x, planes, rows, top_k, bytes, positions, placed, xs, s);
-    if (fits(4)) return dispatch_run<uint32_t>(x, planes, rows, top_k, bytes, positions, placed, xs, s);
-    return dispatch_run<uint16_t>(x, planes, rows, top_k, bytes, positions, placed, xs, s);
+    // moved as 16-bit units
+    const int units = static_cast<int>(width) * (elem_size(dtype) / 2);
+    return with_row_vec<uint16_t>(units, [&](auto v) -> int {
+        constexpr int V = decltype(v)::value;
+        const int GL = row_lanes(ceil_div(units, V));
+        auto kern = k_rows_dispatch<V>;
+        FEQ_LAUNCH("k_rows_dispatch", kern, dim3(std::min(ceil_div(rows, kRowThreads / GL), kMaxRowBlocks), planes),
+                   dim3(kRowThreads), 0, s, static_cast<const uint16_t*>(x), rows, top_k, units, positions, placed,
+                   static_cast<uint16_t*>(xs), GL);
+        return FEQ_OK;
+    });
 }
 
 extern "C" int feq_expert_combine(const void* ys, int64_t planes, int64_t rows, int32_t top_k, int64_t width,
@@ -225,11 +232,11 @@ extern "C" int feq_expert_combine(const void* ys, int64_t planes, int64_t rows, 
         using T = decltype(tt);
         auto run = [&](auto v, auto kb) -> int {
             constexpr int V = decltype(v)::value, KB = decltype(kb)::value;
-            const int GL = row_lanes(width / V);
+            const int GL = row_lanes(ceil_div(width, V));
             auto kern = k_rows_combine<T, V, KB>;
             FEQ_LAUNCH("k_rows_combine", kern, dim3(std::min(ceil_div(rows, kRowThreads / GL), kMaxRowBlocks), planes), dim3(kRowThreads), 0, s,
-                       static_cast<const T*>(ys), rows, top_k, width, positions, placed, weights, weight_dtype,
-                       static_cast<T*>(y), GL);
+                       static_cast<const T*>(ys), rows, top_k, static_cast<int>(width), positions, placed, weights,
+                       weight_dtype, static_cast<T*>(y), GL);
             return FEQ_OK;
         };
         auto with_kb = [&](auto v) -> int {
@@ -237,8 +244,7 @@ extern "C" int feq_expert_combine(const void* ys, int64_t planes, int64_t rows, 
             if (top_k == 2) return run(v, std::integral_constant<int, 2>{});
             return run(v, std::integral_constant<int, 4>{});
         };
-        return rows_vec_ok<T>(width, {ys, y}) ? with_kb(std::integral_constant<int, 16 / sizeof(T)>{})
-                                              : with_kb(std::integral_constant<int, 1>{});
+        return with_row_vec<T>(width, with_kb);
     });
 }
 
@@ -255,14 +261,14 @@ extern "C" int feq_expert_combine_bwd(const void* grad_y, const void* ys, int64_
         using T = decltype(tt);
         auto run = [&](auto v, auto kb) -> int {
             constexpr int V = decltype(v)::value, KB = decltype(kb)::value;
-            const int GL = row_lanes(width / V);
+            const int GL = row_lanes(ceil_div(width, V));
             // groups of a row: as many as fill the chip (eight waves a SIMD), no more than planes.  20000 rows of 9
             // planes, 64 float32 columns: one group 43 us, sixteen (seven of them idle) 83
             int PS = 1;
             while (PS * 2 <= planes && GL * PS * 2 <= kRowThreads && rows * GL * PS < 64 * 8192) PS <<= 1;
             auto kern = k_rows_combine_bwd<T, V, KB>;
             FEQ_LAUNCH("k_rows_combine_bwd", kern, dim3(std::min(ceil_div(rows, kRowThreads / (GL * PS)), kMaxRowBlocks)), dim3(kRowThreads), 0,
-                       s, static_cast<const T*>(grad_y), static_cast<const T*>(ys), rows, top_k, width,
+                       s, static_cast<const T*>(grad_y), static_cast<const T*>(ys), rows, top_k, static_cast<int>(width),
                        static_cast<int>(planes), positions, placed, weights, weight_dtype, static_cast<T*>(grad_ys),
                        grad_weights, GL, PS);
             return FEQ_OK;
@@ -272,7 +278,6 @@ extern "C" int feq_expert_combine_bwd(const void* grad_y, const void* ys, int64_
             if (top_k == 2) return run(v, std::integral_constant<int, 2>{});
             return run(v, std::integral_constant<int, 4>{});
         };
-        return rows_vec_ok<T>(width, {grad_y, ys, grad_ys}) ? with_kb(std::integral_constant<int, 16 / sizeof(T)>{})
-                                                            : with_kb(std::integral_constant<int, 1>{});
+        return with_row_vec<T>(width, with_kb);
     });
 }

@@ -52,7 +52,7 @@ __device__ __forceinline__ void block_sum2(float& a, float& b, float* red) {
     }
 }
 
-// Vectors of V elements; lane `l` of a group of `G` holds vectors l, l + G, ...
+// Vectors of V elements (width >= V; vec_begin, vec_shared); lane `l` of a group of `G` holds vectors l, l + G, ...
 template <class T, int V, int NV, bool BLK>
 __global__ void __launch_bounds__(kLnThreads)
 k_ln_fwd(const T* __restrict__ x, int64_t rows, int width, int64_t ldx, const void* __restrict__ w,
@@ -63,56 +63,49 @@ k_ln_fwd(const T* __restrict__ x, int64_t rows, int width, int64_t ldx, const vo
     const int l = threadIdx.x & (L - 1);
     const int per = kLnThreads / L;
     const int64_t stride = static_cast<int64_t>(gridDim.x) * per;
-    const int nvec = width / V;
+    const int nvec = (width + V - 1) / V;
     const float inv = 1.0f / static_cast<float>(width);
     float wv[NV][V], bv[NV][V];
+    int at[NV], sh[NV];      // a vector's first column, and how many of its columns the vector before has
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int q = l + v * L;
+        at[v] = vec_begin<V>(q, width);
+        sh[v] = vec_shared<V>(q, width);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             wv[v][j] = 1.0f;
             bv[v][j] = 0.0f;
         }
-        if (w && q < nvec) load_any_v<V>(w, pdt, static_cast<int64_t>(q) * V, wv[v]);
-        if (b && q < nvec) load_any_v<V>(b, pdt, static_cast<int64_t>(q) * V, bv[v]);
+        if (w && q < nvec) load_any_v<V>(w, pdt, at[v], wv[v]);
+        if (b && q < nvec) load_any_v<V>(b, pdt, at[v], bv[v]);
     }
     float xv[NV][V], xn[NV][V];
     auto load = [&](int64_t r, float (&o)[NV][V]) {
         const T* xr = x + r * ldx;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const int q = l + v * L;
-            if (q < nvec) {
-                load_f<T, V>(xr + static_cast<int64_t>(q) * V, o[v]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) o[v][j] = 0.0f;
-            }
-        }
+        for (int v = 0; v < NV; ++v) load_f<T, V>(xr + at[v], o[v]);     // a vector of the row in every lane
     };
     int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / L;
     if (r < rows) load(r, xv);
     for (; r < rows; r += stride) {
-        if (r + stride < rows) load(r + stride, xn);      // the next row, in flight during this one's sums
+        load(r + stride < rows ? r + stride : r, xn);     // the next row, in flight during this one's sums
         float s = 0.0f, z = 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
-            for (int j = 0; j < V; ++j) s += xv[v][j];
+            for (int j = 0; j < V; ++j) s += j >= sh[v] ? xv[v][j] : 0.0f;
         if constexpr (BLK) block_sum2<4>(s, z, red);
         else s = group_sum(s, G);
         const float mu = s * inv;
         float q2 = 0.0f;
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const bool in = l + v * L < nvec;
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 xv[v][j] -= mu;
-                q2 += in ? xv[v][j] * xv[v][j] : 0.0f;
+                q2 += j >= sh[v] ? xv[v][j] * xv[v][j] : 0.0f;
             }
-        }
         if constexpr (BLK) block_sum2<4>(q2, z, red);
         else q2 = group_sum(q2, G);
         const float rs = 1.0f / sqrtf(q2 * inv + eps);
@@ -124,7 +117,7 @@ k_ln_fwd(const T* __restrict__ x, int64_t rows, int width, int64_t ldx, const vo
                 float o[V];
 #pragma unroll
                 for (int j = 0; j < V; ++j) o[j] = xv[v][j] * rs * wv[v][j] + bv[v][j];
-                store_f<T, V>(yr + static_cast<int64_t>(q) * V, o);
+                store_f<T, V>(yr + at[v], o);
             }
         }
         if (l == 0 && mean) {
@@ -152,18 +145,21 @@ k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t
     const int l = threadIdx.x & (L - 1);
     const int per = kLnThreads / L;
     const int64_t stride = static_cast<int64_t>(gridDim.x) * per;
-    const int nvec = width / V;
+    const int nvec = (width + V - 1) / V;
     const float inv = 1.0f / static_cast<float>(width);
     float wv[NV][V], dw[NV][V], db[NV][V];
+    int at[NV], sh[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int q = l + v * L;
+        at[v] = vec_begin<V>(q, width);
+        sh[v] = vec_shared<V>(q, width);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             wv[v][j] = 1.0f;
             dw[v][j] = db[v][j] = 0.0f;
         }
-        if (w && q < nvec) load_any_v<V>(w, pdt, static_cast<int64_t>(q) * V, wv[v]);
+        if (w && q < nvec) load_any_v<V>(w, pdt, at[v], wv[v]);
     }
     for (int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / L; r < rows; r += stride) {
         const T* xr = x + r * ldx;
@@ -173,17 +169,8 @@ k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t
         float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
-            const int q = l + v * L;
-            if (q < nvec) {
-                load_f<T, V>(xr + static_cast<int64_t>(q) * V, xh[v]);
-                load_f<T, V>(gr + static_cast<int64_t>(q) * V, h[v]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    xh[v][j] = mu;
-                    h[v][j] = 0.0f;
-                }
-            }
+            load_f<T, V>(xr + at[v], xh[v]);
+            load_f<T, V>(gr + at[v], h[v]);
         }
 #pragma unroll
         for (int v = 0; v < NV; ++v)
@@ -193,8 +180,8 @@ k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t
                 dw[v][j] += h[v][j] * xh[v][j];
                 db[v][j] += h[v][j];
                 h[v][j] *= wv[v][j];
-                s1 += h[v][j];
-                s2 += h[v][j] * xh[v][j];
+                s1 += j >= sh[v] ? h[v][j] : 0.0f;
+                s2 += j >= sh[v] ? h[v][j] * xh[v][j] : 0.0f;
             }
         if (gx) {
             if constexpr (BLK) block_sum2<4>(s1, s2, red);
@@ -212,7 +199,7 @@ k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t
                     float o[V];
 #pragma unroll
                     for (int j = 0; j < V; ++j) o[j] = rs * (h[v][j] - s1 - xh[v][j] * s2);
-                    store_f<T, V>(dr + static_cast<int64_t>(q) * V, o);
+                    store_f<T, V>(dr + at[v], o);
                 }
             }
         }
@@ -224,10 +211,9 @@ k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const int c = (l + v * L) * V + j;
-                if (c < width) {
-                    pw[c] = dw[v][j];
-                    pw[width + c] = db[v][j];
+                if (j >= sh[v]) {
+                    pw[at[v] + j] = dw[v][j];
+                    pw[width + at[v] + j] = db[v][j];
                 }
             }
     } else {
@@ -251,11 +237,12 @@ k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t
             }
         __syncthreads();
         for (int c = threadIdx.x; c < width; c += kLnThreads) {
+            const int last = (nvec - 1) * V, place = c < last ? c : last + c - (width - V);
             float a = 0.0f, d = 0.0f;
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                a += sums[(u * cols + c) * 2];
-                d += sums[(u * cols + c) * 2 + 1];
+                a += sums[(u * cols + place) * 2];
+                d += sums[(u * cols + place) * 2 + 1];
             }
             pw[c] = a;
             pw[width + c] = d;
@@ -383,7 +370,12 @@ inline int ln_nv(int64_t n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 3 ? 3 : n <=
 
 LnForm ln_form(int64_t width, int V) {
     LnForm f{false, false, 64, 1};
-    const int64_t nvec = width / V;
+    const int64_t nvec = ceil_div(width, V);
+    if (V == 1) {                // a column a lane: fewer columns than a vector
+        f.G = 1;
+        while (f.G < nvec) f.G <<= 1;
+        return f;
+    }
     for (int g = 1; g <= 64; g <<= 1) {
         const int nv = ln_nv(ceil_div(nvec, g));
         if (nv * V <= kLnWaveElems) {
@@ -398,20 +390,10 @@ LnForm ln_form(int64_t width, int V) {
     return f;
 }
 
-template <class T>
-bool ln_vec_ok(int64_t width, std::initializer_list<int64_t> lds, std::initializer_list<const void*> ptrs) {
-    constexpr int V = 16 / sizeof(T);
-    if (width % V) return false;
-    for (int64_t l : lds)
-        if (l % V) return false;
-    for (const void* p : ptrs)
-        if (p && !aligned_to(p, 16)) return false;
-    return true;
-}
-
-// f(integral constants V, NV) for the instance that holds `nv` vectors
+// f(NV) for the instance that holds `nv` vectors a lane
 template <int V, class F>
 int ln_with_nv(int nv, F&& f) {
+    if constexpr (V == 1) return f(std::integral_constant<int, 1>{});       // rows narrower than a vector
     switch (nv) {
         case 1: return f(std::integral_constant<int, 1>{});
         case 2: return f(std::integral_constant<int, 2>{});
@@ -496,7 +478,7 @@ extern "C" int feq_layernorm_fwd(const void* x, int64_t rows, int64_t width, int
         constexpr int VV = 16 / sizeof(T);
         const T* xt = static_cast<const T*>(x);
         T* yt = static_cast<T*>(y);
-        const bool vec = ln_vec_ok<T>(width, {ldx}, {x, y, weight, bias});
+        const bool vec = width >= VV;
         const LnForm f = ln_form(width, vec ? VV : 1);
         if (f.wide) {
             auto kern = k_ln_fwd_wide<T>;
@@ -538,7 +520,7 @@ extern "C" int feq_layernorm_bwd(const void* grad_y, int64_t ldg, const void* x,
             constexpr int VV = 16 / sizeof(T);
             const T *gt = static_cast<const T*>(grad_y), *xt = static_cast<const T*>(x);
             T* dt = static_cast<T*>(grad_x);
-            const bool vec = ln_vec_ok<T>(width, {ldx, ldg}, {x, grad_y, grad_x, weight});
+            const bool vec = width >= VV;
             const LnForm f = ln_form(width, vec ? VV : 1);
             if (f.wide) {
                 if (dt) {
