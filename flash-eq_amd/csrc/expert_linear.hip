@@ -125,13 +125,37 @@ __device__ __forceinline__ Table table(const void* p, bool there = true) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, there ? kTableBytes : 0u, 0x00020000);
 }
 
-// 16 bytes of T at byte offset `at` (below 2^31) of the table, of which the first `n` elements exist (n <= 0: none);
-// the others are 0.  VEC: n is a multiple of the 16 bytes.  ONCE: read past the caches.
-template <class T, bool VEC, bool ONCE = false>
-__device__ __forceinline__ uint4 load16(Table t, uint32_t at, int n) {
+// How the rows of a table lie: multiples of 16 bytes, aligned to them (kWhole); of any length of at least 16 bytes and
+// any alignment (kRagged); shorter (kNarrow).
+enum { kWhole, kRagged, kNarrow };
+
+// Rows read in vectors of V elements from multiples of V on.  The last vector of a ragged row (`n` of its elements
+// exist, 0 < n < V) is read from `short_by` = V - n elements before its place, inside the row, and shifted to it
+// when it has arrived (arrived16); an absent one from `safe`, any 16 bytes of the table.
+struct Rows {
+    Table t;
+    const char* base;
+    const char* safe;
+    int short_by;
+};
+template <class T>
+__device__ __forceinline__ Rows rows_at(const T* base, const T* safe, int length) {
+    constexpr int V = 16 / sizeof(T);
+    return Rows{table(base), reinterpret_cast<const char*>(base), reinterpret_cast<const char*>(safe), V - length % V};
+}
+
+// The vector at byte offset `at` (below 2^31) of the rows, of which the first `n` elements exist (n <= 0: none).
+// ONCE: read past the caches.
+template <class T, int HOW, bool ONCE = false>
+__device__ __forceinline__ uint4 load16(const Rows& rows, int at, int n) {
     constexpr int V = 16 / sizeof(T), kPast = ONCE ? 2 : 0;
-    if constexpr (VEC) {
+    const Table t = rows.t;
+    if constexpr (HOW == kWhole) {
         return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(t, n > 0 ? at : kOutside, 0, kPast));
+    } else if constexpr (HOW == kRagged) {
+        const char* p = rows.base + (n < V ? at - rows.short_by * static_cast<int>(sizeof(T)) : at);
+        const typename VecOf<T, V>::type v = *reinterpret_cast<const typename VecOf<T, V>::any*>(n > 0 ? p : rows.safe);
+        return __builtin_bit_cast(uint4, v);
     } else if constexpr (sizeof(T) == 4) {
         uint4 v;
         v.x = __builtin_amdgcn_raw_buffer_load_b32(t, n > 0 ? at : kOutside, 0, kPast);
@@ -146,6 +170,30 @@ __device__ __forceinline__ uint4 load16(Table t, uint32_t at, int n) {
         for (int j = 0; j < V; ++j) v[j] = __builtin_amdgcn_raw_buffer_load_b16(t, n > j ? at + 2 * j : kOutside, 0, kPast);
         return __builtin_bit_cast(uint4, v);
     }
+}
+
+// What load16 returned with its elements in place and zeros for those that do not exist.
+template <class T, int HOW>
+__device__ __forceinline__ uint4 arrived16(const Rows& rows, uint4 v, int n) {
+    if constexpr (HOW == kRagged) {
+        constexpr int V = 16 / sizeof(T);
+        const int s = rows.short_by;             // uniform: 1 .. V - 1, or V where no row has a short vector
+        uint4 z = v;
+        if constexpr (sizeof(T) == 2) {
+            if (s & 4) z = uint4{z.z, z.w, 0, 0};
+            if (s & 2) z = uint4{z.y, z.z, z.w, 0};
+            if (s & 1) z = uint4{z.x >> 16 | z.y << 16, z.y >> 16 | z.z << 16, z.z >> 16 | z.w << 16, z.w >> 16};
+        } else {
+            if (s & 2) z = uint4{z.z, z.w, 0, 0};
+            if (s & 1) z = uint4{z.y, z.z, z.w, 0};
+        }
+        const bool none = n <= 0, part = n < V;
+        v.x = none ? 0 : part ? z.x : v.x;
+        v.y = none ? 0 : part ? z.y : v.y;
+        v.z = none ? 0 : part ? z.z : v.z;
+        v.w = none ? 0 : part ? z.w : v.w;
+    }
+    return v;
 }
 
 // One element as float32, 0 where it does not exist.
@@ -183,16 +231,15 @@ __device__ __forceinline__ void put_dealt(T* row, int n, uint4 v) {
 }
 
 // A lane's V columns of a tile group (accumulators of tile u at acc[u STEP]) to o, of which `n` exist.
-template <class T, bool VEC, int STEP>
+template <class T, int HOW, int STEP>
 __device__ __forceinline__ void store_tiles(T* o, int n, const v4f* acc) {
     constexpr int V = 16 / sizeof(T);
-    if constexpr (VEC) {
-        if (n <= 0) return;
+    if (HOW == kWhole ? n > 0 : n >= V) {
         float f[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) f[v] = acc[v / 4 * STEP][v % 4];
         store_f<T, V>(o, f);
-    } else {
+    } else if constexpr (HOW != kWhole) {
 #pragma unroll
         for (int v = 0; v < V; ++v)
             if (v < n) o[v] = static_cast<T>(acc[v / 4 * STEP][v % 4]);
@@ -276,7 +323,7 @@ inline int64_t xcd_grid(int64_t bound, int64_t subs) { return 8 * ceil_div(bound
 // out[d, p, :] = in[d, p, :] B (+ bias), B = W[e, r]^T (TRANS false: in has Cin columns, out Cout) or W[e, r]
 // (TRANS: in has Cout columns, out Cin).  K: columns of in, N: of out; W rows have wld = Cin elements.
 // WR: waves along the output columns (64 each), 4 / WR along the rows.
-template <class T, bool VEC, bool TRANS, int WR>
+template <class T, int HOW, bool TRANS, int WR>
 __global__ void __launch_bounds__(kXlThreads, 2)
 k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,
         int N, int nreps, XlMap map, const T* __restrict__ bias, int nbias, T* __restrict__ out) {
@@ -301,39 +348,46 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wc = wave / WR;
     const bool none = t.expert == X;                 // uniform: rows without an expert
-    const Table rows_in = table(in + (static_cast<int64_t>(d) * S + t.row0) * K);
+    const Rows rows_in = rows_at(in + (static_cast<int64_t>(d) * S + t.row0) * K, in, K);
     const T* we = W + (static_cast<int64_t>(none ? 0 : t.expert) * nreps + __builtin_amdgcn_readfirstlane(map.rep[d])) * K * N;
 
     auto load = [&](int k0, uint4 (&vin)[NIN], uint4 (&vw)[NW]) {
 #pragma unroll
         for (int i = 0; i < NIN; ++i) {
             const int q = tid + kXlThreads * i, r = q / CH, k = k0 + (q % CH) * V;
-            vin[i] = load16<T, VEC>(rows_in, (r * K + k) * sizeof(T), r < rows ? K - k : 0);
+            vin[i] = load16<T, HOW>(rows_in, (r * K + k) * static_cast<int>(sizeof(T)), r < rows ? K - k : 0);
         }
-        const Table w = table(TRANS ? we + static_cast<int64_t>(k0) * N + n0 : we + static_cast<int64_t>(n0) * K);
+        const Rows w = rows_at(TRANS ? we + static_cast<int64_t>(k0) * N + n0 : we + static_cast<int64_t>(n0) * K, W, TRANS ? N : K);
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             const int q = tid + kXlThreads * i;
             if constexpr (TRANS) {                   // W rows are k, columns n
                 const int r = q / (BN / V), n = (q % (BN / V)) * V;
-                vw[i] = load16<T, VEC>(w, (r * N + n) * sizeof(T), k0 + r < K ? N - n0 - n : 0);
+                vw[i] = load16<T, HOW>(w, (r * N + n) * static_cast<int>(sizeof(T)), k0 + r < K ? N - n0 - n : 0);
             } else {
                 const int r = q / CH, k = k0 + (q % CH) * V;
-                vw[i] = load16<T, VEC>(w, (r * K + k) * sizeof(T), n0 + r < N ? K - k : 0);
+                vw[i] = load16<T, HOW>(w, (r * K + k) * static_cast<int>(sizeof(T)), n0 + r < N ? K - k : 0);
             }
         }
     };
-    auto stage = [&](int u, const uint4 (&vin)[NIN], const uint4 (&vw)[NW]) {
+    const Rows w_rows = rows_at(W, W, TRANS ? N : K);
+    auto stage = [&](int u, int k0, const uint4 (&vin)[NIN], const uint4 (&vw)[NW]) {
 #pragma unroll
         for (int i = 0; i < NIN; ++i) {
-            const int q = tid + kXlThreads * i;
-            *reinterpret_cast<uint4*>(sIn[u] + (q / CH) * LD + (q % CH) * V) = vin[i];
+            const int q = tid + kXlThreads * i, r = q / CH, k = (q % CH) * V;
+            *reinterpret_cast<uint4*>(sIn[u] + r * LD + k) = arrived16<T, HOW>(rows_in, vin[i], r < rows ? K - k0 - k : 0);
         }
 #pragma unroll
         for (int i = 0; i < NW; ++i) {
             const int q = tid + kXlThreads * i;
-            if constexpr (TRANS) put_dealt<T>(sW[u] + (q / (BN / V)) * LDT, (q % (BN / V)) * V, vw[i]);
-            else *reinterpret_cast<uint4*>(sW[u] + dealt<T>(q / CH) * LD + (q % CH) * V) = vw[i];
+            if constexpr (TRANS) {
+                const int r = q / (BN / V), n = (q % (BN / V)) * V;
+                put_dealt<T>(sW[u] + r * LDT, n, arrived16<T, HOW>(w_rows, vw[i], k0 + r < K ? N - n0 - n : 0));
+            } else {
+                const int r = q / CH, k = (q % CH) * V;
+                *reinterpret_cast<uint4*>(sW[u] + dealt<T>(r) * LD + k) =
+                    arrived16<T, HOW>(w_rows, vw[i], n0 + r < N ? K - k0 - k : 0);
+            }
         }
     };
 
@@ -357,7 +411,7 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
     // after it
     uint4 vin[NIN], vw[NW];
     auto step = [&](int k0, int u) {
-        stage(u ^ 1, vin, vw);
+        stage(u ^ 1, k0 + BK, vin, vw);
         load(k0 + 2 * BK, vin, vw);                  // nothing behind K
 #pragma unroll
         for (int ks = 0; ks < BK; ks += M::KS) {
@@ -380,7 +434,7 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
     };
     if (!none) {
         load(0, vin, vw);
-        stage(0, vin, vw);
+        stage(0, 0, vin, vw);
         load(BK, vin, vw);
         __syncthreads();
         for (int k0 = 0; k0 < K; k0 += 2 * BK) {
@@ -395,7 +449,7 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
 #pragma unroll
         for (int j = 0; j < PT; ++j) {
             const int r = 16 * (wc * PT + j) + c;
-            if (r < rows) store_tiles<T, VEC, PT>(od + static_cast<int64_t>(r) * N + n, N - n, &acc[i][j]);
+            if (r < rows) store_tiles<T, HOW, PT>(od + static_cast<int64_t>(r) * N + n, N - n, &acc[i][j]);
         }
     }
 }
@@ -407,8 +461,8 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
 // in the matrix cores' layout (lane (c, g): FE elements of row c), the next block's rows in flight during this
 // one's products.  Nothing but the weight passes through LDS and no barrier stands between blocks of an
 // expert.  NS: reduction steps held (K <= NS KS).
-template <class T, bool VEC, bool TRANS, int NB, int NS>
-__global__ void __launch_bounds__(kXlThreads, NB * NS * Mma<T>::KS * sizeof(T) > 40000 ? 2 : NS == 8 ? 3 : 4)
+template <class T, int HOW, bool TRANS, int NB, int NS>
+__global__ void __launch_bounds__(kXlThreads, NB * NS * Mma<T>::KS * sizeof(T) > 40000 ? 2 : NS == 8 || HOW != kWhole ? 3 : 4)
 k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,
             int N, int nreps, XlMap map, int dim, const T* __restrict__ bias, int nbias, T* __restrict__ out) {
     using M = Mma<T>;
@@ -435,14 +489,22 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
         const T* id = in + (static_cast<int64_t>(d) * S + row0) * K;
         T* od = out + (static_cast<int64_t>(d) * S + row0) * N + n0;
 
+        frag b0[NS], b1[NS];
         auto load = [&](int blk, frag (&b)[NS]) {
-            const Table p = table(id + static_cast<int64_t>(16 * blk) * K);
+            const Rows p = rows_at(id + static_cast<int64_t>(16 * blk) * K, in, K);
             const bool there = 16 * blk + c < rows;
 #pragma unroll
             for (int ks = 0; ks < NS; ++ks) {
                 const int k = ks * M::KS + M::FE * g;
-                b[ks] = __builtin_bit_cast(frag, load16<T, VEC>(p, (c * K + k) * sizeof(T), there ? K - k : 0));
+                b[ks] = __builtin_bit_cast(frag, load16<T, HOW>(p, (c * K + k) * static_cast<int>(sizeof(T)), there ? K - k : 0));
             }
+        };
+        auto arrived = [&](int blk, const frag (&b)[NS]) {
+            const Rows p = rows_at(in, in, K);
+#pragma unroll
+            for (int ks = 0; ks < NS; ++ks)
+                b0[ks] = __builtin_bit_cast(frag, arrived16<T, HOW>(p, __builtin_bit_cast(uint4, b[ks]),
+                                                                    16 * blk + c < rows ? K - ks * M::KS - M::FE * g : 0));
         };
         auto store = [&](int blk, const v4f (&acc)[NT]) {
             const int r = 16 * blk + c;
@@ -451,7 +513,7 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
 #pragma unroll
             for (int i = 0; i < NT; i += kDealt<T>) {
                 const int n = 16 * i + V * g;
-                store_tiles<T, VEC, 1>(o + n, N - n0 - n, &acc[i]);
+                store_tiles<T, HOW, 1>(o + n, N - n0 - n, &acc[i]);
             }
         };
         if (expert == X) {                           // rows without an expert
@@ -461,21 +523,23 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
             for (int blk = wave; blk < nblocks; blk += 4) store(blk, zero);
             continue;
         }
-        frag b0[NS], b1[NS];
-        load(wave, b0);                              // nothing behind the last row
+        load(wave, b1);                              // nothing behind the last row
         __syncthreads();                             // the last expert's weight has been read
         const T* wm = W + (static_cast<int64_t>(expert) * nreps + __builtin_amdgcn_readfirstlane(map.rep[d])) * K * N;
-        const Table we = table(TRANS ? wm + n0 : wm + static_cast<int64_t>(n0) * K);
+        const Rows we = rows_at(TRANS ? wm + n0 : wm + static_cast<int64_t>(n0) * K, W, TRANS ? N : K);
 #pragma unroll
         for (int i = 0; i < KM * NB / V / kXlThreads; ++i) {
             const int q = tid + kXlThreads * i;
             if constexpr (TRANS) {
                 const int k = q / (NB / V), n = (q % (NB / V)) * V;
-                put_dealt<T>(sW + k * LDT, n, load16<T, VEC>(we, (k * N + n) * sizeof(T), k < K ? N - n0 - n : 0));
+                const int there = k < K ? N - n0 - n : 0;
+                put_dealt<T>(sW + k * LDT, n,
+                             arrived16<T, HOW>(we, load16<T, HOW>(we, (k * N + n) * static_cast<int>(sizeof(T)), there), there));
             } else {
                 const int n = q / (KM / V), k = (q % (KM / V)) * V;
+                const int there = n0 + n < N ? K - k : 0;
                 *reinterpret_cast<uint4*>(sW + dealt<T>(n) * LD + k) =
-                    load16<T, VEC>(we, (n * K + k) * sizeof(T), n0 + n < N ? K - k : 0);
+                    arrived16<T, HOW>(we, load16<T, HOW>(we, (n * K + k) * static_cast<int>(sizeof(T)), there), there);
             }
         }
         const int bc = __builtin_amdgcn_readfirstlane(map.bcol[d]);
@@ -484,6 +548,7 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
             sBias[tid] = load1<T>(table(biased ? bias + static_cast<int64_t>(expert) * N * nbias : nullptr, biased),
                                   ((n0 + tid) * nbias + bc) * sizeof(T), n0 + tid < N);
         __syncthreads();
+        arrived(wave, b1);
         for (int blk = wave; blk < nblocks; blk += 4) {
             load(blk + 4, b1);                       // nothing behind the last row
             // the weight is read from LDS for every block: kept in registers it would take them from the rows in flight
@@ -506,8 +571,7 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
                 }
             }
             store(blk, acc);
-#pragma unroll
-            for (int ks = 0; ks < NS; ++ks) b0[ks] = b1[ks];
+            arrived(blk + 4, b1);
         }
     }
 }
@@ -519,7 +583,7 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
 // ONCE: one tile covers the weight, so every row is read once; the rows then go past the caches, which leaves them to
 // the kernels around (20011 x 49 bfloat16 rows, 128 x 128: 137 -> 97 us, and with both maps a pass 376 -> 353).  Rows
 // that several tiles read lose by it (42 -> 52 us for 512 x 1024).
-template <class T, bool VEC, int WR, bool ONCE>
+template <class T, int HOW, int WR, bool ONCE>
 __global__ void __launch_bounds__(kXlThreads)
 k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __restrict__ offsets, int X, int S,
            int ci, int co, int nreps, XlMap map, XlChunks ch, T* __restrict__ gw, T* __restrict__ gb, int nbias,
@@ -552,17 +616,17 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
     auto load = [&](int it) {
         const int d = it < total ? d0 + it / steps : d0, r0 = t.row0 + (it % steps) * BP;
         const int64_t base = static_cast<int64_t>(d) * S + r0;
-        const Table tx = table(x + base * ci + k0), tg = table(gy + base * co + n0);
+        const Rows tx = rows_at(x + base * ci + k0, x, ci), tg = rows_at(gy + base * co + n0, gy, co);
         const int there = it < total ? rend - r0 : 0;
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
             const int q = tid + kXlThreads * i, r = q / (BK / V), k = (q % (BK / V)) * V;
-            vx[i] = load16<T, VEC, ONCE>(tx, (r * ci + k) * sizeof(T), r < there ? ci - k0 - k : 0);
+            vx[i] = load16<T, HOW, ONCE>(tx, (r * ci + k) * static_cast<int>(sizeof(T)), r < there ? ci - k0 - k : 0);
         }
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
             const int q = tid + kXlThreads * i, r = q / (BN / V), n = (q % (BN / V)) * V;
-            vg[i] = load16<T, VEC, ONCE>(tg, (r * co + n) * sizeof(T), r < there ? co - n0 - n : 0);
+            vg[i] = load16<T, HOW, ONCE>(tg, (r * co + n) * static_cast<int>(sizeof(T)), r < there ? co - n0 - n : 0);
         }
     };
     v4f acc[4][NT];
@@ -574,15 +638,17 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
     if (total) load(0);
     for (int it = 0; it < total; ++it) {
         __syncthreads();
+        const int there = rend - (t.row0 + (it % steps) * BP);
+        const Rows tx = rows_at(x, x, ci), tg = rows_at(gy, gy, co);
 #pragma unroll
         for (int i = 0; i < NX; ++i) {
-            const int q = tid + kXlThreads * i;
-            put_dealt<T>(sX + (q / (BK / V)) * LX, (q % (BK / V)) * V, vx[i]);
+            const int q = tid + kXlThreads * i, r = q / (BK / V), k = (q % (BK / V)) * V;
+            put_dealt<T>(sX + r * LX, k, arrived16<T, HOW>(tx, vx[i], r < there ? ci - k0 - k : 0));
         }
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
-            const int q = tid + kXlThreads * i;
-            *reinterpret_cast<uint4*>(sG + (q / (BN / V)) * LG + (q % (BN / V)) * V) = vg[i];
+            const int q = tid + kXlThreads * i, r = q / (BN / V), n = (q % (BN / V)) * V;
+            *reinterpret_cast<uint4*>(sG + r * LG + n) = arrived16<T, HOW>(tg, vg[i], r < there ? co - n0 - n : 0);
         }
         __syncthreads();
         load(it + 1);
@@ -614,11 +680,11 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
         for (int i = 0; i < 4; i += kDealt<T>) {
             const int k = kw + 16 * i;
             if (direct) {
-                store_tiles<T, VEC, NT>(gw + (base + n) * ci + k, ci - k, &acc[i][j]);
+                store_tiles<T, HOW, NT>(gw + (base + n) * ci + k, ci - k, &acc[i][j]);
             } else {
                 float* o = pw + (base + n) * ci + k;
 #pragma unroll
-                for (int u = 0; u < kDealt<T>; ++u) store_tiles<float, VEC, 1>(o + 4 * u, ci - k - 4 * u, &acc[i + u][j]);
+                for (int u = 0; u < kDealt<T>; ++u) store_tiles<float, HOW, 1>(o + 4 * u, ci - k - 4 * u, &acc[i + u][j]);
             }
         }
     }
@@ -716,13 +782,15 @@ int xl_check(const int32_t* lvals, int32_t nreps, int32_t X, int64_t S, int32_t 
     return FEQ_OK;
 }
 
-template <class T>
-bool xl_vec(int ci, int co, std::initializer_list<const void*> ptrs) {
+// f(HOW) for rows of ci and co elements at these addresses.
+template <class T, class F>
+int with_rows(int ci, int co, std::initializer_list<const void*> ptrs, F&& f) {
     constexpr int V = 16 / sizeof(T);
-    if (ci % V || co % V) return false;
-    for (const void* p : ptrs)
-        if (p && !aligned_to(p, 16)) return false;
-    return true;
+    bool whole = ci % V == 0 && co % V == 0;
+    for (const void* p : ptrs) whole = whole && (!p || aligned_to(p, 16));
+    if (whole) return f(std::integral_constant<int, kWhole>{});
+    if (ci >= V && co >= V) return f(std::integral_constant<int, kRagged>{});
+    return f(std::integral_constant<int, kNarrow>{});
 }
 
 // Workgroups of a kernel that the chip holds at once (256 CUs).
@@ -736,12 +804,12 @@ template <class T, bool TRANS>
 int mm_run(const void* in, const void* W, const int32_t* offsets, int X, int64_t S, int ci, int co, int nreps,
            const XlMap& map, const void* bias, int nbias, void* out, hipStream_t s) {
     const int K = TRANS ? co : ci, N = TRANS ? ci : co;
-    const bool vec = xl_vec<T>(ci, co, {in, W, out});
-    if (K <= kXlStreamK) {
-        const int dim = map.first[nreps];
-        auto go = [&](auto v, auto nn, auto ns) -> int {
+    const int dim = map.first[nreps];
+    return with_rows<T>(ci, co, {in, W, out}, [&](auto how) -> int {
+        constexpr int HOW = decltype(how)::value;
+        auto stream = [&](auto nn, auto ns) -> int {
             constexpr int NB = decltype(nn)::value;
-            auto kern = k_xl_stream<T, decltype(v)::value, TRANS, NB, decltype(ns)::value>;
+            auto kern = k_xl_stream<T, HOW, TRANS, NB, decltype(ns)::value>;
             // as many workgroups as run at once
             static const int resident = resident_blocks(reinterpret_cast<const void*>(kern), kXlThreads);
             const int64_t blocks = std::min<int64_t>(resident, tile_bound(S, X, 16) * dim * ceil_div(N, NB));
@@ -750,29 +818,26 @@ int mm_run(const void* in, const void* W, const int32_t* offsets, int X, int64_t
                        dim, static_cast<const T*>(bias), nbias, static_cast<T*>(out));
             return FEQ_OK;
         };
-        constexpr int H = 64 / Mma<T>::KS;           // steps of 64 columns
-        auto with_ns = [&](auto v, auto nn) -> int {
-            return K <= 64 ? go(v, nn, std::integral_constant<int, H>{}) : go(v, nn, std::integral_constant<int, 2 * H>{});
+        auto tile = [&](auto wr) -> int {
+            constexpr int WR = decltype(wr)::value;
+            const int64_t blocks = xcd_grid(tile_bound(S, X, kXlBM), ceil_div(N, 64 * WR));
+            if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
+            auto kern = k_xl_mm<T, HOW, TRANS, WR>;
+            FEQ_LAUNCH(TRANS ? "k_xl_mm_t" : "k_xl_mm", kern, dim3(blocks, dim), dim3(kXlThreads), 0, s,
+                       static_cast<const T*>(in), static_cast<const T*>(W), offsets, X, static_cast<int>(S), K, N, nreps, map,
+                       static_cast<const T*>(bias), nbias, static_cast<T*>(out));
+            return FEQ_OK;
         };
-        if (!vec) return with_ns(std::false_type{}, std::integral_constant<int, 128>{});
-        if (N <= 32) return with_ns(std::true_type{}, std::integral_constant<int, 32>{});
-        if (N <= 64) return with_ns(std::true_type{}, std::integral_constant<int, 64>{});
-        return with_ns(std::true_type{}, std::integral_constant<int, 128>{});
-    }
-    auto run = [&](auto v, auto wr) -> int {
-        constexpr int WR = decltype(wr)::value;
-        const int64_t blocks = xcd_grid(tile_bound(S, X, kXlBM), ceil_div(N, 64 * WR));
-        if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
-        auto kern = k_xl_mm<T, decltype(v)::value, TRANS, WR>;
-        FEQ_LAUNCH(TRANS ? "k_xl_mm_t" : "k_xl_mm", kern, dim3(blocks, map.first[nreps]), dim3(kXlThreads), 0, s,
-                   static_cast<const T*>(in), static_cast<const T*>(W), offsets, X, static_cast<int>(S), K, N, nreps, map,
-                   static_cast<const T*>(bias), nbias, static_cast<T*>(out));
-        return FEQ_OK;
-    };
-    auto with_wr = [&](auto v) -> int {
-        return N <= 64 ? run(v, std::integral_constant<int, 1>{}) : run(v, std::integral_constant<int, 2>{});
-    };
-    return vec ? with_wr(std::true_type{}) : with_wr(std::false_type{});
+        constexpr int H = 64 / Mma<T>::KS;           // steps of 64 columns
+        auto with_ns = [&](auto nn) -> int {
+            return K <= 64 ? stream(nn, std::integral_constant<int, H>{}) : stream(nn, std::integral_constant<int, 2 * H>{});
+        };
+        if (K > kXlStreamK)
+            return N <= 64 ? tile(std::integral_constant<int, 1>{}) : tile(std::integral_constant<int, 2>{});
+        if (N <= 32) return with_ns(std::integral_constant<int, 32>{});
+        if (N <= 64) return with_ns(std::integral_constant<int, 64>{});
+        return with_ns(std::integral_constant<int, 128>{});
+    });
 }
 
 // Weight-gradient chunks: all of about as many row-planes, for about 1024 workgroups, whose partials cost little
@@ -868,27 +933,25 @@ extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int3
     return with_dtype(dtype, [&](auto tt) -> int {
         using T = decltype(tt);
         T *gw = static_cast<T*>(grad_weight), *gb = static_cast<T*>(grad_bias);
-        const bool vec = xl_vec<T>(cin, cout, {grad_y, x, grad_weight});
-        auto run = [&](auto v, auto wr) -> int {
+        return with_rows<T>(cin, cout, {grad_y, x, grad_weight}, [&](auto how) -> int {
+        constexpr int HOW = decltype(how)::value;
+        auto run = [&](auto wr) -> int {
             constexpr int WR = decltype(wr)::value;
             const int64_t blocks = ch.tile0[nreps] * ceil_div(cin, 64 * WR) * ceil_div(cout, 128);
             if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
             auto go = [&](auto once) -> int {
-                auto kern = k_xl_wgrad<T, decltype(v)::value, WR, decltype(once)::value>;
+                auto kern = k_xl_wgrad<T, HOW, WR, decltype(once)::value>;
                 FEQ_LAUNCH("k_xl_wgrad", kern, dim3(blocks), dim3(kXlThreads), 0, s, static_cast<const T*>(grad_y),
                            static_cast<const T*>(x), offsets, experts, static_cast<int>(slots), cin, cout, nreps, map, ch, gw,
                            gb, nb, pw, pb);
                 return FEQ_OK;
             };
-            if constexpr (decltype(v)::value) {
+            if constexpr (HOW == kWhole) {
                 if (cin <= 64 * WR && cout <= 128) return go(std::true_type{});
             }
             return go(std::false_type{});
         };
-        auto with_wr = [&](auto v) -> int {
-            return cin <= 64 ? run(v, std::integral_constant<int, 1>{}) : run(v, std::integral_constant<int, 2>{});
-        };
-        if (const int err = vec ? with_wr(std::true_type{}) : with_wr(std::false_type{})) return err;
+        if (const int err = cin <= 64 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{})) return err;
         if (nslots == 0) return FEQ_OK;               // every expert in one chunk
         const int64_t wsize = static_cast<int64_t>(cin) * cout;
         int least = ch.rows[0];
@@ -901,6 +964,7 @@ extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int3
                        0, s, pw, pb, offsets, experts, ch, wsize, cout, nreps, gw, gb, nb);
             return FEQ_OK;
         };
-        return vec ? sum(std::integral_constant<int, 4>{}) : sum(std::integral_constant<int, 1>{});
+        return HOW == kWhole ? sum(std::integral_constant<int, 4>{}) : sum(std::integral_constant<int, 1>{});
+        });
     });
 }

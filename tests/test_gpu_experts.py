@@ -323,7 +323,8 @@ def check_linear(dev, lvals, counts, unrouted, cin, cout, dtype, bias=True, seed
     assert not y[:, n:].any() and not got[0][:, n:].any()
 
 
-CHANNELS = [(64, 128), (128, 64), (8, 8), (33, 7), (1, 1), (160, 200), (12, 260), (300, 20)]
+CHANNELS = [(64, 128), (128, 64), (8, 8), (33, 7), (1, 1), (160, 200), (12, 260), (300, 20), (301, 133), (131, 9),
+            (22, 26), (9, 98)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
