@@ -249,8 +249,12 @@ k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const 
 #pragma unroll
         for (int j = 0; j < V; ++j) gm[c][j] = (gmean && j >= sh[c]) ? gmean[at[c] + j] * inv_rows : 0.0f;
     const bool full = gmean || (gw && !normalize);      // uniform: the probabilities enter
-    for (int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / G; r < rows;
-         r += static_cast<int64_t>(gridDim.x) * per) {
+    const int64_t stride = static_cast<int64_t>(gridDim.x) * per;
+    int64_t r = static_cast<int64_t>(blockIdx.x) * per + threadIdx.x / G;
+    float x[NC][V], next[NC][V];
+    if (r < rows && full) load_row<T, V, NC>(logits + r * X, at, sh, x);
+    for (; r < rows; r += stride) {
+        if (full) load_row<T, V, NC>(logits + (r + stride < rows ? r + stride : r) * X, at, sh, next);
         float gp[NC][V], d[NC][V];
 #pragma unroll
         for (int c = 0; c < NC; ++c)
@@ -259,8 +263,6 @@ k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const 
                 gp[c][j] = gm[c][j];
                 d[c][j] = 0.0f;
             }
-        float x[NC][V];
-        if (full) load_row<T, V, NC>(logits + r * X, at, sh, x);
         if (gw) {
             float dot = 0.0f;
             if (normalize)
@@ -311,6 +313,10 @@ k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const 
                     if (j >= sh[c]) o[j] = static_cast<T>(d[c][j]);
             }
         }
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+            for (int j = 0; j < V; ++j) x[c][j] = next[c][j];
     }
 }
 
@@ -323,23 +329,27 @@ int topk_check(int64_t rows, int32_t X, int32_t K, int32_t dtype) {
     return FEQ_OK;
 }
 
-// Lanes of a row: 8 logits a lane up to 512 experts, 16 above.
-int topk_lanes(int X) {
+// Logits a lane holds, at least: the forward has most of its work per lane and choice, and takes 16 from 64 experts on
+// (top-6 of 233 bfloat16 for 59000 rows: 34 us, with 8 42); the backward 8 up to 512 (27 us for 58342 rows of 201
+// float16, with 16 31).
+constexpr int kForwardNarrow = 64, kBackwardNarrow = 512;
+// Lanes of a row.
+int topk_lanes(int X, int narrow) {
     int g = 1;
-    while (g < 64 && g * 8 < X) g <<= 1;
+    while (g < 64 && g * (X <= narrow ? 8 : 16) < X) g <<= 1;
     return g;
 }
 int topk_blocks(int64_t rows, int X) {
-    return static_cast<int>(std::min<int64_t>(ceil_div(rows, kTopkThreads / topk_lanes(X)), kTopkMaxBlocks));
+    return static_cast<int>(std::min<int64_t>(ceil_div(rows, kTopkThreads / topk_lanes(X, kForwardNarrow)), kTopkMaxBlocks));
 }
 
-// f(V, NC) for the instance of X experts, vectors where `vec`
+// f(V, NC) for the instance of X experts
 template <class T, class F>
-int with_topk_form(int X, bool vec, F&& f) {
+int with_topk_form(int X, int narrow, F&& f) {
     constexpr int VV = 16 / sizeof(T);
-    if (!vec) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});     // fewer experts than a vector
-    return X <= 512 ? f(std::integral_constant<int, VV>{}, std::integral_constant<int, 8 / VV>{})
-                    : f(std::integral_constant<int, VV>{}, std::integral_constant<int, 16 / VV>{});
+    if (X < VV) return f(std::integral_constant<int, 1>{}, std::integral_constant<int, 8>{});     // fewer than a vector
+    return X <= narrow ? f(std::integral_constant<int, VV>{}, std::integral_constant<int, 8 / VV>{})
+                       : f(std::integral_constant<int, VV>{}, std::integral_constant<int, 16 / VV>{});
 }
 
 // ---- plan ------------------------------------------------------------------------
@@ -583,13 +593,12 @@ extern "C" int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t exp
         return fail(FEQ_ERR_WORKSPACE, "top-k workspace of %zu bytes, %zu needed", ws_bytes,
                     feq_expert_topk_workspace(rows, experts));
     hipStream_t s = stream_of(stream);
-    const int G = topk_lanes(experts), blocks = rows ? topk_blocks(rows, experts) : 0;
+    const int G = topk_lanes(experts, kForwardNarrow), blocks = rows ? topk_blocks(rows, experts) : 0;
     float* part = mean ? static_cast<float*>(workspace) : nullptr;
     if (rows) {
         const int rc = with_dtype(dtype, [&](auto t) -> int {
             using T = decltype(t);
-            const bool vec = experts >= static_cast<int>(16 / sizeof(T));
-            return with_topk_form<T>(experts, vec, [&](auto v, auto nc) -> int {
+            return with_topk_form<T>(experts, kForwardNarrow, [&](auto v, auto nc) -> int {
                 auto run = [&](auto km) -> int {
                     auto kern = k_topk_fwd<T, decltype(v)::value, decltype(nc)::value, decltype(km)::value>;
                     FEQ_LAUNCH("k_topk_fwd", kern, dim3(blocks), dim3(kTopkThreads), 0, s, static_cast<const T*>(logits),
@@ -616,12 +625,11 @@ extern "C" int feq_expert_topk_bwd(const void* logits, const int64_t* ids, const
     if (rows == 0) return FEQ_OK;
     if (!logits || !ids || !weights || !grad_logits) return fail(FEQ_ERR_INVALID, "NULL pointer");
     hipStream_t s = stream_of(stream);
-    const int G = topk_lanes(experts);
-    const int64_t blocks = std::min<int64_t>(ceil_div(rows, kTopkThreads / G), 8192);
+    const int G = topk_lanes(experts, kBackwardNarrow);
+    const int64_t blocks = std::min<int64_t>(ceil_div(rows, kTopkThreads / G), 2048);
     return with_dtype(dtype, [&](auto t) -> int {
         using T = decltype(t);
-        const bool vec = experts >= static_cast<int>(16 / sizeof(T));
-        return with_topk_form<T>(experts, vec, [&](auto v, auto nc) -> int {
+        return with_topk_form<T>(experts, kBackwardNarrow, [&](auto v, auto nc) -> int {
             auto kern = k_topk_bwd<T, decltype(v)::value, decltype(nc)::value>;
             FEQ_LAUNCH("k_topk_bwd", kern, dim3(blocks), dim3(kTopkThreads), 0, s, static_cast<const T*>(logits), ids,
                        weights, grad_weights, grad_mean, rows, experts, top_k, normalize,
