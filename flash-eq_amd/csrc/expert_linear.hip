@@ -6,15 +6,10 @@
 //   grad_b[e, n, j] = sum over the rows p of e of grad_y[d_j, p, n];
 // rows from offsets[X] on (slots without an expert): y and grad_x are 0, and they enter no sum.
 //
-// Products run on the matrix cores: v_mfma_f32_16x16x4_f32 for float32, v_mfma_f32_16x16x32_{f16, bf16}
-// for 16-bit types, float32 accumulators for both, one rounding at the store.  A workgroup of
-// four waves takes a 128-row block of one expert and plane and 64 or 128 output columns; the
-// expert of a block is found by every wave from the offsets (a lane per expert, sums over
-// lanes), so the host never learns the counts and the grid is their upper bound.
-//
-// The weight is the first operand and the rows the second, so a lane's accumulators are
-// columns of one row; the weight rows are dealt to the tiles so that a lane's 16 accumulators are
-// XXX
+// Products run on the matrix cores: v_mfma_f32_16x16x4_f32 for float32, v_mfma_f32_16x16x32_{f16, bf16} for 16-bit
+// types, float32 accumulators for both, one rounding at the store.  The expert of a row block is found by every wave
+// from the offsets (a lane per expert, sums over lanes), so the host never learns the counts and the grid is their
+// upper bound.  The weight is the first operand and the rows the second: a lane's accumulators are columns of one row.
 #include <algorithm>
 
 #include "elem_types.h"
@@ -577,20 +572,20 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
 }
 
 // grad_W and grad_b over row chunks.  A workgroup takes a chunk of one expert, one irrep r (all its
-// planes), 64 WR columns k of x and 128 columns n of grad_y (tiles of k first).  An expert of one chunk gets its
+// planes), 16 TI WR columns k of x and BN columns n of grad_y (tiles of k first).  An expert of one chunk gets its
 // gradient written (zeros without rows), one of several a float32 partial per chunk: pw[slot N K + n K + k],
 // pb[slot N + n], summed by k_xl_wsum.
 // ONCE: one tile covers the weight, so every row is read once; the rows then go past the caches, which leaves them to
 // the kernels around (20011 x 49 bfloat16 rows, 128 x 128: 137 -> 97 us, and with both maps a pass 376 -> 353).  Rows
 // that several tiles read lose by it (42 -> 52 us for 512 x 1024).
-template <class T, int HOW, int WR, bool ONCE>
+template <class T, int HOW, int WR, int TI, int BN, bool ONCE>
 __global__ void __launch_bounds__(kXlThreads)
 k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __restrict__ offsets, int X, int S,
            int ci, int co, int nreps, XlMap map, XlChunks ch, T* __restrict__ gw, T* __restrict__ gb, int nbias,
            float* __restrict__ pw, float* __restrict__ pb) {
     using M = Mma<T>;
     constexpr int V = 16 / sizeof(T), BP = kXlRowBytes / sizeof(T);   // rows staged at a time
-    constexpr int BK = 64 * WR, BN = 128, WC = 4 / WR, NT = BN / (16 * WC);
+    constexpr int BK = 16 * TI * WR, WC = 4 / WR, NT = BN / (16 * WC);
     constexpr int LX = BK + M::PAD, LG = BN + M::PAD;
     constexpr int NX = BP * (BK / V) / kXlThreads, NG = BP * (BN / V) / kXlThreads;
     __shared__ __align__(16) T sX[BP * LX];
@@ -629,12 +624,12 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
             vg[i] = load16<T, HOW, ONCE>(tg, (r * co + n) * static_cast<int>(sizeof(T)), r < there ? co - n0 - n : 0);
         }
     };
-    v4f acc[4][NT];
+    v4f acc[TI][NT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < TI; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) acc[i][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    float bsum = 0.0f;                                             // thread n < 128: column n0 + n
+    float bsum = 0.0f;                                             // thread n < BN: column n0 + n
     if (total) load(0);
     for (int it = 0; it < total; ++it) {
         __syncthreads();
@@ -654,13 +649,13 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
         load(it + 1);
 #pragma unroll
         for (int ks = 0; ks < BP; ks += M::KS) {
-            typename M::frag a[4], b[NT];
+            typename M::frag a[TI], b[NT];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = M::columns(sX, LX, ks, g, c, 64 * wr + 16 * i);
+            for (int i = 0; i < TI; ++i) a[i] = M::columns(sX, LX, ks, g, c, 16 * (wr * TI + i));
 #pragma unroll
             for (int j = 0; j < NT; ++j) b[j] = M::columns(sG, LG, ks, g, c, 16 * (wc * NT + j));
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < TI; ++i)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[i][j] = M::mul(a[i], b[j], acc[i][j]);
         }
@@ -669,7 +664,7 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
     }
     const bool direct = t.count == 1;
     const int64_t slot = ch.slot0[rep] + t.before + t.index;
-    const int kw = k0 + 64 * wr + V * g;
+    const int kw = k0 + 16 * TI * wr + V * g;
     const int64_t base = direct ? (static_cast<int64_t>(t.expert) * nreps + rep) * co
                                 : slot * co;
 #pragma unroll
@@ -677,7 +672,7 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
         const int n = n0 + 16 * (wc * NT + j) + c;
         if (n >= co) continue;
 #pragma unroll
-        for (int i = 0; i < 4; i += kDealt<T>) {
+        for (int i = 0; i < TI; i += kDealt<T>) {
             const int k = kw + 16 * i;
             if (direct) {
                 store_tiles<T, HOW, NT>(gw + (base + n) * ci + k, ci - k, &acc[i][j]);
@@ -934,37 +929,43 @@ extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int3
         using T = decltype(tt);
         T *gw = static_cast<T*>(grad_weight), *gb = static_cast<T*>(grad_bias);
         return with_rows<T>(cin, cout, {grad_y, x, grad_weight}, [&](auto how) -> int {
-        constexpr int HOW = decltype(how)::value;
-        auto run = [&](auto wr) -> int {
-            constexpr int WR = decltype(wr)::value;
-            const int64_t blocks = ch.tile0[nreps] * ceil_div(cin, 64 * WR) * ceil_div(cout, 128);
-            if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
-            auto go = [&](auto once) -> int {
-                auto kern = k_xl_wgrad<T, HOW, WR, decltype(once)::value>;
-                FEQ_LAUNCH("k_xl_wgrad", kern, dim3(blocks), dim3(kXlThreads), 0, s, static_cast<const T*>(grad_y),
-                           static_cast<const T*>(x), offsets, experts, static_cast<int>(slots), cin, cout, nreps, map, ch, gw,
-                           gb, nb, pw, pb);
+            constexpr int HOW = decltype(how)::value;
+            auto run = [&](auto wr, auto ti, auto bn) -> int {
+                constexpr int WR = decltype(wr)::value, TI = decltype(ti)::value, BN = decltype(bn)::value;
+                const int64_t blocks = ch.tile0[nreps] * ceil_div(cin, 16 * TI * WR) * ceil_div(cout, BN);
+                if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
+                auto go = [&](auto once) -> int {
+                    auto kern = k_xl_wgrad<T, HOW, WR, TI, BN, decltype(once)::value>;
+                    FEQ_LAUNCH("k_xl_wgrad", kern, dim3(blocks), dim3(kXlThreads), 0, s, static_cast<const T*>(grad_y),
+                               static_cast<const T*>(x), offsets, experts, static_cast<int>(slots), cin, cout, nreps, map,
+                               ch, gw, gb, nb, pw, pb);
+                    return FEQ_OK;
+                };
+                if constexpr (HOW == kWhole) {
+                    if (cin <= 16 * TI * WR && cout <= BN) return go(std::true_type{});
+                }
+                return go(std::false_type{});
+            };
+            auto with_bn = [&](auto wr, auto ti) -> int {
+                return cout <= 64 ? run(wr, ti, std::integral_constant<int, 64>{}) : run(wr, ti, std::integral_constant<int, 128>{});
+            };
+            constexpr std::integral_constant<int, 1> one{};
+            constexpr std::integral_constant<int, 2> two{};
+            constexpr std::integral_constant<int, 4> four{};
+            if (const int err = cin <= 32 ? with_bn(one, two) : cin <= 64 ? with_bn(one, four) : with_bn(two, four)) return err;
+            if (nslots == 0) return FEQ_OK;               // every expert in one chunk
+            const int64_t wsize = static_cast<int64_t>(cin) * cout;
+            int least = ch.rows[0];
+            for (int r = 1; r < nreps; ++r) least = std::min(least, static_cast<int>(ch.rows[r]));
+            const int64_t many = std::min<int64_t>(experts, slots / least);  // experts of several chunks, at most
+            auto sum = [&](auto vv) -> int {
+                constexpr int V = decltype(vv)::value;
+                auto kern = k_xl_wsum<T, V>;
+                FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(std::max<int64_t>(wsize, cout), 256 * V), many, nreps + nb),
+                           dim3(256), 0, s, pw, pb, offsets, experts, ch, wsize, cout, nreps, gw, gb, nb);
                 return FEQ_OK;
             };
-            if constexpr (HOW == kWhole) {
-                if (cin <= 64 * WR && cout <= 128) return go(std::true_type{});
-            }
-            return go(std::false_type{});
-        };
-        if (const int err = cin <= 64 ? run(std::integral_constant<int, 1>{}) : run(std::integral_constant<int, 2>{})) return err;
-        if (nslots == 0) return FEQ_OK;               // every expert in one chunk
-        const int64_t wsize = static_cast<int64_t>(cin) * cout;
-        int least = ch.rows[0];
-        for (int r = 1; r < nreps; ++r) least = std::min(least, static_cast<int>(ch.rows[r]));
-        const int64_t many = std::min<int64_t>(experts, slots / least);  // experts of several chunks, at most
-        auto sum = [&](auto vv) -> int {
-            constexpr int V = decltype(vv)::value;
-            auto kern = k_xl_wsum<T, V>;
-            FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(std::max<int64_t>(wsize, cout), 256 * V), many, nreps + nb), dim3(256),
-                       0, s, pw, pb, offsets, experts, ch, wsize, cout, nreps, gw, gb, nb);
-            return FEQ_OK;
-        };
-        return HOW == kWhole ? sum(std::integral_constant<int, 4>{}) : sum(std::integral_constant<int, 1>{});
+            return HOW == kWhole ? sum(std::integral_constant<int, 4>{}) : sum(std::integral_constant<int, 1>{});
         });
     });
 }
