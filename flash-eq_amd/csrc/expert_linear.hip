@@ -689,12 +689,16 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
     }
 }
 
-// The gradients of the experts of several chunks: their partials in order.  blockIdx.y: the expert's number among
-// these, blockIdx.z: the irrep, and behind the irreps the bias columns.
-template <class T, int V>
+// The gradients of the experts of several chunks: the sum of their partials, in an order that no launch changes.
+// blockIdx.y: the expert's number among these, blockIdx.z: the irrep, and behind the irreps the bias columns.
+// SPLIT: the four waves of a workgroup take a quarter of the partials each, for experts of many (111 of 34 x 51
+// columns: 22 us in one wave, which waits for its loads in turn, 10 in four; one to two of 512 x 1024 columns: 6 us
+// and 19).
+template <class T, int V, bool SPLIT>
 __global__ void __launch_bounds__(256)
 k_xl_wsum(const float* __restrict__ pw, const float* __restrict__ pb, const int32_t* __restrict__ offsets, int X,
           XlChunks ch, int64_t wsize, int co, int nreps, T* __restrict__ gw, T* __restrict__ gb, int nbias) {
+    __shared__ __align__(16) float part[SPLIT ? 3 : 1][64 * V];
     const int z = blockIdx.z, lane = threadIdx.x & 63, want = blockIdx.y;
     const int rep = z < nreps ? z : ch.brep[z - nreps], rc = ch.rows[rep];
     int expert = -1, first = 0, count = 0, carry = 0, slots = 0;
@@ -720,21 +724,33 @@ k_xl_wsum(const float* __restrict__ pw, const float* __restrict__ pb, const int3
         slots += __shfl(incl, 63, 64);
     }
     if (expert < 0) return;
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) * V;
+    const int64_t i = (static_cast<int64_t>(blockIdx.x) * (SPLIT ? 64 : 256) + (SPLIT ? lane : threadIdx.x)) * V;
+    const int wave = SPLIT ? threadIdx.x >> 6 : 0;
     const bool w = z < nreps;
     const int64_t size = w ? wsize : co;
-    if (i >= size) return;
     const float* p = (w ? pw : pb) + static_cast<int64_t>(ch.slot0[rep] + first) * size + i;
     float a[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) a[v] = 0.0f;
+    if (i < size) {
 #pragma unroll 8
-    for (int q = 0; q < count; ++q) {
-        float f[V];
-        load_f<float, V>(p + q * size, f);
+        for (int q = wave; q < count; q += SPLIT ? 4 : 1) {
+            float f[V];
+            load_f<float, V>(p + q * size, f);
 #pragma unroll
-        for (int v = 0; v < V; ++v) a[v] += f[v];
+            for (int v = 0; v < V; ++v) a[v] += f[v];
+        }
     }
+    if constexpr (SPLIT) {
+        if (wave) store_f<float, V>(part[wave - 1] + lane * V, a);
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+            for (int v = 0; v < V; ++v) a[v] += part[q][lane * V + v];
+    }
+    if (i >= size) return;
     if (w) {
         store_f<T, V>(gw + (static_cast<int64_t>(expert) * nreps + z) * wsize + i, a);
     } else {
@@ -958,14 +974,17 @@ extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int3
             int least = ch.rows[0];
             for (int r = 1; r < nreps; ++r) least = std::min(least, static_cast<int>(ch.rows[r]));
             const int64_t many = std::min<int64_t>(experts, slots / least);  // experts of several chunks, at most
-            auto sum = [&](auto vv) -> int {
+            const bool split = slots / least > 8 * experts;                  // more than eight chunks an expert, on average
+            auto sum = [&](auto vv, auto sp) -> int {
                 constexpr int V = decltype(vv)::value;
-                auto kern = k_xl_wsum<T, V>;
-                FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(std::max<int64_t>(wsize, cout), 256 * V), many, nreps + nb),
+                constexpr bool SPLIT = decltype(sp)::value;
+                auto kern = k_xl_wsum<T, V, SPLIT>;
+                FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(std::max<int64_t>(wsize, cout), (SPLIT ? 64 : 256) * V), many, nreps + nb),
                            dim3(256), 0, s, pw, pb, offsets, experts, ch, wsize, cout, nreps, gw, gb, nb);
                 return FEQ_OK;
             };
-            return HOW == kWhole ? sum(std::integral_constant<int, 4>{}) : sum(std::integral_constant<int, 1>{});
+            auto with_split = [&](auto vv) -> int { return split ? sum(vv, std::true_type{}) : sum(vv, std::false_type{}); };
+            return HOW == kWhole ? with_split(four) : with_split(one);
         });
     });
 }
