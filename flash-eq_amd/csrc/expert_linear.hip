@@ -887,6 +887,7 @@ extern "C" int feq_expert_linear_fwd(const int32_t* lvals, int32_t nreps, int32_
                                      void* y, feq_stream_t stream) {
     XlMap map;
     if (int rc = xl_check(lvals, nreps, experts, slots, cin, cout, dtype, bias ? bias_cols : nullptr, nbias, &map)) return rc;
+    if (bias && (!bias_cols || nbias < 1)) return fail(FEQ_ERR_INVALID, "a bias needs bias columns");
     if (slots == 0) return FEQ_OK;
     if (!x || !weight || !offsets || !y) return fail(FEQ_ERR_INVALID, "NULL pointer");
     return with_dtype(dtype, [&](auto t) -> int {

@@ -16,11 +16,11 @@
 // sum per lane, summed over lanes, waves and workgroups in a fixed order.
 //
 // Plan.  A stable counting sort: per 2048-slot tile a histogram (k_plan_hist), per bucket the
-// tiles' exclusive sums (k_plan_scan; up to 64 tiles sum them themselves), then every tile ranks its
-// slots (k_plan_place).  Up to 8192 slots one workgroup does all three (k_plan_one).  Lanes with equal keys find each other by one
-// ballot per key bit, so a slot's rank needs no atomics and the order is the slots' own.  Slots
-// whose expert lies outside [0, X) fill a last bucket.  The plan is integer work on 8 bytes
-// per slot: launches and latency bound it.
+// tiles' exclusive sums (k_plan_scan; up to 64 tiles sum them themselves), then every tile ranks
+// its slots (k_plan_place).  Up to 8192 slots one workgroup does all three (k_plan_one).  Lanes
+// with equal keys find each other by one ballot per key bit, so a slot's rank needs no atomics and
+// the order is the slots' own.  Slots whose expert lies outside [0, X) fill a last bucket.  The
+// plan is integer work on 8 bytes per slot: launches and latency bound it.
 #include <algorithm>
 
 #include "elem_types.h"
@@ -99,8 +99,8 @@ __device__ __forceinline__ float row_exp(const float (&x)[NC][V], int G, float (
     return group_sum(s, G);
 }
 
-// X >= V.  KMAX: the choices are kept
-// in registers until the weights' sum is known (K <= KMAX); 0: they wait in memory.
+// X >= V.  KMAX: the choices are kept in registers until the weights' sum is known (K <= KMAX); 0: they wait in
+// memory.
 template <class T, int V, int NC, int KMAX>
 __global__ void __launch_bounds__(kTopkThreads)
 k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normalize, int64_t* __restrict__ ids,
@@ -329,9 +329,9 @@ int topk_check(int64_t rows, int32_t X, int32_t K, int32_t dtype) {
     return FEQ_OK;
 }
 
-// Logits a lane holds, at least: the forward has most of its work per lane and choice, and takes 16 from 64 experts on
-// (top-6 of 233 bfloat16 for 59000 rows: 34 us, with 8 42); the backward 8 up to 512 (27 us for 58342 rows of 201
-// float16, with 16 31).
+// A lane holds up to 8 logits of rows up to these many, above them up to 16: the forward's work is per lane and choice
+// (top-6 of 233 bfloat16 for 59000 rows: 34 us with 16, 42 with 8), the backward's per logit (58342 rows of 201
+// float16: 31 us with 16, 27 with 8).
 constexpr int kForwardNarrow = 64, kBackwardNarrow = 512;
 // Lanes of a row.
 int topk_lanes(int X, int narrow) {
@@ -571,8 +571,8 @@ __global__ void k_plan_empty(int32_t* offsets, int X) {
     if (i <= X) offsets[i] = 0;
 }
 
-// The one-workgroup form: its 17 (X + 2) counters fit 64 KB.
-bool plan_one(int64_t slots, int X) { return slots <= kPlanOne && 17 * (X + 2) * sizeof(int) <= 64 * 1024; }
+// The one-workgroup form: its counters, 17 (X + 2) and 16, fit 64 KB.
+bool plan_one(int64_t slots, int X) { return slots <= kPlanOne && (17 * (X + 2) + 16) * sizeof(int) <= 64 * 1024; }
 
 }  // namespace
 }  // namespace feq

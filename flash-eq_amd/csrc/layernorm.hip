@@ -31,6 +31,7 @@ constexpr int kLnBlockElems = 32;   // and in the workgroup form
 constexpr int kLnFwdBlocks = 2048;   // workgroups of the forward: what the chip holds, each over many rows
 constexpr int kLnMaxBlocks = 1024;  // workgroups of the backward, and weight-gradient partials
 constexpr int kLnWide = 1024;       // threads of the _wide kernels
+constexpr int kLnWideBlocks = 64;   // their weight-gradient partials
 
 // Sum over the workgroup of NW waves; red holds 2 NW floats, one use per call.
 template <int NW>
@@ -447,7 +448,7 @@ int ln_bwd_run(const T* gy, int64_t ldg, const T* x, int64_t rows, int width, in
 int ln_check(int64_t rows, int64_t width, int64_t ldx, int32_t dtype, const void* x, const void* w, const void* b,
              int32_t pdt) {
     if (rows < 0 || width < 1) return fail(FEQ_ERR_INVALID, "layer norm of %lld rows of width %lld", (long long)rows, (long long)width);
-    if (width > INT32_MAX / 2) return fail(FEQ_ERR_UNSUPPORTED, "layer norm width %lld exceeds 2^30", (long long)width);
+    if (width > 1 << 24) return fail(FEQ_ERR_UNSUPPORTED, "layer norm width %lld exceeds 2^24", (long long)width);
     if (ldx < width) return fail(FEQ_ERR_INVALID, "row stride %lld is smaller than the width %lld", (long long)ldx, (long long)width);
     if (!dtype_ok(dtype)) return fail(FEQ_ERR_INVALID, "unknown element type %d", dtype);
     if ((w || b) && !dtype_ok(pdt)) return fail(FEQ_ERR_INVALID, "unknown parameter type %d", pdt);
@@ -455,9 +456,11 @@ int ln_check(int64_t rows, int64_t width, int64_t ldx, int32_t dtype, const void
     return FEQ_OK;
 }
 
-// Workgroups of the backward (and partials of the weight gradients).
+// Workgroups of the backward, and partials of the weight gradients: at most (those of few wide rows would take more
+// memory than the rows).
 int ln_bwd_blocks(int64_t rows, int64_t width) {
-    return static_cast<int>(std::min<int64_t>(std::max<int64_t>(rows, 1), kLnMaxBlocks));
+    return static_cast<int>(std::min<int64_t>(std::max<int64_t>(rows, 1),
+                                              width > kLnThreads * kLnBlockElems ? kLnWideBlocks : kLnMaxBlocks));
 }
 
 }  // namespace
@@ -529,7 +532,7 @@ extern "C" int feq_layernorm_bwd(const void* grad_y, int64_t ldg, const void* x,
                                xt, rows, width, ldx, weight, param_dtype, mean, rstd, dt);
                 }
                 if (part) {
-                    const int64_t per = ceil_div(rows, std::min<int64_t>(ln_bwd_blocks(rows, width), 64));
+                    const int64_t per = ceil_div(rows, ln_bwd_blocks(rows, width));
                     groups = static_cast<int>(ceil_div(rows, per));
                     auto kern = k_ln_cols_wide<T>;
                     FEQ_LAUNCH("k_ln_cols_wide", kern, dim3(ceil_div(width, 256), groups), dim3(256), 0, s, gt, ldg, xt,

@@ -327,6 +327,15 @@ std::tuple<Tensor, Tensor, Tensor> expert_plan(const Tensor& ids, int64_t expert
     return {order, positions, offsets};
 }
 
+// The kernels write to the places a plan holds, so one whose tensors are not those that expert_plan
+// returned, as it returned them, is refused.
+void check_plan(const Tensor& t, const char* name, int64_t dims) {
+    need_gpu(t, name);
+    if (t.scalar_type() != at::kInt || t.dim() != dims || !t.is_contiguous())
+        value_error("not an ExpertPlan's ", name, ": ", dtype_name(t.scalar_type()), " of shape ", t.sizes());
+    TORCH_CHECK(t.is_inference() || t._version() == 0, "the ", name, " of an ExpertPlan have been modified in place");
+}
+
 // A plan as the row moves need it.
 struct Places {
     Tensor positions, offsets;
@@ -334,10 +343,15 @@ struct Places {
     int64_t k() const { return positions.size(1); }
     int64_t slots() const { return positions.numel(); }
     const int32_t* placed() const { return ptr_as<int32_t>(offsets) + offsets.numel() - 1; }
+    void check() const {
+        check_plan(positions, "positions", 2);
+        check_plan(offsets, "offsets", 1);
+    }
 };
 
 void check_table(const Tensor& t, const char* name, int64_t rows, const Places& p) {
     code_of(t, name);
+    p.check();
     same_device(p.positions, t);
     if (t.dim() < 2 || t.size(-2) != rows) value_error(name, " must be (..., ", rows, ", width), got shape ", t.sizes());
 }
@@ -366,6 +380,7 @@ struct DispatchNode final : OnceNode {
     Places places;
     variable_list backward(variable_list& grads) override {
         variable_list out(1);
+        places.check();
         if (grads[0].defined()) out[0] = combined(places, dense(grads[0]), Tensor());
         return out;
     }
@@ -401,6 +416,7 @@ struct CombineNode final : OnceNode {
     variable_list backward(variable_list& grads) override {
         variable_list out(2);
         if (!grads[0].defined()) return out;
+        places.check();
         const Tensor in = ys.unpack(), w = weights.unpack(), g = dense(grads[0]);
         if (need(0)) out[0] = make(in.sizes(), in, in.scalar_type());
         if (need(1)) out[1] = make(w.sizes(), w, w.scalar_type());
@@ -475,6 +491,7 @@ struct ExpertLinearNode final : OnceNode {
     variable_list backward(variable_list& grads) override {
         variable_list out(3);
         if (!grads[0].defined()) return out;
+        check_plan(offsets, "offsets", 1);
         const Tensor xs = x.unpack(), w = weight.unpack(), g = dense(grads[0]);
         const int64_t experts = w.size(0), co = w.size(2), ci = w.size(3), slots = xs.size(-2);
         const int code = code_of(xs, "x");
@@ -519,6 +536,7 @@ Tensor expert_linear(const Tensor& x, const Tensor& weight, const OptTensor& bia
             type_error("x and ", name, " of different dtypes: ", dtype_name(x.scalar_type()), " and ", dtype_name(t.scalar_type()));
         same_device(x, t);
     }
+    check_plan(offsets, "offsets", 1);
     same_device(x, offsets);
     const int64_t experts = offsets.size(0) - 1;
     if (weight.dim() != 4 || weight.size(0) != experts || weight.size(1) != irreps.n())

@@ -14,6 +14,9 @@ import torch
 
 from . import _native as N
 
+MAX_EXPERTS = 1024
+MAX_TOP_K = 64
+
 
 def expert_topk(logits: torch.Tensor, top_k: int,
                 normalize: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -41,25 +44,43 @@ class ExpertPlan:
     * ``offsets`` (num_experts + 1,) int32: every expert's first place; the last one is the number
       of slots with an expert.
 
-    ``dispatch`` copies rows to their places, ``combine`` sums them back with weights."""
+    They are for reading: kernels write where they point, and a plan whose positions or offsets have
+    been modified in place is refused.  ``dispatch`` copies rows to their places, ``combine`` sums them
+    back with weights."""
 
     def __init__(self, ids: torch.Tensor, num_experts: int) -> None:
-        self.order, self.positions, self.offsets = N.nodes().expert_plan(ids, num_experts)
+        self._order, self._positions, self._offsets = N.nodes().expert_plan(ids, num_experts)
         self.num_experts = num_experts
-        self.num_rows, self.top_k = self.positions.shape
+        self.num_rows, self.top_k = self._positions.shape
         self.num_slots = self.num_rows * self.top_k
+
+    @property
+    def order(self) -> torch.Tensor:
+        return self._order
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._positions
+
+    @property
+    def offsets(self) -> torch.Tensor:
+        return self._offsets
+
+    def __setstate__(self, state: dict) -> None:
+        # of a copy or a pickle, whose tensors were filled in place
+        self.__dict__.update({k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in state.items()})
 
     def dispatch(self, x: torch.Tensor) -> torch.Tensor:
         """x (..., rows, width) to (..., slots, width): every place its slot's row, zeros at the
         places without an expert.  The gradient of a row is the sum over its places, in the order of
         its choices."""
-        return N.nodes().expert_dispatch(x, self.positions, self.offsets)
+        return N.nodes().expert_dispatch(x, self._positions, self._offsets)
 
     def combine(self, ys: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
         """ys (..., slots, width) to (..., rows, width): the sum over a row's choices of weight times
         the row at the choice's place, over the choices with an expert (none: zeros).  weights (rows,
         top_k), float32, float16 or bfloat16.  Gradients for both."""
-        return N.nodes().expert_combine(ys, weights, self.positions, self.offsets)
+        return N.nodes().expert_combine(ys, weights, self._positions, self._offsets)
 
     def __repr__(self) -> str:
         return f"ExpertPlan(rows={self.num_rows}, top_k={self.top_k}, num_experts={self.num_experts})"

@@ -7,12 +7,12 @@ equivariant.  No counterpart in the reference.
 """
 from __future__ import annotations
 
-from typing import Tuple
+from typing import List, Optional, Tuple
 
 import torch
 import torch.nn as nn
 
-from ..experts import ExpertPlan, expert_linear, expert_topk
+from ..experts import MAX_EXPERTS, MAX_TOP_K, ExpertPlan, expert_linear, expert_topk
 from ..representations import Repr
 from .gating import EquivariantGating
 from .norm import InvariantLayerNorm, RepNorm
@@ -24,8 +24,10 @@ class ExpertRouter(nn.Module):
 
     def __init__(self, repr: Repr, num_experts: int, top_k: int = 2, normalize: bool = True) -> None:
         super().__init__()
-        if not 1 <= top_k <= num_experts:
-            raise ValueError(f"top_k must be 1 to num_experts, got {top_k} of {num_experts}")
+        if not 1 <= num_experts <= MAX_EXPERTS:
+            raise ValueError(f"num_experts must be 1 to {MAX_EXPERTS}, got {num_experts}")
+        if not 1 <= top_k <= min(num_experts, MAX_TOP_K):
+            raise ValueError(f"top_k must be 1 to num_experts (at most {MAX_TOP_K}), got {top_k} of {num_experts}")
         self.num_experts = num_experts
         self.top_k = top_k
         self.normalize = normalize
@@ -86,8 +88,8 @@ class EquivariantExpertMLP(nn.Module):
 
     Every node's row goes to its ``top_k`` experts (``ExpertRouter``), through their maps up, the
     gating (shared by the experts) and their maps down, and the results are summed with the
-    router's weights.  After a forward ``balance`` holds the router's balancing term of that call, for
-    the training loss."""
+    router's weights.  ``forward(x, balance=terms)`` appends the router's balancing term to the list
+    ``terms``, for the training loss (the module keeps nothing of a call, so no graph outlives it)."""
 
     def __init__(self, repr: Repr, num_experts: int, top_k: int = 2, mlp_ratio: int = 2, use_gating: bool = True,
                  normalize: bool = True) -> None:
@@ -98,14 +100,14 @@ class EquivariantExpertMLP(nn.Module):
         self.up = EquivariantExpertLinear(repr, hidden, num_experts)
         self.act: nn.Module = EquivariantGating(hidden) if use_gating else nn.Identity()
         self.down = EquivariantExpertLinear(hidden, repr, num_experts)
-        self.balance: torch.Tensor | None = None
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, balance: Optional[List[torch.Tensor]] = None) -> torch.Tensor:
         if x.dim() != 3 or x.shape[1:] != (self.repr.mult, self.repr.dim()):
             raise ValueError(f"node features must be (nodes, {self.repr.mult}, {self.repr.dim()}), got {tuple(x.shape)}")
         ids, weights, mean = self.router(x)
         plan = ExpertPlan(ids, self.router.num_experts)
-        self.balance = self.router.balance(plan, mean)
+        if balance is not None:
+            balance.append(self.router.balance(plan, mean))
         # component-major (dim, nodes, mult): the layout of the maps and the gating
         h = self.up(plan.dispatch(x.permute(2, 0, 1).contiguous()), plan)
         if isinstance(self.act, EquivariantGating):

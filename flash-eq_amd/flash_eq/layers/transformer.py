@@ -64,7 +64,8 @@ class EquivariantTransformerBlock(nn.Module):
     """norm -> attention (-> residual when reprs match) -> norm -> gated MLP -> residual.
 
     With ``num_experts`` > 0 the MLP is a mixture of experts (``EquivariantExpertMLP``), each node
-    taking ``experts_per_node`` of them; the reference has no such option."""
+    taking ``experts_per_node`` of them; ``forward(..., balance=terms)`` appends its balancing term to
+    the list ``terms``.  The reference has no such option."""
 
     def __init__(self, in_repr: Repr, out_repr: Repr, num_heads: int = 1, num_bins: int = 100,
                  rank: int = 4, hidden_dim: int = 64, min_dist: float = 0.0,
@@ -90,6 +91,8 @@ class EquivariantTransformerBlock(nn.Module):
             dropout=dropout, reduce="sum", distance_decay_scale=distance_decay_scale)
         self.norm2 = SeparableEquivariantLayerNorm(out_repr)
         self.experts: EquivariantExpertMLP | None = None
+        if num_experts < 0:
+            raise ValueError(f"num_experts must not be negative, got {num_experts}")
         if num_experts > 0:
             self.experts = EquivariantExpertMLP(out_repr, num_experts, experts_per_node, mlp_ratio, use_gating)
         else:
@@ -107,11 +110,12 @@ class EquivariantTransformerBlock(nn.Module):
 
     def forward(self, P: torch.Tensor, Q: torch.Tensor, node_features: torch.Tensor,
                 distances: torch.Tensor, graph: Graph,
-                edge_features: torch.Tensor | None = None) -> torch.Tensor:
+                edge_features: torch.Tensor | None = None,
+                balance: list[torch.Tensor] | None = None) -> torch.Tensor:
         half = half_dtype(node_features)
         if half is not None:
             return run_float32(self, half, (P, Q, node_features, distances, graph),
-                               dict(edge_features=edge_features))
+                               dict(edge_features=edge_features, balance=balance))
         # With the residual connection, the norm also returns the features for
         # it (forward_pair): the residual's gradient is then added inside the
         # norm's backward kernel instead of by autograd in a separate pass.
@@ -126,7 +130,7 @@ class EquivariantTransformerBlock(nn.Module):
             x = attn_out
         if self.experts is not None:
             h, xr = self.norm2.forward_pair(x) if self.norm2.cm_ok(x) else (self.norm2(x), x)
-            return _residual(xr, self.experts(h), self.layer_scale_mlp, self.drop_path)
+            return _residual(xr, self.experts(h, balance), self.layer_scale_mlp, self.drop_path)
         if (isinstance(self.mlp_act, EquivariantGating) and self.mlp_act.kernels_ok(x)
                 and self.mlp_up.fused_ok(x) and self.mlp_down.fused_ok(x)):
             # the MLP runs component-major (dim, N, c) from the norm's output to
@@ -153,7 +157,8 @@ class EquivariantTransformerBlock(nn.Module):
 
 class EquivariantTransformer(nn.Module):
     """Stack of blocks: in -> hidden -> ... -> hidden -> out, basis computed from coordinates.
-    ``num_experts`` > 0 makes every block's MLP a mixture of experts."""
+    ``num_experts`` > 0 makes every block's MLP a mixture of experts, and ``forward(..., balance=terms)``
+    appends every block's balancing term to the list ``terms``."""
 
     def __init__(self, in_repr: Repr, hidden_repr: Repr, out_repr: Repr, num_layers: int = 6,
                  num_heads: int = 1, num_bins: int = 100, rank: int = 4, hidden_dim: int = 64,
@@ -185,10 +190,10 @@ class EquivariantTransformer(nn.Module):
         self.final_norm = SeparableEquivariantLayerNorm(out_repr)
 
     def forward(self, coordinates: torch.Tensor, node_features: torch.Tensor,
-                graph: Graph) -> torch.Tensor:
+                graph: Graph, balance: list[torch.Tensor] | None = None) -> torch.Tensor:
         half = half_dtype(node_features)
         if half is not None:
-            return run_float32(self, half, (coordinates, node_features, graph), {})
+            return run_float32(self, half, (coordinates, node_features, graph), dict(balance=balance))
         # src - dst, as transformer.py:406.  In float32 through the graph's CSR
         # gathers: their backward (the coordinate gradient) is a fixed-order
         # segmented sum, where torch's indexing backward sorts the indices
@@ -211,7 +216,7 @@ class EquivariantTransformer(nn.Module):
                 uses = [(next(views) if P is m_hidden else P, next(views) if Q is m_hidden else Q)
                         for P, Q in uses]
         for layer, (P, Q) in zip(self.layers, uses):
-            x = layer(P, Q, x, distances, graph)
+            x = layer(P, Q, x, distances, graph, balance=balance)
         return self.final_norm(x)
 
     def extra_repr(self) -> str:

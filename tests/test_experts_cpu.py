@@ -131,3 +131,22 @@ def test_blocks_without_experts_are_unchanged():
     assert shared and all(torch.equal(plain.state_dict()[k], mixed.state_dict()[k]) for k in shared)
     model = fe.EquivariantTransformer(rp, rp, rp, num_layers=2, num_experts=3, experts_per_node=1)
     assert all(layer.experts.router.top_k == 1 for layer in model.layers)
+
+
+def test_numbers_of_experts():
+    rp = fe.Repr([0, 1], 8)
+    for n, k in ((0, 1), (1025, 2)):
+        with pytest.raises(ValueError, match="num_experts must be 1 to 1024"):
+            fe.ExpertRouter(rp, n, k)
+    with pytest.raises(ValueError, match="at most 64"):
+        fe.ExpertRouter(rp, 100, 65)
+    with pytest.raises(ValueError, match="must not be negative"):
+        fe.EquivariantTransformerBlock(rp, rp, num_experts=-1)
+
+
+def test_linear_abi_refuses_a_bias_without_columns():
+    lib = N.load_library()
+    one = (ctypes.c_int32 * 1)(0)
+    for cols, n in ((None, 1), (one, 0)):
+        assert lib.feq_expert_linear_fwd(one, 1, 2, 10, 4, 4, 0, FAKE, FAKE, FAKE, FAKE, n, cols, FAKE, None) != 0
+        assert "bias" in lib.feq_last_error().decode()

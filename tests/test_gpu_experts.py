@@ -72,7 +72,8 @@ def check_topk(dev, logits, k, normalize, seed=0):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows,experts,k", [(1, 1, 1), (5, 2, 1), (9, 7, 7), (100, 8, 2), (64, 16, 4), (33, 64, 8),
                                             (17, 100, 3), (9, 256, 5), (5, 512, 2), (4, 513, 4), (3, 1000, 64),
-                                            (3, 1024, 1), (3001, 8, 2)])
+                                            (3, 1024, 1), (3001, 8, 2), (50, 9, 2), (41, 61, 9), (19, 65, 4), (23, 201, 6),
+                                            (12, 515, 8), (5, 1021, 33)])
 def test_topk_sizes(dev, rows, experts, k, dtype):
     logits = (2 * torch.randn(rows, experts, generator=gen(rows + experts))).to(dev, dtype)
     for normalize in (True, False):
@@ -139,6 +140,20 @@ def test_topk_gradients_one_by_one_shapes_and_no_rows(dev):
     assert ge.shape == (0, 12)
 
 
+@pytest.mark.parametrize("experts", [5, 24, 67, 530])
+def test_topk_of_unaligned_logits(dev, experts):
+    for dtype in TYPES:
+        l = torch.randn(31, experts, generator=gen(experts)).to(dev, dtype)
+        apart = torch.cat([l.new_zeros(1), l.reshape(-1)])[1:].view(l.shape)
+        both = []
+        for t in (l, apart):
+            t = t.detach().requires_grad_()
+            ids, w, mean = fe.expert_topk(t, 3, False)
+            both.append((ids, w, mean, torch.autograd.grad(w.square().sum() + mean.square().sum(), [t])[0]))
+        for a, b in zip(*both):
+            assert torch.equal(a, b)
+
+
 def test_topk_gradient_against_differences(dev):
     l = torch.randn(3, 6, generator=gen(7), dtype=torch.float64)
     gw = torch.randn(3, 2, generator=gen(8), dtype=torch.float64)
@@ -171,7 +186,7 @@ def some_ids(g, rows, k, experts, bad=0.1):
 
 @pytest.mark.parametrize("rows,k,experts", [(0, 2, 4), (1, 1, 1), (5, 1, 3), (100, 2, 8), (64, 1, 64), (333, 3, 65),
                                             (4096, 2, 8), (8193, 1, 5), (1000, 64, 9), (3000, 4, 1024), (2049, 8, 100),
-                                            (30011, 2, 16), (700, 2, 1024)])
+                                            (30011, 2, 16), (700, 2, 1024), (4095, 2, 960), (4095, 2, 962), (70000, 2, 1023)])
 def test_plan_is_exact(dev, rows, k, experts):
     ids = some_ids(gen(rows + k), rows, k, experts)
     order, positions, offsets = OE.plan(ids, experts)
@@ -195,7 +210,8 @@ def test_plan_of_one_expert_none_and_small_integer_types(dev):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("lead,rows,k,width,experts", [
     ((), 1, 1, 1, 1), ((), 7, 2, 3, 4), ((9,), 50, 2, 64, 8), ((2, 3), 33, 3, 20, 5), ((49,), 20, 4, 128, 16),
-    ((4,), 100, 5, 33, 8), ((), 300, 8, 576, 12), ((1,), 65, 1, 1152, 3), ((3,), 41, 9, 6, 10)])
+    ((4,), 100, 5, 33, 8), ((), 300, 8, 576, 12), ((1,), 65, 1, 1152, 3), ((3,), 41, 9, 6, 10),
+    ((4,), 30, 2, 5, 3), ((9,), 12, 3, 13, 4), ((16,), 11, 4, 259, 5)])
 def test_rows_and_their_gradients(dev, lead, rows, k, width, experts, dtype):
     g = gen(rows * k + width)
     ids = some_ids(g, rows, k, experts)
@@ -324,7 +340,7 @@ def check_linear(dev, lvals, counts, unrouted, cin, cout, dtype, bias=True, seed
 
 
 CHANNELS = [(64, 128), (128, 64), (8, 8), (33, 7), (1, 1), (160, 200), (12, 260), (300, 20), (301, 133), (131, 9),
-            (22, 26), (9, 98)]
+            (22, 26), (9, 98), (32, 64), (30, 70), (48, 61), (72, 9), (5, 129), (136, 72), (129, 65)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -352,6 +368,8 @@ def test_linear_many_chunks(dev):
     """Experts of several weight-gradient chunks beside ones of one and none."""
     check_linear(dev, (0, 1), [5000, 100, 0, 2000, 129], 50, 16, 24, torch.float32, seed=3)
     check_linear(dev, (0,), [3000, 64, 1500], 0, 64, 64, torch.bfloat16, seed=4)
+    check_linear(dev, (0, 0), [30000, 1], 3, 34, 51, torch.float32, seed=5)      # more than eight chunks an expert
+    check_linear(dev, (0,), [9000, 40000], 0, 32, 32, torch.float16, seed=6)
 
 
 def test_linear_views_and_two_dimensions(dev):
@@ -366,6 +384,34 @@ def test_linear_views_and_two_dimensions(dev):
     flat = torch.randn(4 * 16 + 1, generator=g).to(dev)[1:].view(4, 16)     # 4-byte aligned
     w16 = torch.randn(2, 1, 8, 16, generator=g).to(dev)
     assert torch.equal(fe.expert_linear(flat, w16, plan), fe.expert_linear(flat.clone(), w16, plan))
+
+
+@pytest.mark.parametrize("cin,cout", [(5, 6), (24, 40), (41, 30), (150, 136), (137, 9)])
+def test_linear_of_unaligned_tables(dev, cin, cout):
+    """Every table one element further on: as far from the formula as aligned ones, and zeros behind the last row."""
+    for dtype in TYPES:
+        g = gen(cin)
+        ids = some_ids(g, 70, 1, 3)
+        plan = fe.ExpertPlan(ids.to(dev), 3)
+        n = plan.offsets[-1].item()
+
+        def apart(*shape):
+            return torch.randn(torch.Size(shape).numel() + 1, generator=g).to(dtype)[1:].view(shape)
+        x, w, b, gy = apart(4, 70, cin), apart(3, 2, cout, cin), apart(3, cout, 1), apart(4, 70, cout)
+        # moved to the device with the element before them
+        far = [torch.cat([t.new_zeros(1), t.reshape(-1)]).to(dev)[1:].view(t.shape) for t in (x, w, b, gy)]
+        leaves = [t.requires_grad_() for t in far[:3]]
+        y = fe.expert_linear(*leaves[:2], plan, (0, 1), leaves[2])
+        got = (y, *torch.autograd.grad(y, leaves, far[3]))
+
+        def reference(f):
+            l64 = [f(t.double()).requires_grad_() for t in (x, w, b)]
+            y64 = OE.linear(*l64[:2], plan.offsets.cpu(), (0, 1), l64[2])
+            return (y64.detach(), *torch.autograd.grad(y64, l64, f(gy.double())))
+        want, mass = reference(lambda t: t.clone()), reference(torch.abs)
+        for a, r, m, terms in zip(got, want, mass, (2 * cin + 2, 2 * cout, 700, 700)):
+            within(a, r, HALF[dtype] * r.abs() + U * terms * m)
+        assert not y[:, n:].any() and not got[1][:, n:].any()
 
 
 def test_linear_infinity_stays_in_its_row_and_expert(dev):
@@ -425,6 +471,127 @@ def test_refusals(dev):
         fe.expert_linear(xs, w.half(), plan)
 
 
+def test_a_plan_is_for_reading(dev):
+    """Places that a kernel would write to are those of the sort, or the call is refused; copies are plans too."""
+    import copy
+    import pickle
+    ids = torch.tensor([[0, 1], [2, 0], [-1, 1]], device=dev)
+    x, w = torch.randn(3, 8, device=dev, requires_grad=True), torch.ones(3, 2, device=dev, requires_grad=True)
+    lw = torch.randn(3, 1, 8, 8, device=dev, requires_grad=True)
+    plan = fe.ExpertPlan(ids, 3)
+    with pytest.raises(AttributeError):
+        plan.positions = plan.positions.long()
+    for other in (copy.deepcopy(plan), pickle.loads(pickle.dumps(plan))):
+        assert torch.equal(other.order, plan.order) and torch.equal(other.dispatch(x), plan.dispatch(x))
+    xs = plan.dispatch(x)
+    ys = fe.expert_linear(xs, lw, plan)
+    y = plan.combine(ys, w)
+    plan.offsets[-1] += 1
+    with pytest.raises(RuntimeError, match="offsets of an ExpertPlan have been modified"):
+        plan.dispatch(x)
+    with pytest.raises(RuntimeError, match="have been modified"):
+        fe.expert_linear(xs, lw, plan)
+    for out, leaf in ((y, w), (ys, lw), (xs, x)):
+        with pytest.raises(RuntimeError, match="have been modified"):
+            torch.autograd.grad(out.sum(), [leaf], retain_graph=True)
+    plan = fe.ExpertPlan(ids, 3)
+    plan.positions.clamp_(max=2)
+    with pytest.raises(RuntimeError, match="positions of an ExpertPlan have been modified"):
+        plan.combine(ys, w)
+    with torch.inference_mode():
+        plan = fe.ExpertPlan(ids, 3)
+        assert plan.combine(plan.dispatch(x), w).shape == (3, 8)
+
+
+def test_derivatives_that_there_are_not(dev):
+    """Inputs changed before the backward, second derivatives and forward mode raise; none gives a wrong gradient."""
+    ids = torch.tensor([[0, 1], [1, 0]], device=dev)
+    plan = fe.ExpertPlan(ids, 2)
+    calls = [(lambda l: fe.expert_topk(l, 2, False)[1], [(5, 4)]),
+             (lambda x: plan.dispatch(x), [(2, 6)]),
+             (lambda ys, w: plan.combine(ys, w), [(4, 6), (2, 2)]),
+             (lambda x, w: fe.expert_linear(x, w, plan), [(4, 6), (2, 1, 3, 6)])]
+    for k, (call, shapes) in enumerate(calls):
+        for i in range(len(shapes)):
+            args = [torch.randn(s, generator=gen(i)).to(dev).requires_grad_() for s in shapes]
+            out = call(*args)
+            grads = torch.autograd.grad(out.square().sum(), args, create_graph=True)
+            with pytest.raises(RuntimeError, match="no second derivative"):
+                grads[i].sum().backward()
+            if k != 1:                           # dispatch keeps none of its input
+                out = call(*args)
+                with torch.no_grad():
+                    args[i].add_(1.0)
+                with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                    out.sum().backward()
+            with torch.autograd.forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+                duals = [torch.autograd.forward_ad.make_dual(a.detach(), torch.ones_like(a)) if j == i else a.detach()
+                         for j, a in enumerate(args)]
+                call(*duals)
+    l = torch.randn(5, 4, device=dev, requires_grad=True)
+    chosen, w, _ = fe.expert_topk(l, 2)
+    chosen.clamp_(max=1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        w.square().sum().backward()
+
+
+def test_past_32_bit_offsets(dev):
+    """Rows whose elements lie behind the first 2^31, read and written at their places."""
+    rows, width = 2 ** 20 + 5, 1030                  # two slots a row: 2.2e9 elements in expert order
+    g = gen(17)
+    ids = torch.zeros(rows, 2, dtype=torch.int64, device=dev)
+    ids[:, 1], ids[0], ids[-1, 1] = 1, 1, -1
+    plan = fe.ExpertPlan(ids, 2)
+    x = torch.zeros(rows, width, device=dev, dtype=torch.bfloat16)
+    x[0], x[-1] = torch.randn(2, width, generator=g).to(dev, torch.bfloat16)
+    xs = plan.dispatch(x)
+    slots = 2 * rows
+    places = plan.positions[[0, -1]].tolist()        # row 0 behind the expert 0's, the last slot unrouted
+    assert places[1][1] == slots - 1 and places[0][0] == rows - 1
+    assert torch.equal(xs[rows - 1], x[0]) and torch.equal(xs[rows], x[0]) and torch.equal(xs[rows - 2], x[-1])
+    assert not xs[-1].any() and not xs[slots // 2 + 9].any()
+    w = torch.ones(rows, 2, device=dev)
+    xs[slots - 2] = 1.0                              # row rows - 2's second slot, in the last places
+    y = plan.combine(xs, w)
+    assert torch.equal(y[0], (2 * x[0].float()).bfloat16()) and torch.equal(y[-1], x[-1])
+    assert (y[-2] == 1).all() and not y[-3].any()
+    del xs, y
+    lw = torch.randn(2, 1, 8, 1030, generator=g).to(dev, torch.bfloat16)
+    big = torch.zeros(slots, width, device=dev, dtype=torch.bfloat16)
+    big[slots - 2], big[3] = x[0], x[-1]
+    out = fe.expert_linear(big, lw, plan)
+    small = fe.ExpertPlan(torch.tensor([0, 1], device=dev), 2)
+    want = fe.expert_linear(torch.stack([x[-1], x[0]]), lw, small)
+    assert torch.equal(out[3], want[0]) and torch.equal(out[slots - 2], want[1]) and not out[slots - 1].any()
+    del big
+    gy = torch.zeros(slots, 8, device=dev, dtype=torch.bfloat16)
+    gy[slots - 2], gy[3] = 1.0, 2.0
+    lx = torch.zeros(slots, width, device=dev, dtype=torch.bfloat16)
+    lx[slots - 2], lx[3] = x[0], x[-1]
+    lx.requires_grad_()
+    gx, gw = torch.autograd.grad(fe.expert_linear(lx, lw.requires_grad_(), plan), [lx, lw], gy)
+    sx = torch.stack([x[-1], x[0]]).requires_grad_()
+    gx2, gw2 = torch.autograd.grad(fe.expert_linear(sx, lw, small), [sx, lw], gy[[3, slots - 2]])
+    assert torch.equal(gx[3], gx2[0]) and torch.equal(gx[slots - 2], gx2[1]) and torch.equal(gw, gw2)
+
+
+def test_topk_past_32_bit_offsets(dev):
+    rows, experts = 2 ** 25 + 7, 64                  # 2.1e9 logits
+    l = torch.zeros(rows, experts, device=dev, dtype=torch.float16)
+    tail = torch.randn(9, experts, generator=gen(18)).to(dev, torch.float16)
+    l[-9:] = tail
+    l.requires_grad_()
+    ids, w, _ = fe.expert_topk(l, 2)
+    t = tail.clone().requires_grad_()
+    ids2, w2, _ = fe.expert_topk(t, 2)
+    assert torch.equal(ids[-9:], ids2) and torch.equal(w[-9:], w2) and (ids[0] == torch.tensor([0, 1], device=dev)).all()
+    gw = torch.zeros_like(w)
+    gw[-9:, 0] = 1.0
+    (gl,) = torch.autograd.grad(w, [l], gw)
+    (gt,) = torch.autograd.grad(w2, [t], gw[-9:].clone())
+    assert torch.equal(gl[-9:], gt) and not gl[:9].any()
+
+
 # ---- a run of them together ------------------------------------------------------------
 
 @pytest.mark.parametrize("top_k", [1, 2])
@@ -437,10 +604,12 @@ def test_expert_mlp_matches_the_oracle(dev, top_k):
             b.normal_(generator=torch.Generator(device=dev).manual_seed(1))
     x = torch.randn(403, 32, 9, generator=gen(6))
     xl = x.to(dev).requires_grad_()
-    y = mlp(xl)
+    terms = []
+    y = mlp(xl, balance=terms)
+    (own,) = terms
     gy = torch.randn(403, 32, 9, generator=gen(7))
     params = dict(mlp.named_parameters())
-    grads = torch.autograd.grad((y * gy.to(dev)).sum() + mlp.balance, [xl, *params.values()])
+    grads = torch.autograd.grad((y * gy.to(dev)).sum() + own, [xl, *params.values()])
 
     x64 = x.double().requires_grad_()
     p64 = {k: v.detach().double().cpu().requires_grad_() for k, v in params.items()}
@@ -459,7 +628,7 @@ def test_expert_mlp_matches_the_oracle(dev, top_k):
     y64 = OE.expert_mlp(x64, ids, w, {k: p64[v] for k, v in names.items()}, (0, 1, 2), 1e-8)
     want = torch.autograd.grad((y64 * gy.double()).sum() + balance, [x64, *p64.values()])
     rel = lambda a, b: ((a.detach().double().cpu() - b).abs().max() / b.abs().max()).item()
-    assert rel(y, y64.detach()) < 1e-5 and rel(mlp.balance, balance.detach()) < 1e-5
+    assert rel(y, y64.detach()) < 1e-5 and rel(own, balance.detach()) < 1e-5
     for name, a, b in zip(["x", *params], grads, want):
         if top_k == 1 and name.startswith("router"):     # one weight of 1: only the balance is left, tiny
             assert (a.detach().double().cpu() - b).abs().max() < 1e-5
@@ -488,7 +657,10 @@ def test_expert_block_is_equivariant_and_trains(dev):
     y2 = model((xyz @ R.t()).to(dev), (x @ D.t()).to(dev), graph)
     err = ((y2 - y @ D.t().to(dev)).abs().max() / y.abs().max()).item()
     assert err < 1e-2, err           # the bar of the model's other equivariance tests
-    loss = y.pow(2).mean() + 0.01 * sum(layer.experts.balance for layer in model.layers)
+    terms = []
+    y = model(xyz.to(dev), x.to(dev), graph, balance=terms)
+    assert len(terms) == 2
+    loss = y.pow(2).mean() + 0.01 * sum(terms)
     loss.backward()
     missing = [k for k, p in model.named_parameters() if p.grad is None]
     assert not missing, missing
@@ -503,15 +675,17 @@ def test_half_precision_block_and_mlp(dev, dtype):
     rp = fe.Repr([0, 1], 16)
     mlp = fe.EquivariantExpertMLP(rp, 4, 2).to(dev, dtype)
     x = torch.randn(50, 16, 4, generator=gen(8)).to(dev, dtype).requires_grad_()
-    y = mlp(x)
-    (gx,) = torch.autograd.grad(y.sum() + mlp.balance, [x])
+    terms = []
+    y = mlp(x, terms)
+    (gx,) = torch.autograd.grad(y.sum() + terms[0], [x])
     assert y.dtype == gx.dtype == dtype and torch.isfinite(y).all() and torch.isfinite(gx).all()
     block = fe.EquivariantTransformerBlock(rp, rp, num_heads=2, num_experts=4).to(dev, dtype)
     graph = fe.Graph.random(50, 300, device=dev)
     vec = torch.randn(300, 3, generator=gen(9)).to(dev)
     (P,) = fe.WignerDBasis([rp]).to(dev)(vec)
-    out = block(P.to(dtype), P.to(dtype), x, vec.norm(dim=-1).to(dtype), graph)
+    out = block(P.to(dtype), P.to(dtype), x, vec.norm(dim=-1).to(dtype), graph, balance=terms)
     assert out.dtype == dtype and torch.isfinite(out).all()
+    assert len(terms) == 2 and torch.isfinite(terms[1])
     with pytest.raises(TypeError, match="float64"):
         fe.EquivariantExpertMLP(rp, 4, 2).to(dev).double()(x.double())
 
@@ -527,7 +701,8 @@ def test_captured_training_step(dev):
     leaves = [x, *mlp.parameters()]
 
     def step():
-        loss = (mlp(x) * gy).sum((1, 2)).mean() + mlp.balance
+        terms = []
+        loss = (mlp(x, terms) * gy).sum((1, 2)).mean() + terms[0]
         loss.backward()
         return loss
 
@@ -538,7 +713,8 @@ def test_captured_training_step(dev):
         graph.replay()
         torch.cuda.synchronize()
         got = [t.grad.clone() for t in leaves]
-        y = (mlp(x) * gy).sum((1, 2)).mean() + mlp.balance
+        terms = []
+        y = (mlp(x, terms) * gy).sum((1, 2)).mean() + terms[0]
         want = torch.autograd.grad(y, leaves)
         for a, b in zip(got, want):
             assert torch.allclose(a, b, rtol=1e-5, atol=1e-6 * b.abs().max().item())
@@ -564,3 +740,71 @@ def test_another_stream_and_the_same_bits(dev):
     torch.cuda.current_stream().wait_stream(side)
     for a, b, c in zip(first, other, step()):
         assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_two_graphs_two_threads_and_an_empty_input(dev):
+    """Captured steps replayed in turn, with eager work between, and threads on streams of their own: each call's
+    results are its own."""
+    import threading
+    from flash_eq.capture import capture_step
+    torch.manual_seed(8)
+    rp = fe.Repr([0, 1], 16)
+    mlps = [fe.EquivariantExpertMLP(rp, n, 2).to(dev) for n in (4, 9)]
+    xs = [torch.randn(n, 16, 4, generator=gen(n)).to(dev).requires_grad_() for n in (700, 5001)]
+
+    def eager(i):
+        terms = []
+        loss = mlps[i](xs[i], terms).square().sum((1, 2)).mean() + terms[0]
+        return loss, [xs[i], *mlps[i].parameters()]
+
+    def step_of(i):
+        def step():
+            loss, _ = eager(i)
+            loss.backward()
+            return loss
+        return step
+    graphs = [capture_step(step_of(i), eager(i)[1]) for i in range(2)]
+    for k in range(3):
+        for x in xs:
+            with torch.no_grad():
+                x.copy_(torch.randn(x.shape, generator=gen(60 + k)))
+        for graph, _ in graphs:
+            graph.replay()
+        for i in range(2):
+            torch.cuda.synchronize()
+            loss, leaves = eager(i)
+            for leaf, want in zip(leaves, torch.autograd.grad(loss, leaves)):
+                assert torch.allclose(leaf.grad, want, rtol=1e-5, atol=1e-6 * want.abs().max().item())
+        torch.cuda.synchronize()
+
+    want = [torch.autograd.grad(*eager(i)) for i in range(2)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(5):
+                got = torch.autograd.grad(*eager(i))
+                torch.cuda.current_stream().synchronize()
+                wrong.extend(i for a, b in zip(got, want[i]) if not torch.allclose(a, b, rtol=1e-5, atol=1e-6 * b.abs().max().item()))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+    terms = []
+    e = torch.empty(0, 16, 4, device=dev, requires_grad=True)
+    y = mlps[0](e, terms)
+    grads = torch.autograd.grad(y.sum() + terms[0], [e, *mlps[0].parameters()], allow_unused=True)
+    assert y.shape == (0, 16, 4) and terms[0] == 0 and not any(g.any() for g in grads if g is not None)
+
+
+def test_a_module_is_copied_and_saved_after_a_call(dev):
+    import copy
+    mlp = fe.EquivariantExpertMLP(fe.Repr([0, 1], 8), 4, 2).to(dev)
+    x = torch.randn(30, 8, 4, generator=gen(1)).to(dev)
+    terms = []
+    y = mlp(x, terms)
+    assert torch.equal(copy.deepcopy(mlp)(x), y) and torch.equal(mlp(x), y)

@@ -20,7 +20,9 @@ TINY = {torch.float32: 0.0, torch.float16: 2.0 ** -25, torch.bfloat16: 0.0}     
 TYPES = [torch.float32, torch.float16, torch.bfloat16]
 # one element; no spread; odd; each lane-group form; a workgroup a row; rows beyond its registers, odd too
 SIZES = [(1, 1), (3, 2), (5, 7), (100, 192), (33, 55), (7, 1000), (64, 1024), (17, 1152), (9, 4096), (3, 8192),
-         (2, 8200), (2, 20000), (3, 16391), (2050, 64), (5000, 8), (300, 896), (4, 2049)]
+         (2, 8200), (2, 20000), (3, 16391), (2050, 64), (5000, 8), (300, 896), (4, 2049),
+         # a last vector that shares elements, in each form
+         (6, 9), (40, 63), (21, 257), (8, 515), (5, 1027), (3, 6978), (3, 8191), (70, 8193)]
 
 
 def within(got, want, tol, dtype):
@@ -127,8 +129,7 @@ def test_rows_of_a_wider_table_and_strided_gradients(dev, width, cut):
     check(dev, x, w, b, gy)
     a = ops.layer_norm(x, w, b)
     assert a.is_contiguous()
-    if cut[0] % 4 == 0 or width % 4:     # else one reads vectors and one elements, whose sums differ in order
-        assert torch.equal(a, ops.layer_norm(x.contiguous(), w, b))
+    assert torch.equal(a, ops.layer_norm(x.contiguous(), w, b))
 
 
 def test_shapes_and_broadcast_gradients(dev):
@@ -212,8 +213,64 @@ def test_captured_step_and_another_stream(dev):
     assert torch.equal(y2, y)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [5, 17, 100, 1030, 8200])
+def test_unaligned_tables(dev, width, dtype):
+    """Tables and parameters from an address that is a multiple of their element alone: the bits of aligned ones."""
+    x, w, b, gy = inputs(dev, 23, width, dtype, width)
+
+    def apart(t):
+        return torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+
+    def step(x, w, b, gy):
+        x, w, b = (t.detach().requires_grad_() for t in (x, w, b))
+        y = ops.layer_norm(x, w, b)
+        return (y.detach(), *torch.autograd.grad(y, [x, w, b], gy))
+
+    for one, two in zip(step(x, w, b, gy), step(*(apart(t) for t in (x, w, b, gy)))):
+        assert torch.equal(one, two)
+
+
+def test_past_32_bit_offsets(dev):
+    """Rows whose elements lie behind the first 2^31, read and written at their places."""
+    rows, width = 2 ** 21 + 3, 1030              # 2.2e9 elements
+    x = torch.empty(rows, width, device=dev, dtype=torch.bfloat16)
+    x[-4:] = torch.randn(4, width, generator=torch.Generator().manual_seed(1)).to(dev, torch.bfloat16)
+    x[:-4] = 0
+    x.requires_grad_()
+    y = ops.layer_norm(x)
+    y0 = ops.layer_norm(x.detach()[-4:].clone().requires_grad_())
+    assert torch.equal(y[-4:], y0) and not y[:4].any() and not y[rows // 2].any()
+    gy = torch.zeros_like(x)
+    gy[-4:] = 1.0
+    (gx,) = torch.autograd.grad(y, [x], gy)
+    x0 = x.detach()[-4:].clone().requires_grad_()
+    (g0,) = torch.autograd.grad(ops.layer_norm(x0), [x0], gy[-4:].clone())
+    assert torch.equal(gx[-4:], g0) and not gx[:4].any()
+
+
+def test_inputs_changed_before_the_backward_are_refused(dev):
+    x, w, b, gy = inputs(dev, 8, 40, torch.float32, 12)
+    for i in range(2):
+        args = [x.clone().requires_grad_(), w.clone().requires_grad_(), b.clone().requires_grad_()]
+        y = ops.layer_norm(*args)
+        with torch.no_grad():
+            args[i].add_(1.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward(gy)
+
+
+def test_no_forward_mode(dev):
+    x = torch.randn(4, 8, device=dev)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            ops.layer_norm(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+
+
 def test_refusals(dev):
     x = torch.randn(4, 8, device=dev)
+    with pytest.raises(RuntimeError, match="exceeds 2\\^24"):
+        ops.layer_norm(torch.zeros(1, 2 ** 24 + 1, device=dev))
     with pytest.raises(TypeError, match="float64"):
         ops.layer_norm(x.double())
     with pytest.raises(ValueError, match=r"weight must have shape \(8,\)"):
