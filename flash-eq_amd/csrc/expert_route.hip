@@ -100,11 +100,12 @@ __device__ __forceinline__ float row_exp(const float (&x)[NC][V], int G, float (
 }
 
 // X >= V.  KMAX: the choices are kept in registers until the weights' sum is known (K <= KMAX); 0: they wait in
-// memory.
+// memory.  The workgroups' sums of probabilities go to part (gridDim.x, X), or as means to mean (X) where there is
+// one workgroup (a launch of 4 us less); neither: not wanted.
 template <class T, int V, int NC, int KMAX>
 __global__ void __launch_bounds__(kTopkThreads)
 k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normalize, int64_t* __restrict__ ids,
-           float* __restrict__ weights, float* __restrict__ part, int G) {
+           float* __restrict__ weights, float* __restrict__ part, float* __restrict__ mean_out, float inv_rows, int G) {
     __shared__ float sums[4 * kMaxExperts];
     const int l = threadIdx.x & (G - 1);
     const int per = kTopkThreads / G;
@@ -199,7 +200,7 @@ k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normali
 #pragma unroll
             for (int j = 0; j < V; ++j) x[c][j] = next[c][j];
     }
-    if (!part) return;
+    if (!part && !mean_out) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -210,9 +211,11 @@ k_topk_fwd(const T* __restrict__ logits, int64_t rows, int X, int K, int normali
             if (lane < G && j >= sh[c]) sums[wave * X + at[c] + j] = a;
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < X; i += kTopkThreads)
-        part[static_cast<int64_t>(blockIdx.x) * X + i] =
-            (sums[i] + sums[X + i]) + (sums[2 * X + i] + sums[3 * X + i]);
+    for (int i = threadIdx.x; i < X; i += kTopkThreads) {
+        const float a = (sums[i] + sums[X + i]) + (sums[2 * X + i] + sums[3 * X + i]);
+        if (part) part[static_cast<int64_t>(blockIdx.x) * X + i] = a;
+        else mean_out[i] = a * inv_rows;
+    }
 }
 
 // mean[i] = (sum of the workgroups' sums) / rows, 16 experts a workgroup.
@@ -581,7 +584,8 @@ using namespace feq;
 
 extern "C" size_t feq_expert_topk_workspace(int64_t rows, int32_t experts) {
     if (rows < 1 || experts < 1 || experts > kMaxExperts) return 0;
-    return sizeof(float) * static_cast<size_t>(experts) * topk_blocks(rows, experts);
+    const int blocks = topk_blocks(rows, experts);
+    return blocks > 1 ? sizeof(float) * static_cast<size_t>(experts) * blocks : 0;
 }
 
 extern "C" int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t experts, int32_t dtype, int32_t top_k,
@@ -589,12 +593,13 @@ extern "C" int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t exp
                                    size_t ws_bytes, feq_stream_t stream) {
     if (int rc = topk_check(rows, experts, top_k, dtype)) return rc;
     if (rows && (!logits || !ids || !weights)) return fail(FEQ_ERR_INVALID, "NULL pointer");
-    if (mean && rows && (!workspace || ws_bytes < feq_expert_topk_workspace(rows, experts)))
-        return fail(FEQ_ERR_WORKSPACE, "top-k workspace of %zu bytes, %zu needed", ws_bytes,
-                    feq_expert_topk_workspace(rows, experts));
+    const size_t need = mean ? feq_expert_topk_workspace(rows, experts) : 0;
+    if (need && (!workspace || ws_bytes < need))
+        return fail(FEQ_ERR_WORKSPACE, "top-k workspace of %zu bytes, %zu needed", ws_bytes, need);
     hipStream_t s = stream_of(stream);
     const int G = topk_lanes(experts, kForwardNarrow), blocks = rows ? topk_blocks(rows, experts) : 0;
-    float* part = mean ? static_cast<float*>(workspace) : nullptr;
+    float* part = need ? static_cast<float*>(workspace) : nullptr;
+    const float inv_rows = rows ? 1.0f / static_cast<float>(rows) : 0.0f;
     if (rows) {
         const int rc = with_dtype(dtype, [&](auto t) -> int {
             using T = decltype(t);
@@ -602,7 +607,7 @@ extern "C" int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t exp
                 auto run = [&](auto km) -> int {
                     auto kern = k_topk_fwd<T, decltype(v)::value, decltype(nc)::value, decltype(km)::value>;
                     FEQ_LAUNCH("k_topk_fwd", kern, dim3(blocks), dim3(kTopkThreads), 0, s, static_cast<const T*>(logits),
-                               rows, experts, top_k, normalize, ids, weights, part, G);
+                               rows, experts, top_k, normalize, ids, weights, part, part ? nullptr : mean, inv_rows, G);
                     return FEQ_OK;
                 };
                 if (top_k <= 2) return run(std::integral_constant<int, 2>{});
@@ -612,9 +617,9 @@ extern "C" int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t exp
         });
         if (rc) return rc;
     }
-    if (mean)     // of no rows: 0
+    if (mean && blocks != 1)     // of no rows: 0
         FEQ_LAUNCH("k_topk_mean", k_topk_mean, dim3(ceil_div(experts, 16)), dim3(1024), 0, s, part, blocks, experts,
-                   rows ? 1.0f / static_cast<float>(rows) : 0.0f, mean);
+                   inv_rows, mean);
     return FEQ_OK;
 }
 

@@ -30,8 +30,10 @@ constexpr int kLnWaveElems = 16;    // elements a lane holds in the lane-group f
 constexpr int kLnBlockElems = 32;   // and in the workgroup form
 constexpr int kLnFwdBlocks = 2048;   // workgroups of the forward: what the chip holds, each over many rows
 constexpr int kLnMaxBlocks = 1024;  // workgroups of the backward, and weight-gradient partials
+constexpr int64_t kLnMaxWidth = 1 << 24;
 constexpr int kLnWide = 1024;       // threads of the _wide kernels
 constexpr int kLnWideBlocks = 64;   // their weight-gradient partials
+constexpr int kLnOneRows = 8;       // rows of a lane group up to which one workgroup makes the backward
 
 // Sum over the workgroup of NW waves; red holds 2 NW floats, one use per call.
 template <int NW>
@@ -132,13 +134,13 @@ k_ln_fwd(const T* __restrict__ x, int64_t rows, int width, int64_t ldx, const vo
     }
 }
 
-// part: (gridDim.x, 2, width) sums of grad_w and grad_b, or NULL where neither
-// is wanted; gx may be NULL.
+// The workgroups' sums of grad_w and grad_b go to part (gridDim.x, 2, width), or as gradients to gw and gb where there
+// is one workgroup; all NULL: not wanted.  gx may be NULL.
 template <class T, int V, int NV, bool BLK>
 __global__ void __launch_bounds__(kLnThreads)
 k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t rows, int width, int64_t ldx,
          const void* __restrict__ w, int pdt, const float* __restrict__ mean, const float* __restrict__ rstd,
-         T* __restrict__ gx, float* __restrict__ part, int G) {
+         T* __restrict__ gx, float* __restrict__ part, void* __restrict__ gw, void* __restrict__ gb, int G) {
     __shared__ float red[8];
     // the waves' column sums: 4 waves x (64 lanes x NV V columns) x 2
     __shared__ float sums[BLK ? 1 : 4 * 64 * NV * V * 2];
@@ -205,17 +207,23 @@ k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t
             }
         }
     }
-    if (!part) return;
+    if (!part && !gw && !gb) return;
     float* pw = part + static_cast<int64_t>(blockIdx.x) * 2 * width;
+    auto put = [&](int c, float a, float d) {
+        if (part) {
+            pw[c] = a;
+            pw[width + c] = d;
+        } else {
+            if (gw) store_any(gw, pdt, c, a);
+            if (gb) store_any(gb, pdt, c, d);
+        }
+    };
     if constexpr (BLK) {
 #pragma unroll
         for (int v = 0; v < NV; ++v)
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                if (j >= sh[v]) {
-                    pw[at[v] + j] = dw[v][j];
-                    pw[width + at[v] + j] = db[v][j];
-                }
+                if (j >= sh[v]) put(at[v] + j, dw[v][j], db[v][j]);
             }
     } else {
         // the groups of a wave, then the waves
@@ -245,8 +253,7 @@ k_ln_bwd(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t
                 a += sums[(u * cols + place) * 2];
                 d += sums[(u * cols + place) * 2 + 1];
             }
-            pw[c] = a;
-            pw[width + c] = d;
+            put(c, a, d);
         }
     }
 }
@@ -339,12 +346,12 @@ k_ln_bwd_wide(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, in
     }
 }
 
-// part (gridDim.y, 2, width): a thread per column, a run of rows per blockIdx.y.
+// part (gridDim.y, 2, width): a thread per column, a run of rows per blockIdx.y; NULL (one run): gradients to gw, gb.
 template <class T>
 __global__ void __launch_bounds__(256)
 k_ln_cols_wide(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, int64_t rows, int64_t width,
                int64_t ldx, const float* __restrict__ mean, const float* __restrict__ rstd, int64_t per,
-               float* __restrict__ part) {
+               float* __restrict__ part, void* __restrict__ gw, void* __restrict__ gb, int pdt) {
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
     if (c >= width) return;
     const int64_t r0 = blockIdx.y * per, r1 = r0 + per < rows ? r0 + per : rows;
@@ -354,23 +361,28 @@ k_ln_cols_wide(const T* __restrict__ gy, int64_t ldg, const T* __restrict__ x, i
         a += g * ((static_cast<float>(x[r * ldx + c]) - mean[r]) * rstd[r]);
         d += g;
     }
-    float* pw = part + static_cast<int64_t>(blockIdx.y) * 2 * width;
-    pw[c] = a;
-    pw[width + c] = d;
+    if (part) {
+        float* pw = part + static_cast<int64_t>(blockIdx.y) * 2 * width;
+        pw[c] = a;
+        pw[width + c] = d;
+    } else {
+        if (gw) store_any(gw, pdt, c, a);
+        if (gb) store_any(gb, pdt, c, d);
+    }
 }
 
 // ---- which form takes a width ----------------------------------------------------
 struct LnForm {
-    bool wide;   // the _wide kernels
     bool blk;    // a workgroup per row, else a group of G lanes
     int G, NV;
 };
+bool ln_wide(int64_t width) { return width > kLnThreads * kLnBlockElems; }     // the _wide kernels
 
 // NV of the instances: the smallest that covers.
 inline int ln_nv(int64_t n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 3 ? 3 : n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32; }
 
 LnForm ln_form(int64_t width, int V) {
-    LnForm f{false, false, 64, 1};
+    LnForm f{false, 64, 1};
     const int64_t nvec = ceil_div(width, V);
     if (V == 1) {                // a column a lane: fewer columns than a vector
         f.G = 1;
@@ -387,7 +399,6 @@ LnForm ln_form(int64_t width, int V) {
     }
     f.blk = true;
     f.NV = ln_nv(ceil_div(nvec, kLnThreads));
-    f.wide = ceil_div(nvec, kLnThreads) * V > kLnBlockElems;
     return f;
 }
 
@@ -429,17 +440,18 @@ int ln_fwd_run(const T* x, int64_t rows, int width, int64_t ldx, const void* w, 
 
 template <class T, int V>
 int ln_bwd_run(const T* gy, int64_t ldg, const T* x, int64_t rows, int width, int64_t ldx, const void* w, int pdt,
-               const float* mean, const float* rstd, T* gx, float* part, int blocks, const LnForm& f, hipStream_t s) {
+               const float* mean, const float* rstd, T* gx, float* part, void* gw, void* gb, int blocks, const LnForm& f,
+               hipStream_t s) {
     return ln_with_nv<V>(f.NV, [&](auto nv) -> int {
         constexpr int NV = decltype(nv)::value;
         if (f.blk) {
             auto kern = k_ln_bwd<T, V, NV, true>;
             FEQ_LAUNCH("k_ln_bwd", kern, dim3(blocks), dim3(kLnThreads), 0, s, gy, ldg, x, rows, width, ldx, w, pdt,
-                       mean, rstd, gx, part, f.G);
+                       mean, rstd, gx, part, gw, gb, f.G);
         } else if constexpr (NV * V <= kLnWaveElems) {
             auto kern = k_ln_bwd<T, V, NV, false>;
             FEQ_LAUNCH("k_ln_bwd", kern, dim3(blocks), dim3(kLnThreads), 0, s, gy, ldg, x, rows, width, ldx, w, pdt,
-                       mean, rstd, gx, part, f.G);
+                       mean, rstd, gx, part, gw, gb, f.G);
         }
         return FEQ_OK;
     });
@@ -448,7 +460,7 @@ int ln_bwd_run(const T* gy, int64_t ldg, const T* x, int64_t rows, int width, in
 int ln_check(int64_t rows, int64_t width, int64_t ldx, int32_t dtype, const void* x, const void* w, const void* b,
              int32_t pdt) {
     if (rows < 0 || width < 1) return fail(FEQ_ERR_INVALID, "layer norm of %lld rows of width %lld", (long long)rows, (long long)width);
-    if (width > 1 << 24) return fail(FEQ_ERR_UNSUPPORTED, "layer norm width %lld exceeds 2^24", (long long)width);
+    if (width > kLnMaxWidth) return fail(FEQ_ERR_UNSUPPORTED, "layer norm width %lld exceeds 2^24", (long long)width);
     if (ldx < width) return fail(FEQ_ERR_INVALID, "row stride %lld is smaller than the width %lld", (long long)ldx, (long long)width);
     if (!dtype_ok(dtype)) return fail(FEQ_ERR_INVALID, "unknown element type %d", dtype);
     if ((w || b) && !dtype_ok(pdt)) return fail(FEQ_ERR_INVALID, "unknown parameter type %d", pdt);
@@ -456,11 +468,15 @@ int ln_check(int64_t rows, int64_t width, int64_t ldx, int32_t dtype, const void
     return FEQ_OK;
 }
 
-// Workgroups of the backward, and partials of the weight gradients: at most (those of few wide rows would take more
-// memory than the rows).
-int ln_bwd_blocks(int64_t rows, int64_t width) {
-    return static_cast<int>(std::min<int64_t>(std::max<int64_t>(rows, 1),
-                                              width > kLnThreads * kLnBlockElems ? kLnWideBlocks : kLnMaxBlocks));
+// Workgroups of the backward, each with a partial of the weight gradients.  Few rows (kLnOneRows a lane group) take
+// one workgroup, which writes the gradients itself: launches bound such calls (100 rows of 192 with their gradients:
+// 60 -> 55 us).  Partials of many wide rows would take more memory than the rows: at most kLnWideBlocks.
+int ln_bwd_blocks(int64_t rows, int64_t width, int32_t dtype) {
+    if (ln_wide(width)) return static_cast<int>(std::min<int64_t>(rows, kLnWideBlocks));
+    const int V = 16 / elem_size(dtype);
+    const LnForm f = ln_form(width, width >= V ? V : 1);
+    const int64_t rounds = ceil_div(rows, f.blk ? 1 : kLnThreads / f.G);
+    return rounds <= kLnOneRows ? 1 : static_cast<int>(std::min<int64_t>(rounds, kLnMaxBlocks));
 }
 
 }  // namespace
@@ -483,7 +499,7 @@ extern "C" int feq_layernorm_fwd(const void* x, int64_t rows, int64_t width, int
         T* yt = static_cast<T*>(y);
         const bool vec = width >= VV;
         const LnForm f = ln_form(width, vec ? VV : 1);
-        if (f.wide) {
+        if (ln_wide(width)) {
             auto kern = k_ln_fwd_wide<T>;
             FEQ_LAUNCH("k_ln_fwd_wide", kern, dim3(std::min<int64_t>(rows, 4096)), dim3(kLnWide), 0, s, xt, rows, width,
                        ldx, weight, bias, param_dtype, eps, yt, mean, rstd);
@@ -495,9 +511,10 @@ extern "C" int feq_layernorm_fwd(const void* x, int64_t rows, int64_t width, int
     });
 }
 
-extern "C" size_t feq_layernorm_bwd_workspace(int64_t rows, int64_t width) {
-    if (rows < 1 || width < 1) return 0;
-    return sizeof(float) * 2 * static_cast<size_t>(width) * ln_bwd_blocks(rows, width);
+extern "C" size_t feq_layernorm_bwd_workspace(int64_t rows, int64_t width, int32_t dtype) {
+    if (rows < 1 || width < 1 || width > kLnMaxWidth || !dtype_ok(dtype)) return 0;
+    const int blocks = ln_bwd_blocks(rows, width, dtype);
+    return blocks > 1 ? sizeof(float) * 2 * static_cast<size_t>(width) * blocks : 0;
 }
 
 extern "C" int feq_layernorm_bwd(const void* grad_y, int64_t ldg, const void* x, int64_t rows, int64_t width,
@@ -510,13 +527,12 @@ extern "C" int feq_layernorm_bwd(const void* grad_y, int64_t ldg, const void* x,
     if (params && !dtype_ok(param_dtype)) return fail(FEQ_ERR_INVALID, "unknown parameter type %d", param_dtype);
     if (rows && (!grad_y || !mean || !rstd)) return fail(FEQ_ERR_INVALID, "NULL pointer");
     if (!grad_x && !params) return FEQ_OK;
-    if (params && ws_bytes < feq_layernorm_bwd_workspace(rows, width))
-        return fail(FEQ_ERR_WORKSPACE, "layer norm workspace of %zu bytes, %zu needed", ws_bytes,
-                    feq_layernorm_bwd_workspace(rows, width));
-    if (params && rows && !workspace) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    const size_t need = params ? feq_layernorm_bwd_workspace(rows, width, dtype) : 0;
+    if (need && (!workspace || ws_bytes < need))
+        return fail(FEQ_ERR_WORKSPACE, "layer norm workspace of %zu bytes, %zu needed", ws_bytes, need);
     hipStream_t s = stream_of(stream);
-    float* part = params ? static_cast<float*>(workspace) : nullptr;
-    int groups = 0;
+    float* part = need ? static_cast<float*>(workspace) : nullptr;
+    int blocks = rows ? ln_bwd_blocks(rows, width, dtype) : 0;
     if (rows) {
         const int rc = with_dtype(dtype, [&](auto t) -> int {
             using T = decltype(t);
@@ -525,31 +541,30 @@ extern "C" int feq_layernorm_bwd(const void* grad_y, int64_t ldg, const void* x,
             T* dt = static_cast<T*>(grad_x);
             const bool vec = width >= VV;
             const LnForm f = ln_form(width, vec ? VV : 1);
-            if (f.wide) {
+            if (ln_wide(width)) {
                 if (dt) {
                     auto kern = k_ln_bwd_wide<T>;
                     FEQ_LAUNCH("k_ln_bwd_wide", kern, dim3(std::min<int64_t>(rows, 4096)), dim3(kLnWide), 0, s, gt, ldg,
                                xt, rows, width, ldx, weight, param_dtype, mean, rstd, dt);
                 }
-                if (part) {
-                    const int64_t per = ceil_div(rows, ln_bwd_blocks(rows, width));
-                    groups = static_cast<int>(ceil_div(rows, per));
+                if (params) {
+                    const int64_t per = ceil_div(rows, blocks);
+                    blocks = static_cast<int>(ceil_div(rows, per));
                     auto kern = k_ln_cols_wide<T>;
-                    FEQ_LAUNCH("k_ln_cols_wide", kern, dim3(ceil_div(width, 256), groups), dim3(256), 0, s, gt, ldg, xt,
-                               rows, width, ldx, mean, rstd, per, part);
+                    FEQ_LAUNCH("k_ln_cols_wide", kern, dim3(ceil_div(width, 256), blocks), dim3(256), 0, s, gt, ldg, xt,
+                               rows, width, ldx, mean, rstd, per, part, grad_w, grad_b, param_dtype);
                 }
                 return FEQ_OK;
             }
-            const int per = f.blk ? 1 : kLnThreads / f.G;
-            groups = static_cast<int>(std::min<int64_t>(ceil_div(rows, per), ln_bwd_blocks(rows, width)));
             const int w32 = static_cast<int>(width);
-            return vec ? ln_bwd_run<T, VV>(gt, ldg, xt, rows, w32, ldx, weight, param_dtype, mean, rstd, dt, part, groups, f, s)
-                       : ln_bwd_run<T, 1>(gt, ldg, xt, rows, w32, ldx, weight, param_dtype, mean, rstd, dt, part, groups, f, s);
+            void *gw = part ? nullptr : grad_w, *gb = part ? nullptr : grad_b;
+            return vec ? ln_bwd_run<T, VV>(gt, ldg, xt, rows, w32, ldx, weight, param_dtype, mean, rstd, dt, part, gw, gb, blocks, f, s)
+                       : ln_bwd_run<T, 1>(gt, ldg, xt, rows, w32, ldx, weight, param_dtype, mean, rstd, dt, part, gw, gb, blocks, f, s);
         });
         if (rc) return rc;
     }
-    if (params)     // with no rows: the sums of no partials, zeros
-        FEQ_LAUNCH("k_ln_wsum", k_ln_wsum, dim3(ceil_div(2 * width, 16)), dim3(1024), 0, s, part, groups,
+    if (params && (part || rows == 0))     // with no rows: the sums of no partials, zeros
+        FEQ_LAUNCH("k_ln_wsum", k_ln_wsum, dim3(ceil_div(2 * width, 16)), dim3(1024), 0, s, part, blocks,
                    static_cast<int>(width), grad_w, grad_b, param_dtype);
     return FEQ_OK;
 }

@@ -179,7 +179,7 @@ struct LayerNormNode final : OnceNode {
         if (nx) out[0] = make(xr.sizes(), xr, xr.scalar_type());
         if (nw) out[1] = make({width}, xr, ptype);
         if (nb) out[2] = make({width}, xr, ptype);
-        const Tensor ws_ = (nw || nb) ? scratch(feq_layernorm_bwd_workspace(rows, width), xr) : Tensor();
+        const Tensor ws_ = (nw || nb) ? scratch(feq_layernorm_bwd_workspace(rows, width, code_of(xr, "x")), xr) : Tensor();
         On on(xr);
         done(feq_layernorm_bwd(ptr(g), ldg, ptr(xr), rows, width, ldx, code_of(xr, "x"), ptr(ws), pdtype,
                                ptr_as<float>(stats), ptr_as<float>(stats) + rows, ptr(out[0]), ptr(out[1]), ptr(out[2]),

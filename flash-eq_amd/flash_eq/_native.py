@@ -188,7 +188,7 @@ _SIGS = {
     "feq_attn_pool_grad_attn": ([_P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _P, _P], ctypes.c_int),
     # mixture-of-experts node MLP
     "feq_layernorm_fwd": ([_P, _I64, _I64, _I64, _I32, _P, _P, _I32, _F, _P, _P, _P, _P], ctypes.c_int),
-    "feq_layernorm_bwd_workspace": ([_I64, _I64], _SZ),
+    "feq_layernorm_bwd_workspace": ([_I64, _I64, _I32], _SZ),
     "feq_layernorm_bwd": ([_P, _I64, _P, _I64, _I64, _I64, _I32, _P, _I32, _P, _P, _P, _P, _P, _P, _SZ, _P],
                           ctypes.c_int),
     "feq_expert_topk_workspace": ([_I64, _I32], _SZ),

@@ -750,9 +750,9 @@ int feq_layernorm_fwd(const void* x, int64_t rows, int64_t width, int64_t ldx, i
                       feq_stream_t stream);
 /* Its gradients from grad_y (rows ldg apart): grad_x (contiguous), grad_w, grad_b of
  * param_dtype, any of them NULL.  The parameters' sums over rows run in a fixed order.
- * rows = 0 writes zero parameter gradients.  Workspace feq_layernorm_bwd_workspace bytes
- * when a parameter gradient is wanted. */
-size_t feq_layernorm_bwd_workspace(int64_t rows, int64_t width);
+ * rows = 0 writes zero parameter gradients.  Workspace feq_layernorm_bwd_workspace bytes (dtype
+ * that of x; 0: none) when a parameter gradient is wanted.  width <= 2^24. */
+size_t feq_layernorm_bwd_workspace(int64_t rows, int64_t width, int32_t dtype);
 int feq_layernorm_bwd(const void* grad_y, int64_t ldg, const void* x, int64_t rows, int64_t width, int64_t ldx,
                       int32_t dtype, const void* weight, int32_t param_dtype, const float* mean, const float* rstd,
                       void* grad_x, void* grad_w, void* grad_b, void* workspace, size_t ws_bytes,
@@ -763,7 +763,7 @@ int feq_layernorm_bwd(const void* grad_y, int64_t ldg, const void* x, int64_t ro
  * at the chosen ones, divided by their sum where normalize is set.  A logit of -inf is
  * never chosen: its place holds id -1 and weight 0.  mean (experts, may be NULL): the mean
  * over the rows of the softmax (a row of -inf alone counts 0; of no rows: 0); it needs a workspace of
- * feq_expert_topk_workspace bytes.  experts <= 1024, top_k <= 64. */
+ * feq_expert_topk_workspace bytes (0: none).  experts <= 1024, top_k <= 64. */
 size_t feq_expert_topk_workspace(int64_t rows, int32_t experts);
 int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t experts, int32_t dtype, int32_t top_k,
                         int32_t normalize, int64_t* ids, float* weights, float* mean, void* workspace,

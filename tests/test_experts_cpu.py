@@ -49,9 +49,9 @@ def test_layernorm_abi_refusals():
     refused(fwd(dt=3), "unknown element type 3")
     refused(fwd(mean=FAKE), "together")
     assert fwd(rows=0) == 0
-    need = lib.feq_layernorm_bwd_workspace(100, 192)
-    assert 0 < need <= 100 * 2 * 192 * 4
-    refused(lib.feq_layernorm_bwd(FAKE, 192, FAKE, 100, 192, 192, 0, None, 0, FAKE, FAKE, None, FAKE, None, FAKE,
+    need = lib.feq_layernorm_bwd_workspace(1000, 192, 0)
+    assert 0 < need <= 1000 * 2 * 192 * 4
+    refused(lib.feq_layernorm_bwd(FAKE, 192, FAKE, 1000, 192, 192, 0, None, 0, FAKE, FAKE, None, FAKE, None, FAKE,
                                   need - 1, None), "workspace")
 
 
@@ -64,7 +64,7 @@ def test_topk_abi_refusals():
     refused(fwd(x=1025), "more than 1024 experts")
     refused(fwd(x=100, k=65), "more than 64 choices")
     refused(fwd(dt=7), "unknown element type")
-    refused(fwd(mean=FAKE), "workspace")
+    refused(fwd(rows=1000, mean=FAKE), "workspace")
     assert fwd(rows=0) == 0
 
 
