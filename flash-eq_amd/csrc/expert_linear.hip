@@ -575,34 +575,71 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
 // planes), 16 TI WR columns k of x and BN columns n of grad_y (tiles of k first).  An expert of one chunk gets its
 // gradient written (zeros without rows), one of several a float32 partial per chunk: pw[slot N K + n K + k],
 // pb[slot N + n], summed by k_xl_wsum.
+// GX: grad_x too, from the same rows of grad_y, where one tile covers the weight (20011 x 49 bfloat16 rows, 128 x 128:
+// 162 us, where grad_x took 121 and grad_W 105; 40000 x 9 float32 rows, 64 x 128: 143, where they took 84 and 75.  A
+// second pair of row buffers, filled during the products, gained nothing: HBM bounds the first, the matrix cores' 77 us
+// the second).
 // ONCE: one tile covers the weight, so every row is read once; the rows then go past the caches, which leaves them to
 // the kernels around (20011 x 49 bfloat16 rows, 128 x 128: 137 -> 97 us, and with both maps a pass 376 -> 353).  Rows
 // that several tiles read lose by it (42 -> 52 us for 512 x 1024).
-template <class T, int HOW, int WR, int TI, int BN, bool ONCE>
-__global__ void __launch_bounds__(kXlThreads)
-k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __restrict__ offsets, int X, int S,
-           int ci, int co, int nreps, XlMap map, XlChunks ch, T* __restrict__ gw, T* __restrict__ gb, int nbias,
-           float* __restrict__ pw, float* __restrict__ pb) {
+template <class T, int HOW, int WR, int TI, int BN, bool ONCE, bool GX>
+__global__ void __launch_bounds__(kXlThreads, GX ? 2 : 1)
+k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const T* __restrict__ W, const int32_t* __restrict__ offsets,
+           int X, int S, int ci, int co, int nreps, XlMap map, XlChunks ch, T* __restrict__ gx, T* __restrict__ gw,
+           T* __restrict__ gb, int nbias, float* __restrict__ pw, float* __restrict__ pb) {
     using M = Mma<T>;
     constexpr int V = 16 / sizeof(T), BP = kXlRowBytes / sizeof(T);   // rows staged at a time
     constexpr int BK = 16 * TI * WR, WC = 4 / WR, NT = BN / (16 * WC);
     constexpr int LX = BK + M::PAD, LG = BN + M::PAD;
     constexpr int NX = BP * (BK / V) / kXlThreads, NG = BP * (BN / V) / kXlThreads;
-    __shared__ __align__(16) T sX[BP * LX];
-    __shared__ __align__(16) T sG[BP * LG];
+    constexpr int SIZE = BP * (LX + LG), WSIZE = GX ? BN * LX : 0;
+    __shared__ __align__(16) T lds[SIZE > WSIZE ? SIZE : WSIZE];
+    T *sX = lds, *sG = lds + BP * LX;
     const int nk = (ci + BK - 1) / BK, nn = (co + BN - 1) / BN;
     const int block = blockIdx.x / (nk * nn), sub = blockIdx.x % (nk * nn);
     int rep = nreps - 1;                             // the irreps of most planes first
     while (rep > 0 && block >= ch.tile0[rep - 1]) --rep;
     const int rc = ch.rows[rep];
     const XlTile t = find_tile<true>(offsets, X, S, rc, block - ch.tile0[rep]);
-    if (t.expert < 0 || t.expert == X) return;
+    if (t.expert < 0 || (!GX && t.expert == X)) return;
     const int k0 = (sub % nk) * BK, n0 = (sub / nk) * BN;
     const int rend = t.row1 - t.row0 < rc ? t.row1 : t.row0 + rc;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wr = wave % WR, wc = wave / WR;
     const int d0 = __builtin_amdgcn_readfirstlane(map.first[rep]), d1 = __builtin_amdgcn_readfirstlane(map.first[rep + 1]);
+    // GX: a wave takes CT column tiles of grad_x, the weight's fragments of which it keeps, and RP row tiles of a step
+    constexpr int KT = BK / 16, CT = KT / 4 > kDealt<T> ? KT / 4 : kDealt<T>, CW = KT / CT, RP = BP / 16 * CW / 4;
+    constexpr int GS = GX ? BN / M::KS : 1;
+    const int gc = wave % CW, gr = wave / CW * RP;
+    typename M::frag wf[GS][CT];
+    if constexpr (GX) {
+        if (t.expert == X) {                         // rows without an expert: grad_x is 0
+            const int n = (rend - t.row0) * ci;      // of a plane, in one piece
+            for (int d = d0; d < d1; ++d) {
+                T* o = gx + (static_cast<int64_t>(d) * S + t.row0) * ci;
+                const float zero[V] = {};
+                for (int i = tid * V; i < n; i += kXlThreads * V) {
+                    if (i + V <= n) store_f<T, V>(o + i, zero);
+                    else
+                        for (int j = i; j < n; ++j) o[j] = static_cast<T>(0.0f);
+                }
+            }
+            return;
+        }
+        const Rows w = rows_at(W + (static_cast<int64_t>(t.expert) * nreps + rep) * co * ci, W, ci);
+#pragma unroll
+        for (int i = 0; i < BN * (BK / V) / kXlThreads; ++i) {
+            const int q = tid + kXlThreads * i, r = q / (BK / V), k = (q % (BK / V)) * V;
+            const int there = r < co ? ci - k : 0;
+            put_dealt<T>(lds + r * LX, k, arrived16<T, HOW>(w, load16<T, HOW>(w, (r * ci + k) * static_cast<int>(sizeof(T)), there), there));
+        }
+        __syncthreads();
+#pragma unroll
+        for (int ks = 0; ks < GS; ++ks)
+#pragma unroll
+            for (int j = 0; j < CT; ++j) wf[ks][j] = M::columns(lds, LX, ks * M::KS, g, c, 16 * (gc * CT + j));
+    }
     const int steps = (rend - t.row0 + BP - 1) / BP, total = steps * (d1 - d0);
     const int bc = __builtin_amdgcn_readfirstlane(map.bcol[d0]);
     const bool sums = gb && bc >= 0 && k0 == 0;                    // uniform
@@ -658,6 +695,30 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const int32_t* __r
             for (int i = 0; i < TI; ++i)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) acc[i][j] = M::mul(a[i], b[j], acc[i][j]);
+        }
+        if constexpr (GX) {
+            v4f o[RP][CT];
+#pragma unroll
+            for (int r = 0; r < RP; ++r)
+#pragma unroll
+                for (int j = 0; j < CT; ++j) o[r][j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < GS; ++ks)
+#pragma unroll
+                for (int r = 0; r < RP; ++r)
+                    M::template mul_all<CT>(wf[ks], *reinterpret_cast<const typename M::frag*>(
+                                                sG + (16 * (gr + r) + c) * LG + ks * M::KS + M::FE * g), o[r]);
+#pragma unroll
+            for (int r = 0; r < RP; ++r) {
+                const int row = 16 * (gr + r) + c;
+                if (row >= there) continue;
+                T* at = gx + (static_cast<int64_t>(d0 + it / steps) * S + t.row0 + (it % steps) * BP + row) * ci;
+#pragma unroll
+                for (int j = 0; j < CT; j += kDealt<T>) {
+                    const int n = 16 * (gc * CT + j) + V * g;
+                    store_tiles<T, HOW, 1>(at + n, ci - n, &o[r][j]);
+                }
+            }
         }
         if (sums && tid < BN)
             for (int p = 0; p < BP; ++p) bsum += static_cast<float>(sG[p * LG + tid]);
@@ -841,10 +902,15 @@ int mm_run(const void* in, const void* W, const int32_t* offsets, int X, int64_t
         };
         constexpr int H = 64 / Mma<T>::KS;           // steps of 64 columns
         auto with_ns = [&](auto nn) -> int {
-            return K <= 64 ? stream(nn, std::integral_constant<int, H>{}) : stream(nn, std::integral_constant<int, 2 * H>{});
+            if (K <= 64) return stream(nn, std::integral_constant<int, H>{});
+            if constexpr (HOW == kNarrow && decltype(nn)::value > 32) return FEQ_ERR_INVALID;        // neither is narrow
+            else return stream(nn, std::integral_constant<int, 2 * H>{});
         };
-        if (K > kXlStreamK)
-            return N <= 64 ? tile(std::integral_constant<int, 1>{}) : tile(std::integral_constant<int, 2>{});
+        if (K > kXlStreamK) {
+            if (N <= 64) return tile(std::integral_constant<int, 1>{});
+            if constexpr (HOW == kNarrow) return FEQ_ERR_INVALID;
+            else return tile(std::integral_constant<int, 2>{});
+        }
         if (N <= 32) return with_ns(std::integral_constant<int, 32>{});
         if (N <= 64) return with_ns(std::integral_constant<int, 64>{});
         return with_ns(std::integral_constant<int, 128>{});
@@ -868,12 +934,83 @@ int64_t wgrad_chunks(int64_t S, int X, const int32_t* lvals, int nreps, int ci, 
         ch->rows[r] = static_cast<int32_t>(rows);
         ch->tile0[r] = static_cast<int32_t>(tiles);
         ch->slot0[r] = static_cast<int32_t>(slots);
-        tiles += S / rows + X;
+        tiles += S / rows + X + 1;                       // the rows without an expert last
         slots += S > rows ? 2 * S / rows : 0;
     }
     ch->tile0[nreps] = static_cast<int32_t>(tiles);      // all
     ch->slot0[nreps] = static_cast<int32_t>(slots);
     return slots;
+}
+
+// Whether one kernel makes grad_x and grad_W: where one tile covers the weight.
+bool bwd_fused(int ci, int co) { return ci <= 128 && co <= 128; }
+
+// grad_W, grad_b (gb NULL: not wanted) and, for gx, with the weight W, grad_x in the same kernel.
+int bwd_w_run(const int32_t* lvals, int nreps, int experts, int64_t slots, int cin, int cout, int dtype, const XlMap& map,
+              const void* grad_y, const void* x, const void* weight, const int32_t* offsets, int nb, const int32_t* bias_cols,
+              void* grad_x, void* grad_weight, void* grad_bias, void* workspace, size_t ws_bytes, hipStream_t s) {
+    const size_t need = feq_expert_linear_bwd_workspace(lvals, nreps, experts, slots, cin, cout, nb);
+    if (ws_bytes < need) return fail(FEQ_ERR_WORKSPACE, "weight-gradient workspace of %zu bytes, %zu needed", ws_bytes, need);
+    if (need && !workspace) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    XlChunks ch;
+    const int64_t nslots = wgrad_chunks(slots, experts, lvals, nreps, cin, cout, &ch);
+    for (int r = 0; r < nreps; ++r)
+        if (nb && bias_cols[r] >= 0) ch.brep[bias_cols[r]] = static_cast<int8_t>(r);
+    Carver c(workspace);
+    float* pw = c.take<float>(static_cast<size_t>(nslots) * cin * cout);
+    float* pb = c.take<float>(nb ? static_cast<size_t>(nslots) * cout : 0);
+    return with_dtype(dtype, [&](auto tt) -> int {
+        using T = decltype(tt);
+        T *gx = static_cast<T*>(grad_x), *gw = static_cast<T*>(grad_weight), *gb = static_cast<T*>(grad_bias);
+        return with_rows<T>(cin, cout, {grad_y, x, weight, grad_x, grad_weight}, [&](auto how) -> int {
+            constexpr int HOW = decltype(how)::value;
+            auto run = [&](auto wr, auto ti, auto bn) -> int {
+                constexpr int WR = decltype(wr)::value, TI = decltype(ti)::value, BN = decltype(bn)::value;
+                constexpr int BK = 16 * TI * WR;
+                const int64_t blocks = ch.tile0[nreps] * ceil_div(cin, BK) * ceil_div(cout, BN);
+                if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
+                auto go = [&](auto once, auto with_gx) -> int {
+                    constexpr bool GX = decltype(with_gx)::value;
+                    auto kern = k_xl_wgrad<T, HOW, WR, TI, BN, decltype(once)::value, GX>;
+                    FEQ_LAUNCH(GX ? "k_xl_bwd" : "k_xl_wgrad", kern, dim3(blocks), dim3(kXlThreads), 0, s,
+                               static_cast<const T*>(grad_y), static_cast<const T*>(x), static_cast<const T*>(weight),
+                               offsets, experts, static_cast<int>(slots), cin, cout, nreps, map, ch, gx, gw, gb, nb, pw, pb);
+                    return FEQ_OK;
+                };
+                constexpr std::integral_constant<bool, HOW == kWhole> past{};
+                if (gx) return go(past, std::true_type{});
+                if constexpr (HOW == kWhole) {
+                    if (cin <= BK && cout <= BN) return go(past, std::false_type{});
+                }
+                return go(std::false_type{}, std::false_type{});
+            };
+            auto with_bn = [&](auto wr, auto ti) -> int {
+                if (cout <= 64) return run(wr, ti, std::integral_constant<int, 64>{});
+                if constexpr (HOW == kNarrow && decltype(ti)::value > 2) return FEQ_ERR_INVALID;     // neither is narrow
+                else return run(wr, ti, std::integral_constant<int, 128>{});
+            };
+            constexpr std::integral_constant<int, 1> one{};
+            constexpr std::integral_constant<int, 2> two{};
+            constexpr std::integral_constant<int, 4> four{};
+            if (const int err = cin <= 32 ? with_bn(one, two) : cin <= 64 ? with_bn(one, four) : with_bn(two, four)) return err;
+            if (nslots == 0) return FEQ_OK;               // every expert in one chunk
+            const int64_t wsize = static_cast<int64_t>(cin) * cout;
+            int least = ch.rows[0];
+            for (int r = 1; r < nreps; ++r) least = std::min(least, static_cast<int>(ch.rows[r]));
+            const int64_t many = std::min<int64_t>(experts, slots / least);  // experts of several chunks, at most
+            const bool split = slots / least > 8 * experts;                  // more than eight chunks an expert, on average
+            auto sum = [&](auto vv, auto sp) -> int {
+                constexpr int V = decltype(vv)::value;
+                constexpr bool SPLIT = decltype(sp)::value;
+                auto kern = k_xl_wsum<T, V, SPLIT>;
+                FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(std::max<int64_t>(wsize, cout), (SPLIT ? 64 : 256) * V), many, nreps + nb),
+                           dim3(256), 0, s, pw, pb, offsets, experts, ch, wsize, cout, nreps, gw, gb, nb);
+                return FEQ_OK;
+            };
+            auto with_split = [&](auto vv) -> int { return split ? sum(vv, std::true_type{}) : sum(vv, std::false_type{}); };
+            return HOW == kWhole ? with_split(four) : with_split(one);
+        });
+    });
 }
 
 }  // namespace
@@ -909,14 +1046,14 @@ extern "C" int feq_expert_linear_bwd_x(const int32_t* lvals, int32_t nreps, int3
     });
 }
 
-extern "C" size_t feq_expert_linear_bwd_w_workspace(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots,
-                                                    int32_t cin, int32_t cout, int32_t nbias) {
+extern "C" size_t feq_expert_linear_bwd_workspace(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots,
+                                                  int32_t cin, int32_t cout, int32_t nbias) {
     if (!lvals || nreps < 1 || nreps > kXlMaxReps || experts < 1 || slots < 1 || cin < 1 || cout < 1 || nbias < 0) return 0;
     for (int r = 0; r < nreps; ++r)
         if (lvals[r] < 0 || lvals[r] > kXlMaxPlanes) return 0;
     XlChunks ch;
     const int64_t n = wgrad_chunks(slots, experts, lvals, nreps, cin, cout, &ch);
-    Carver c(nullptr);
+    Carver c(nullptr);                                   // the partials
     c.take<float>(static_cast<size_t>(n) * cin * cout);
     c.take<float>(nbias ? static_cast<size_t>(n) * cout : 0);
     return c.used;
@@ -930,62 +1067,24 @@ extern "C" int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int3
     if (int rc = xl_check(lvals, nreps, experts, slots, cin, cout, dtype, grad_bias ? bias_cols : nullptr, nbias, &map)) return rc;
     if (!grad_weight || !offsets || (slots && (!grad_y || !x))) return fail(FEQ_ERR_INVALID, "NULL pointer");
     if (grad_bias && (!bias_cols || nbias < 1)) return fail(FEQ_ERR_INVALID, "a bias gradient needs bias columns");
-    const int nb = grad_bias ? nbias : 0;
-    const size_t need = feq_expert_linear_bwd_w_workspace(lvals, nreps, experts, slots, cin, cout, nb);
-    if (ws_bytes < need) return fail(FEQ_ERR_WORKSPACE, "weight-gradient workspace of %zu bytes, %zu needed", ws_bytes, need);
-    if (need && !workspace) return fail(FEQ_ERR_INVALID, "NULL pointer");
-    hipStream_t s = stream_of(stream);
-    XlChunks ch;
-    const int64_t nslots = wgrad_chunks(slots, experts, lvals, nreps, cin, cout, &ch);
-    for (int r = 0; r < nreps; ++r)
-        if (nb && bias_cols[r] >= 0) ch.brep[bias_cols[r]] = static_cast<int8_t>(r);
-    Carver c(workspace);
-    float* pw = c.take<float>(static_cast<size_t>(nslots) * cin * cout);
-    float* pb = c.take<float>(nb ? static_cast<size_t>(nslots) * cout : 0);
-    return with_dtype(dtype, [&](auto tt) -> int {
-        using T = decltype(tt);
-        T *gw = static_cast<T*>(grad_weight), *gb = static_cast<T*>(grad_bias);
-        return with_rows<T>(cin, cout, {grad_y, x, grad_weight}, [&](auto how) -> int {
-            constexpr int HOW = decltype(how)::value;
-            auto run = [&](auto wr, auto ti, auto bn) -> int {
-                constexpr int WR = decltype(wr)::value, TI = decltype(ti)::value, BN = decltype(bn)::value;
-                const int64_t blocks = ch.tile0[nreps] * ceil_div(cin, 16 * TI * WR) * ceil_div(cout, BN);
-                if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
-                auto go = [&](auto once) -> int {
-                    auto kern = k_xl_wgrad<T, HOW, WR, TI, BN, decltype(once)::value>;
-                    FEQ_LAUNCH("k_xl_wgrad", kern, dim3(blocks), dim3(kXlThreads), 0, s, static_cast<const T*>(grad_y),
-                               static_cast<const T*>(x), offsets, experts, static_cast<int>(slots), cin, cout, nreps, map,
-                               ch, gw, gb, nb, pw, pb);
-                    return FEQ_OK;
-                };
-                if constexpr (HOW == kWhole) {
-                    if (cin <= 16 * TI * WR && cout <= BN) return go(std::true_type{});
-                }
-                return go(std::false_type{});
-            };
-            auto with_bn = [&](auto wr, auto ti) -> int {
-                return cout <= 64 ? run(wr, ti, std::integral_constant<int, 64>{}) : run(wr, ti, std::integral_constant<int, 128>{});
-            };
-            constexpr std::integral_constant<int, 1> one{};
-            constexpr std::integral_constant<int, 2> two{};
-            constexpr std::integral_constant<int, 4> four{};
-            if (const int err = cin <= 32 ? with_bn(one, two) : cin <= 64 ? with_bn(one, four) : with_bn(two, four)) return err;
-            if (nslots == 0) return FEQ_OK;               // every expert in one chunk
-            const int64_t wsize = static_cast<int64_t>(cin) * cout;
-            int least = ch.rows[0];
-            for (int r = 1; r < nreps; ++r) least = std::min(least, static_cast<int>(ch.rows[r]));
-            const int64_t many = std::min<int64_t>(experts, slots / least);  // experts of several chunks, at most
-            const bool split = slots / least > 8 * experts;                  // more than eight chunks an expert, on average
-            auto sum = [&](auto vv, auto sp) -> int {
-                constexpr int V = decltype(vv)::value;
-                constexpr bool SPLIT = decltype(sp)::value;
-                auto kern = k_xl_wsum<T, V, SPLIT>;
-                FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(std::max<int64_t>(wsize, cout), (SPLIT ? 64 : 256) * V), many, nreps + nb),
-                           dim3(256), 0, s, pw, pb, offsets, experts, ch, wsize, cout, nreps, gw, gb, nb);
-                return FEQ_OK;
-            };
-            auto with_split = [&](auto vv) -> int { return split ? sum(vv, std::true_type{}) : sum(vv, std::false_type{}); };
-            return HOW == kWhole ? with_split(four) : with_split(one);
-        });
-    });
+    return bwd_w_run(lvals, nreps, experts, slots, cin, cout, dtype, map, grad_y, x, nullptr, offsets, grad_bias ? nbias : 0,
+                     bias_cols, nullptr, grad_weight, grad_bias, workspace, ws_bytes, stream_of(stream));
+}
+
+extern "C" int feq_expert_linear_bwd(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
+                                     int32_t cout, int32_t dtype, const void* grad_y, const void* x, const void* weight,
+                                     const int32_t* offsets, int32_t nbias, const int32_t* bias_cols, void* grad_x,
+                                     void* grad_weight, void* grad_bias, void* workspace, size_t ws_bytes,
+                                     feq_stream_t stream) {
+    XlMap map;
+    if (int rc = xl_check(lvals, nreps, experts, slots, cin, cout, dtype, grad_bias ? bias_cols : nullptr, nbias, &map)) return rc;
+    if (!grad_weight || !offsets || (slots && (!grad_y || !x || !weight || !grad_x))) return fail(FEQ_ERR_INVALID, "NULL pointer");
+    if (grad_bias && (!bias_cols || nbias < 1)) return fail(FEQ_ERR_INVALID, "a bias gradient needs bias columns");
+    const bool fused = slots && bwd_fused(cin, cout);
+    if (const int rc = bwd_w_run(lvals, nreps, experts, slots, cin, cout, dtype, map, grad_y, x, fused ? weight : nullptr,
+                                 offsets, grad_bias ? nbias : 0, bias_cols, fused ? grad_x : nullptr, grad_weight, grad_bias,
+                                 workspace, ws_bytes, stream_of(stream)))
+        return rc;
+    if (fused || slots == 0) return FEQ_OK;
+    return feq_expert_linear_bwd_x(lvals, nreps, experts, slots, cin, cout, dtype, grad_y, weight, offsets, grad_x, stream);
 }

@@ -496,24 +496,26 @@ struct ExpertLinearNode final : OnceNode {
         const int64_t experts = w.size(0), co = w.size(2), ci = w.size(3), slots = xs.size(-2);
         const int code = code_of(xs, "x");
         On on(xs);
-        if (need(0)) {
-            out[0] = make(xs.sizes(), xs, xs.scalar_type());
-            done(feq_expert_linear_bwd_x(irreps.lvals.data(), irreps.n(), experts, slots, ci, co, code, ptr(g), ptr(w),
-                                         ptr_as<int32_t>(offsets), ptr(out[0]), on.stream),
+        const int32_t *lv = irreps.lvals.data(), n = irreps.n(), *off = ptr_as<int32_t>(offsets);
+        const int32_t nb = need(2) ? static_cast<int32_t>(nbias) : 0;
+        Tensor gw, gb, ws;
+        if (need(0)) out[0] = make(xs.sizes(), xs, xs.scalar_type());
+        if (need(1) || need(2)) gw = make(w.sizes(), w, w.scalar_type());
+        if (nb) gb = make({experts, co, nbias}, w, w.scalar_type());
+        if (gw.defined()) ws = scratch(feq_expert_linear_bwd_workspace(lv, n, experts, slots, ci, co, nb), xs);
+        if (need(0) && gw.defined())
+            done(feq_expert_linear_bwd(lv, n, experts, slots, ci, co, code, ptr(g), ptr(xs), ptr(w), off, nb, irreps.cols.data(),
+                                       ptr(out[0]), ptr(gw), ptr(gb), ptr(ws), bytes_of(ws), on.stream),
+                 "feq_expert_linear_bwd");
+        else if (need(0))
+            done(feq_expert_linear_bwd_x(lv, n, experts, slots, ci, co, code, ptr(g), ptr(w), off, ptr(out[0]), on.stream),
                  "feq_expert_linear_bwd_x");
-        }
-        if (need(1) || need(2)) {
-            const int32_t nb = need(2) ? static_cast<int32_t>(nbias) : 0;
-            Tensor gw = make(w.sizes(), w, w.scalar_type()), gb;
-            if (nb) gb = make({experts, co, nbias}, w, w.scalar_type());
-            const Tensor ws = scratch(feq_expert_linear_bwd_w_workspace(irreps.lvals.data(), irreps.n(), experts, slots, ci, co, nb), xs);
-            done(feq_expert_linear_bwd_w(irreps.lvals.data(), irreps.n(), experts, slots, ci, co, code, ptr(g), ptr(xs),
-                                         ptr_as<int32_t>(offsets), nb, irreps.cols.data(), ptr(gw), ptr(gb), ptr(ws),
-                                         bytes_of(ws), on.stream),
+        else if (gw.defined())
+            done(feq_expert_linear_bwd_w(lv, n, experts, slots, ci, co, code, ptr(g), ptr(xs), off, nb, irreps.cols.data(),
+                                         ptr(gw), ptr(gb), ptr(ws), bytes_of(ws), on.stream),
                  "feq_expert_linear_bwd_w");
-            if (need(1)) out[1] = gw;
-            if (need(2)) out[2] = gb;
-        }
+        if (need(1)) out[1] = gw;
+        if (need(2)) out[2] = gb;
         return out;
     }
     void release_variables() override {

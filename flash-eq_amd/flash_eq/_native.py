@@ -202,7 +202,9 @@ _SIGS = {
     "feq_expert_linear_fwd": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I32, _P, _P, _P],
                               ctypes.c_int),
     "feq_expert_linear_bwd_x": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _P], ctypes.c_int),
-    "feq_expert_linear_bwd_w_workspace": ([_P, _I32, _I32, _I64, _I32, _I32, _I32], _SZ),
+    "feq_expert_linear_bwd_workspace": ([_P, _I32, _I32, _I64, _I32, _I32, _I32], _SZ),
+    "feq_expert_linear_bwd": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _P, _I32, _P, _P, _P, _P, _P, _SZ, _P],
+                              ctypes.c_int),
     "feq_expert_linear_bwd_w": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _I32, _P, _P, _P, _P, _SZ, _P],
                                 ctypes.c_int),
 }

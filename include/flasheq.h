@@ -810,13 +810,19 @@ int feq_expert_linear_bwd_x(const int32_t* lvals, int32_t nreps, int32_t experts
                             int32_t cout, int32_t dtype, const void* grad_y, const void* weight,
                             const int32_t* offsets, void* grad_x, feq_stream_t stream);
 /* grad_weight and, unless NULL, grad_bias: sums in a fixed order, zeros for an expert without rows.
- * Workspace feq_expert_linear_bwd_w_workspace bytes (nbias 0 without grad_bias). */
-size_t feq_expert_linear_bwd_w_workspace(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots,
-                                         int32_t cin, int32_t cout, int32_t nbias);
+ * Workspace feq_expert_linear_bwd_workspace bytes (nbias 0 without grad_bias). */
+size_t feq_expert_linear_bwd_workspace(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots,
+                                       int32_t cin, int32_t cout, int32_t nbias);
 int feq_expert_linear_bwd_w(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
                             int32_t cout, int32_t dtype, const void* grad_y, const void* x, const int32_t* offsets,
                             int32_t nbias, const int32_t* bias_cols, void* grad_weight, void* grad_bias,
                             void* workspace, size_t ws_bytes, feq_stream_t stream);
+/* grad_x as well: channels of at most 128 both ways take one pass over grad_y, others bwd_w and bwd_x.
+ * The workspace is bwd_w's. */
+int feq_expert_linear_bwd(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
+                          int32_t cout, int32_t dtype, const void* grad_y, const void* x, const void* weight,
+                          const int32_t* offsets, int32_t nbias, const int32_t* bias_cols, void* grad_x,
+                          void* grad_weight, void* grad_bias, void* workspace, size_t ws_bytes, feq_stream_t stream);
 
 #ifdef __cplusplus
 }

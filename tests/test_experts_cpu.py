@@ -100,7 +100,7 @@ def test_linear_abi_refusals():
     refused(fwd(lv=(0, 0), nb=2, cols=(0, 0)), "bias column 0 of irrep 1")
     refused(fwd(lv=(0, 0), nb=2, cols=(0, -1)), "not each of them")
     refused(fwd(dt=5), "unknown element type")
-    lib_ws = lib.feq_expert_linear_bwd_w_workspace(i32(0, 1), 2, 4, 10000, 64, 64, 1)
+    lib_ws = lib.feq_expert_linear_bwd_workspace(i32(0, 1), 2, 4, 10000, 64, 64, 1)
     assert lib_ws > 0
     refused(lib.feq_expert_linear_bwd_w(i32(0, 1), 2, 4, 10000, 64, 64, 0, FAKE, FAKE, FAKE, 1, i32(0, -1), FAKE, FAKE, FAKE,
                                         lib_ws - 1, None), "workspace")

@@ -337,6 +337,11 @@ def check_linear(dev, lvals, counts, unrouted, cin, cout, dtype, bias=True, seed
     for i, (a, r, m) in enumerate(zip((y, *got), want, mass)):
         within(a, r, HALF[dtype] * r.abs() + U * (terms[i] or rows) * m)
     assert not y[:, n:].any() and not got[0][:, n:].any()
+    for i, leaf in enumerate(leaves):            # each gradient without the others
+        args = [t.detach().requires_grad_(t is leaf) if t is not None else None for t in (xl, wl, bl)]
+        (one,) = torch.autograd.grad(fe.expert_linear(*args[:2], plan, lvals, args[2]), [args[i]], gyd.to(dev))
+        within(one, want[1 + i], HALF[dtype] * want[1 + i].abs() + U * (terms[1 + i] or rows) * mass[1 + i])
+        assert i or not one[:, n:].any()
 
 
 CHANNELS = [(64, 128), (128, 64), (8, 8), (33, 7), (1, 1), (160, 200), (12, 260), (300, 20), (301, 133), (131, 9),
