@@ -8,12 +8,13 @@
 //
 // Products run on the matrix cores: v_mfma_f32_16x16x4_f32 for float32, v_mfma_f32_16x16x32_{f16, bf16} for 16-bit
 // types, float32 accumulators for both, one rounding at the store.  The expert of a row block is found by every wave
-// from the offsets (a lane per expert, sums over lanes), so the host never learns the counts and the grid is their
+// from the offsets (experts over the lanes, a sum along the wave), so the host never learns the counts and the grid is their
 // upper bound.  The weight is the first operand and the rows the second: a lane's accumulators are columns of one row.
 #include <algorithm>
 
 #include "elem_types.h"
 #include "feq_internal.h"
+#include "lane_math.h"
 #include "tile_math.h"
 
 namespace feq {
@@ -249,60 +250,61 @@ struct XlTile {
     int count;       // the expert's blocks
 };
 
-// Block `want` of the row blocks (of `bm` rows) of the experts in order, the rows behind them last.  Called
-// by whole waves; the result is uniform.  EMPTY: an expert without rows has one block.
+// The row blocks (of `bm` rows) of the experts in order, the rows behind them last.  A lane has `per` experts next to
+// each other, so one sum along the wave numbers the blocks of all.  EMPTY: an expert without rows has one block.
+// Built and asked by whole waves; results are uniform.
 template <bool EMPTY = false>
-__device__ __forceinline__ XlTile find_tile(const int32_t* __restrict__ offsets, int X, int S, int bm, int want) {
-    const int lane = threadIdx.x & 63;
-    int carry = 0, many = 0;
-    for (int e0 = 0; e0 <= X; e0 += 64) {
-        const int e = e0 + lane;
-        int a = 0, z = 0;
-        if (e <= X) {
-            a = offsets[e];
-            z = e < X ? offsets[e + 1] : S;
-        }
-        int n = (z - a + bm - 1) / bm;
-        if (EMPTY && n == 0 && e < X) n = 1;
-        int incl = n, multi = (e < X && n > 1) ? n : 0, mincl = multi;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(incl, o, 64), w = __shfl_up(mincl, o, 64);
-            if (lane >= o) {
-                incl += u;
-                mincl += w;
-            }
-        }
-        const uint64_t hit = __ballot(carry + incl > want);
-        if (hit) {
-            const int f = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-            const int begin = carry + __builtin_amdgcn_readlane(incl - n, f);
-            XlTile t;
-            t.expert = e0 + f;
-            t.index = want - begin;
-            t.row0 = __builtin_amdgcn_readlane(a, f) + t.index * bm;
-            t.row1 = __builtin_amdgcn_readlane(z, f);
-            t.before = many + __builtin_amdgcn_readlane(mincl - multi, f);
-            t.count = __builtin_amdgcn_readlane(n, f);
-            return t;
-        }
-        carry += __builtin_amdgcn_readlane(incl, 63);
-        many += __builtin_amdgcn_readlane(mincl, 63);
+struct XlBlocks {
+    const int32_t* offsets;
+    int X, S, bm, per;
+    int own, upto;       // blocks of the lane's experts, and of those up to them
+    int many, many_upto; // the same of experts of more than one block
+
+    __device__ __forceinline__ int blocks(int e, int a, int z) const {
+        const int n = (z - a + bm - 1) / bm;
+        return EMPTY && n == 0 && e < X ? 1 : n;
     }
-    return XlTile{-1, 0, 0, 0, 0, 0};
-}
+    __device__ __forceinline__ XlBlocks(const int32_t* __restrict__ offs, int X_, int S_, int bm_)
+        : offsets(offs), X(X_), S(S_), bm(bm_), per(X_ / 64 + 1), own(0), many(0) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll 2
+        for (int i = 0; i < per; ++i) {
+            const int e = lane * per + i;
+            const int n = e <= X ? blocks(e, offsets[e], e < X ? offsets[e + 1] : S) : 0;
+            own += n;
+            many += e < X && n > 1 ? n : 0;
+        }
+        upto = inclusive_sum(own);
+        many_upto = inclusive_sum(many);
+    }
+    __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(upto, 63); }
+    __device__ __forceinline__ XlTile find(int want) const {
+        const uint64_t hit = __ballot(upto > want);
+        if (!hit) return XlTile{-1, 0, 0, 0, 0, 0};
+        const int f = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+        int at = __builtin_amdgcn_readlane(upto - own, f), before = __builtin_amdgcn_readlane(many_upto - many, f);
+        int e = f * per, ea, ez, n;
+        for (;; ++e) {                           // ends by the lane's last expert
+            ea = __builtin_amdgcn_readfirstlane(offsets[e]);
+            ez = e < X ? __builtin_amdgcn_readfirstlane(offsets[e + 1]) : S;
+            n = blocks(e, ea, ez);
+            if (at + n > want || e >= X) break;
+            at += n;
+            before += n > 1 ? n : 0;
+        }
+        XlTile t;
+        t.expert = e;
+        t.index = want - at;
+        t.row0 = ea + t.index * bm;
+        t.row1 = ez;
+        t.before = before;
+        t.count = n;
+        return t;
+    }
+};
 
 // Blocks of `bm` rows that X experts and the rows behind them can make of S rows.
 inline int64_t tile_bound(int64_t S, int X, int bm) { return S / bm + std::min<int64_t>(S, X + 1); }
-
-// The blocks (of `bm` rows) that find_tile numbers.  Called by whole waves.
-__device__ __forceinline__ int count_tiles(const int32_t* __restrict__ offsets, int X, int S, int bm) {
-    int n = 0;
-    for (int e = threadIdx.x & 63; e <= X; e += 64) {
-        n += ((e < X ? offsets[e + 1] : S) - offsets[e] + bm - 1) / bm;
-    }
-    for (int o = 32; o; o >>= 1) n += __shfl_xor(n, o, 64);
-    return __builtin_amdgcn_readfirstlane(n);
-}
 
 // The row block of a workgroup of a grid of 8 ceil(bound / 8) subs workgroups (a plane's), -1: none; `sub` its column
 // block.  Workgroups go to the 8 XCDs in turn.  An XCD takes neighbouring row blocks, whole: an expert's weight and
@@ -333,9 +335,10 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
     __shared__ __align__(16) T sW[2][TRANS ? BK * LDT : BN * LD];
     const int d = blockIdx.y;
     int sub;
-    const int tile = xcd_tile(blockIdx.x, (N + BN - 1) / BN, count_tiles(offsets, X, S, kXlBM), sub);
+    const XlBlocks<> experts(offsets, X, S, kXlBM);
+    const int tile = xcd_tile(blockIdx.x, (N + BN - 1) / BN, experts.total(), sub);
     if (tile < 0) return;
-    const XlTile t = find_tile(offsets, X, S, kXlBM, tile);
+    const XlTile t = experts.find(tile);
     const int n0 = sub * BN;
     const int rows = t.row1 - t.row0 < kXlBM ? t.row1 - t.row0 : kXlBM;
     T* od = out + (static_cast<int64_t>(d) * S + t.row0) * N;
@@ -470,14 +473,15 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int nb = (N + NB - 1) / NB;
-    const int per_plane = count_tiles(offsets, X, S, 16);
+    const XlBlocks<> experts(offsets, X, S, 16);
+    const int per_plane = experts.total();
     const int64_t total = static_cast<int64_t>(per_plane) * dim * nb;
     const int64_t share = total / gridDim.x, more = total % gridDim.x;
     int64_t at = blockIdx.x * share + (blockIdx.x < more ? blockIdx.x : more);
     const int64_t end = at + share + (blockIdx.x < more ? 1 : 0);
     while (at < end) {
         const int line = static_cast<int>(at / per_plane), d = line / nb, n0 = line % nb * NB;
-        const XlTile t = find_tile(offsets, X, S, 16, static_cast<int>(at % per_plane));
+        const XlTile t = experts.find(static_cast<int>(at % per_plane));
         const int expert = t.expert, row0 = t.row0, rows = t.row1 - t.row0, left = t.count - t.index;
         const int nblocks = static_cast<int>(end - at < left ? end - at : left);
         at += nblocks;
@@ -580,8 +584,8 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
 // second pair of row buffers, filled during the products, gained nothing: HBM bounds the first, the matrix cores' 77 us
 // the second).
 // ONCE: one tile covers the weight, so every row is read once; the rows then go past the caches, which leaves them to
-// the kernels around (20011 x 49 bfloat16 rows, 128 x 128: 137 -> 97 us, and with both maps a pass 376 -> 353).  Rows
-// that several tiles read lose by it (42 -> 52 us for 512 x 1024).
+// the kernels around (grad_W alone for 20011 x 49 bfloat16 rows, 128 x 128: 137 -> 97 us).  Rows that several tiles read
+// lose by it (42 -> 52 us for 512 x 1024).
 template <class T, int HOW, int WR, int TI, int BN, bool ONCE, bool GX>
 __global__ void __launch_bounds__(kXlThreads, GX ? 2 : 1)
 k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const T* __restrict__ W, const int32_t* __restrict__ offsets,
@@ -600,7 +604,7 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const T* __restric
     int rep = nreps - 1;                             // the irreps of most planes first
     while (rep > 0 && block >= ch.tile0[rep - 1]) --rep;
     const int rc = ch.rows[rep];
-    const XlTile t = find_tile<true>(offsets, X, S, rc, block - ch.tile0[rep]);
+    const XlTile t = XlBlocks<true>(offsets, X, S, rc).find(block - ch.tile0[rep]);
     if (t.expert < 0 || (!GX && t.expert == X)) return;
     const int k0 = (sub % nk) * BK, n0 = (sub / nk) * BN;
     const int rend = t.row1 - t.row0 < rc ? t.row1 : t.row0 + rc;
@@ -768,21 +772,17 @@ k_xl_wsum(const float* __restrict__ pw, const float* __restrict__ pb, const int3
         const int n = e < X ? (offsets[e + 1] - offsets[e] + rc - 1) / rc : 0;
         const int m = n > 1 ? n : 0;
         const uint64_t many = __ballot(n > 1);
-        int incl = m;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(incl, o, 64);
-            if (lane >= o) incl += u;
-        }
+        const int incl = inclusive_sum(m);
         const uint64_t hit = __ballot(n > 1 && carry + static_cast<int>(__popcll(many & ((1ull << lane) - 1ull))) == want);
         if (hit) {
             const int f = __ffsll(static_cast<unsigned long long>(hit)) - 1;
             expert = e0 + f;
-            first = slots + __shfl(incl - m, f, 64);
-            count = __shfl(n, f, 64);
+            first = slots + __builtin_amdgcn_readlane(incl - m, f);
+            count = __builtin_amdgcn_readlane(n, f);
             break;
         }
         carry += static_cast<int>(__popcll(many));
-        slots += __shfl(incl, 63, 64);
+        slots += __builtin_amdgcn_readlane(incl, 63);
     }
     if (expert < 0) return;
     const int64_t i = (static_cast<int64_t>(blockIdx.x) * (SPLIT ? 64 : 256) + (SPLIT ? lane : threadIdx.x)) * V;

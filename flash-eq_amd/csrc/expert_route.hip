@@ -408,11 +408,7 @@ __device__ __forceinline__ int scan_buckets(int* v, int X, int* tmp) {
         own[i] = b < X ? v[b] : 0;
         s += own[i];
     }
-    int incl = s;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(incl, o, 64);
-        if ((threadIdx.x & 63) >= static_cast<unsigned>(o)) incl += u;
-    }
+    const int incl = inclusive_sum(s);
     const int wave = threadIdx.x >> 6;
     if ((threadIdx.x & 63) == 63) tmp[wave] = incl;
     __syncthreads();
@@ -495,11 +491,7 @@ k_plan_scan(int32_t* __restrict__ hist, int64_t ntiles, int32_t* __restrict__ to
     for (int64_t t0 = 0; t0 < ntiles; t0 += 256) {
         const int64_t t = t0 + threadIdx.x;
         const int v = t < ntiles ? h[t] : 0;
-        int incl = v;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(incl, o, 64);
-            if ((threadIdx.x & 63) >= static_cast<unsigned>(o)) incl += u;
-        }
+        const int incl = inclusive_sum(v);
         __syncthreads();
         if ((threadIdx.x & 63) == 63) tmp[threadIdx.x >> 6] = incl;
         __syncthreads();

@@ -1,4 +1,4 @@
-// Reductions over groups of 1, 2, 4, ... 64 neighbouring lanes; every lane of a group gets the result.
+// Reductions over groups of 1, 2, 4, ... 64 neighbouring lanes, of which every lane gets the result; sums along a wave.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -48,6 +48,21 @@ __device__ __forceinline__ uint32_t group_max_u(uint32_t v, int g) {
 }
 __device__ __forceinline__ uint32_t group_min_u(uint32_t v, int g) {
     return group_op(v, g, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+}
+
+// The sum over the lanes up to this one, by a whole wave: within 16 lanes by shifts, the rows before by broadcasts of
+// their last lane (masks: rows 1 and 3, then 2 and 3).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ int inclusive_sum(int v) {
+    v = dpp_add<0x111, 0xF>(v);      // row_shr 1
+    v = dpp_add<0x112, 0xF>(v);      // 2
+    v = dpp_add<0x114, 0xF>(v);      // 4
+    v = dpp_add<0x118, 0xF>(v);      // 8
+    v = dpp_add<0x142, 0xA>(v);      // row_bcast 15
+    return dpp_add<0x143, 0xC>(v);   // row_bcast 31
 }
 
 }  // namespace
