@@ -320,6 +320,9 @@ inline int64_t xcd_grid(int64_t bound, int64_t subs) { return 8 * ceil_div(bound
 // out[d, p, :] = in[d, p, :] B (+ bias), B = W[e, r]^T (TRANS false: in has Cin columns, out Cout) or W[e, r]
 // (TRANS: in has Cout columns, out Cin).  K: columns of in, N: of out; W rows have wld = Cin elements.
 // WR: waves along the output columns (64 each), 4 / WR along the rows.
+// 8191 bfloat16 rows of 64 experts, 512 to 1024 columns: 30 us forward, 28 grad_x (290 TFLOP/s): the workgroups run
+// in two rounds of 8 and 16 steps that wait for LDS and for each other.  Steps of half the columns with three
+// workgroups on a CU instead of two: 45 and 49 us.
 template <class T, int HOW, bool TRANS, int WR>
 __global__ void __launch_bounds__(kXlThreads, 2)
 k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,
@@ -459,6 +462,9 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
 // in the matrix cores' layout (lane (c, g): FE elements of row c), the next block's rows in flight during this
 // one's products.  Nothing but the weight passes through LDS and no barrier stands between blocks of an
 // expert.  NS: reduction steps held (K <= NS KS).
+// Forward and grad_x, against the tile kernel: 78 and 75 us (95 and 91) for 40000 x 9 float32 rows, 64 x 128 (3.5 TB/s;
+// the matrix cores' share is 38 us); 117 and 116 (140 and 139) for 20011 x 49 bfloat16 rows, 128 x 128 (4.3 TB/s).
+// Column blocks no wider than the output: 16 columns take 28 us in blocks of 32, 52 in blocks of 128.
 template <class T, int HOW, bool TRANS, int NB, int NS>
 __global__ void __launch_bounds__(kXlThreads, NB * NS * Mma<T>::KS * sizeof(T) > 40000 ? 2 : NS == 8 || HOW != kWhole ? 3 : 4)
 k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,

@@ -186,7 +186,8 @@ def some_ids(g, rows, k, experts, bad=0.1):
 
 @pytest.mark.parametrize("rows,k,experts", [(0, 2, 4), (1, 1, 1), (5, 1, 3), (100, 2, 8), (64, 1, 64), (333, 3, 65),
                                             (4096, 2, 8), (8193, 1, 5), (1000, 64, 9), (3000, 4, 1024), (2049, 8, 100),
-                                            (30011, 2, 16), (700, 2, 1024), (4095, 2, 960), (4095, 2, 962), (70000, 2, 1023)])
+                                            (30011, 2, 16), (700, 2, 1024), (4095, 2, 960), (4095, 2, 962), (70000, 2, 1023),
+                                            (9000, 1, 255), (9000, 1, 256)])
 def test_plan_is_exact(dev, rows, k, experts):
     ids = some_ids(gen(rows + k), rows, k, experts)
     order, positions, offsets = OE.plan(ids, experts)
