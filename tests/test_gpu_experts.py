@@ -477,6 +477,29 @@ def test_refusals(dev):
         fe.expert_linear(xs, w.half(), plan)
 
 
+def test_broadcast_inputs_and_gradients(dev):
+    """Expanded inputs give what their copies give, and their sources the copies' gradients summed."""
+    g = gen(14)
+    plan = fe.ExpertPlan(some_ids(g, 40, 2, 3).to(dev), 3)
+    x, ys = torch.randn(1, 40, 8, generator=g).to(dev), torch.randn(4, 1, 8, generator=g).to(dev)
+    w, lw = torch.rand(1, 2, generator=g).to(dev), torch.randn(3, 1, 6, 8, generator=g).to(dev)
+    l = torch.randn(1, 3, generator=g).to(dev)
+    calls = [(lambda a: plan.dispatch(a), x, (4, 40, 8)),
+             (lambda a: plan.combine(a, w.expand(40, 2)), ys, (4, 80, 8)),
+             (lambda a: plan.combine(ys.expand(4, 80, 8), a), w, (40, 2)),
+             (lambda a: fe.expert_linear(ys.expand(4, 80, 8), a, plan, (0, 1)), lw, (3, 2, 6, 8)),
+             (lambda a: fe.expert_linear(a, lw.expand(3, 2, 6, 8), plan, (0, 1)), ys, (4, 80, 8)),
+             (lambda a: fe.expert_topk(a, 2)[1], l, (40, 3))]
+    for call, small, shape in calls:
+        a = small.clone().requires_grad_()
+        b = small.expand(shape).contiguous().requires_grad_()
+        ya, yb = call(a.expand(shape)), call(b)
+        assert torch.equal(ya, yb)
+        gy = torch.ones(1, device=dev).expand(ya.shape)              # as of a sum, stride 0
+        (ga,), (gb,) = torch.autograd.grad(ya, [a], gy), torch.autograd.grad(yb, [b], gy.contiguous())
+        assert torch.allclose(ga, gb.sum_to_size(small.shape), rtol=1e-5, atol=1e-6 * max(1.0, gb.abs().max().item()))
+
+
 def test_a_plan_is_for_reading(dev):
     """Places that a kernel would write to are those of the sort, or the call is refused; copies are plans too."""
     import copy
