@@ -273,7 +273,8 @@ k_topk_bwd(const T* __restrict__ logits, const int64_t* __restrict__ ids, const 
             float dot = 0.0f;
             if (normalize)
 #pragma unroll 4
-                for (int k = 0; k < K; ++k) dot += weights[r * K + k] * gw[r * K + k];
+                for (int k = 0; k < K; ++k)      // a place without an expert is no function of the logits: not 0 g
+                    dot += ids[r * K + k] >= 0 ? weights[r * K + k] * gw[r * K + k] : 0.0f;
 #pragma unroll 4
             for (int k = 0; k < K; ++k) {
                 const int id = static_cast<int>(ids[r * K + k]);

@@ -870,3 +870,27 @@ def test_one_expert_is_the_dense_mlp(dev, lvals, mult, gating):
     rel = lambda a, b: ((a.detach().double().cpu() - b).abs().max() / b.abs().max()).item()
     # sums of up to 2 mult terms twice and a gate: 64 steps of float32 at the largest value are 4e-6
     assert rel(y, y64.detach()) < 1e-5 and rel(gx, gx64) < 2e-5
+
+
+# ---- gradients at places without an expert ---------------------------------------------
+
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("experts,k", [(5, 2), (9, 4), (70, 12)])
+def test_topk_gradient_at_places_without_an_expert_is_not_read(dev, experts, k, dtype, normalize):
+    """Whatever gradient meets the constant weight 0 of a place without an expert, infinity and NaN too: the others
+    are those of a 0 there."""
+    l = torch.randn(6, experts, generator=gen(experts)).to(dev, dtype)
+    l[0] = -INF
+    l[1, 1:] = -INF
+    l[2, k // 2:] = -INF
+    l.requires_grad_()
+    ids, w, _ = fe.expert_topk(l, k, normalize)
+    gw = torch.randn(6, k, generator=gen(k)).to(dev)
+    got = []
+    for garbage in (0.0, INF, -INF, NAN):
+        g = torch.where(ids < 0, torch.full_like(gw, garbage), gw)
+        got.append(torch.autograd.grad([w], [l], [g], retain_graph=True)[0])
+    assert (ids < 0).any() and torch.isfinite(got[0]).all()
+    for other in got[1:]:
+        assert torch.equal(other, got[0])
