@@ -416,8 +416,8 @@ struct CombineNode final : OnceNode {
     variable_list backward(variable_list& grads) override {
         variable_list out(2);
         if (!grads[0].defined()) return out;
+        const Tensor in = ys.unpack(), w = weights.unpack(), g = dense(grads[0]);   // an error when they have been freed
         places.check();
-        const Tensor in = ys.unpack(), w = weights.unpack(), g = dense(grads[0]);
         if (need(0)) out[0] = make(in.sizes(), in, in.scalar_type());
         if (need(1)) out[1] = make(w.sizes(), w, w.scalar_type());
         if (in.numel()) {
@@ -491,8 +491,8 @@ struct ExpertLinearNode final : OnceNode {
     variable_list backward(variable_list& grads) override {
         variable_list out(3);
         if (!grads[0].defined()) return out;
+        const Tensor xs = x.unpack(), w = weight.unpack(), g = dense(grads[0]);     // an error when they have been freed
         check_plan(offsets, "offsets", 1);
-        const Tensor xs = x.unpack(), w = weight.unpack(), g = dense(grads[0]);
         const int64_t experts = w.size(0), co = w.size(2), ci = w.size(3), slots = xs.size(-2);
         const int code = code_of(xs, "x");
         On on(xs);

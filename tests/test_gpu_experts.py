@@ -894,3 +894,14 @@ def test_topk_gradient_at_places_without_an_expert_is_not_read(dev, experts, k, 
     assert (ids < 0).any() and torch.isfinite(got[0]).all()
     for other in got[1:]:
         assert torch.equal(other, got[0])
+
+
+def test_a_second_backward_names_what_was_freed(dev):
+    plan = fe.ExpertPlan(torch.tensor([[0, 1], [1, 0]], device=dev), 2)
+    w = torch.randn(2, 1, 3, 6, device=dev, requires_grad=True)
+    for call in (lambda a: plan.combine(a, torch.ones(2, 2, device=dev)), lambda a: fe.expert_linear(a, w, plan),
+                 lambda a: fe.expert_topk(a, 2)[1], lambda a: fe.ops.layer_norm(a)):
+        y = call(torch.randn(4, 6, device=dev, requires_grad=True)).sum()
+        y.backward()
+        with pytest.raises(RuntimeError, match="backward through the graph a second time"):
+            y.backward()
