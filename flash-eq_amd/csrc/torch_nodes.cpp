@@ -316,6 +316,7 @@ std::tuple<Tensor, Tensor, Tensor> expert_plan(const Tensor& ids, int64_t expert
     const int64_t slots = ids.size(0) * k;
     if (slots > (int64_t{1} << 30)) value_error("more than 2^30 slots: ", slots);
     at::NoGradGuard none;
+    c10::InferenceMode tracked(false);      // in-place changes of a plan made in inference mode are counted too (check_plan)
     const Tensor flat = dense(ids.scalar_type() == at::kLong ? ids : ids.to(at::kLong));
     Tensor order = make({slots}, flat, at::kInt), positions = make({ids.size(0), k}, flat, at::kInt),
            offsets = make({experts + 1}, flat, at::kInt);
@@ -328,12 +329,19 @@ std::tuple<Tensor, Tensor, Tensor> expert_plan(const Tensor& ids, int64_t expert
 }
 
 // The kernels write to the places a plan holds, so one whose tensors are not those that expert_plan
-// returned, as it returned them, is refused.
+// returned, as it returned them, is refused.  Theirs are no inference tensors, whose changes nothing counts.
 void check_plan(const Tensor& t, const char* name, int64_t dims) {
     need_gpu(t, name);
-    if (t.scalar_type() != at::kInt || t.dim() != dims || !t.is_contiguous())
+    if (t.scalar_type() != at::kInt || t.dim() != dims || !t.is_contiguous() || t.is_inference())
         value_error("not an ExpertPlan's ", name, ": ", dtype_name(t.scalar_type()), " of shape ", t.sizes());
-    TORCH_CHECK(t.is_inference() || t._version() == 0, "the ", name, " of an ExpertPlan have been modified in place");
+    TORCH_CHECK(t._version() == 0, "the ", name, " of an ExpertPlan have been modified in place");
+}
+
+// A copy of a plan's tensor (any device) that check_plan takes: of version 0, no inference tensor.
+Tensor plan_copy(const Tensor& t) {
+    c10::InferenceMode tracked(false);
+    at::AutoDispatchBelowADInplaceOrView uncounted;      // a clone of an inference tensor is filled in place
+    return t.clone();
 }
 
 // A plan as the row moves need it.
@@ -592,6 +600,7 @@ PYBIND11_MODULE(flasheq_torch, m) {
     m.def("layer_norm", &layer_norm, released);
     m.def("expert_topk", &expert_topk, released);
     m.def("expert_plan", &expert_plan, released);
+    m.def("plan_copy", &plan_copy, released);
     m.def("expert_dispatch", &expert_dispatch, released);
     m.def("expert_combine", &expert_combine, released);
     m.def("expert_linear", &expert_linear, released);

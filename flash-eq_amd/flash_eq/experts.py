@@ -68,7 +68,8 @@ class ExpertPlan:
 
     def __setstate__(self, state: dict) -> None:
         # of a copy or a pickle, whose tensors were filled in place
-        self.__dict__.update({k: v.clone() if isinstance(v, torch.Tensor) else v for k, v in state.items()})
+        copy = N.nodes().plan_copy
+        self.__dict__.update({k: copy(v) if isinstance(v, torch.Tensor) else v for k, v in state.items()})
 
     def dispatch(self, x: torch.Tensor) -> torch.Tensor:
         """x (..., rows, width) to (..., slots, width): every place its slot's row, zeros at the

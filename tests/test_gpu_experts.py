@@ -905,3 +905,30 @@ def test_a_second_backward_names_what_was_freed(dev):
         y.backward()
         with pytest.raises(RuntimeError, match="backward through the graph a second time"):
             y.backward()
+
+
+def test_plans_made_in_inference_mode_are_for_reading(dev):
+    """Changes in place are refused there as elsewhere, of copies too; unchanged plans serve in and out of the mode."""
+    import copy
+    x, w = torch.randn(3, 8, device=dev), torch.ones(3, 2, device=dev)
+    lw = torch.randn(3, 1, 8, 8, device=dev)
+    for inside in (True, False):
+        with torch.inference_mode():
+            ids = torch.tensor([[0, 1], [2, 0], [-1, 1]], device=dev)
+            plan = fe.ExpertPlan(ids, 3)
+            copied = copy.deepcopy(plan)
+            late = fe.ExpertPlan(ids.int(), 3)
+            ys = fe.expert_linear(plan.dispatch(x), lw, copied)
+            assert torch.equal(late.combine(ys, w), plan.combine(ys, w))
+        a = x.clone().requires_grad_()
+        assert torch.equal(torch.autograd.grad(plan.dispatch(a).sum(), [a])[0][2], torch.ones(8, device=dev))
+        for p in (plan, copied):
+            with torch.inference_mode(inside):
+                p.positions.clamp_(max=2)
+            for mode in (True, False):
+                with torch.inference_mode(mode), pytest.raises(RuntimeError, match="positions of an ExpertPlan have been modified"):
+                    p.dispatch(x)
+        with torch.inference_mode(inside):
+            late.offsets[-1] += 1
+            with pytest.raises(RuntimeError, match="offsets of an ExpertPlan have been modified"):
+                fe.expert_linear(ys, lw, late)
