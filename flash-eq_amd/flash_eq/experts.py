@@ -66,6 +66,13 @@ class ExpertPlan:
     def offsets(self) -> torch.Tensor:
         return self._offsets
 
+    def __getstate__(self) -> dict:
+        # a copy counts changes from its own beginning: one of a changed plan would be taken
+        for name in ("order", "positions", "offsets"):
+            if getattr(self, name)._version != 0:
+                raise RuntimeError(f"the {name} of an ExpertPlan have been modified in place")
+        return self.__dict__
+
     def __setstate__(self, state: dict) -> None:
         # of a copy or a pickle, whose tensors were filled in place
         copy = N.nodes().plan_copy

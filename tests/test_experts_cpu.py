@@ -1,6 +1,9 @@
 """Host-side behaviour of the layer norm's and the expert routing's entry points: refusals, sizes,
 construction (no GPU work: pointers are never dereferenced)."""
+import copy
 import ctypes
+import pickle
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -150,3 +153,31 @@ def test_linear_abi_refuses_a_bias_without_columns():
     for cols, n in ((None, 1), (one, 0)):
         assert lib.feq_expert_linear_fwd(one, 1, 2, 10, 4, 4, 0, FAKE, FAKE, FAKE, FAKE, n, cols, FAKE, None) != 0
         assert "bias" in lib.feq_last_error().decode()
+
+
+@pytest.fixture
+def host_plan(monkeypatch):
+    """A function that makes plans of host tensors: one row for each of two experts, as the kernels would return it."""
+    real = N.nodes()
+
+    def expert_plan(ids, num_experts):
+        n = ids.shape[0]
+        place = torch.arange(n, dtype=torch.int32)
+        return place, place[:, None].clone(), torch.arange(num_experts + 1, dtype=torch.int32)
+    monkeypatch.setattr(N, "nodes", lambda: SimpleNamespace(expert_plan=expert_plan, plan_copy=real.plan_copy,
+                                                            expert_linear=lambda *a: a))
+    return lambda: fe.ExpertPlan(torch.tensor([0, 1]), 2)
+
+
+def test_a_changed_plan_is_not_copied(host_plan):
+    """A copy's tensors count their changes anew, so the plan's have to be looked at before."""
+    for copied in (copy.copy, copy.deepcopy, lambda p: pickle.loads(pickle.dumps(p))):
+        plan = host_plan()
+        other = copied(copied(plan))
+        assert other.positions.tolist() == plan.positions.tolist() and other.positions._version == 0
+        assert other.positions.data_ptr() != plan.positions.data_ptr()
+        for name in ("order", "positions", "offsets"):
+            for plan in (host_plan(), other, copied(host_plan())):
+                getattr(plan, name).add_(2 ** 30)
+                with pytest.raises(RuntimeError, match="of an ExpertPlan have been modified"):
+                    copied(plan)
