@@ -44,15 +44,28 @@ class ExpertPlan:
     * ``offsets`` (num_experts + 1,) int32: every expert's first place; the last one is the number
       of slots with an expert.
 
-    They are for reading: kernels write where they point, and a plan whose positions or offsets have
-    been modified in place is refused.  ``dispatch`` copies rows to their places, ``combine`` sums them
+    They and the sizes are for reading: kernels write where they point, and a plan whose positions or offsets
+    have been modified in place is refused.  ``dispatch`` copies rows to their places, ``combine`` sums them
     back with weights."""
 
     def __init__(self, ids: torch.Tensor, num_experts: int) -> None:
         self._order, self._positions, self._offsets = N.nodes().expert_plan(ids, num_experts)
-        self.num_experts = num_experts
-        self.num_rows, self.top_k = self._positions.shape
-        self.num_slots = self.num_rows * self.top_k
+
+    @property
+    def num_experts(self) -> int:
+        return self._offsets.shape[0] - 1
+
+    @property
+    def num_rows(self) -> int:
+        return self._positions.shape[0]
+
+    @property
+    def top_k(self) -> int:
+        return self._positions.shape[1]
+
+    @property
+    def num_slots(self) -> int:
+        return self._positions.numel()
 
     @property
     def order(self) -> torch.Tensor:
@@ -103,4 +116,6 @@ def expert_linear(x: torch.Tensor, weight: torch.Tensor, plan: ExpertPlan, lvals
     alone, lvals (0,)); weight (experts, irreps, cout, cin); bias (experts, cout, scalar irreps) or
     None, added to the scalar irreps; all of one dtype (float32, float16 or bfloat16).  Returns (dim,
     slots, cout); zeros in the rows without an expert, which enter no gradient."""
+    if not isinstance(plan, ExpertPlan):
+        raise TypeError(f"plan must be an ExpertPlan, got {type(plan).__name__}")
     return N.nodes().expert_linear(x, weight, bias, plan.offsets, plan.num_slots, lvals)

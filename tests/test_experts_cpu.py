@@ -181,3 +181,17 @@ def test_a_changed_plan_is_not_copied(host_plan):
                 getattr(plan, name).add_(2 ** 30)
                 with pytest.raises(RuntimeError, match="of an ExpertPlan have been modified"):
                     copied(plan)
+
+
+def test_a_plans_sizes_are_those_of_its_tensors(host_plan):
+    """The kernels' bounds come from them: none can be set, and no other object stands for a plan."""
+    plan = host_plan()
+    assert (plan.num_experts, plan.num_rows, plan.top_k, plan.num_slots) == (2, 2, 1, 2)
+    for name in ("num_experts", "num_rows", "top_k", "num_slots", "order", "positions", "offsets"):
+        with pytest.raises(AttributeError):
+            setattr(plan, name, 1)
+    assert repr(plan) == "ExpertPlan(rows=2, top_k=1, num_experts=2)"
+    x, w = torch.randn(1, 8), torch.randn(2, 1, 4, 8)
+    assert fe.expert_linear(x, w, plan)[4] == 2
+    with pytest.raises(TypeError, match="plan must be an ExpertPlan, got SimpleNamespace"):
+        fe.expert_linear(x, w, SimpleNamespace(offsets=plan.offsets, num_slots=1))
