@@ -37,7 +37,7 @@ def _up(v):
     return v
 
 
-def _up_all(named) -> dict:
+def up_all(named) -> dict:
     """float32 copies of named tensors: those of one half-precision dtype and
     device are cast together (one concatenation and one cast, split back into
     views: two launches instead of one per tensor, and one for their
@@ -63,8 +63,8 @@ def _up_all(named) -> dict:
 def run_float32(module: nn.Module, dtype: torch.dtype, args: tuple, kwargs: dict):
     """``module(*args, **kwargs)`` with float32 copies of its floating
     parameters, buffers and tensor arguments; the output cast to ``dtype``."""
-    state = _up_all(module.named_parameters())
-    state.update(_up_all(module.named_buffers()))
+    state = up_all(module.named_parameters())
+    state.update(up_all(module.named_buffers()))
     seen = {}
 
     def up(v):   # one float32 copy per distinct argument (P passed as P and Q: one cast)

@@ -14,13 +14,18 @@ import torch.nn as nn
 
 from ..experts import MAX_EXPERTS, MAX_TOP_K, ExpertPlan, expert_linear, expert_topk
 from ..representations import Repr
+from ..utils import epsilon_dtype
+from ._precision import half_dtype, run_float32, up_all
 from .gating import EquivariantGating
 from .norm import InvariantLayerNorm, RepNorm
 
 
 class ExpertRouter(nn.Module):
     """The experts of every node: layer norm of its invariants, a linear map to one logit per
-    expert, the ``top_k`` largest with softmax weights (``expert_topk``)."""
+    expert, the ``top_k`` largest with softmax weights (``expert_topk``).
+
+    float16 and bfloat16 features and parameters go through it in float32 (the squares of float16 features
+    pass its range from 256 on, and logits of 16 bits tie)."""
 
     def __init__(self, repr: Repr, num_experts: int, top_k: int = 2, normalize: bool = True) -> None:
         super().__init__()
@@ -39,6 +44,10 @@ class ExpertRouter(nn.Module):
 
     def forward(self, st: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """(nodes, mult, dim) to ids (nodes, top_k), weights (nodes, top_k), mean probabilities."""
+        half = half_dtype(st)
+        if half is not None:
+            with epsilon_dtype(half):
+                return torch.func.functional_call(self, up_all(self.named_parameters()), (st.float(),))
         invariants = self.norm(st).flatten(-2, -1)
         return expert_topk(self.linear(self.lnorm(invariants)), self.top_k, self.normalize)
 
@@ -88,7 +97,8 @@ class EquivariantExpertMLP(nn.Module):
 
     Every node's row goes to its ``top_k`` experts (``ExpertRouter``), through their maps up, the
     gating (shared by the experts) and their maps down, and the results are summed with the
-    router's weights.  ``forward(x, balance=terms)`` appends the router's balancing term to the list
+    router's weights.  float16 and bfloat16 features keep their type between these steps; router and gating
+    run in float32 inside.  ``forward(x, balance=terms)`` appends the router's balancing term to the list
     ``terms``, for the training loss (the module keeps nothing of a call, so no graph outlives it)."""
 
     def __init__(self, repr: Repr, num_experts: int, top_k: int = 2, mlp_ratio: int = 2, use_gating: bool = True,
@@ -114,7 +124,9 @@ class EquivariantExpertMLP(nn.Module):
             if self.act.kernels_ok(h):
                 h = self.act.forward_cm(h)
             else:
-                h = self.act(h.permute(1, 2, 0)).permute(2, 0, 1).contiguous()
+                nodes, half = h.permute(1, 2, 0), half_dtype(h)
+                nodes = self.act(nodes) if half is None else run_float32(self.act, half, (nodes,), {})
+                h = nodes.permute(2, 0, 1).contiguous()
         return plan.combine(self.down(h, plan), weights).permute(1, 2, 0).contiguous()
 
     def extra_repr(self) -> str:

@@ -932,3 +932,102 @@ def test_plans_made_in_inference_mode_are_for_reading(dev):
             late.offsets[-1] += 1
             with pytest.raises(RuntimeError, match="offsets of an ExpertPlan have been modified"):
                 fe.expert_linear(ys, lw, late)
+
+
+# ---- the 16-bit mixture ----------------------------------------------------------------
+
+def check_half_mlp(dev, dtype, gating, scale):
+    """Values and gradients against the float64 formulas on the same 16-bit values, with the module's choice.
+
+    Norms (Frobenius, |.|) bound the errors.  A table stored in the type is off by h |table|, its half step with room
+    for the float32 sums; a map multiplies errors by at most its largest singular value; with the gate's matrix L,
+    lambda = |L|, and rows of irrep norms n of at most N, the gate u s(L n) by 1 + lambda N / 4 (|s'| <= 1/4), and its
+    derivative's own error has, relative to the gradient that comes in, h lambda N / 4 from s, and
+    h lambda N (1/4 + lambda N / 10 + 1/2) from <u, g>, s' (|s''| < 1/10) and u / n."""
+    torch.manual_seed(11)
+    rp, k, lvals = fe.Repr([0, 1, 2], 16), 2, (0, 1, 2)
+    mlp = fe.EquivariantExpertMLP(rp, 4, k, use_gating=gating).to(dev, dtype)
+    on_dev = torch.Generator(device=dev).manual_seed(1)
+    names = ["up.weight", "up.bias", "down.weight", "down.bias"] + ["act.linear.weight", "act.linear.bias"] * gating
+    params = [dict(mlp.named_parameters())[n] for n in names]
+    with torch.no_grad():
+        for b in params[1::2]:
+            b.normal_(generator=on_dev)
+    x = (scale * torch.randn(60, 16, 9, generator=gen(12))).to(dtype)
+    gy = torch.randn(60, 16, 9, generator=gen(13)).to(dtype)
+    xl = x.to(dev).requires_grad_()
+    with torch.no_grad():
+        ids, w, mean = mlp.router(xl)
+    assert w.dtype == mean.dtype == torch.float32
+    y = mlp(xl)
+    got = dict(zip(["y", "x"] + names, (y, *torch.autograd.grad(y, [xl, *params], gy.to(dev)))))
+    assert all(t.dtype == dtype for t in got.values())
+
+    x64, gy64 = x.double().requires_grad_(), gy.double().permute(2, 0, 1)
+    p = {n: t.detach().double().cpu().requires_grad_() for n, t in mlp.named_parameters()}
+    irreps = ((0, 1), (1, 4), (4, 9))
+    norms = lambda t, eps: torch.stack([(t[a:b] ** 2).sum(0) + eps for a, b in irreps], -1).sqrt()
+    ids = ids.cpu()
+    invariants = norms(x64.permute(2, 0, 1), 1e-5).flatten(-2)
+    logits = OE.layer_norm(invariants, p["router.lnorm.weight"], p["router.lnorm.bias"]) @ p["router.linear.weight"].t()
+    w64, _ = OE.topk_weights(logits, ids, True)
+    assert (w.double().cpu() - w64).abs().max() < 1e-5       # float32 logits are off by less
+    _, _, offsets = OE.plan(ids, 4)
+    xs = OE.dispatch(x64.permute(2, 0, 1), ids, 4)
+    u = OE.linear(xs, p["up.weight"], offsets, lvals, p["up.bias"])
+    a, n = u, torch.zeros(1, 1, dtype=torch.float64)
+    if gating:
+        n = norms(u, 1e-5)
+        gate = torch.sigmoid(n.flatten(-2) @ p["act.linear.weight"].t() + p["act.linear.bias"]).view(n.shape)
+        a = torch.cat([u[i:j] * gate[..., r] for r, (i, j) in enumerate(irreps)])
+        n = n.flatten(-2)
+    s = OE.linear(a, p["down.weight"], offsets, lvals, p["down.bias"])
+    y64 = OE.combine(s, w64, ids, 4)
+    *gp, gx, gxs, gu, ga, gs, gw = (t.detach() for t in torch.autograd.grad(
+        y64, [*(p[m] for m in names), x64, xs, u, a, s, w64], gy64, retain_graph=True))
+    jac = sum(torch.autograd.grad(w64[:, i].sum(), x64, retain_graph=True)[0].flatten(1).norm(dim=1) ** 2 for i in range(k))
+
+    f = lambda t: t.detach().norm().item()
+    top = lambda t: torch.linalg.matrix_norm(t.detach(), ord=2).max().item()
+    h, root = HALF[dtype] + 2.0 ** -18, ids.numel() ** 0.5
+    up, down, lam = top(p["up.weight"]), top(p["down.weight"]), top(p["act.linear.weight"]) if gating else 0.0
+    N = n.detach().norm(dim=-1).max().item()
+    lip = 1 + lam * N / 4
+    e_u = h * f(u)
+    e_a = lip * e_u + h * f(a)
+    e_s = down * e_a + h * f(s)
+    e_y = e_s + 2e-5 * f(s) + h * f(y64)                     # weights of a row: together at most 1
+    e_gs = h * f(gs) + 2e-5 * f(gy64)
+    e_ga = down * e_gs + h * f(ga)
+    e_gu = lip * e_ga + h * lam * N * (1 + lam * N / 10) * f(ga) + h * f(gu)
+    e_gxs = up * e_gu + h * f(gxs)
+    rows = OE.combine(gxs, torch.ones_like(w64), ids, 4).permute(1, 2, 0)
+    e_rows = k ** 0.5 * e_gxs + h * f(rows)
+    e_router = jac.max().sqrt().item() * (gy64.permute(1, 0, 2).flatten(1).norm(dim=1).max().item() * e_s + 2.0 ** -14 * f(gw)) \
+        + h * f(gx - rows)
+    e_q = N / 4 * e_ga + h * N * (1 / 4 + lam * N / 10) * f(ga)
+    bounds = dict(zip(["y", "x"] + names, (
+        e_y, e_rows + e_router + h * (f(rows) + f(gx - rows) + f(gx)),
+        e_gu * f(xs) + h * f(gp[0]), root * e_gu + h * f(gp[1]),
+        e_gs * (f(a) + e_a) + f(gs) * e_a + h * f(gp[2]), root * e_gs + h * f(gp[3]))))
+    if gating:
+        q = N / 4 * f(ga)
+        bounds["act.linear.weight"] = (e_q + q * h) * f(n) + h * f(gp[4])
+        bounds["act.linear.bias"] = root * e_q + h * f(gp[5])
+    want = dict(zip(["y", "x"] + names, (y64.permute(1, 2, 0), gx, *gp)))
+    for name, bound in bounds.items():
+        err = f(got[name].double().cpu() - want[name])
+        assert err <= bound + TINY[dtype] * got[name].numel(), (name, err, bound, f(want[name]))
+
+
+@pytest.mark.parametrize("gating", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_half_precision_mlp_values(dev, dtype, gating):
+    check_half_mlp(dev, dtype, gating, 1.0)
+
+
+@pytest.mark.parametrize("gating", [True, False])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_half_precision_mlp_of_large_features(dev, dtype, gating):
+    """Features whose squares a float16 does not hold."""
+    check_half_mlp(dev, dtype, gating, 300.0)
