@@ -120,13 +120,12 @@ class EquivariantExpertMLP(nn.Module):
             balance.append(self.router.balance(plan, mean))
         # component-major (dim, nodes, mult): the layout of the maps and the gating
         h = self.up(plan.dispatch(x.permute(2, 0, 1).contiguous()), plan)
-        if isinstance(self.act, EquivariantGating):
-            if self.act.kernels_ok(h):
-                h = self.act.forward_cm(h)
-            else:
-                nodes, half = h.permute(1, 2, 0), half_dtype(h)
-                nodes = self.act(nodes) if half is None else run_float32(self.act, half, (nodes,), {})
-                h = nodes.permute(2, 0, 1).contiguous()
+        if isinstance(self.act, EquivariantGating) and self.act.kernels_ok(h):
+            h = self.act.forward_cm(h)
+        elif type(self.act) is not nn.Identity:
+            nodes, half = h.permute(1, 2, 0), half_dtype(h)
+            nodes = self.act(nodes) if half is None else run_float32(self.act, half, (nodes,), {})
+            h = nodes.permute(2, 0, 1).contiguous()
         return plan.combine(self.down(h, plan), weights).permute(1, 2, 0).contiguous()
 
     def extra_repr(self) -> str:

@@ -1031,3 +1031,18 @@ def test_half_precision_mlp_values(dev, dtype, gating):
 def test_half_precision_mlp_of_large_features(dev, dtype, gating):
     """Features whose squares a float16 does not hold."""
     check_half_mlp(dev, dtype, gating, 300.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_another_activation_is_called(dev, dtype):
+    """A module put in the place of the gating gets (slots, hidden, dim) features; here it scales by a power of two."""
+    class Scale(torch.nn.Module):
+        def forward(self, st):
+            assert st.shape[1:] == (16, 4)
+            return 4 * st
+    torch.manual_seed(12)
+    mlp = fe.EquivariantExpertMLP(fe.Repr([0, 1], 8), 3, 2, use_gating=False).to(dev, dtype)
+    x = torch.randn(20, 8, 4, generator=gen(14)).to(dev, dtype)
+    y = mlp(x)                                   # biases are zero
+    mlp.act = Scale()
+    assert y.any() and torch.equal(mlp(x), 4 * y)
