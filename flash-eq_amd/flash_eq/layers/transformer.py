@@ -60,6 +60,11 @@ class DropPath(nn.Module):
         return x / (1 - self.drop_prob)
 
 
+def _wanted(balance: list[torch.Tensor] | None) -> dict:
+    """The keyword of a call, where there is a list: blocks and subclasses without it stay callable."""
+    return {} if balance is None else {"balance": balance}
+
+
 class EquivariantTransformerBlock(nn.Module):
     """norm -> attention (-> residual when reprs match) -> norm -> gated MLP -> residual.
 
@@ -115,7 +120,7 @@ class EquivariantTransformerBlock(nn.Module):
         half = half_dtype(node_features)
         if half is not None:
             return run_float32(self, half, (P, Q, node_features, distances, graph),
-                               dict(edge_features=edge_features, balance=balance))
+                               dict(edge_features=edge_features, **_wanted(balance)))
         # With the residual connection, the norm also returns the features for
         # it (forward_pair): the residual's gradient is then added inside the
         # norm's backward kernel instead of by autograd in a separate pass.
@@ -193,7 +198,7 @@ class EquivariantTransformer(nn.Module):
                 graph: Graph, balance: list[torch.Tensor] | None = None) -> torch.Tensor:
         half = half_dtype(node_features)
         if half is not None:
-            return run_float32(self, half, (coordinates, node_features, graph), dict(balance=balance))
+            return run_float32(self, half, (coordinates, node_features, graph), _wanted(balance))
         # src - dst, as transformer.py:406.  In float32 through the graph's CSR
         # gathers: their backward (the coordinate gradient) is a fixed-order
         # segmented sum, where torch's indexing backward sorts the indices
@@ -216,7 +221,7 @@ class EquivariantTransformer(nn.Module):
                 uses = [(next(views) if P is m_hidden else P, next(views) if Q is m_hidden else Q)
                         for P, Q in uses]
         for layer, (P, Q) in zip(self.layers, uses):
-            x = layer(P, Q, x, distances, graph, balance=balance)
+            x = layer(P, Q, x, distances, graph, **_wanted(balance))
         return self.final_norm(x)
 
     def extra_repr(self) -> str:

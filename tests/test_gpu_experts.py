@@ -1046,3 +1046,30 @@ def test_another_activation_is_called(dev, dtype):
     y = mlp(x)                                   # biases are zero
     mlp.act = Scale()
     assert y.any() and torch.equal(mlp(x), 4 * y)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_blocks_and_subclasses_without_the_balance_argument(dev, dtype):
+    """Only a call that asks for the balancing terms passes the list on."""
+    class Block(fe.EquivariantTransformerBlock):
+        def forward(self, P, Q, node_features, distances, graph, edge_features=None):
+            return super().forward(P, Q, node_features, distances, graph, edge_features)
+
+    class Model(fe.EquivariantTransformer):
+        def forward(self, coordinates, node_features, graph):
+            return super().forward(coordinates, node_features, graph)
+    torch.manual_seed(13)
+    rp = fe.Repr([0, 1], 16)
+    model = Model(rp, rp, rp, num_layers=2, num_heads=2).to(dev, dtype)
+    graph = fe.Graph.random(40, 200, device=dev)
+    xyz = torch.randn(40, 3, generator=gen(15)).to(dev, dtype)
+    x = torch.randn(40, 16, 4, generator=gen(16)).to(dev, dtype)
+    want = fe.EquivariantTransformer.forward(model, xyz, x, graph) if dtype == torch.float32 else None
+    for i in range(2):
+        block = Block(rp, rp, num_heads=2).to(dev, dtype)
+        block.load_state_dict(model.layers[i].state_dict())
+        model.layers[i] = block
+    y = model(xyz, x, graph)
+    assert y.dtype == dtype and torch.isfinite(y).all() and (want is None or torch.equal(y, want))
+    with pytest.raises(TypeError, match="balance"):
+        fe.EquivariantTransformer.forward(model, xyz.float(), x.float(), graph, balance=[])
