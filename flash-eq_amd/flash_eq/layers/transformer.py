@@ -113,6 +113,11 @@ class EquivariantTransformerBlock(nn.Module):
                                            if layer_scale_init is not None else nn.Identity())
         self.drop_path: nn.Module = DropPath(drop_path) if drop_path > 0.0 else nn.Identity()
 
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        if "experts" not in self._modules:       # a block pickled before there were any
+            self.__dict__.setdefault("experts", None)
+
     def forward(self, P: torch.Tensor, Q: torch.Tensor, node_features: torch.Tensor,
                 distances: torch.Tensor, graph: Graph,
                 edge_features: torch.Tensor | None = None,

@@ -195,3 +195,12 @@ def test_a_plans_sizes_are_those_of_its_tensors(host_plan):
     assert fe.expert_linear(x, w, plan)[4] == 2
     with pytest.raises(TypeError, match="plan must be an ExpertPlan, got SimpleNamespace"):
         fe.expert_linear(x, w, SimpleNamespace(offsets=plan.offsets, num_slots=1))
+
+
+def test_blocks_pickled_before_the_experts_option():
+    rp = fe.Repr([0, 1], 8)
+    block = fe.EquivariantTransformerBlock(rp, rp)
+    del block.experts
+    assert pickle.loads(pickle.dumps(block)).experts is None
+    mixed = pickle.loads(pickle.dumps(fe.EquivariantTransformerBlock(rp, rp, num_experts=2)))
+    assert isinstance(mixed.experts, fe.EquivariantExpertMLP)
