@@ -73,14 +73,16 @@ def _link_nodes(obj: str) -> None:
 
 
 def build(verbose: bool = False) -> str:
-    """Compile every source and link the shared library and the PyTorch module; returns the library's path."""
+    """Compile every source and link the shared library and the PyTorch module; returns the library's path.
+
+    The library is in place before anything of the module can fail, and is built alone where there is
+    no PyTorch.  A module that could not be built leaves none of an earlier library behind."""
     os.makedirs(BUILD_DIR, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
     srcs = sorted(glob.glob(os.path.join(CSRC, "*.hip")))
-    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs))) as ex:
-        nodes = ex.submit(_compile_nodes)
+    with cf.ThreadPoolExecutor(max_workers=min(8, len(srcs) + 1)) as ex:
+        nodes = ex.submit(_compile_nodes) if importlib.util.find_spec("torch") else None
         objs = list(ex.map(_compile, srcs))
-        nodes = nodes.result()
     tmp = LIB_PATH + ".tmp"
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp, *objs,
            "-L/opt/rocm/lib", "-Wl,-rpath,/opt/rocm/lib"]
@@ -88,9 +90,13 @@ def build(verbose: bool = False) -> str:
     if res.returncode != 0:
         raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
     os.replace(tmp, LIB_PATH)
-    _link_nodes(nodes)
+    if os.path.exists(NODES_PATH):
+        os.remove(NODES_PATH)
+    if nodes is not None:
+        _link_nodes(nodes.result())
     if verbose:
-        print(f"built {LIB_PATH} and {NODES_PATH}", file=sys.stderr)
+        built = f"{LIB_PATH} and {NODES_PATH}" if nodes is not None else f"{LIB_PATH} (no PyTorch: no {NODES_PATH})"
+        print(f"built {built}", file=sys.stderr)
     return LIB_PATH
 
 
