@@ -23,6 +23,7 @@ namespace {
 constexpr int kXlMaxPlanes = FEQ_MAX_SLOTS;
 constexpr int kXlMaxReps = FEQ_MAX_IRREPS;
 constexpr int kXlMaxExperts = 1024;
+constexpr int64_t kXlMaxRows = int64_t{1} << 30;     // a row's number and a chunk's length more fit 32 bits
 constexpr int kXlThreads = 256;
 constexpr int kXlBM = 128;          // rows of a block
 constexpr int kXlStreamK = 128;     // reduction columns of the streaming kernel
@@ -838,7 +839,7 @@ int xl_check(const int32_t* lvals, int32_t nreps, int32_t X, int64_t S, int32_t 
     if (X < 1 || S < 0 || ci < 1 || co < 1)
         return fail(FEQ_ERR_INVALID, "%lld rows of %d experts, %d to %d channels", (long long)S, X, ci, co);
     if (X > kXlMaxExperts) return fail(FEQ_ERR_UNSUPPORTED, "more than %d experts", kXlMaxExperts);
-    if (S > INT32_MAX / 2) return fail(FEQ_ERR_UNSUPPORTED, "more than 2^30 rows");
+    if (S > kXlMaxRows) return fail(FEQ_ERR_UNSUPPORTED, "more than 2^30 rows");
     if (ci > 65536 || co > 65536) return fail(FEQ_ERR_UNSUPPORTED, "more than 65536 channels");
     if (!dtype_ok(dtype)) return fail(FEQ_ERR_INVALID, "unknown element type %d", dtype);
     int d = 0;

@@ -204,3 +204,13 @@ def test_blocks_pickled_before_the_experts_option():
     assert pickle.loads(pickle.dumps(block)).experts is None
     mixed = pickle.loads(pickle.dumps(fe.EquivariantTransformerBlock(rp, rp, num_experts=2)))
     assert isinstance(mixed.experts, fe.EquivariantExpertMLP)
+
+
+def test_linear_takes_all_the_slots_of_a_plan():
+    """2^30 rows pass the check of sizes (and meet the next one, of the type)."""
+    lib = N.load_library()
+    one = (ctypes.c_int32 * 1)(0)
+    for slots, text in ((2 ** 30, "unknown element type"), (2 ** 30 + 1, "more than 2^30 rows")):
+        refused(lib.feq_expert_linear_fwd(one, 1, 2, slots, 1, 1, 9, FAKE, FAKE, FAKE, None, 0, None, FAKE, None), text)
+        refused(lib.feq_expert_linear_bwd_w(one, 1, 2, slots, 1, 1, 9, FAKE, FAKE, FAKE, 0, None, FAKE, None, FAKE, 0, None),
+                text)

@@ -1073,3 +1073,31 @@ def test_blocks_and_subclasses_without_the_balance_argument(dev, dtype):
     assert y.dtype == dtype and torch.isfinite(y).all() and (want is None or torch.equal(y, want))
     with pytest.raises(TypeError, match="balance"):
         fe.EquivariantTransformer.forward(model, xyz.float(), x.float(), graph, balance=[])
+
+
+def test_the_most_slots(dev):
+    """2^30 slots of one channel: the sort, the move and the maps at the last places and the first."""
+    slots = 2 ** 30
+    ids = torch.zeros(slots, dtype=torch.int8, device=dev)
+    ids[0], ids[5], ids[-1], ids[-2] = 1, -1, 1, 1
+    plan = fe.ExpertPlan(ids, 2)
+    del ids
+    assert plan.offsets.tolist() == [0, slots - 4, slots - 1]
+    assert plan.order[[0, 4, slots - 4, slots - 3, slots - 2, slots - 1]].tolist() == [1, 6, 0, slots - 2, slots - 1, 5]
+    assert plan.positions[[0, 1, 5, 6, slots - 1], 0].tolist() == [slots - 4, 0, slots - 1, 4, slots - 2]
+    x = torch.zeros(slots, 1, device=dev, dtype=torch.bfloat16)
+    x[0], x[1], x[5], x[-1] = 2.0, 3.0, NAN, 5.0
+    xs = plan.dispatch(x)
+    del x
+    at = [0, 1, slots - 4, slots - 3, slots - 2, slots - 1]
+    assert xs[at, 0].tolist() == [3, 0, 2, 0, 5, 0]
+    xs[-1] = NAN
+    xs.requires_grad_()
+    w = torch.tensor([[[[1.0]]], [[[4.0]]]], device=dev, dtype=torch.bfloat16, requires_grad=True)
+    y = fe.expert_linear(xs, w, plan)
+    assert y[at, 0].tolist() == [3, 0, 8, 0, 20, 0] and not y[2:-4].any()
+    gy = torch.zeros_like(y)
+    gy[at] = torch.tensor([1, 2, 3, 4, 5, NAN], device=dev, dtype=torch.bfloat16)[:, None]
+    gx, gw = torch.autograd.grad(y, [xs, w], gy)
+    assert gx[at, 0].tolist() == [1, 2, 12, 16, 20, 0] and not gx[2:-4].any()
+    assert gw.flatten().tolist() == [3, 31]
