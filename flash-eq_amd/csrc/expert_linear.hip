@@ -842,15 +842,17 @@ int xl_check(const int32_t* lvals, int32_t nreps, int32_t X, int64_t S, int32_t 
     if (S > kXlMaxRows) return fail(FEQ_ERR_UNSUPPORTED, "more than 2^30 rows");
     if (ci > 65536 || co > 65536) return fail(FEQ_ERR_UNSUPPORTED, "more than 65536 channels");
     if (!dtype_ok(dtype)) return fail(FEQ_ERR_INVALID, "unknown element type %d", dtype);
+    const char* const unused = "%d bias columns, not each of them a scalar irrep's";
+    if (bias_cols && nbias > nreps) return fail(FEQ_ERR_INVALID, unused, nbias);     // at most 32: a bit of `used` each
     int d = 0;
     uint32_t used = 0;
     for (int r = 0; r < nreps; ++r) {
         if (lvals[r] < 0) return fail(FEQ_ERR_INVALID, "negative degree");
         const int n = 2 * lvals[r] + 1;
         if (d + n > kXlMaxPlanes) return fail(FEQ_ERR_UNSUPPORTED, "representation dimension exceeds %d", kXlMaxPlanes);
-        const int bc = bias_cols ? bias_cols[r] : -1;   // at most 32 irreps: columns below 32
-        if (bc >= 0) {
-            if (bc >= nbias || n != 1 || (used >> bc & 1))
+        const int bc = bias_cols ? bias_cols[r] : -1;
+        if (bc != -1) {
+            if (bc < 0 || bc >= nbias || n != 1 || (used >> bc & 1))
                 return fail(FEQ_ERR_INVALID, "bias column %d of irrep %d (degree %d, %d columns)", bc, r, lvals[r], nbias);
             used |= 1u << bc;
         }
@@ -861,8 +863,7 @@ int xl_check(const int32_t* lvals, int32_t nreps, int32_t X, int64_t S, int32_t 
         }
     }
     map->first[nreps] = static_cast<int16_t>(d);
-    if (bias_cols && (nbias > nreps || used != (nbias >= 32 ? ~0u : (1u << nbias) - 1u)))
-        return fail(FEQ_ERR_INVALID, "%d bias columns, not each of them a scalar irrep's", nbias);
+    if (bias_cols && nbias > 0 && used != ~0u >> (32 - nbias)) return fail(FEQ_ERR_INVALID, unused, nbias);
     return FEQ_OK;
 }
 

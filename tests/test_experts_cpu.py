@@ -214,3 +214,19 @@ def test_linear_takes_all_the_slots_of_a_plan():
         refused(lib.feq_expert_linear_fwd(one, 1, 2, slots, 1, 1, 9, FAKE, FAKE, FAKE, None, 0, None, FAKE, None), text)
         refused(lib.feq_expert_linear_bwd_w(one, 1, 2, slots, 1, 1, 9, FAKE, FAKE, FAKE, 0, None, FAKE, None, FAKE, 0, None),
                 text)
+
+
+def test_linear_abi_refuses_columns_that_there_are_not():
+    """Numbers that would wrap around in the kernels' tables: below -1, and of 32 and more."""
+    lib = N.load_library()
+    i32 = lambda *v: (ctypes.c_int32 * len(v))(*v)
+
+    def calls(lv, nb, cols):
+        common = (i32(*lv), len(lv), 2, 10, 8, 8, 0)
+        yield lib.feq_expert_linear_fwd(*common, FAKE, FAKE, FAKE, FAKE, nb, i32(*cols), FAKE, None)
+        yield lib.feq_expert_linear_bwd_w(*common, FAKE, FAKE, FAKE, nb, i32(*cols), FAKE, FAKE, None, 0, None)
+    for lv, nb, cols, text in (((0,), 1, (-200,), "bias column -200 of irrep 0"), ((0, 0), 1, (0, -2), "bias column -2 of irrep 1"),
+                               ((0, 0), 34, (33, 1), "34 bias columns"), ((0,), 300, (256,), "300 bias columns"),
+                               ((0, 0), 33, (32, 0), "33 bias columns")):
+        for rc in calls(lv, nb, cols):
+            refused(rc, text)
