@@ -797,38 +797,42 @@ k_xl_wsum(const float* __restrict__ pw, const float* __restrict__ pb, const int3
         slots += __builtin_amdgcn_readlane(incl, 63);
     }
     if (expert < 0) return;
-    const int64_t i = (static_cast<int64_t>(blockIdx.x) * (SPLIT ? 64 : 256) + (SPLIT ? lane : threadIdx.x)) * V;
+    constexpr int EACH = (SPLIT ? 64 : 256) * V;
     const int wave = SPLIT ? threadIdx.x >> 6 : 0;
     const bool w = z < nreps;
     const int64_t size = w ? wsize : co;
-    const float* p = (w ? pw : pb) + static_cast<int64_t>(ch.slot0[rep] + first) * size + i;
-    float a[V];
+    for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * EACH; i0 < size; i0 += static_cast<int64_t>(gridDim.x) * EACH) {
+        const int64_t i = i0 + (SPLIT ? lane : threadIdx.x) * V;
+        const float* p = (w ? pw : pb) + static_cast<int64_t>(ch.slot0[rep] + first) * size + i;
+        float a[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) a[v] = 0.0f;
-    if (i < size) {
+        for (int v = 0; v < V; ++v) a[v] = 0.0f;
+        if (i < size) {
 #pragma unroll 8
-        for (int q = wave; q < count; q += SPLIT ? 4 : 1) {
-            float f[V];
-            load_f<float, V>(p + q * size, f);
+            for (int q = wave; q < count; q += SPLIT ? 4 : 1) {
+                float f[V];
+                load_f<float, V>(p + q * size, f);
 #pragma unroll
-            for (int v = 0; v < V; ++v) a[v] += f[v];
+                for (int v = 0; v < V; ++v) a[v] += f[v];
+            }
         }
-    }
-    if constexpr (SPLIT) {
-        if (wave) store_f<float, V>(part[wave - 1] + lane * V, a);
-        __syncthreads();
-        if (wave) return;
+        if constexpr (SPLIT) {
+            __syncthreads();                         // the last sums have been read
+            if (wave) store_f<float, V>(part[wave - 1] + lane * V, a);
+            __syncthreads();
+            if (wave) continue;
 #pragma unroll
-        for (int q = 0; q < 3; ++q)
+            for (int q = 0; q < 3; ++q)
 #pragma unroll
-            for (int v = 0; v < V; ++v) a[v] += part[q][lane * V + v];
-    }
-    if (i >= size) return;
-    if (w) {
-        store_f<T, V>(gw + (static_cast<int64_t>(expert) * nreps + z) * wsize + i, a);
-    } else {
+                for (int v = 0; v < V; ++v) a[v] += part[q][lane * V + v];
+        }
+        if (i >= size) continue;
+        if (w) {
+            store_f<T, V>(gw + (static_cast<int64_t>(expert) * nreps + z) * wsize + i, a);
+        } else {
 #pragma unroll
-        for (int v = 0; v < V; ++v) gb[(static_cast<int64_t>(expert) * co + i + v) * nbias + (z - nreps)] = static_cast<T>(a[v]);
+            for (int v = 0; v < V; ++v) gb[(static_cast<int64_t>(expert) * co + i + v) * nbias + (z - nreps)] = static_cast<T>(a[v]);
+        }
     }
 }
 
@@ -1018,8 +1022,10 @@ int bwd_w_run(const int32_t* lvals, int nreps, int experts, int64_t slots, int c
                 constexpr int V = decltype(vv)::value;
                 constexpr bool SPLIT = decltype(sp)::value;
                 auto kern = k_xl_wsum<T, V, SPLIT>;
-                FEQ_LAUNCH("k_xl_wsum", kern, dim3(ceil_div(std::max<int64_t>(wsize, cout), (SPLIT ? 64 : 256) * V), many, nreps + nb),
-                           dim3(256), 0, s, pw, pb, offsets, experts, ch, wsize, cout, nreps, gw, gb, nb);
+                // a grid of 2^32 threads and more loses its last workgroups without an error
+                const int64_t blocks = std::min<int64_t>(ceil_div(std::max<int64_t>(wsize, cout), (SPLIT ? 64 : 256) * V), 1 << 20);
+                FEQ_LAUNCH("k_xl_wsum", kern, dim3(blocks, many, nreps + nb), dim3(256), 0, s, pw, pb, offsets, experts, ch,
+                           wsize, cout, nreps, gw, gb, nb);
                 return FEQ_OK;
             };
             auto with_split = [&](auto vv) -> int { return split ? sum(vv, std::true_type{}) : sum(vv, std::false_type{}); };

@@ -1101,3 +1101,23 @@ def test_the_most_slots(dev):
     gx, gw = torch.autograd.grad(y, [xs, w], gy)
     assert gx[at, 0].tolist() == [1, 2, 12, 16, 20, 0] and not gx[2:-4].any()
     assert gw.flatten().tolist() == [3, 31]
+
+
+def test_weight_gradient_of_many_rows_and_a_very_large_weight(dev):
+    """More than 2^30 elements of a weight whose gradient is summed from many chunks of rows."""
+    from flash_eq import _native as N
+    c, slots = 33001, 74000
+    x, gy = (torch.zeros(1, slots, c, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    plan = fe.ExpertPlan(torch.zeros(slots, 1, dtype=torch.int64, device=dev), 1)
+    rows = torch.arange(0, slots, 4000, device=dev)          # 19 rows, in every chunk
+    x[0, rows[:, None], torch.tensor([0, 17, c - 1], device=dev)] = torch.tensor([1.0, 2.0, 3.0], device=dev, dtype=torch.bfloat16)
+    gy[0, rows[:, None], torch.tensor([1, 99, c - 1], device=dev)] = torch.tensor([1.0, 4.0, 8.0], device=dev, dtype=torch.bfloat16)
+    w = torch.zeros(1, 1, c, c, device=dev, dtype=torch.bfloat16, requires_grad=True)
+    lvals = (N.ctypes.c_int32 * 1)(0)
+    assert N.lib().feq_expert_linear_bwd_workspace(lvals, 1, 1, slots, c, c, 0) >= 18 * 4 * c * c
+    y = fe.expert_linear(x, w, plan)
+    (gw,) = torch.autograd.grad(y, [w], gy)
+    out, inp = [0, 1, 99, c - 1], [0, 1, 17, c - 1]
+    got = gw[0, 0][out][:, inp].float().cpu()
+    want = 19 * torch.tensor([0.0, 1, 4, 8])[:, None] * torch.tensor([1.0, 0, 2, 3])
+    assert torch.equal(got, want) and gw.count_nonzero().item() == 9
