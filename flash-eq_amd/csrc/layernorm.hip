@@ -470,15 +470,16 @@ int ln_check(int64_t rows, int64_t width, int64_t ldx, int32_t dtype, const void
     return FEQ_OK;
 }
 
-// Workgroups of the backward, each with a partial of the weight gradients.  Few rows (kLnOneRows a lane group) take
-// one workgroup, which writes the gradients itself: launches bound such calls (100 rows of 192 with their gradients:
-// 60 -> 55 us).  Partials of many wide rows would take more memory than the rows: at most kLnWideBlocks.
-int ln_bwd_blocks(int64_t rows, int64_t width, int32_t dtype) {
+// Workgroups of the backward, each with a partial of the weight gradients where `params` wants them.  Few rows
+// (kLnOneRows a lane group) then take one workgroup, which writes the gradients itself: launches bound such calls (100
+// rows of 192 with their gradients: 60 -> 55 us).  grad_x alone has no launch to save (8 rows of 8000 bfloat16 columns:
+// 13.0 us in one workgroup, 4.6 in eight; 128 x 192 float32: 7.8 and 3.5).  Partials of many wide rows would take more memory than the rows: at most kLnWideBlocks.
+int ln_bwd_blocks(int64_t rows, int64_t width, int32_t dtype, bool params) {
     if (ln_wide(width)) return static_cast<int>(std::min<int64_t>(rows, kLnWideBlocks));
     const int V = 16 / elem_size(dtype);
     const LnForm f = ln_form(width, width >= V ? V : 1);
     const int64_t rounds = ceil_div(rows, f.blk ? 1 : kLnThreads / f.G);
-    return rounds <= kLnOneRows ? 1 : static_cast<int>(std::min<int64_t>(rounds, kLnMaxBlocks));
+    return params && rounds <= kLnOneRows ? 1 : static_cast<int>(std::min<int64_t>(rounds, kLnMaxBlocks));
 }
 
 }  // namespace
@@ -515,7 +516,7 @@ extern "C" int feq_layernorm_fwd(const void* x, int64_t rows, int64_t width, int
 
 extern "C" size_t feq_layernorm_bwd_workspace(int64_t rows, int64_t width, int32_t dtype) {
     if (rows < 1 || width < 1 || width > kLnMaxWidth || !dtype_ok(dtype)) return 0;
-    const int blocks = ln_bwd_blocks(rows, width, dtype);
+    const int blocks = ln_bwd_blocks(rows, width, dtype, true);
     return blocks > 1 ? sizeof(float) * 2 * static_cast<size_t>(width) * blocks : 0;
 }
 
@@ -534,7 +535,7 @@ extern "C" int feq_layernorm_bwd(const void* grad_y, int64_t ldg, const void* x,
         return fail(FEQ_ERR_WORKSPACE, "layer norm workspace of %zu bytes, %zu needed", ws_bytes, need);
     hipStream_t s = stream_of(stream);
     float* part = need ? static_cast<float*>(workspace) : nullptr;
-    int blocks = rows ? ln_bwd_blocks(rows, width, dtype) : 0;
+    int blocks = rows ? ln_bwd_blocks(rows, width, dtype, params) : 0;
     if (rows) {
         const int rc = with_dtype(dtype, [&](auto t) -> int {
             using T = decltype(t);

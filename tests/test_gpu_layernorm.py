@@ -288,3 +288,21 @@ def test_refusals(dev):
     # float64 modules take PyTorch's layer norm, as the other norms do
     norm = fe.InvariantLayerNorm(8).to(dev).double()
     assert torch.equal(norm(x.double()), torch.nn.functional.layer_norm(x.double(), (8,), norm.weight, norm.bias, 1e-5))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_gradient_of_the_rows_alone(dev, dtype):
+    """Frozen or absent parameters: the bits of the call that has their gradients too, in each form of few rows."""
+    for rows, width in ((1, 5), (8, 3000), (7, 8192), (128, 192), (20, 1000), (256, 40), (3, 9000), (40, 9001)):
+        g = torch.Generator().manual_seed(rows)
+        x, gy = (torch.randn(rows, width, generator=g).to(dev, dtype) for _ in range(2))
+        w, b = (torch.randn(width, generator=g).to(dev, dtype).requires_grad_() for _ in range(2))
+        x.requires_grad_()
+        y = ops.layer_norm(x, w, b)
+        both = torch.autograd.grad(y, [x, w, b], gy, retain_graph=True)[0]
+        assert torch.equal(torch.autograd.grad(y, [x], gy)[0], both)
+        frozen = ops.layer_norm(x, w.detach(), b.detach())
+        assert torch.equal(torch.autograd.grad(frozen, [x], gy)[0], both)
+        ones = torch.ones(width, device=dev, dtype=dtype, requires_grad=True)
+        plain = torch.autograd.grad(ops.layer_norm(x, ones), [x, ones], gy)[0]
+        assert torch.equal(torch.autograd.grad(ops.layer_norm(x), [x], gy)[0], plain)
