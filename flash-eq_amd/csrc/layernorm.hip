@@ -380,8 +380,8 @@ struct LnForm {
 };
 bool ln_wide(int64_t width) { return width > kLnThreads * kLnBlockElems; }     // the _wide kernels
 
-// NV of the instances: the smallest that covers.
-inline int ln_nv(int64_t n) { return n <= 1 ? 1 : n <= 2 ? 2 : n <= 3 ? 3 : n <= 4 ? 4 : n <= 8 ? 8 : n <= 16 ? 16 : 32; }
+// NV of the instances: the smallest that covers (n <= 8: kLnBlockElems elements of at least four a vector).
+inline int ln_nv(int64_t n) { return n <= 4 ? static_cast<int>(n) : 8; }
 
 LnForm ln_form(int64_t width, int V) {
     LnForm f{false, 64, 1};
@@ -414,8 +414,6 @@ int ln_with_nv(int nv, F&& f) {
         case 3: return f(std::integral_constant<int, 3>{});
         case 4: return f(std::integral_constant<int, 4>{});
         case 8: if constexpr (8 * V <= kLnBlockElems) return f(std::integral_constant<int, 8>{}); else break;
-        case 16: if constexpr (16 * V <= kLnBlockElems) return f(std::integral_constant<int, 16>{}); else break;
-        case 32: if constexpr (32 * V <= kLnBlockElems) return f(std::integral_constant<int, 32>{}); else break;
     }
     return fail(FEQ_ERR_INVALID, "internal: layer norm form");
 }
