@@ -1121,3 +1121,18 @@ def test_weight_gradient_of_many_rows_and_a_very_large_weight(dev):
     got = gw[0, 0][out][:, inp].float().cpu()
     want = 19 * torch.tensor([0.0, 1, 4, 8])[:, None] * torch.tensor([1.0, 0, 2, 3])
     assert torch.equal(got, want) and gw.count_nonzero().item() == 9
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("lvals", [(0,), (0, 1)])
+def test_linear_of_many_large_uneven_experts(dev, lvals, dtype):
+    """Weights that outweigh the rows take longer chunks (512 and more tiles of 128 columns both ways over the
+    experts and irreps): tiles in both directions, experts of no, one and several chunks, rows without an expert."""
+    from flash_eq import _native as N
+    cin, cout = 300, 520
+    counts = [(7 * e) % 23 for e in range(64)]
+    counts[40], counts[63], counts[9] = 2500, 700, 0
+    assert -(-cin // 128) * -(-cout // 128) * 64 >= 512 and 0 in counts
+    arr = (N.ctypes.c_int32 * len(lvals))(*lvals)
+    assert N.lib().feq_expert_linear_bwd_workspace(arr, len(lvals), 64, sum(counts) + 37, cin, cout, 1) > 4 * cin * cout
+    check_linear(dev, lvals, counts, 37, cin, cout, dtype, seed=21)
