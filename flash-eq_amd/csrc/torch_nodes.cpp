@@ -145,8 +145,42 @@ std::shared_ptr<N> node_for(const In&... in) {
     return node;
 }
 
-// Keeps `t` (an input or an intermediate, not an output) for the backward; in-place changes until then are errors.
-SavedVariable keep(const Tensor& t) { return SavedVariable(t, false); }
+// A tensor kept for the backward; in-place changes until then are errors.  A saved-tensor hook may hand out
+// another tensor: one of other strides is copied, one that could not stand for the kept one is refused.
+class Kept {
+   public:
+    // `output`: of the node that keeps it
+    void keep(const Tensor& t, bool output = false) {
+        saved_ = SavedVariable(t, output);
+        defined_ = t.defined();
+        if (!defined_) return;
+        sizes_.assign(t.sizes().begin(), t.sizes().end());
+        type_ = t.scalar_type();
+        device_ = t.device();
+    }
+    // As kept, its rows apart where they were (rows_of takes those).
+    Tensor get(std::shared_ptr<torch::autograd::Node> node = nullptr) const {
+        Tensor t = saved_.unpack(std::move(node));
+        TORCH_CHECK(t.defined() == defined_, "a saved-tensor hook returned no tensor");
+        if (defined_)
+            TORCH_CHECK(t.sizes() == at::IntArrayRef(sizes_) && t.scalar_type() == type_ && t.device() == device_,
+                        "a saved-tensor hook returned a ", dtype_name(t.scalar_type()), " tensor of shape ", t.sizes(), " on ",
+                        t.device(), " for a ", dtype_name(type_), " one of shape ", at::IntArrayRef(sizes_), " on ", device_);
+        return t;
+    }
+    Tensor get_dense(std::shared_ptr<torch::autograd::Node> node = nullptr) const {
+        const Tensor t = get(std::move(node));
+        return t.defined() ? dense(t) : t;
+    }
+    void reset_data() { saved_.reset_data(); }
+
+   private:
+    SavedVariable saved_;
+    bool defined_ = false;
+    c10::SmallVector<int64_t, 4> sizes_;
+    at::ScalarType type_ = at::kFloat;
+    c10::Device device_ = at::kCPU;
+};
 
 // ---- layer norm ----------------------------------------------------------------------
 
@@ -163,7 +197,7 @@ Tensor rows_of(const Tensor& t, int64_t& ld) {
 }
 
 struct LayerNormNode final : OnceNode {
-    SavedVariable x, w;
+    Kept x, w;
     Tensor stats;             // (2, rows): mean, 1 / standard deviation
     int pdtype = 0;           // feq_dtype of the parameters
     at::ScalarType ptype = at::kFloat;
@@ -171,9 +205,9 @@ struct LayerNormNode final : OnceNode {
     variable_list backward(variable_list& grads) override {
         variable_list out(3);
         if (!grads[0].defined()) return out;
-        const Tensor xs = x.unpack(), ws = w.unpack();
+        const Tensor xs = x.get(), ws = w.get_dense();
         int64_t ldx, ldg;
-        const Tensor xr = rows_of(xs, ldx), g = rows_of(grads[0], ldg);     // xs was saved as read
+        const Tensor xr = rows_of(xs, ldx), g = rows_of(grads[0], ldg);
         const int64_t width = xr.size(-1), rows = xr.numel() / width;
         const bool nx = need(0), nw = need(1), nb = need(2);
         if (nx) out[0] = make(xr.sizes(), xr, xr.scalar_type());
@@ -224,8 +258,8 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
                                ptr_as<float>(stats), stats.defined() ? ptr_as<float>(stats) + rows : nullptr, on.stream),
              "feq_layernorm_fwd");
         if (node) {
-            node->x = keep(xs);
-            node->w = keep(wc);
+            node->x.keep(xs);
+            node->w.keep(wc);
             node->stats = stats;
             node->pdtype = pcode;
             node->ptype = w.defined() ? w.scalar_type() : b.defined() ? b.scalar_type() : at::kFloat;
@@ -238,13 +272,13 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
 // ---- top-k ---------------------------------------------------------------------------
 
 struct TopkNode final : OnceNode {
-    SavedVariable logits, ids, weights;      // weights: the node's own first output
+    Kept logits, ids, weights;      // weights: the node's own first output
     bool normalize = true;
 
     variable_list backward(variable_list& grads) override {
         variable_list out(1);
         if (!grads[0].defined() && !grads[1].defined()) return out;
-        const Tensor l = logits.unpack(), chosen = ids.unpack(), w = weights.unpack(shared_from_this());
+        const Tensor l = logits.get_dense(), chosen = ids.get_dense(), w = weights.get_dense(shared_from_this());
         const Tensor gw = grads[0].defined() ? dense(grads[0]) : Tensor(), gm = grads[1].defined() ? dense(grads[1]) : Tensor();
         out[0] = make(l.sizes(), l, l.scalar_type());
         On on(l);
@@ -285,15 +319,15 @@ std::tuple<Tensor, Tensor, Tensor> expert_topk(const Tensor& logits, int64_t top
                                  ptr_as<float>(mean), ptr(ws), bytes_of(ws), on.stream),
              "feq_expert_topk_fwd");
         if (node) {
-            node->logits = keep(lc);
-            node->ids = keep(ids);
+            node->logits.keep(lc);
+            node->ids.keep(ids);
             node->normalize = normalize;
         }
     }
     if (node) {
         torch::autograd::set_history(weights, node);
         torch::autograd::set_history(mean, node);
-        node->weights = SavedVariable(weights, true);
+        node->weights.keep(weights, true);
     }
     if (logits.dim() != 2) {
         auto shape = logits.sizes().vec();
@@ -419,12 +453,12 @@ Tensor expert_dispatch(const Tensor& x, const Tensor& positions, const Tensor& o
 }
 
 struct CombineNode final : OnceNode {
-    SavedVariable ys, weights;
+    Kept ys, weights;
     Places places;
     variable_list backward(variable_list& grads) override {
         variable_list out(2);
         if (!grads[0].defined()) return out;
-        const Tensor in = ys.unpack(), w = weights.unpack(), g = dense(grads[0]);   // an error when they have been freed
+        const Tensor in = ys.get_dense(), w = weights.get_dense(), g = dense(grads[0]);   // an error when they have been freed
         places.check();
         if (need(0)) out[0] = make(in.sizes(), in, in.scalar_type());
         if (need(1)) out[1] = make(w.sizes(), w, w.scalar_type());
@@ -463,8 +497,8 @@ Tensor expert_combine(const Tensor& ys, const Tensor& weights, const Tensor& pos
         const Tensor yc = dense(ys), wc = dense(weights);
         y = combined(p, yc, wc);
         if (node) {
-            node->ys = keep(yc);
-            node->weights = keep(wc);
+            node->ys.keep(yc);
+            node->weights.keep(wc);
             node->places = p;
         }
     }
@@ -491,7 +525,7 @@ struct Irreps {
 };
 
 struct ExpertLinearNode final : OnceNode {
-    SavedVariable x, weight;
+    Kept x, weight;
     Tensor offsets;
     Irreps irreps{{0}};
     int64_t nbias = 0;
@@ -499,7 +533,7 @@ struct ExpertLinearNode final : OnceNode {
     variable_list backward(variable_list& grads) override {
         variable_list out(3);
         if (!grads[0].defined()) return out;
-        const Tensor xs = x.unpack(), w = weight.unpack(), g = dense(grads[0]);     // an error when they have been freed
+        const Tensor xs = x.get_dense(), w = weight.get_dense(), g = dense(grads[0]);     // an error when they have been freed
         check_plan(offsets, "offsets", 1);
         const int64_t experts = w.size(0), co = w.size(2), ci = w.size(3), slots = xs.size(-2);
         const int code = code_of(xs, "x");
@@ -573,8 +607,8 @@ Tensor expert_linear(const Tensor& x, const Tensor& weight, const OptTensor& bia
                                    ptr(y), on.stream),
              "feq_expert_linear_fwd");
         if (node) {
-            node->x = keep(xc);
-            node->weight = keep(wc);
+            node->x.keep(xc);
+            node->weight.keep(wc);
             node->offsets = offsets;
             node->irreps = irreps;
             node->nbias = irreps.nscalar;

@@ -1136,3 +1136,42 @@ def test_linear_of_many_large_uneven_experts(dev, lvals, dtype):
     arr = (N.ctypes.c_int32 * len(lvals))(*lvals)
     assert N.lib().feq_expert_linear_bwd_workspace(arr, len(lvals), 64, sum(counts) + 37, cin, cout, 1) > 4 * cin * cout
     check_linear(dev, lvals, counts, 37, cin, cout, dtype, seed=21)
+
+
+def hooked_calls(dev):
+    """(call, its leaves) of every operator that keeps tensors for its backward."""
+    g = gen(22)
+    plan = fe.ExpertPlan(torch.tensor([[0, 1], [1, 0], [1, 1]], device=dev), 2)
+    leaf = lambda *s: torch.randn(*s, generator=g).to(dev).requires_grad_()
+    return [(lambda x, w: fe.ops.layer_norm(x, w), (leaf(5, 24), leaf(24))),
+            (lambda l: fe.expert_topk(l, 2)[1], (leaf(5, 24),)),
+            (lambda ys, w: plan.combine(ys, w), (leaf(4, 6, 24), leaf(3, 2))),
+            (lambda x, w: fe.expert_linear(x, w, plan, (0, 1)), (leaf(4, 6, 24), leaf(2, 2, 7, 24)))]
+
+
+def test_saved_tensors_come_back_in_any_layout(dev):
+    """A hook may hand out a saved tensor's values with other strides."""
+    turn = lambda t: t.permute(*range(t.dim() - 1, -1, -1))
+    for call, leaves in hooked_calls(dev):
+        gy = torch.randn(call(*leaves).shape, generator=gen(23)).to(dev)
+        want = torch.autograd.grad(call(*leaves), leaves, gy)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: turn(t).contiguous(), turn):
+            y = call(*leaves)
+        for a, b in zip(torch.autograd.grad(y, leaves, gy), want):
+            assert torch.equal(a, b)
+        with torch.autograd.graph.save_on_cpu():
+            y = call(*leaves)
+        for a, b in zip(torch.autograd.grad(y, leaves, gy), want):
+            assert torch.equal(a, b)
+
+
+def test_saved_tensors_of_another_kind_are_refused(dev):
+    """What a hook hands out has the kept tensor's shape, type and device, or the backward raises."""
+    others = [lambda t: t.cpu(), lambda t: t[:1], lambda t: t.double() if t.is_floating_point() else t.int(),
+              lambda t: t.reshape(-1)]
+    for other in others:
+        for call, leaves in hooked_calls(dev):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, other):
+                y = call(*leaves)
+            with pytest.raises(RuntimeError, match="a saved-tensor hook returned a"):
+                y.sum().backward()
