@@ -125,12 +125,18 @@ struct OnceNode : torch::autograd::Node {
     variable_list apply(variable_list&& grads) final {
         variable_list out;
         {
+            std::lock_guard<std::mutex> lock(mutex_);      // a backward of the same graph in another thread frees
             at::NoGradGuard none;
             out = backward(grads);
         }
         return once(std::move(out));
     }
+    void release_variables() final {
+        std::lock_guard<std::mutex> lock(mutex_);
+        release();
+    }
     virtual variable_list backward(variable_list& grads) = 0;
+    virtual void release() {}
     bool need(size_t i) const { return task_should_compute_output(i); }
 };
 
@@ -221,7 +227,7 @@ struct LayerNormNode final : OnceNode {
              "feq_layernorm_bwd");
         return out;
     }
-    void release_variables() override {
+    void release() override {
         x.reset_data();
         w.reset_data();
         stats.reset();
@@ -287,7 +293,7 @@ struct TopkNode final : OnceNode {
              "feq_expert_topk_bwd");
         return out;
     }
-    void release_variables() override {
+    void release() override {
         logits.reset_data();
         ids.reset_data();
         weights.reset_data();
@@ -473,7 +479,7 @@ struct CombineNode final : OnceNode {
         }
         return out;
     }
-    void release_variables() override {
+    void release() override {
         ys.reset_data();
         weights.reset_data();
         places = Places();
@@ -560,7 +566,7 @@ struct ExpertLinearNode final : OnceNode {
         if (need(2)) out[2] = gb;
         return out;
     }
-    void release_variables() override {
+    void release() override {
         x.reset_data();
         weight.reset_data();
         offsets.reset();

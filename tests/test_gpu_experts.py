@@ -1175,3 +1175,26 @@ def test_saved_tensors_of_another_kind_are_refused(dev):
                 y = call(*leaves)
             with pytest.raises(RuntimeError, match="a saved-tensor hook returned a"):
                 y.sum().backward()
+
+
+def test_two_threads_take_one_graph_backward(dev):
+    """One frees what the other may be reading: each ends with the gradient or with the error of a second backward."""
+    import threading
+    for call, leaves in hooked_calls(dev):
+        want = torch.autograd.grad(call(*leaves).sum(), leaves)
+        torch.cuda.synchronize()
+        for _ in range(20):
+            y = call(*leaves).sum()
+            ends = []
+
+            def work():
+                try:
+                    ends.append(all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves), want)))
+                except RuntimeError as e:
+                    ends.append("a second time" in str(e))
+            threads = [threading.Thread(target=work) for _ in range(2)]
+            for t in threads:
+                t.start()
+            for t in threads:
+                t.join()
+            assert ends == [True, True]
