@@ -24,7 +24,6 @@ constexpr int kXlMaxPlanes = FEQ_MAX_SLOTS;
 constexpr int kXlMaxReps = FEQ_MAX_IRREPS;
 constexpr int kXlMaxExperts = 1024;
 constexpr int64_t kXlMaxRows = int64_t{1} << 30;     // a row's number and a chunk's length more fit 32 bits
-constexpr int kXcds = 8;            // XCDs, each with an L2 of its own
 constexpr int kXlThreads = 256;
 constexpr int kXlBM = 128;          // rows of a block
 constexpr int kXlStreamK = 128;     // reduction columns of the streaming kernel
@@ -44,12 +43,13 @@ struct XlMap {
 };
 
 // Weight-gradient chunks, which the irreps of many planes have shorter: rows of a chunk, the first chunk's number over
-// kXcds (irreps in descending order, as launched) and first partial of every irrep; irrep of every bias column.
+// `xcds` (irreps in descending order, as launched) and first partial of every irrep; irrep of every bias column.
 struct XlChunks {
     int32_t rows[kXlMaxReps];
     int32_t tile0[kXlMaxReps + 1];
     int32_t slot0[kXlMaxReps + 1];
     int8_t brep[kXlMaxReps];
+    int32_t xcds;        // XCDs that chunks are dealt to, each with all its tiles; 1: the tiles are
 };
 
 // One reduction step of a 16 x 16 tile: KS elements, a lane holding FE of them.
@@ -608,16 +608,17 @@ k_xl_wgrad(const T* __restrict__ gy, const T* __restrict__ x, const T* __restric
     __shared__ __align__(16) T lds[SIZE > WSIZE ? SIZE : WSIZE];
     T *sX = lds, *sG = lds + BP * LX;
     const int nk = (ci + BK - 1) / BK, nn = (co + BN - 1) / BN;
-    // workgroups go to the XCDs in turn; the tiles of a chunk go to one, whose L2 passes its rows to all of them.  Dealt
-    // by tiles: 20000 x 9 bfloat16 rows, 256 x 256: 93 us, so 86; float32: 279 and 262; of 64 uneven experts 8191 x 512
-    // x 1024 bfloat16 rows: 39.8 and 37.8 us, 20000 x 4 x 256 x 256: 47.9 and 41.6; 4000 x 1024 x 1024 of 16: 34.2 and
-    // 36.3 (few chunks, unevenly dealt)
-    const int block = blockIdx.x / (kXcds * nk * nn);
+    // workgroups go to the 8 XCDs in turn; the tiles of a chunk go to one, whose L2 passes its rows to all of them
+    // (20000 x 9 bfloat16 rows, 256 x 256: 93 -> 86 us; float32: 279 -> 262), unless chunks are long and few
+    // (wgrad_chunks): those leave XCDs idle.  A map with all its gradients, dealt by tiles and by chunks: 15000 x 400 x
+    // 1000 float32 of 32 experts 606 and 633 us, bfloat16 8191 x 1024 x 512 of 64 101 and 104, 4000 x 1024 x 1024 of 8 85 and
+    // 91; where there are more chunks, 20000 x 4 x 256 x 256 of 64 129 and 121, 60000 x 256 x 512 146 and 142
+    const int xcds = ch.xcds, block = blockIdx.x / (xcds * nk * nn);
     int rep = nreps - 1;                             // the irreps of most planes first
     while (rep > 0 && block >= ch.tile0[rep - 1]) --rep;
     const int rc = ch.rows[rep];
-    const int i0 = blockIdx.x / kXcds - ch.tile0[rep] * nk * nn, sub = i0 % (nk * nn);
-    const XlTile t = XlBlocks<true>(offsets, X, S, rc).find(i0 / (nk * nn) * kXcds + blockIdx.x % kXcds);
+    const int i0 = blockIdx.x / xcds - ch.tile0[rep] * nk * nn, sub = i0 % (nk * nn);
+    const XlTile t = XlBlocks<true>(offsets, X, S, rc).find(i0 / (nk * nn) * xcds + blockIdx.x % xcds);
     if (t.expert < 0 || (!GX && t.expert == X)) return;
     const int k0 = (sub % nk) * BK, n0 = (sub / nk) * BN;
     const int rend = t.row1 - t.row0 < rc ? t.row1 : t.row0 + rc;
@@ -946,6 +947,7 @@ int64_t wgrad_chunks(int64_t S, int X, const int32_t* lvals, int nreps, int ci, 
     for (int r = 0; r < nreps; ++r) dim += 2 * lvals[r] + 1;
     const bool heavy = sub * nreps * X >= 512;
     const int64_t want = heavy ? 256 : 1024;
+    ch->xcds = heavy ? 1 : 8;
     const int64_t unit = ceil_div(std::max<int64_t>(S, 1) * dim * sub, want);
     int64_t tiles = 0, slots = 0;
     for (int r = nreps - 1; r >= 0; --r) {
@@ -953,7 +955,7 @@ int64_t wgrad_chunks(int64_t S, int X, const int32_t* lvals, int nreps, int ci, 
         ch->rows[r] = static_cast<int32_t>(rows);
         ch->tile0[r] = static_cast<int32_t>(tiles);
         ch->slot0[r] = static_cast<int32_t>(slots);
-        tiles += ceil_div(S / rows + X + 1, kXcds);          // the rows without an expert last
+        tiles += ceil_div(S / rows + X + 1, ch->xcds);          // the rows without an expert last
         slots += S > rows ? 2 * S / rows : 0;
     }
     ch->tile0[nreps] = static_cast<int32_t>(tiles);      // all
@@ -986,7 +988,7 @@ int bwd_w_run(const int32_t* lvals, int nreps, int experts, int64_t slots, int c
             auto run = [&](auto wr, auto ti, auto bn) -> int {
                 constexpr int WR = decltype(wr)::value, TI = decltype(ti)::value, BN = decltype(bn)::value;
                 constexpr int BK = 16 * TI * WR;
-                const int64_t blocks = static_cast<int64_t>(kXcds) * ch.tile0[nreps] * ceil_div(cin, BK) * ceil_div(cout, BN);
+                const int64_t blocks = ch.xcds * static_cast<int64_t>(ch.tile0[nreps]) * ceil_div(cin, BK) * ceil_div(cout, BN);
                 if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
                 auto go = [&](auto once, auto with_gx) -> int {
                     constexpr bool GX = decltype(with_gx)::value;
