@@ -10,6 +10,8 @@
 // types, float32 accumulators for both, one rounding at the store.  The expert of a row block is found by every wave
 // from the offsets (experts over the lanes, a sum along the wave), so the host never learns the counts and the grid is their
 // upper bound.  The weight is the first operand and the rows the second: a lane's accumulators are columns of one row.
+//
+// Times below are medians of a kernel's launches in training passes unless a comment says otherwise.
 #include <algorithm>
 
 #include "elem_types.h"
@@ -322,9 +324,9 @@ inline int64_t xcd_grid(int64_t bound, int64_t subs) { return 8 * ceil_div(bound
 // out[d, p, :] = in[d, p, :] B (+ bias), B = W[e, r]^T (TRANS false: in has Cin columns, out Cout) or W[e, r]
 // (TRANS: in has Cout columns, out Cin).  K: columns of in, N: of out; W rows have wld = Cin elements.
 // WR: waves along the output columns (64 each), 4 / WR along the rows.
-// 8191 bfloat16 rows of 64 experts, 512 to 1024 columns: 30 us forward, 28 grad_x (290 TFLOP/s): the workgroups run
-// in two rounds of 8 and 16 steps that wait for LDS and for each other.  Steps of half the columns with three
-// workgroups on a CU instead of two: 45 and 49 us.
+// 8191 bfloat16 rows of 64 experts, 512 to 1024 columns: 35 us forward, 28 grad_x (246 and 303 TFLOP/s): the
+// workgroups run in two rounds of 8 and 16 steps that wait for LDS and for each other.  Steps of half the columns with
+// three workgroups on a CU instead of two, against these (31 and 28 us in runs of their own): 45 and 49 us.
 template <class T, int HOW, bool TRANS, int WR>
 __global__ void __launch_bounds__(kXlThreads, 2)
 k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,
@@ -464,9 +466,10 @@ k_xl_mm(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __rest
 // in the matrix cores' layout (lane (c, g): FE elements of row c), the next block's rows in flight during this
 // one's products.  Nothing but the weight passes through LDS and no barrier stands between blocks of an
 // expert.  NS: reduction steps held (K <= NS KS).
-// Forward and grad_x, against the tile kernel: 78 and 75 us (95 and 91) for 40000 x 9 float32 rows, 64 x 128 (3.5 TB/s;
-// the matrix cores' share is 38 us); 117 and 116 (140 and 139) for 20011 x 49 bfloat16 rows, 128 x 128 (4.3 TB/s).
-// Column blocks no wider than the output: 16 columns take 28 us in blocks of 32, 52 in blocks of 128.
+// Forward and grad_x alone, against the tile kernel: 93 and 90 us (107 and 105) for 40000 x 9 float32 rows, 64 x 128 (3.0
+// TB/s; the matrix cores' share is 38 us); 122 and 121 (140 and 141) for 20011 x 49 bfloat16 rows, 128 x 128 (4.1 TB/s;
+// 137, 3.7 TB/s, where the fused gradients run between the calls).  Column blocks no wider than the output: 16 columns
+// take 28 us in blocks of 32, 52 in blocks of 128.
 template <class T, int HOW, bool TRANS, int NB, int NS>
 __global__ void __launch_bounds__(kXlThreads, NB * NS * Mma<T>::KS * sizeof(T) > 40000 ? 2 : NS == 8 || HOW != kWhole ? 3 : 4)
 k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __restrict__ offsets, int X, int S, int K,
@@ -588,9 +591,9 @@ k_xl_stream(const T* __restrict__ in, const T* __restrict__ W, const int32_t* __
 // gradient written (zeros without rows), one of several a float32 partial per chunk: pw[slot N K + n K + k],
 // pb[slot N + n], summed by k_xl_wsum.
 // GX: grad_x too, from the same rows of grad_y, where one tile covers the weight (20011 x 49 bfloat16 rows, 128 x 128:
-// 162 us, where grad_x took 121 and grad_W 105; 40000 x 9 float32 rows, 64 x 128: 143, where they took 84 and 75.  A
-// second pair of row buffers, filled during the products, gained nothing: HBM bounds the first, the matrix cores' 77 us
-// the second).
+// 164 us, where grad_x took 121 and grad_W 105; 40000 x 9 float32 rows, 64 x 128: 145, where they took 84 and 75).  HBM
+// bounds the first (4.6 TB/s).  The second has 78 us of bytes and 77 of products; its chunks, whose rows are rounded up
+// (wgrad_chunks), are no even load.  A second pair of row buffers, filled during the products, gained nothing.
 // ONCE: one tile covers the weight, so every row is read once; the rows then go past the caches, which leaves them to
 // the kernels around (grad_W alone for 20011 x 49 bfloat16 rows, 128 x 128: 137 -> 97 us).  Rows that several tiles read
 // lose by it (42 -> 52 us for 512 x 1024).
@@ -937,7 +940,8 @@ int mm_run(const void* in, const void* W, const int32_t* offsets, int X, int64_t
 }
 
 // Weight-gradient chunks: all of about as many row-planes, for about 1024 workgroups, whose partials cost little
-// beside the rows.  Where the experts' weights alone make half of that (64 experts, 512 to 1024 channels: 2048),
+// beside the rows.  Rows are rounded up to 64, so that short chunks are uneven: 40000 slots of degrees 0 to 2, 352
+// row-planes wanted each, have chunks of 384, 128 x 3 and 128 x 5.  Where the experts' weights alone make half of that (64 experts, 512 to 1024 channels: 2048),
 // chunks four times as long: a chunk's partial is written and read at 8 bytes an element, which 1024 rows are
 // worth and 256 are not (8191 bfloat16 rows: the sums took 166 us beside 44 of products).  A partial is needed for
 // an expert of several chunks; those have at most 2 S / rows.  Returns the number of partials.
