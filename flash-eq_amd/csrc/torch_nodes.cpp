@@ -357,6 +357,7 @@ std::tuple<Tensor, Tensor, Tensor> expert_plan(const Tensor& ids, int64_t expert
     if (slots > (int64_t{1} << 30)) value_error("more than 2^30 slots: ", slots);
     at::NoGradGuard none;
     c10::InferenceMode tracked(false);      // in-place changes of a plan made in inference mode are counted too (check_plan)
+    at::AutoDispatchBelowADInplaceOrView uncounted;   // at::empty fills what it makes where algorithms have to be deterministic
     const Tensor flat = dense(ids.scalar_type() == at::kLong ? ids : ids.to(at::kLong));
     Tensor order = make({slots}, flat, at::kInt), positions = make({ids.size(0), k}, flat, at::kInt),
            offsets = make({experts + 1}, flat, at::kInt);

@@ -1198,3 +1198,57 @@ def test_two_threads_take_one_graph_backward(dev):
             for t in threads:
                 t.join()
             assert ends == [True, True]
+
+
+@pytest.mark.parametrize("lout,mult", [([0, 1, 2], 32), ([0, 1], 20)])
+def test_a_block_of_one_expert_is_the_dense_block(dev, lout, mult):
+    """Values and all gradients of the whole block, its residual and layer scales included."""
+    torch.manual_seed(14)
+    rin, rout = fe.Repr([0, 1], mult), fe.Repr(lout, mult)
+    args = dict(num_heads=4, layer_scale_init=0.3)
+    dense = fe.EquivariantTransformerBlock(rin, rout, **args).to(dev)
+    mixed = fe.EquivariantTransformerBlock(rin, rout, num_experts=1, experts_per_node=1, **args).to(dev)
+    state = {k: v for k, v in dense.state_dict().items() if not k.startswith("mlp_")}
+    own = mixed.experts.state_dict()
+    for name in ("up", "down"):
+        own[f"{name}.weight"] = getattr(dense, f"mlp_{name}").weight.detach().view(own[f"{name}.weight"].shape)
+        own[f"{name}.bias"] = torch.randn(own[f"{name}.bias"].shape, generator=gen(24)).to(dev)
+        with torch.no_grad():
+            getattr(dense, f"mlp_{name}").bias.copy_(own[f"{name}.bias"].view(getattr(dense, f"mlp_{name}").bias.shape))
+    own.update({f"act.{k}": v for k, v in dense.mlp_act.state_dict().items()})
+    mixed.load_state_dict({**state, **{f"experts.{k}": v for k, v in own.items()}})
+    graph = fe.Graph.random(300, 2400, device=dev)
+    vec = torch.randn(2400, 3, generator=gen(25)).to(dev)
+    P, Q = fe.WignerDBasis([rin, rout]).to(dev)(vec)
+    x = torch.randn(300, mult, rin.dim(), generator=gen(26)).to(dev).requires_grad_()
+    gy = torch.randn(300, mult, rout.dim(), generator=gen(27)).to(dev)
+    got = []
+    for block in (dense, mixed):
+        y = block(P, Q, x, vec.norm(dim=-1), graph)
+        names = [k for k, _ in block.named_parameters() if "router" not in k]
+        grads = torch.autograd.grad(y, [x] + [block.get_parameter(k) for k in names], gy)
+        got.append(dict(zip(["y", "x"] + [k.replace("experts.", "mlp_") for k in names], (y.detach(), *grads))))
+    assert got[0].keys() == got[1].keys()
+    for k, a in got[0].items():
+        b = got[1][k].view(a.shape)
+        assert (a - b).abs().max() <= 2e-5 * a.abs().max(), k       # the bar of the mixture against 64 bits
+
+
+def test_deterministic_algorithms(dev):
+    """The setting, which fills new tensors in place, changes nothing and refuses nothing."""
+    torch.manual_seed(15)
+    mlp = fe.EquivariantExpertMLP(fe.Repr([0, 1], 8), 4, 2).to(dev)
+    x = torch.randn(50, 8, 4, generator=gen(28)).to(dev).requires_grad_()
+    leaves = [x, *mlp.parameters()]
+    step = lambda: torch.autograd.grad(mlp(x).square().sum(), leaves)
+    want = step()
+    torch.use_deterministic_algorithms(True)
+    try:
+        got = step()
+        with torch.inference_mode():
+            y = mlp(x)
+    finally:
+        torch.use_deterministic_algorithms(False)
+    assert torch.equal(y, mlp(x))
+    for a, b in zip(got, want):
+        assert torch.allclose(a, b, rtol=1e-5, atol=1e-6 * b.abs().max().item())
