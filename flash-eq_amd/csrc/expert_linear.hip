@@ -941,10 +941,11 @@ int mm_run(const void* in, const void* W, const int32_t* offsets, int X, int64_t
 
 // Weight-gradient chunks: all of about as many row-planes, for about 1024 workgroups, whose partials cost little
 // beside the rows.  Rows are rounded up to 64, so that short chunks are uneven: 40000 slots of degrees 0 to 2, 352
-// row-planes wanted each, have chunks of 384, 128 x 3 and 128 x 5.  Where the experts' weights alone make half of that (64 experts, 512 to 1024 channels: 2048),
-// chunks four times as long: a chunk's partial is written and read at 8 bytes an element, which 1024 rows are
-// worth and 256 are not (8191 bfloat16 rows: the sums took 166 us beside 44 of products).  A partial is needed for
-// an expert of several chunks; those have at most 2 S / rows.  Returns the number of partials.
+// row-planes wanted each, have chunks of 384, 128 x 3 and 128 x 5.  Where the experts' weights alone make half of
+// that (64 experts, 512 to 1024 channels: 2048), chunks four times as long: a chunk's partial is written and read at 8
+// bytes an element, which 1024 rows are worth and 256 are not (8191 bfloat16 rows: the sums took 166 us beside 44 of
+// products).  A partial is needed for an expert of several chunks; those have at most 2 S / rows.  Returns the number
+// of partials.
 int64_t wgrad_chunks(int64_t S, int X, const int32_t* lvals, int nreps, int ci, int co, XlChunks* ch) {
     const int64_t sub = ceil_div(ci, ci <= 64 ? 64 : 128) * ceil_div(co, 128);
     int64_t dim = 0;

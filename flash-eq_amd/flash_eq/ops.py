@@ -1334,7 +1334,9 @@ class GatingFn(torch.autograd.Function):
             rc = lib.feq_gate_norms(arr, nreps, mult, n, int(cm), N.ptr(xs), eps, N.ptr(norms),
                                     N.stream_ptr(dev))
         N.check(rc, "feq_gate_norms")
-        lin = torch.addmm(bias.detach(), norms, weight.detach().t())
+        # into tables of their own: autocast would make these products 16-bit, and the kernels read float32
+        lin = torch.empty_like(norms)
+        torch.addmm(bias.detach(), norms, weight.detach().t(), out=lin)
         y = torch.empty_like(xs)
         with N.on_device(dev):
             rc = lib.feq_gate_apply(arr, nreps, mult, n, int(cm), N.ptr(xs), N.ptr(lin), N.ptr(y),
@@ -1358,7 +1360,8 @@ class GatingFn(torch.autograd.Function):
             rc = lib.feq_gate_bwd_lin(arr, nreps, mult, n, int(cm), N.ptr(gy), N.ptr(xs),
                                       N.ptr(lin), N.ptr(dlin), N.stream_ptr(dev))
         N.check(rc, "feq_gate_bwd_lin")
-        dnorms = torch.mm(dlin, weight.detach())
+        dnorms = torch.empty_like(norms)
+        torch.mm(dlin, weight.detach(), out=dnorms)
         gw = rows_weight_grad(dlin, norms, weight.dtype) if ctx.needs_input_grad[1] else None
         gb = column_sums(dlin) if ctx.needs_input_grad[2] else None
         gx = torch.empty_like(xs)

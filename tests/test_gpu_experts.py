@@ -1252,3 +1252,24 @@ def test_deterministic_algorithms(dev):
     assert torch.equal(y, mlp(x))
     for a, b in zip(got, want):
         assert torch.allclose(a, b, rtol=1e-5, atol=1e-6 * b.abs().max().item())
+
+
+def test_gating_and_mixture_under_autocast(dev):
+    """The kernels around the gating's products read float32: autocast leaves them so, forward and backward."""
+    torch.manual_seed(16)
+    rp = fe.Repr([0, 1], 24)
+    gating, mlp = fe.EquivariantGating(rp).to(dev), fe.EquivariantExpertMLP(rp, 1, 1).to(dev)
+    x = torch.randn(70, 24, 4, generator=gen(29)).to(dev).requires_grad_()
+    gy = torch.randn(70, 24, 4, generator=gen(30)).to(dev)
+    for module in (gating, mlp):
+        leaves = [x] + [p for k, p in module.named_parameters() if "router" not in k]
+        y = module(x)
+        want = (y, *torch.autograd.grad(y, leaves, gy))
+        for dtype in (torch.bfloat16, torch.float16):
+            with torch.autocast("cuda", dtype=dtype):
+                y = module(x)
+                outside = torch.autograd.grad(y, leaves[:1], gy, retain_graph=True)
+            got = (y, *torch.autograd.grad(y, leaves, gy))
+            assert torch.equal(outside[0], got[1])
+            for a, b in zip(got, want):
+                assert a.dtype == torch.float32 and torch.equal(a, b)
