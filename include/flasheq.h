@@ -769,7 +769,7 @@ int feq_expert_topk_fwd(const void* logits, int64_t rows, int32_t experts, int32
                         int32_t normalize, int64_t* ids, float* weights, float* mean, void* workspace,
                         size_t ws_bytes, feq_stream_t stream);
 /* grad_logits from the gradients of weights and mean (either may be NULL), with the
- * forward's ids and weights. */
+ * forward's ids and weights; the gradient of a weight whose id is -1 is not read. */
 int feq_expert_topk_bwd(const void* logits, const int64_t* ids, const float* weights, const float* grad_weights,
                         const float* grad_mean, int64_t rows, int32_t experts, int32_t dtype, int32_t top_k,
                         int32_t normalize, void* grad_logits, feq_stream_t stream);
@@ -787,7 +787,8 @@ int feq_expert_plan(const int64_t* ids, int64_t slots, int32_t experts, int32_t*
  * dispatch: xs[d, positions[t, k]] = x[d, t]; zeros at places without an expert.
  * combine: y[d, t] = sum_k weights[t, k] ys[d, positions[t, k]] over the slots with an expert;
  * weights (rows, top_k) of weight_dtype, NULL for 1 (the gradient of dispatch).
- * combine_bwd: grad_ys (zeros at places without an expert) and grad_weights (0 there), either NULL. */
+ * combine_bwd: grad_ys (zeros at places without an expert) and grad_weights (0 there), either NULL.
+ * planes <= 65535, width <= 2^29, top_k <= 64, rows top_k < 2^31. */
 int feq_expert_dispatch(const void* x, int64_t planes, int64_t rows, int32_t top_k, int64_t width, int32_t dtype,
                         const int32_t* positions, const int32_t* placed, void* xs, feq_stream_t stream);
 int feq_expert_combine(const void* ys, int64_t planes, int64_t rows, int32_t top_k, int64_t width, int32_t dtype,
@@ -802,7 +803,8 @@ int feq_expert_combine_bwd(const void* grad_y, const void* ys, int64_t planes, i
  * cin), y (dim, slots, cout), weight (experts, nreps, cout, cin), bias (experts, cout, nbias) or NULL,
  * all of dtype; offsets of the plan.  Rows offsets[e] .. offsets[e + 1] of the plane of a component of irrep r
  * are multiplied by weight[e, r]^T; bias column bias_cols[r] (-1: none; each column one scalar irrep's) is added;
- * rows from offsets[experts] on are 0 and enter no gradient.  experts <= 1024, nreps <= 32, dim <= 128. */
+ * rows from offsets[experts] on are 0 and enter no gradient.  experts <= 1024, slots <= 2^30, cin, cout <= 65536, nreps <= 32,
+ * dim <= 128; nbias <= nreps, bias_cols from -1 to nbias - 1. */
 int feq_expert_linear_fwd(const int32_t* lvals, int32_t nreps, int32_t experts, int64_t slots, int32_t cin,
                           int32_t cout, int32_t dtype, const void* x, const void* weight, const int32_t* offsets,
                           const void* bias, int32_t nbias, const int32_t* bias_cols, void* y, feq_stream_t stream);
