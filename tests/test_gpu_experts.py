@@ -1273,3 +1273,16 @@ def test_gating_and_mixture_under_autocast(dev):
             assert torch.equal(outside[0], got[1])
             for a, b in zip(got, want):
                 assert a.dtype == torch.float32 and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("cin,cout,dtype", [(65536, 9, torch.bfloat16), (40, 65536, torch.float32),
+                                            (65535, 130, torch.float32), (136, 65533, torch.bfloat16)])
+def test_linear_of_the_most_channels(dev, cin, cout, dtype):
+    check_linear(dev, (0, 1), [9, 0, 140], 2, cin, cout, dtype, seed=31)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("lead,rows,k,width,experts", [((65535,), 3, 2, 3, 4), ((3, 5), 37, 64, 9, 100), ((), 3, 64, 4099, 64),
+                                                       ((300,), 2, 7, 130, 9)])
+def test_rows_of_the_most_planes_and_choices(dev, lead, rows, k, width, experts, dtype):
+    test_rows_and_their_gradients(dev, lead, rows, k, width, experts, dtype)

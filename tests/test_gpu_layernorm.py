@@ -306,3 +306,9 @@ def test_gradient_of_the_rows_alone(dev, dtype):
         ones = torch.ones(width, device=dev, dtype=dtype, requires_grad=True)
         plain = torch.autograd.grad(ops.layer_norm(x, ones), [x, ones], gy)[0]
         assert torch.equal(torch.autograd.grad(ops.layer_norm(x), [x], gy)[0], plain)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_the_widest_rows(dev, dtype):
+    x, w, b, gy = inputs(dev, 3, 2 ** 24, dtype, 40)
+    check(dev, x, w, b, gy)
