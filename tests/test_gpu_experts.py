@@ -1286,3 +1286,34 @@ def test_linear_of_the_most_channels(dev, cin, cout, dtype):
                                                        ((300,), 2, 7, 130, 9)])
 def test_rows_of_the_most_planes_and_choices(dev, lead, rows, k, width, experts, dtype):
     test_rows_and_their_gradients(dev, lead, rows, k, width, experts, dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_captured_half_precision_step(dev, dtype):
+    """Router and gating in float32 inside, recorded as the rest; replays on new inputs give the eager step's values."""
+    from flash_eq.capture import capture_step
+    torch.manual_seed(17)
+    mlp = fe.EquivariantExpertMLP(fe.Repr([0, 1], 16), 4, 2).to(dev, dtype)
+    x = torch.randn(900, 16, 4, generator=gen(32)).to(dev, dtype).requires_grad_()
+    gy = torch.randn(900, 16, 4, generator=gen(33)).to(dev, dtype)
+    leaves = [x, *mlp.parameters()]
+
+    def loss_of():
+        terms = []
+        return (mlp(x, terms) * gy).float().sum((1, 2)).mean() + terms[0]
+
+    def step():
+        loss = loss_of()
+        loss.backward()
+        return loss
+    graph, _ = capture_step(step, leaves)
+    for k in range(3):
+        with torch.no_grad():
+            x.copy_(torch.randn(900, 16, 4, generator=gen(50 + k)))
+        graph.replay()
+        torch.cuda.synchronize()
+        for leaf, want in zip(leaves, torch.autograd.grad(loss_of(), leaves)):
+            assert torch.isfinite(leaf.grad).all()
+            # one step of the type, and what float32 sums in another order make of it
+            assert torch.allclose(leaf.grad.float(), want.float(), rtol=2 * HALF[dtype], atol=HALF[dtype] * want.abs().max().item())
+        torch.cuda.synchronize()
