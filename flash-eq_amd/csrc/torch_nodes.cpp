@@ -1,5 +1,5 @@
-// PyTorch bindings of the layer norm and the expert routing: argument checks, outputs and
-// workspaces from the caching allocator, autograd nodes, and the calls of the C ABI
+// PyTorch bindings of the layer norm, the expert routing and the fine-tuning operators (dropout, biased edge
+// attention): argument checks, outputs and workspaces from the caching allocator, autograd nodes, and the calls of the C ABI
 // (flasheq.h) on the tensors' device and its current stream.
 //
 // A training call of a small graph is host work: a torch.autograd.Function spends about 20 us forward
@@ -87,6 +87,9 @@ const Tensor& get(const OptTensor& t) {
     return t.has_value() ? *t : none;
 }
 
+Tensor dense_long(const Tensor& t) {
+    return !t.defined() ? t : (t.scalar_type() == at::kLong ? t : t.to(at::kLong)).contiguous();
+}
 Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 template <class T>
@@ -112,16 +115,17 @@ struct On {
 
 // The backward of every node below runs once: under create_graph its results carry an error
 // for a second derivative instead of being constants without one.
-variable_list once(variable_list&& grads) {
+variable_list once(variable_list&& grads, const char* ops) {
     if (!at::GradMode::is_enabled()) return std::move(grads);
     for (auto& g : grads)
         if (g.defined()) g = g.detach().requires_grad_();
     auto error = std::make_shared<torch::autograd::DelayedError>(
-        "the layer norm and the expert routing of flash_eq have no second derivative", static_cast<int64_t>(grads.size()));
+        c10::str(ops, " of flash_eq have no second derivative"), static_cast<int64_t>(grads.size()));
     return (*error)(std::move(grads));
 }
 
 struct OnceNode : torch::autograd::Node {
+    static constexpr const char* kOps = "the layer norm and the expert routing";     // as errors name them
     variable_list apply(variable_list&& grads) final {
         variable_list out;
         {
@@ -129,7 +133,7 @@ struct OnceNode : torch::autograd::Node {
             at::NoGradGuard none;
             out = backward(grads);
         }
-        return once(std::move(out));
+        return once(std::move(out), ops());
     }
     void release_variables() final {
         std::lock_guard<std::mutex> lock(mutex_);
@@ -137,6 +141,7 @@ struct OnceNode : torch::autograd::Node {
     }
     virtual variable_list backward(variable_list& grads) = 0;
     virtual void release() {}
+    virtual const char* ops() const { return kOps; }
     bool need(size_t i) const { return task_should_compute_output(i); }
 };
 
@@ -144,7 +149,7 @@ struct OnceNode : torch::autograd::Node {
 template <class N, class... In>
 std::shared_ptr<N> node_for(const In&... in) {
     TORCH_CHECK_NOT_IMPLEMENTED(!(torch::autograd::isFwGradDefined(in) || ...),
-                                "the layer norm and the expert routing of flash_eq have no forward-mode derivative");
+                                N::kOps, " of flash_eq have no forward-mode derivative");
     if (!at::GradMode::is_enabled() || !(wants_grad(in) || ...)) return nullptr;
     std::shared_ptr<N> node(new N(), torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(in...));
@@ -625,10 +630,324 @@ Tensor expert_linear(const Tensor& x, const Tensor& weight, const OptTensor& bia
     return y;
 }
 
+// ---- dropout -------------------------------------------------------------------------
+
+struct TuneNode : OnceNode {
+    static constexpr const char* kOps = "the dropout, edge attention and adapters";
+    const char* ops() const override { return kOps; }
+};
+
+void check_share(double p) {
+    if (!(p >= 0.0 && p <= 1.0)) value_error("dropout must be between 0 and 1, got ", p);
+}
+
+// The seed of a dropout of `like`: one int64 on its device.
+void check_seed(const Tensor& seed, const Tensor& like) {
+    need_gpu(seed, "seed");
+    if (seed.scalar_type() != at::kLong || seed.numel() != 1)
+        value_error("seed must be one int64 (dropout_seed), got ", dtype_name(seed.scalar_type()), " of shape ", seed.sizes());
+    same_device(like, seed);
+}
+
+struct DropoutCall {
+    std::vector<int32_t> lvals;
+    bool cm = false;
+    double p = 0.0;
+
+    Tensor run(const Tensor& x, const Tensor& seed) const {
+        Tensor y = make(x.sizes(), x, x.scalar_type());
+        int64_t dim = 0;
+        for (const int32_t l : lvals) dim += 2 * l + 1;
+        On on(x);
+        done(feq_dropout(lvals.data(), static_cast<int32_t>(lvals.size()), x.numel() / dim, cm, code_of(x, "x"), ptr(x), p,
+                         ptr_as<int64_t>(seed), ptr(y), on.stream),
+             "feq_dropout");
+        return y;
+    }
+};
+
+struct DropoutNode final : TuneNode {
+    Kept seed;
+    DropoutCall call;
+
+    variable_list backward(variable_list& grads) override {
+        const Tensor s = seed.get();                     // an error when it has been freed
+        if (!grads[0].defined()) return {Tensor()};
+        return {call.run(dense(grads[0]), s)};
+    }
+    void release() override { seed.reset_data(); }
+    std::string name() const override { return "FeqDropoutBackward"; }
+};
+
+// `lvals` none: element by element.
+Tensor feature_dropout(const Tensor& x, double p, const Tensor& seed, const std::optional<std::vector<int64_t>>& lvals, bool cm) {
+    code_of(x, "x");
+    check_share(p);
+    check_seed(seed, x);
+    DropoutCall call{{0}, cm && lvals.has_value(), p};
+    if (lvals) {
+        const Irreps irreps(*lvals);
+        call.lvals = irreps.lvals;
+        if (irreps.n() > FEQ_MAX_IRREPS || irreps.dim > FEQ_MAX_SLOTS)
+            value_error("at most ", FEQ_MAX_IRREPS, " irreps and ", FEQ_MAX_SLOTS, " components, got ", irreps.n(), " and ", irreps.dim);
+        if (x.dim() < 1 || x.size(cm ? 0 : -1) != irreps.dim)
+            value_error("x must be ", cm ? "(" : "(..., ", irreps.dim, cm ? ", ...)" : ")", ", got shape ", x.sizes());
+    }
+    const auto node = node_for<DropoutNode>(x);
+    Tensor y;
+    {
+        at::NoGradGuard none;
+        y = call.run(dense(x), seed);
+        if (node) {
+            node->seed.keep(seed);
+            node->call = call;
+        }
+    }
+    if (node) torch::autograd::set_history(y, node);
+    return y;
+}
+
+// ---- biased edge attention -----------------------------------------------------------
+
+Tensor distance_buckets(const Tensor& dist, const Tensor& bounds) {
+    need_gpu(dist, "distances");
+    need_gpu(bounds, "boundaries");
+    for (const auto& [t, name] : {std::pair<const Tensor&, const char*>{dist, "distances"}, {bounds, "boundaries"}})
+        if (t.scalar_type() != at::kFloat) type_error(name, " must be float32, got ", dtype_name(t.scalar_type()));
+    if (dist.dim() != 1 || bounds.dim() != 1)
+        value_error("distances (edges,) and boundaries (buckets - 1,) expected, got shapes ", dist.sizes(), " and ", bounds.sizes());
+    same_device(dist, bounds);
+    if (bounds.size(0) > INT32_MAX) value_error("more than 2^31 - 1 boundaries");
+    at::NoGradGuard none;
+    const Tensor d = dense(dist), b = dense(bounds);
+    Tensor out = make({d.size(0)}, d, at::kInt);
+    On on(d);
+    done(feq_distance_buckets(ptr_as<float>(d), d.size(0), ptr_as<float>(b), static_cast<int32_t>(b.size(0)), ptr_as<int32_t>(out),
+                              on.stream),
+         "feq_distance_buckets");
+    return out;
+}
+
+// The edges of a graph: indices by destination and source, and their CSRs.
+struct EdgeIndex {
+    Tensor src, dst, perm, offsets, perm_s, offsets_s;
+    int64_t nodes = 0;
+};
+
+struct EdgeAttentionCall {
+    bool node_form, cm;
+    int64_t nodes, heads;
+    double decay, p;
+
+    // The ABI's view of a call on these (contiguous) tensors.
+    feq_edge_attn on(const Tensor& qt, const Tensor& kt, const Tensor& ls, const Tensor& b, const Tensor& d, const Tensor& bk,
+                       const Tensor& sd, const EdgeIndex& g) const {
+        feq_edge_attn a{};
+        a.num_nodes = nodes;
+        a.heads = static_cast<int32_t>(heads);
+        a.dtype = code_of(qt, "q");
+        const int64_t size = qt.element_size();
+        char* base = static_cast<char*>(ptr(qt));
+        a.q = base;
+        if (node_form) {
+            const int64_t mult = qt.size(cm ? 2 : 1) / 2, dim = qt.size(cm ? 0 : 2), n = qt.size(cm ? 1 : 0);
+            a.num_edges = g.src.size(0);
+            a.num_k = n;
+            a.head_len = static_cast<int32_t>(cm ? mult / heads : mult / heads * dim);
+            a.head_runs = static_cast<int32_t>(cm ? dim : 1);
+            a.ldq = a.ldk = cm ? 2 * mult : 2 * mult * dim;
+            a.head_stride = a.head_len;
+            a.run_stride = cm ? n * 2 * mult : 0;
+            a.k = base ? base + size * (cm ? mult : mult * dim) : nullptr;
+            a.q_idx = ptr_as<int64_t>(g.dst);
+            a.k_idx = ptr_as<int64_t>(g.src);
+        } else {
+            a.num_edges = qt.size(0);
+            a.head_len = static_cast<int32_t>(qt.size(2));
+            a.head_runs = 1;
+            a.ldq = a.ldk = heads * qt.size(2);
+            a.head_stride = a.head_len;
+            a.k = ptr(kt);
+        }
+        a.perm = ptr_as<int32_t>(g.perm);
+        a.offsets = ptr_as<int32_t>(g.offsets);
+        a.log_scale = ptr(ls);
+        a.scale_dtype = code_of(ls, "log_scale");
+        a.decay = static_cast<float>(decay);
+        a.dist = ptr_as<float>(d);
+        if (b.defined()) {
+            a.bias = ptr(b);
+            a.bias_dtype = code_of(b, "bias");
+            a.num_buckets = static_cast<int32_t>(b.size(0));
+            a.buckets = ptr(bk);
+            a.wide_buckets = bk.scalar_type() == at::kLong;
+        }
+        a.dropout = p;
+        a.seed = ptr_as<int64_t>(sd);
+        return a;
+    }
+};
+
+struct EdgeAttentionNode final : TuneNode {
+    // inputs: qk (node form) or q, then k (edge form), log_scale, bias, distances
+    Kept q, k, log_scale, bias, dist, buckets, seed, weights;
+    Kept src, dst, perm, offsets, perm_s, offsets_s;
+    EdgeAttentionCall call{};
+    bool own_weights = false;
+    at::ScalarType dist_type = at::kFloat;
+
+    variable_list backward(variable_list& grads) override {
+        variable_list out(5);
+        if (!grads[0].defined()) return out;
+        const Tensor qt = q.get_dense(), kt = k.get_dense(), ls = log_scale.get_dense(), b = bias.get_dense(), d = dist.get_dense(),
+                     bk = buckets.get_dense(), sd = seed.get();
+        const Tensor w = own_weights ? weights.get_dense() : weights.get_dense(shared_from_this());
+        const EdgeIndex ix{src.get_dense(), dst.get_dense(), perm.get_dense(), offsets.get_dense(), perm_s.get_dense(), offsets_s.get_dense(), call.nodes};
+        const Tensor g = dense(grads[0]);
+        const feq_edge_attn a = call.on(qt, kt, ls, b, d, bk, sd, ix);
+        const bool rows = need(0) || need(1) || need(2);
+        Tensor gq, gk, gls, gb, gd;
+        if (rows) gq = make(qt.sizes(), qt, qt.scalar_type());
+        if (rows && !call.node_form) gk = make(kt.sizes(), kt, kt.scalar_type());
+        if (need(2)) gls = make(ls.sizes(), ls, ls.scalar_type());
+        if (need(3)) gb = make(b.sizes(), b, b.scalar_type());
+        if (need(4)) gd = make(d.sizes(), d, at::kFloat);
+        if (a.num_edges == 0) {
+            for (Tensor* t : {&gq, &gk, &gls, &gb, &gd})
+                if (t->defined()) t->zero_();
+        } else {
+            const Tensor gz = make(w.sizes(), w, at::kFloat);
+            const Tensor ws = scratch(feq_edge_attn_bwd_workspace(&a, gb.defined(), gls.defined()), qt);
+            const char* kbase = static_cast<const char*>(static_cast<const void*>(a.k));
+            char* gkp = !rows ? nullptr
+                        : call.node_form ? static_cast<char*>(ptr(gq)) + (kbase - static_cast<const char*>(a.q))
+                                    : static_cast<char*>(ptr(gk));
+            On on(qt);
+            done(feq_edge_attn_bwd(&a, ptr_as<int32_t>(ix.perm_s), ptr_as<int32_t>(ix.offsets_s), ptr_as<float>(w), ptr(g),
+                                   ptr_as<float>(gz), ptr(gq), a.ldq, gkp, a.ldk, ptr(gb), ptr(gls), ptr_as<float>(gd), ptr(ws),
+                                   bytes_of(ws), on.stream),
+                 "feq_edge_attn_bwd");
+        }
+        if (need(0)) out[0] = gq;
+        if (need(1)) out[1] = gk;
+        out[2] = gls;
+        out[3] = gb;
+        if (need(4)) out[4] = gd.to(dist_type);
+        return out;
+    }
+    void release() override {
+        for (Kept* t : {&q, &k, &log_scale, &bias, &dist, &buckets, &seed, &weights, &src, &dst, &perm, &offsets, &perm_s, &offsets_s})
+            t->reset_data();
+    }
+    std::string name() const override { return "FeqEdgeAttentionBackward"; }
+};
+
+// q: (nodes, 2 mult, dim), component-major (dim, nodes, 2 mult), or with k the edges' (edges, heads, head dim).
+Tensor edge_attention(const Tensor& q, const OptTensor& k_, const OptTensor& src_, const OptTensor& dst_, const Tensor& perm,
+                      const Tensor& offsets, const OptTensor& perm_s_, const OptTensor& offsets_s_, int64_t nodes, int64_t edges,
+                      int64_t heads, const Tensor& log_scale, bool cm, const OptTensor& dist_, double decay, const OptTensor& bias_,
+                      const OptTensor& buckets_, double p, const OptTensor& seed_) {
+    const Tensor &k = get(k_), &dist = get(dist_), &b = get(bias_), &buckets = get(buckets_), &seed = get(seed_);
+    const bool node_form = !k.defined();
+    code_of(q, node_form ? "qk" : "Q");
+    if (heads < 1 || heads > 1024) value_error("num_heads must be 1 to 1024, got ", heads);
+    if (node_form) {
+        if (q.dim() != 3 || q.size(cm ? 2 : 1) % 2 || q.size(cm ? 2 : 1) / 2 % heads || q.size(cm ? 2 : 1) == 0 || q.size(cm ? 0 : 2) < 1)
+            value_error("qk must be ", cm ? "(dim, nodes, 2 mult)" : "(nodes, 2 mult, dim)", " with ", heads,
+                        " heads dividing mult, got shape ", q.sizes());
+        if (cm && q.size(0) > FEQ_MAX_SLOTS) value_error("at most ", FEQ_MAX_SLOTS, " components, got ", q.size(0));
+        if (q.size(cm ? 1 : 0) != nodes) value_error("qk has ", q.size(cm ? 1 : 0), " rows but the graph has ", nodes, " nodes");
+    } else {
+        code_of(k, "K");
+        if (q.scalar_type() != k.scalar_type())
+            type_error("Q and K of different dtypes: ", dtype_name(q.scalar_type()), " and ", dtype_name(k.scalar_type()));
+        if (q.dim() != 3 || q.size(0) != edges || q.size(1) != heads || q.size(2) < 1 || q.sizes() != k.sizes())
+            value_error("Q and K must be (", edges, ", ", heads, ", head dim), got shapes ", q.sizes(), " and ", k.sizes());
+        same_device(q, k);
+    }
+    const int64_t head = node_form ? q.numel() / std::max<int64_t>(nodes, 1) / 2 / heads : q.size(2);
+    if (head > 1 << 20) value_error("heads of more than 2^20 elements");
+    code_of(log_scale, "log_scale");
+    if (log_scale.numel() != 1) value_error("log_scale must be one number, got shape ", log_scale.sizes());
+    same_device(q, log_scale);
+    same_device(q, perm);
+    if (!(decay >= 0.0)) value_error("distance decay must not be negative, got ", decay);
+    if (decay > 0.0) {
+        if (!dist.defined()) value_error("distance decay needs distances");
+        code_of(dist, "distances");
+        if (dist.dim() != 1 || dist.size(0) != edges) value_error("distances must be (", edges, ",), got shape ", dist.sizes());
+        same_device(q, dist);
+    }
+    if (b.defined() != buckets.defined()) value_error("bias and buckets come together");
+    if (b.defined()) {
+        code_of(b, "bias");
+        if (b.dim() != 2 || b.size(1) != heads || b.size(0) < 1 || b.size(0) > 4096)
+            value_error("bias must be (1 to 4096 buckets, ", heads, "), got shape ", b.sizes());
+        same_device(q, b);
+        need_gpu(buckets, "buckets");
+        if (buckets.scalar_type() != at::kInt && buckets.scalar_type() != at::kLong)
+            type_error("buckets must be int32 or int64, got ", dtype_name(buckets.scalar_type()));
+        if (buckets.dim() != 1 || buckets.size(0) != edges) value_error("buckets must be (", edges, ",), got shape ", buckets.sizes());
+        same_device(q, buckets);
+    }
+    check_share(p);
+    if (p > 0.0) {
+        if (!seed.defined()) value_error("dropout needs a seed (dropout_seed)");
+        check_seed(seed, q);
+    }
+    const Tensor used_dist = decay > 0.0 ? dist : Tensor();
+    const auto node = node_for<EdgeAttentionNode>(q, k, log_scale, b, used_dist);
+    Tensor out;
+    {
+        at::NoGradGuard none;
+        EdgeIndex ix{dense_long(get(src_)), dense_long(get(dst_)), dense(perm), dense(offsets), get(perm_s_), get(offsets_s_), nodes};
+        if (ix.perm.size(0) != edges || ix.offsets.size(0) != nodes + 1 ||
+            (node_form && (ix.src.size(0) != edges || ix.dst.size(0) != edges || ix.perm_s.size(0) != edges || ix.offsets_s.size(0) != nodes + 1)))
+            value_error("the graph's CSRs do not cover ", edges, " edges and ", nodes, " nodes");
+        const EdgeAttentionCall call{node_form, cm, nodes, heads, decay, p};
+        const Tensor qc = dense(q), kc = k.defined() ? dense(k) : k, ls = dense(log_scale), bc = b.defined() ? dense(b) : b,
+                     bk = b.defined() ? dense(buckets) : Tensor(),
+                     dc = used_dist.defined() ? dense(used_dist.scalar_type() == at::kFloat ? used_dist : used_dist.to(at::kFloat)) : used_dist;
+        const Tensor sd = p > 0.0 ? seed : Tensor();
+        out = make({edges, heads}, q, q.scalar_type());
+        const bool same = q.scalar_type() == at::kFloat && p == 0.0;
+        const Tensor w = same ? out : make({edges, heads}, q, at::kFloat);
+        if (edges) {
+            const feq_edge_attn a = call.on(qc, kc, ls, bc, dc, bk, sd, ix);
+            On on(q);
+            done(feq_edge_attn_fwd(&a, ptr_as<float>(w), same ? nullptr : ptr(out), on.stream), "feq_edge_attn_fwd");
+        }
+        if (node) {
+            node->call = call;
+            node->own_weights = !same;
+            if (used_dist.defined()) node->dist_type = used_dist.scalar_type();
+            node->q.keep(qc);
+            node->k.keep(kc);
+            node->log_scale.keep(ls);
+            node->bias.keep(bc);
+            node->dist.keep(dc);
+            node->buckets.keep(bk);
+            node->seed.keep(sd);
+            node->src.keep(ix.src);
+            node->dst.keep(ix.dst);
+            node->perm.keep(ix.perm);
+            node->offsets.keep(ix.offsets);
+            node->perm_s.keep(ix.perm_s);
+            node->offsets_s.keep(ix.offsets_s);
+            if (!same) node->weights.keep(w);
+        }
+    }
+    if (node) {
+        torch::autograd::set_history(out, node);
+        if (!node->own_weights) node->weights.keep(out, true);
+    }
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(flasheq_torch, m) {
-    m.doc() = "Layer norm and expert routing of flash_eq on PyTorch tensors";
+    m.doc() = "Layer norm, expert routing and fine-tuning operators of flash_eq on PyTorch tensors";
     py::register_exception_translator([](std::exception_ptr p) {
         try {
             if (p) std::rethrow_exception(p);
@@ -645,4 +964,7 @@ PYBIND11_MODULE(flasheq_torch, m) {
     m.def("expert_dispatch", &expert_dispatch, released);
     m.def("expert_combine", &expert_combine, released);
     m.def("expert_linear", &expert_linear, released);
+    m.def("feature_dropout", &feature_dropout, released);
+    m.def("distance_buckets", &distance_buckets, released);
+    m.def("edge_attention", &edge_attention, released);
 }

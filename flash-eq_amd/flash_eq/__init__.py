@@ -10,6 +10,8 @@ from .representations import (Irrep, ProductIrrep, Repr, ProductRepr, WignerD, W
                               random_rotation)
 from .graph import Graph
 from .experts import ExpertPlan, expert_linear, expert_topk
+from .dropout import dropout_seed, feature_dropout
+from .edge_attention import distance_buckets, edge_attention_weights, edge_attention_weights_qk
 from .layers.radial import RadialBasisFunctions, RadialMLP, SeparableRadialNet
 from .layers import (
     EquivariantEdgewiseLinear,
@@ -40,6 +42,7 @@ __all__ = [
     "WignerDBasis",
     "InvariantLayerNorm", "ExpertPlan", "expert_topk", "expert_linear",
     "ExpertRouter", "EquivariantExpertLinear", "EquivariantExpertMLP",
+    "dropout_seed", "feature_dropout", "distance_buckets", "edge_attention_weights", "edge_attention_weights_qk",
     "RadialBasisFunctions", "RadialMLP", "SeparableRadialNet",
     "CUDANotAvailableError",
 ]

@@ -48,6 +48,19 @@ class FeqBinning(ctypes.Structure):
     ]
 
 
+class FeqEdgeAttn(ctypes.Structure):
+    _fields_ = [
+        ("num_edges", ctypes.c_int64), ("num_nodes", ctypes.c_int64), ("num_k", ctypes.c_int64),
+        ("heads", ctypes.c_int32), ("head_len", ctypes.c_int32), ("head_runs", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("ldq", ctypes.c_int64), ("ldk", ctypes.c_int64), ("head_stride", ctypes.c_int64), ("run_stride", ctypes.c_int64),
+        ("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("q_idx", ctypes.c_void_p), ("k_idx", ctypes.c_void_p),
+        ("perm", ctypes.c_void_p), ("offsets", ctypes.c_void_p), ("log_scale", ctypes.c_void_p),
+        ("scale_dtype", ctypes.c_int32), ("decay", ctypes.c_float), ("dist", ctypes.c_void_p), ("bias", ctypes.c_void_p),
+        ("buckets", ctypes.c_void_p), ("bias_dtype", ctypes.c_int32), ("num_buckets", ctypes.c_int32),
+        ("wide_buckets", ctypes.c_int32), ("dropout", ctypes.c_double), ("seed", ctypes.c_void_p),
+    ]
+
+
 _lib: Optional[ctypes.CDLL] = None
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
@@ -207,6 +220,12 @@ _SIGS = {
                               ctypes.c_int),
     "feq_expert_linear_bwd_w": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _P, _P, _P, _I32, _P, _P, _P, _P, _SZ, _P],
                                 ctypes.c_int),
+    # fine-tuning: dropout, biased edge attention (feq_edge_attn by pointer)
+    "feq_dropout": ([_P, _I32, _I64, _I32, _I32, _P, ctypes.c_double, _P, _P, _P], ctypes.c_int),
+    "feq_distance_buckets": ([_P, _I64, _P, _I32, _P, _P], ctypes.c_int),
+    "feq_edge_attn_fwd": ([_P, _P, _P, _P], ctypes.c_int),
+    "feq_edge_attn_bwd_workspace": ([_P, _I32, _I32], _SZ),
+    "feq_edge_attn_bwd": ([_P, _P, _P, _P, _P, _P, _P, _I64, _P, _I64, _P, _P, _P, _P, _SZ, _P], ctypes.c_int),
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGS)

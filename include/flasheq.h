@@ -826,6 +826,64 @@ int feq_expert_linear_bwd(const int32_t* lvals, int32_t nreps, int32_t experts, 
                           const int32_t* offsets, int32_t nbias, const int32_t* bias_cols, void* grad_x,
                           void* grad_weight, void* grad_bias, void* workspace, size_t ws_bytes, feq_stream_t stream);
 
+/* ---- fine-tuning: dropout, biased edge attention, low-rank adapters --------------------------------
+ * No counterpart in the reference (whose attention has a fixed distance decay and PyTorch's dropout).
+ *
+ * Random numbers are Philox 4 x 32 with ten rounds: key = the seed (one int64 on the device), block b with the
+ * counter (b mod 2^32, b / 2^32, 0, 0), its four words eight numbers of 16 bits, the lower half first.  Unit u has
+ * number u mod 8 of block u / 8, is dropped where that is below t = round(65536 p), and is else multiplied by
+ * 65536 / (65536 - t); p = 1 drops all. */
+
+/* Dropout of whole irreps: y = x times the factor of its unit, 0 where that is dropped; the gradient is the same
+ * call on grad_y.  channels = rows x channels of the table; component d of row-channel rc lies at rc dim + d
+ * (component_major 0) or d channels + rc and belongs to unit rc nreps + (irrep of d).  dim <= 128, nreps <= 32. */
+int feq_dropout(const int32_t* lvals, int32_t nreps, int64_t channels, int32_t component_major, int32_t dtype,
+                const void* x, double p, const int64_t* seed, void* y, feq_stream_t stream);
+
+/* buckets[e] = the number of the num_bounds ascending bounds that are at most dist[e] (NaN: 0). */
+int feq_distance_buckets(const float* dist, int64_t num_edges, const float* bounds, int32_t num_bounds,
+                         int32_t* buckets, feq_stream_t stream);
+
+/* The attention weights of edges over their destination, with a bias for each head and bucket and dropout.  Row
+ * r of q starts at r ldq, its head h at h head_stride from there, head_runs runs of head_len elements run_stride apart
+ * (k the same).  Node form: q is read at the edge's destination (q_idx, the index that perm and offsets group by)
+ * and k at k_idx (num_k rows; an index outside reads zeros); edge form (both NULL): both at the edge.
+ *   z[e, h] = exp(log_scale) <q, k> - dist[e] / decay (decay > 0) + bias[buckets[e], h] (an index outside: none),
+ *   weights[e, h] = exp(z - max) / (sum + 1e-8) over the edges of a destination, 0 where z is -inf and for edges
+ *   whose destination lies outside [0, num_nodes);  out = weights times the dropout's factor of unit e heads + h.
+ * heads <= 1024, buckets <= 4096, num_nodes and num_k <= 2^25, num_edges < 2^31. */
+typedef struct feq_edge_attn {
+    int64_t num_edges, num_nodes, num_k;
+    int32_t heads, head_len, head_runs, dtype;
+    int64_t ldq, ldk, head_stride, run_stride;
+    const void* q;
+    const void* k;
+    const int64_t* q_idx;
+    const int64_t* k_idx;
+    const int32_t* perm;       /* CSR of the edges by destination */
+    const int32_t* offsets;
+    const void* log_scale;     /* one element of scale_dtype */
+    int32_t scale_dtype;
+    float decay;
+    const float* dist;
+    const void* bias;          /* (num_buckets, heads) of bias_dtype, or NULL */
+    const void* buckets;       /* of every edge, int32, or int64 where wide_buckets */
+    int32_t bias_dtype, num_buckets, wide_buckets;
+    double dropout;
+    const int64_t* seed;
+} feq_edge_attn;
+/* weights (num_edges, heads) float32, for the backward; out of dtype, NULL where it would be the same (float32
+ * without dropout). */
+int feq_edge_attn_fwd(const feq_edge_attn* a, float* weights, void* out, feq_stream_t stream);
+/* From grad_out (of dtype): grad_logits (num_edges, heads) float32; grad_q and grad_k (both or neither, laid out
+ * as q and k with row strides ldgq, ldgk, every row written; the node form needs the CSR of the edges by k_idx);
+ * grad_bias, grad_log_scale (with grad_q), grad_dist or NULL.  Sums in a fixed order.  num_edges > 0. */
+size_t feq_edge_attn_bwd_workspace(const feq_edge_attn* a, int32_t want_bias, int32_t want_scale);
+int feq_edge_attn_bwd(const feq_edge_attn* a, const int32_t* perm_k, const int32_t* offsets_k, const float* weights,
+                      const void* grad_out, float* grad_logits, void* grad_q, int64_t ldgq, void* grad_k, int64_t ldgk,
+                      void* grad_bias, void* grad_log_scale, float* grad_dist, void* workspace, size_t ws_bytes,
+                      feq_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
