@@ -1,5 +1,5 @@
 // PyTorch bindings of the layer norm, the expert routing and the fine-tuning operators (dropout, biased edge
-// attention): argument checks, outputs and workspaces from the caching allocator, autograd nodes, and the calls of the C ABI
+// attention, adapters): argument checks, outputs and workspaces from the caching allocator, autograd nodes, and the calls of the C ABI
 // (flasheq.h) on the tensors' device and its current stream.
 //
 // A training call of a small graph is host work: a torch.autograd.Function spends about 20 us forward
@@ -944,6 +944,123 @@ Tensor edge_attention(const Tensor& q, const OptTensor& k_, const OptTensor& src
     return out;
 }
 
+// ---- adapters beside a shared map ----------------------------------------------------
+
+struct AdapterLinearNode final : TuneNode {
+    Kept x, weight, down, up, low;
+    Tensor order, offsets;
+    Irreps irreps{{0}};
+    int64_t nbias = 0;
+    float scale = 1.0f;
+
+    variable_list backward(variable_list& grads) override {
+        variable_list out(5);
+        if (!grads[0].defined()) return out;
+        const Tensor xs = x.get_dense(), w = weight.get_dense(), dn = down.get_dense(), u = up.get_dense(), lo = low.get_dense(),
+                     g = dense(grads[0]);
+        check_plan(order, "order", 1);
+        check_plan(offsets, "offsets", 1);
+        const int64_t adapters = dn.size(0), rank = dn.size(2), ci = dn.size(3), co = u.size(2), rows = xs.size(-2);
+        const int32_t *lv = irreps.lvals.data(), n = irreps.n();
+        const bool shared = need(1) || need(4);
+        const int32_t nb = need(4) ? static_cast<int32_t>(nbias) : 0;
+        Tensor gx, gw, gd, gu, gb;
+        if (need(0) || need(2)) gx = make(xs.sizes(), xs, xs.scalar_type());
+        if (shared) gw = make(w.sizes(), w, w.scalar_type());
+        if (need(2)) gd = make(dn.sizes(), dn, dn.scalar_type());
+        if (need(3)) gu = make(u.sizes(), u, u.scalar_type());
+        if (nb) gb = make({co, nbias}, w, w.scalar_type());
+        if (rows == 0) {
+            for (Tensor* t : {&gx, &gw, &gd, &gu, &gb})
+                if (t->defined()) t->zero_();
+        } else {
+            const Tensor ws = scratch(feq_adapter_linear_bwd_workspace(lv, n, adapters, rows, ci, co, rank, shared, nb), xs);
+            On on(xs);
+            done(feq_adapter_linear_bwd(lv, n, adapters, rows, ci, co, rank, code_of(xs, "x"), ptr(g), ptr(xs), ptr(w), ptr(dn), ptr(u),
+                                        scale, ptr_as<int32_t>(order), ptr_as<int32_t>(offsets), ptr_as<float>(lo), nb,
+                                        irreps.cols.data(), ptr(gx), ptr(gd), ptr(gu), ptr(gw), ptr(gb), ptr(ws), bytes_of(ws), on.stream),
+                 "feq_adapter_linear_bwd");
+        }
+        if (need(0)) out[0] = gx;
+        if (need(1)) out[1] = gw;
+        out[2] = gd;
+        out[3] = gu;
+        out[4] = gb;
+        return out;
+    }
+    void release() override {
+        for (Kept* t : {&x, &weight, &down, &up, &low}) t->reset_data();
+        order.reset();
+        offsets.reset();
+    }
+    std::string name() const override { return "FeqAdapterLinearBackward"; }
+};
+
+Tensor adapter_linear(const Tensor& x, const Tensor& weight, const Tensor& down, const Tensor& up, const OptTensor& bias, const Tensor& order,
+                      const Tensor& offsets, int64_t rows, int64_t top_k, const std::vector<int64_t>& lvals, double scale) {
+    const Irreps irreps(lvals);
+    const int code = code_of(x, "x");
+    const Tensor& b = get(bias);
+    for (const auto& [t, name] : {std::pair<const Tensor&, const char*>{weight, "weight"}, {down, "down"}, {up, "up"}, {b, "bias"}}) {
+        if (!t.defined()) continue;
+        code_of(t, name);
+        if (t.scalar_type() != x.scalar_type())
+            type_error("x and ", name, " of different dtypes: ", dtype_name(x.scalar_type()), " and ", dtype_name(t.scalar_type()));
+        same_device(x, t);
+    }
+    check_plan(order, "order", 1);
+    check_plan(offsets, "offsets", 1);
+    same_device(x, offsets);
+    if (top_k != 1) value_error("a row has one adapter: a plan of ids (rows,) or (rows, 1), got top_k ", top_k);
+    const int64_t adapters = offsets.size(0) - 1, n = irreps.n();
+    if (down.dim() != 4 || down.size(0) != adapters || down.size(1) != n || down.size(2) < 1 || down.size(2) > 64 || down.size(3) < 1)
+        value_error("down must be (", adapters, ", ", n, ", rank 1 to 64, cin), got shape ", down.sizes());
+    const int64_t rank = down.size(2), ci = down.size(3);
+    if (up.dim() != 4 || up.size(0) != adapters || up.size(1) != n || up.size(2) < 1 || up.size(3) != rank)
+        value_error("up must be (", adapters, ", ", n, ", cout, ", rank, "), got shape ", up.sizes());
+    const int64_t co = up.size(2);
+    if (!(weight.dim() == 3 && weight.size(0) == n && weight.size(1) == co && weight.size(2) == ci) &&
+        !(weight.dim() == 2 && weight.size(0) == n * co && weight.size(1) == ci))
+        value_error("weight must be (", n, ", ", co, ", ", ci, ") or (", n * co, ", ", ci, "), got shape ", weight.sizes());
+    const bool flat = x.dim() == 2 && n == 1 && irreps.dim == 1;
+    if (!(flat && x.size(0) == rows && x.size(1) == ci) && !(x.dim() == 3 && x.size(0) == irreps.dim && x.size(1) == rows && x.size(2) == ci))
+        value_error("x must be (", irreps.dim, ", ", rows, ", ", ci, "), got shape ", x.sizes());
+    if (b.defined() && (irreps.nscalar == 0 || b.dim() != 2 || b.size(0) != co || b.size(1) != irreps.nscalar))
+        value_error("bias must be (", co, ", ", irreps.nscalar, "), one column per scalar irrep, got shape ", b.sizes());
+    if (!(scale - scale == 0.0)) value_error("scale must be finite, got ", scale);
+    const auto node = node_for<AdapterLinearNode>(x, weight, down, up, b);
+    Tensor y;
+    {
+        at::NoGradGuard none;
+        const Tensor xc = dense(x), wc = dense(weight), dc = dense(down), uc = dense(up), bc = b.defined() ? dense(b) : b;
+        c10::SmallVector<int64_t, 3> shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = co;
+        y = make(shape, x, x.scalar_type());
+        Tensor low;
+        if (rows && (ci > 128 || (node && wants_grad(up))))
+            low = make({static_cast<int64_t>(feq_adapter_linear_low_floats(irreps.lvals.data(), irreps.n(), rows, rank))}, x, at::kFloat);
+        On on(x);
+        done(feq_adapter_linear_fwd(irreps.lvals.data(), irreps.n(), adapters, rows, ci, co, rank, code, ptr(xc), ptr(wc), ptr(dc), ptr(uc),
+                                    static_cast<float>(scale), ptr_as<int32_t>(order), ptr_as<int32_t>(offsets), ptr(bc),
+                                    static_cast<int32_t>(irreps.nscalar), irreps.cols.data(), ptr(y), ptr_as<float>(low), on.stream),
+             "feq_adapter_linear_fwd");
+        if (node) {
+            node->x.keep(xc);
+            node->weight.keep(wc);
+            node->down.keep(dc);
+            node->up.keep(uc);
+            node->low.keep(low);
+            node->order = order;
+            node->offsets = offsets;
+            node->irreps = irreps;
+            node->nbias = irreps.nscalar;
+            node->scale = static_cast<float>(scale);
+        }
+    }
+    if (node) torch::autograd::set_history(y, node);
+    return y;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(flasheq_torch, m) {
@@ -967,4 +1084,5 @@ PYBIND11_MODULE(flasheq_torch, m) {
     m.def("feature_dropout", &feature_dropout, released);
     m.def("distance_buckets", &distance_buckets, released);
     m.def("edge_attention", &edge_attention, released);
+    m.def("adapter_linear", &adapter_linear, released);
 }

@@ -10,6 +10,7 @@ from .representations import (Irrep, ProductIrrep, Repr, ProductRepr, WignerD, W
                               random_rotation)
 from .graph import Graph
 from .experts import ExpertPlan, expert_linear, expert_topk
+from .adapters import adapter_linear
 from .dropout import dropout_seed, feature_dropout
 from .edge_attention import distance_buckets, edge_attention_weights, edge_attention_weights_qk
 from .layers.radial import RadialBasisFunctions, RadialMLP, SeparableRadialNet
@@ -43,6 +44,7 @@ __all__ = [
     "InvariantLayerNorm", "ExpertPlan", "expert_topk", "expert_linear",
     "ExpertRouter", "EquivariantExpertLinear", "EquivariantExpertMLP",
     "dropout_seed", "feature_dropout", "distance_buckets", "edge_attention_weights", "edge_attention_weights_qk",
+    "adapter_linear",
     "RadialBasisFunctions", "RadialMLP", "SeparableRadialNet",
     "CUDANotAvailableError",
 ]

@@ -101,17 +101,19 @@ def node_qk(qk, heads, src, dst, component_major=False):
 
 def adapter_linear(x, weight, down, up, ids, lvals, bias=None, scale=1.0):
     """x (dim, rows, cin), weight (irreps, cout, cin), down (adapters, irreps, rank, cin), up (adapters, irreps, cout, rank)."""
-    rep = irreps(lvals).tolist()
+    rep = irreps(lvals)
     scalars = [r for r, l in enumerate(lvals) if l == 0]
-    rows = []
-    for i, a in enumerate(ids.tolist()):
-        planes = []
-        for d, r in enumerate(rep):
-            y = weight[r] @ x[d, i]
-            if 0 <= a < down.shape[0]:
-                y = y + scale * (up[a, r] @ (down[a, r] @ x[d, i]))
-            if bias is not None and lvals[r] == 0:
-                y = y + bias[:, scalars.index(r)]
-            planes.append(y)
-        rows.append(torch.stack(planes))
-    return torch.stack(rows, 1) if rows else x.new_zeros(len(rep), 0, weight.shape[1])
+    y = torch.stack([x[d] @ weight[r].t() for d, r in enumerate(rep.tolist())])
+    low = torch.zeros_like(y)
+    for a in range(down.shape[0]):
+        at = (ids == a).nonzero()[:, 0]
+        if at.numel():
+            own = torch.stack([(x[d, at] @ down[a, r].t()) @ up[a, r].t() for d, r in enumerate(rep.tolist())])
+            low = low.index_copy(1, at, own)
+    y = y + scale * low
+    if bias is not None:
+        column = torch.zeros(len(rep), weight.shape[1], dtype=y.dtype)
+        for j, r in enumerate(scalars):
+            column = column + (rep == r).to(y.dtype)[:, None] * bias[:, j]
+        y = y + column[:, None]
+    return y
