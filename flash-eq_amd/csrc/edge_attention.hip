@@ -37,6 +37,7 @@ constexpr int kEaBiasThreads = 256;
 struct EaHead {
     int64_t hs, cs;        // from head to head, from run to run
     int len, cpd, vecs;    // vectors of a run, of a head
+    int ragged;            // whether a run's last vector shares elements with the one before
 };
 
 struct EaBias {
@@ -92,43 +93,86 @@ struct EaLane {
     }
 };
 
-// Offsets of the lane's vectors of a slice within a head, and how many of their first elements belong to the vector
+// Offsets of the lane's vectors of a slice within a row, and how many of their first elements belong to the vector
 // before (V: there is no such vector, and the head's first is read in its place).
 template <int V, int NT>
 struct EaVecs {
     int64_t off[NT];
     int shared[NT];
-    __device__ __forceinline__ EaVecs(const EaHead& hd, int j, int G, int slice) {
+    __device__ __forceinline__ EaVecs(const EaHead& hd, int64_t h, int j, int G, int slice) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             const int c = j + G * (t + NT * slice);
             const int run = c / hd.cpd, i = (c - run * hd.cpd) * V;
             const bool there = c < hd.vecs;
             const int last = hd.len - V;
-            off[t] = there ? run * hd.cs + (i < last ? i : last) : 0;
+            off[t] = h * hd.hs + (there ? run * hd.cs + (i < last ? i : last) : 0);
             shared[t] = there ? (i > last ? i - last : 0) : V;
         }
     }
 };
 
+// A row that all lanes read, by buffer loads: the base is a scalar, the lane's offsets are 32 bits, and what lies outside (a
+// lane's absent vectors, all of an absent row) is 0 without a memory access or a select.
+typedef __amdgpu_buffer_rsrc_t EaTable;
+constexpr uint32_t kEaInside = 0x7ffffff0u, kEaOutside = 0x80000000u;
+
+// A row's vectors, in the table's type until they are used (16-bit rows in flight take half the registers).
 template <class T, int V, int NT>
-__device__ __forceinline__ void ea_load(const T* __restrict__ row, const EaVecs<V, NT>& v, float (&o)[NT][V]) {
+struct EaRow {
+    typedef typename VecOf<T, V>::type vec;
+    vec v[NT];
+    __device__ __forceinline__ void load(const T* __restrict__ row, const EaVecs<V, NT>& vecs) {
 #pragma unroll
-    for (int t = 0; t < NT; ++t) load_f<T, V>(row + v.off[t], o[t]);
-}
+        for (int t = 0; t < NT; ++t) v[t] = *reinterpret_cast<const typename VecOf<T, V>::any*>(row + vecs.off[t]);
+    }
+    __device__ __forceinline__ void load_uniform(const T* row, bool there, const uint32_t (&at)[NT]) {
+        const EaTable r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row), 0, there ? kEaInside : 0u, 0x00020000);
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            if constexpr (sizeof(vec) == 16) v[t] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b128(r, at[t], 0, 0));
+            else if constexpr (sizeof(vec) == 8) v[t] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b64(r, at[t], 0, 0));
+            else if constexpr (sizeof(vec) == 4) v[t] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b32(r, at[t], 0, 0));
+            else v[t] = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b16(r, at[t], 0, 0));
+        }
+    }
+    __device__ __forceinline__ float get(int t, int u) const {
+        if constexpr (V == 1) return static_cast<float>(v[t]);
+        else return static_cast<float>(v[t][u]);
+    }
+};
 
 // The part of a dot product that the lane's vectors make.
-template <int V, int NT>
-__device__ __forceinline__ float ea_dot(const float (&a)[NT][V], const float (&b)[NT][V], const EaVecs<V, NT>& v) {
+template <bool UNI, class T, int V, int NT>
+__device__ __forceinline__ float ea_dot(const float (&a)[NT][V], const EaRow<T, V, NT>& b, const EaVecs<V, NT>& v, int ragged) {
     float sum = 0.0f;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         float d = 0.0f;
+        if (!UNI && ragged) {                    // uniform
 #pragma unroll
-        for (int u = 0; u < V; ++u) d += u < v.shared[t] ? 0.0f : a[t][u] * b[t][u];
-        sum += d;
+            for (int u = 0; u < V; ++u) d += u < v.shared[t] ? 0.0f : a[t][u] * b.get(t, u);
+        } else {
+#pragma unroll
+            for (int u = 0; u < V; ++u) d += a[t][u] * b.get(t, u);
+        }
+        sum += UNI || v.shared[t] < V ? d : 0.0f;
     }
     return sum;
+}
+template <class T, int V, int NT>
+__device__ __forceinline__ void ea_floats(const EaRow<T, V, NT>& r, float (&o)[NT][V]) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int u = 0; u < V; ++u) o[t][u] = r.get(t, u);
+}
+
+// The lane's offsets in bytes for load_uniform.
+template <class T, int V, int NT>
+__device__ __forceinline__ void ea_bytes(const EaVecs<V, NT>& v, uint32_t (&at)[NT]) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) at[t] = v.shared[t] < V ? static_cast<uint32_t>(v.off[t]) * static_cast<uint32_t>(sizeof(T)) : kEaOutside;
 }
 
 template <int V, int NT>
@@ -142,15 +186,58 @@ __device__ __forceinline__ bool ea_segment(const int32_t* __restrict__ offsets, 
     return true;
 }
 
-// w (float32; out where that is NULL is the result itself) holds the logits between the two passes.
-template <class T, int V, int NT, bool NODE>
+// The sums of N values over their lane groups of g lanes (uniform), as group_sum.
+template <int N>
+__device__ __forceinline__ void group_sums(float (&v)[N], int g) {
+    auto step = [&](auto move) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += move(v[i]);
+    };
+    auto dpp = [](float x, auto c) { return __uint_as_float(dpp_u<decltype(c)::value>(__float_as_uint(x))); };
+    if (g > 1) step([&](float x) { return dpp(x, std::integral_constant<int, 0xB1>{}); });
+    if (g > 2) step([&](float x) { return dpp(x, std::integral_constant<int, 0x4E>{}); });
+    if (g > 4) step([&](float x) { return dpp(x, std::integral_constant<int, 0x141>{}); });
+    if (g > 8) step([&](float x) { return dpp(x, std::integral_constant<int, 0x140>{}); });
+    if (g > 16)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = group_sum16(v[i]);
+    if (g > 32)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = group_sum32(v[i]);
+}
+
+// The edges of 64 places of a segment, one a lane: number, row (-1: outside the table) and bucket (-1: none).
+template <class T>
+struct EaEdges {
+    int e, row, bucket;
+    template <bool NODE, bool BUCKETS>
+    __device__ __forceinline__ void load(const EaArgs<T>& a, int b, int cnt, int s0) {
+        const int at = s0 + static_cast<int>(threadIdx.x & 63);
+        const bool there = at < cnt;
+        e = a.perm[b + (there ? at : 0)];
+        row = e;
+        bucket = -1;
+        if constexpr (NODE) {
+            const int64_t r = a.kidx[e];
+            row = r >= 0 && r < a.nk ? static_cast<int>(r) : -1;
+        }
+        if (!there) row = -1;
+        if (BUCKETS && a.bias.table) bucket = bucket_of(a.bias, e);
+    }
+    __device__ __forceinline__ int edge(int i) const { return __shfl(e, i, 64); }
+};
+
+// w (float32; out where that is NULL is the result itself) holds the logits between the two passes of a segment of more than
+// 64 edges, LDS those of a shorter one.
+template <class T, int V, int NT, bool NODE, bool UNI>
 __global__ void __launch_bounds__(64 * kEaWaves)
 k_ea_fwd(EaArgs<T> a, float* __restrict__ w, T* __restrict__ out) {
+    __shared__ float kept_z[kEaWaves][64 * kEaMaxHeadLanes];
     int64_t n;
     int b, cnt;
     if (!ea_segment(a.offsets, a.N, a.E, n, b, cnt)) return;
-    const int H = a.H, L = 1 << a.lgL, G = 1 << a.lgG, lgE = a.lgL - a.lgG;
-    const EaLane me(H, a.lgL, a.lgG);
+    const int H = a.H, lgL = a.lgL, L = 1 << lgL, G = 1 << a.lgG, lgE = lgL - a.lgG, lane = threadIdx.x & 63;
+    const EaLane me(H, lgL, a.lgG);
     const int64_t h = me.hv ? me.h : 0;
     if (n == a.N) {                              // destinations outside the graph
         for (int i = me.pos; i < cnt; i += L) {
@@ -161,70 +248,117 @@ k_ea_fwd(EaArgs<T> a, float* __restrict__ w, T* __restrict__ out) {
         }
         return;
     }
+    if (cnt == 0) return;
+    float* const zs = kept_z[threadIdx.x >> 6];
     const float scale = expf(load_any(a.log_scale, a.scale_dtype, 0));
     constexpr int UE = kEaRows<V, NT>;
+    const int sub = UNI ? 0 : (lane & (L - 1)) >> a.lgG, per = UE << lgE;      // subgroup; places of a step
+    const int lg_per = lgE + (UE == 4 ? 2 : 1);
+    const bool one = UNI || a.slices == 1;
     float q[NT][V];
+    const EaVecs<V, NT> first(a.head, h, me.j, G, 0);
+    uint32_t bytes[NT];
+    if constexpr (UNI) ea_bytes<T>(first, bytes);
+    auto load_row = [&](EaRow<T, V, NT>& k, const T* table, int64_t ld, int64_t r, const EaVecs<V, NT>& vecs) {
+        if constexpr (UNI) k.load_uniform(table + (r < 0 ? 0 : r) * ld, r >= 0, bytes);
+        else k.load(table + (r < 0 ? 0 : r) * ld, vecs);
+    };
+    auto queries = [&](const EaVecs<V, NT>& vecs) {
+        EaRow<T, V, NT> own;
+        load_row(own, a.q, a.ldq, n, vecs);
+        ea_floats(own, q);
+    };
     float top = -INFINITY, sum = 0.0f;
-    for (int c0 = 0; c0 < cnt; c0 += L) {
-        const int at = c0 + me.pos;
-        const bool there = at < cnt;
-        const int64_t e = there ? a.perm[b + at] : 0;
-        int row = -1;
-        float bias = 0.0f;
-        if (there) {
-            if constexpr (NODE) {
-                const int64_t r = a.kidx[e];
-                row = r >= 0 && r < a.nk ? static_cast<int>(r) : -1;
-            } else {
-                row = static_cast<int>(e);
-            }
-            if (a.bias.table) {
-                const int j = bucket_of(a.bias, e);
-                if (j >= 0) bias = load_any(a.bias.table, a.bias.dtype, static_cast<int64_t>(j) * H + h);
-            }
+    EaEdges<T> ed;
+    for (int s0 = 0; s0 < cnt; s0 += 64) {
+        ed.template load<NODE, true>(a, b, cnt, s0);
+        const int left = cnt - s0 < 64 ? cnt - s0 : 64, steps = (left + per - 1) >> lg_per;
+        float z = 0.0f, bias = 0.0f;
+        bool there = false;
+        int64_t e = 0;
+        auto begin = [&](int c0) {               // the lane's edge of the chunk at place c0
+            there = c0 + me.pos < left;
+            e = ed.edge((c0 + me.pos) & 63);
+            const int j = __shfl(ed.bucket, (c0 + me.pos) & 63, 64);
+            bias = j >= 0 ? load_any(a.bias.table, a.bias.dtype, static_cast<int64_t>(j) * H + h) : 0.0f;
             if (a.decay > 0.0f) bias -= a.dist[e] / a.decay;
-        }
-        float z = 0.0f;
-        for (int sl = 0; sl < a.slices; ++sl) {
-            const EaVecs<V, NT> vecs(a.head, me.j, G, sl);
-            if (NODE && (a.slices > 1 || c0 == 0)) ea_load<T, V, NT>(a.q + n * a.ldq + h * a.head.hs, vecs, q);
-            for (int u0 = 0; u0 < G && c0 + (u0 << lgE) < cnt; u0 += UE) {
-                float k[UE][NT][V];
+            z = 0.0f;
+        };
+        auto finish = [&](int c0) {
+            const int row = __shfl(ed.row, (c0 + me.pos) & 63, 64);
+            z = row < 0 ? 0.0f : z * scale;      // an edge from outside the graph: a row of zeros
+            z = !there || bias == -INFINITY ? -INFINITY : z + bias;
+            if (cnt <= 64) zs[(c0 >> lgL) * 64 + lane] = z;
+            else if (there && me.hv) w[e * H + h] = z;
+            const float most = group_max(fmaxf(z, top), L);
+            const float base = most == -INFINITY ? 0.0f : most;
+            sum = sum * expf(top - base) + group_sum(expf(z - base), L);
+            top = most;
+        };
+        auto row_at = [&](int i) {               // of the edge at place i of the 64
+            return UNI ? __builtin_amdgcn_readlane(ed.row, i & 63) : __shfl(ed.row, i & 63, 64);
+        };
+        auto rows_of = [&](const EaVecs<V, NT>& vecs, int t, EaRow<T, V, NT> (&k)[UE]) {
 #pragma unroll
-                for (int u = 0; u < UE; ++u) {
-                    const int r = __shfl(row, me.base | (u0 + u), 64);
-                    ea_load<T, V, NT>(a.k + static_cast<int64_t>(r < 0 ? 0 : r) * a.ldk + h * a.head.hs, vecs, k[u]);
+            for (int u = 0; u < UE; ++u) load_row(k[u], a.k, a.ldk, row_at(t * per + (u << lgE) + sub), vecs);
+        };
+        auto dots = [&](const EaVecs<V, NT>& vecs, int t, const EaRow<T, V, NT> (&k)[UE]) {
+            float d[UE];
+#pragma unroll
+            for (int u = 0; u < UE; ++u) {
+                if constexpr (!NODE) {
+                    EaRow<T, V, NT> own;
+                    load_row(own, a.q, a.ldq, row_at(t * per + (u << lgE) + sub), vecs);
+                    ea_floats(own, q);
                 }
+                d[u] = ea_dot<UNI>(q, k[u], vecs, a.head.ragged);
+            }
+            group_sums<UE>(d, G);
+            const int u0 = t * UE & (G - 1);
 #pragma unroll
-                for (int u = 0; u < UE; ++u) {
-                    if constexpr (!NODE) {
-                        const int r = __shfl(row, me.base | (u0 + u), 64);
-                        ea_load<T, V, NT>(a.q + static_cast<int64_t>(r < 0 ? 0 : r) * a.ldq + h * a.head.hs, vecs, q);
+            for (int u = 0; u < UE; ++u)
+                if (me.j == u0 + u) z += d[u];
+        };
+        const int su = G >> (UE == 4 ? 2 : 1);   // steps of a chunk
+        if (one) {
+            if (NODE && s0 == 0) queries(first);
+            for (int t = 0; t < steps; ++t) {
+                EaRow<T, V, NT> k[UE];
+                rows_of(first, t, k);
+                if ((t & (su - 1)) == 0) begin(t * per);
+                dots(first, t, k);
+                if (((t + 1) & (su - 1)) == 0 || t + 1 == steps) finish((t * per) & ~(L - 1));
+            }
+        } else {
+            for (int t0 = 0; t0 < steps; t0 += su) {
+                begin(t0 * per);
+                for (int sl = 0; sl < a.slices; ++sl) {
+                    const EaVecs<V, NT> vecs(a.head, h, me.j, G, sl);
+                    if (NODE) queries(vecs);
+                    for (int t = t0; t < steps && t < t0 + su; ++t) {
+                        EaRow<T, V, NT> k[UE];
+                        rows_of(vecs, t, k);
+                        dots(vecs, t, k);
                     }
-                    const float d = group_sum(ea_dot<V, NT>(q, k[u], vecs), G);
-                    if (me.j == u0 + u) z += d;
                 }
+                finish(t0 * per);
             }
         }
-        z = row < 0 ? 0.0f : z * scale;          // an edge from outside the graph: a row of zeros
-        z = !there || bias == -INFINITY ? -INFINITY : z + bias;
-        if (there && me.hv) w[e * H + h] = z;
-        const float most = group_max(fmaxf(z, top), L);
-        const float base = most == -INFINITY ? 0.0f : most;
-        sum = sum * expf(top - base) + group_sum(expf(z - base), L);
-        top = most;
     }
     const float base = top == -INFINITY ? 0.0f : top;
     const float inv = 1.0f / (sum + 1e-8f);
     const uint64_t key = a.drop.limit ? static_cast<uint64_t>(*a.drop.seed) : 0;
-    if (!me.hv) return;
-    for (int i = me.pos; i < cnt; i += L) {      // by the lane that stored them
-        const int64_t at = static_cast<int64_t>(a.perm[b + i]) * H + h;
-        const float v = expf(w[at] - base) * inv;
-        w[at] = v;
-        if (out) {
-            const bool keep = !a.drop.limit || kept(key, at, a.drop.limit);
-            out[at] = static_cast<T>(a.drop.limit ? (keep ? v * a.drop.scale : 0.0f) : v);
+    for (int s0 = 0; s0 < cnt; s0 += 64) {
+        if (cnt > 64) ed.e = a.perm[b + (s0 + lane < cnt ? s0 + lane : 0)];
+        for (int c0 = 0; c0 < 64 && s0 + c0 < cnt; c0 += L) {        // by the lane that stored them
+            const int64_t at = static_cast<int64_t>(ed.edge((c0 + me.pos) & 63)) * H + h;
+            if (s0 + c0 + me.pos >= cnt || !me.hv) continue;
+            const float v = expf((cnt <= 64 ? zs[(c0 >> lgL) * 64 + lane] : w[at]) - base) * inv;
+            w[at] = v;
+            if (out) {
+                const bool keep = !a.drop.limit || kept(key, at, a.drop.limit);
+                out[at] = static_cast<T>(a.drop.limit ? (keep ? v * a.drop.scale : 0.0f) : v);
+            }
         }
     }
 }
@@ -239,14 +373,14 @@ __device__ __forceinline__ float ea_grad(const T* __restrict__ g, int64_t at, co
 // Rows of a segment summed with grad_z: out[n] = scale sum of grad_z[e] rows[.].  DST: by destination, grad_z is formed from w and
 // the gradient and written, rows are K's; else by source, it is read, rows are Q's.  ROWS false: grad_z alone (edge form).
 // dots (DST): the wave's share of sum over n of <Q[n], grad_Q[n]>, one for every node and group of heads.
-template <class T, int V, int NT, bool DST, bool ROWS>
+template <class T, int V, int NT, bool DST, bool ROWS, bool UNI>
 __global__ void __launch_bounds__(64 * kEaWaves)
 k_ea_bwd(EaArgs<T> a, const float* __restrict__ w, const T* __restrict__ g, float* __restrict__ gz, T* __restrict__ out,
          int64_t ldo, float* __restrict__ dots) {
     int64_t n;
     int b, cnt;
     if (!ea_segment(a.offsets, a.N, a.E, n, b, cnt)) return;
-    const int H = a.H, L = 1 << a.lgL, G = 1 << a.lgG, lgE = a.lgL - a.lgG;
+    const int H = a.H, L = 1 << a.lgL, G = 1 << a.lgG, lgE = a.lgL - a.lgG, lane = threadIdx.x & 63;
     const EaLane me(H, a.lgL, a.lgG);
     const int64_t h = me.hv ? me.h : 0;
     if (n == a.N) {
@@ -259,59 +393,90 @@ k_ea_bwd(EaArgs<T> a, const float* __restrict__ w, const T* __restrict__ g, floa
     const float scale = ROWS ? expf(load_any(a.log_scale, a.scale_dtype, 0)) : 0.0f;
     // an edge of weight 0 passes no gradient, whatever the gradient of its weight holds
     float total = 0.0f;
+    EaEdges<T> ed;
     if constexpr (DST) {
-        for (int i = me.pos; i < cnt; i += L) {
-            const int64_t at = static_cast<int64_t>(a.perm[b + i]) * H + h;
-            const float v = me.hv ? w[at] : 0.0f;
-            if (v != 0.0f) total += v * ea_grad(g, at, a.drop, key);
+        for (int s0 = 0; s0 < cnt; s0 += 64) {
+            ed.template load<ROWS, false>(a, b, cnt, s0);
+            const int left = cnt - s0 < 64 ? cnt - s0 : 64;
+#pragma unroll 4
+            for (int c0 = 0; c0 < left; c0 += L) {
+                const int64_t at = static_cast<int64_t>(ed.edge((c0 + me.pos) & 63)) * H + h;
+                const float v = c0 + me.pos < left && me.hv ? w[at] : 0.0f;
+                if (v != 0.0f) total += v * ea_grad(g, at, a.drop, key);
+            }
         }
         total = group_sum(total, L);
     }
     constexpr int UE = kEaRows<V, NT>;
+    const int per = UE << lgE, lg_per = lgE + (UE == 4 ? 2 : 1), su = G >> (UE == 4 ? 2 : 1), sub = UNI ? 0 : (lane & (L - 1)) >> a.lgG;
     float dot = 0.0f;
-    for (int sl = 0; sl < (ROWS ? a.slices : 1); ++sl) {
-        const EaVecs<V, NT> vecs(a.head, me.j, G, sl);
+    for (int sl = 0; sl < (ROWS && !UNI ? a.slices : 1); ++sl) {
+        const EaVecs<V, NT> vecs(a.head, h, me.j, G, sl);
+        uint32_t bytes[NT];
+        if constexpr (UNI) ea_bytes<T>(vecs, bytes);
         float acc[NT][V];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int u = 0; u < V; ++u) acc[t][u] = 0.0f;
-        for (int c0 = 0; c0 < cnt; c0 += L) {
-            const int at = c0 + me.pos;
-            const bool there = at < cnt && me.hv;
-            const int64_t e = at < cnt ? a.perm[b + at] : 0;
+        for (int s0 = 0; s0 < cnt; s0 += 64) {
+            if (cnt > 64 || (sl == 0 && !DST)) ed.template load<ROWS, false>(a, b, cnt, s0);
+            const int left = cnt - s0 < 64 ? cnt - s0 : 64, steps = (left + per - 1) >> lg_per;
             float c = 0.0f;
-            if (there) {
-                if constexpr (DST) {
-                    const float v = w[e * H + h];
-                    if (v != 0.0f) c = v * (ea_grad(g, e * H + h, a.drop, key) - total);
-                    if (sl == 0) gz[e * H + h] = c;
-                } else {
-                    c = gz[e * H + h];
+            auto begin = [&](int c0) {           // the lane's edge of the chunk at place c0
+                const int at = c0 + me.pos;
+                const int64_t e = ed.edge(at & 63);
+                c = 0.0f;
+                if (at < left && me.hv) {
+                    if constexpr (DST) {
+                        const float v = w[e * H + h];
+                        if (v != 0.0f) c = v * (ea_grad(g, e * H + h, a.drop, key) - total);
+                        if (sl == 0) gz[e * H + h] = c;
+                    } else {
+                        c = gz[e * H + h];
+                    }
                 }
-            }
+                c = __shfl(ed.row, at & 63, 64) < 0 ? 0.0f : c * scale;
+            };
             if constexpr (ROWS) {
-                int row = -1;
-                if (at < cnt) {
-                    const int64_t r = a.kidx[e];
-                    row = r >= 0 && r < a.nk ? static_cast<int>(r) : -1;
-                }
-                c = row < 0 ? 0.0f : c * scale;
-                for (int u0 = 0; u0 < G && c0 + (u0 << lgE) < cnt; u0 += UE) {
-                    float k[UE][NT][V], cu[UE];
+                auto rows_of = [&](int t, EaRow<T, V, NT> (&k)[UE]) {
 #pragma unroll
                     for (int u = 0; u < UE; ++u) {
-                        const int r = __shfl(row, me.base | (u0 + u), 64);
-                        cu[u] = __shfl(c, me.base | (u0 + u), 64);
-                        ea_load<T, V, NT>(a.k + static_cast<int64_t>(r < 0 ? 0 : r) * a.ldk + h * a.head.hs, vecs, k[u]);
+                        const int i = (t * per + (u << lgE) + sub) & 63;
+                        const int r = UNI ? __builtin_amdgcn_readlane(ed.row, i) : __shfl(ed.row, i, 64);
+                        const T* at = a.k + static_cast<int64_t>(r < 0 ? 0 : r) * a.ldk;
+                        if constexpr (UNI) k[u].load_uniform(at, r >= 0, bytes);
+                        else k[u].load(at, vecs);
                     }
+                };
+                auto add = [&](int t, const EaRow<T, V, NT> (&k)[UE]) {
+                    const int u0 = t * UE & (G - 1);
+                    float cu[UE];
 #pragma unroll
-                    for (int u = 0; u < UE; ++u)
+                    for (int u = 0; u < UE; ++u) cu[u] = __shfl(c, me.base | (u0 + u), 64);
 #pragma unroll
-                        for (int t = 0; t < NT; ++t)
+                    for (int u = 0; u < UE; ++u) {
+                        if (__any(cu[u] == 0.0f)) {      // 0 times what an absent or forbidden edge's row holds may be NaN
 #pragma unroll
-                            for (int v = 0; v < V; ++v) acc[t][v] += cu[u] == 0.0f ? 0.0f : cu[u] * k[u][t][v];
+                            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                                for (int v = 0; v < V; ++v) acc[i][v] += cu[u] == 0.0f ? 0.0f : cu[u] * k[u].get(i, v);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < NT; ++i)
+#pragma unroll
+                                for (int v = 0; v < V; ++v) acc[i][v] += cu[u] * k[u].get(i, v);
+                        }
+                    }
+                };
+                for (int t = 0; t < steps; ++t) {
+                    EaRow<T, V, NT> k[UE];
+                    rows_of(t, k);
+                    if ((t & (su - 1)) == 0) begin(t * per);
+                    add(t, k);
                 }
+            } else {
+                for (int c0 = 0; c0 < left; c0 += L) begin(c0);
             }
         }
         if constexpr (ROWS) {
@@ -321,18 +486,20 @@ k_ea_bwd(EaArgs<T> a, const float* __restrict__ w, const T* __restrict__ g, floa
                 for (int v = 0; v < V; ++v)
                     for (int o = G; o < L; o <<= 1) acc[t][v] += __shfl_xor(acc[t][v], o, 64);
             if (me.hv && (me.pos & ((1 << lgE) - 1)) == 0) {      // the first subgroup
-                T* o = out + n * ldo + h * a.head.hs;
+                T* o = out + n * ldo;
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
                     if (vecs.shared[t] < V) store_f<T, V>(o + vecs.off[t], acc[t]);
                 if (DST && dots) {
+                    EaRow<T, V, NT> own;
+                    own.load(a.q + n * a.ldq, vecs);
                     float q[NT][V];
-                    ea_load<T, V, NT>(a.q + n * a.ldq + h * a.head.hs, vecs, q);
+                    ea_floats(own, q);
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
 #pragma unroll
-                        for (int v = 0; v < V; ++v) q[t][v] = acc[t][v] == 0.0f ? 0.0f : q[t][v];
-                    dot += ea_dot<V, NT>(q, acc, vecs);
+                        for (int v = 0; v < V; ++v)
+                            if (v >= vecs.shared[t] && acc[t][v] != 0.0f) dot += q[t][v] * acc[t][v];
                 }
             }
         }
@@ -356,20 +523,20 @@ k_ea_edge_rows(EaArgs<T> a, const float* __restrict__ gz, T* __restrict__ gq, in
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t eh = i / a.head.vecs, e = eh / a.H;
         const int c = static_cast<int>(i % a.head.vecs), h = static_cast<int>(eh % a.H);
-        const EaVecs<V, 1> vec(a.head, c, 1, 0);
-        const int64_t at = h * a.head.hs + vec.off[0];
+        const EaVecs<V, 1> vec(a.head, h, c, 1, 0);
         const float s = gz[eh] * scale;
-        float q[1][V], k[1][V], o[V], p[V];
-        load_f<T, V>(a.q + e * a.ldq + at, q[0]);
-        load_f<T, V>(a.k + e * a.ldk + at, k[0]);
+        EaRow<T, V, 1> q, k;
+        q.load(a.q + e * a.ldq, vec);
+        k.load(a.k + e * a.ldk, vec);
+        float o[V], p[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            o[v] = s == 0.0f ? 0.0f : s * k[0][v];
-            p[v] = s == 0.0f ? 0.0f : s * q[0][v];
+            o[v] = s == 0.0f ? 0.0f : s * k.get(0, v);
+            p[v] = s == 0.0f ? 0.0f : s * q.get(0, v);
+            if (v >= vec.shared[0] && s != 0.0f) dot += q.get(0, v) * o[v];
         }
-        store_f<T, V>(gq + e * ldgq + at, o);
-        store_f<T, V>(gk + e * ldgk + at, p);
-        if (s != 0.0f) dot += s * ea_dot<V, 1>(q, k, vec);
+        store_f<T, V>(gq + e * ldgq + vec.off[0], o);
+        store_f<T, V>(gk + e * ldgk + vec.off[0], p);
     }
     if (!dots) return;
     dot = group_sum(dot, 64);
@@ -378,23 +545,12 @@ k_ea_edge_rows(EaArgs<T> a, const float* __restrict__ gz, T* __restrict__ gq, in
     if (threadIdx.x == 0) dots[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
 }
 
-// out[0] = the sum of n floats, in float64 and a fixed order.
-__global__ void __launch_bounds__(1024) k_ea_total(const float* __restrict__ in, int64_t n, void* out, int dtype) {
-    __shared__ double part[1024];
-    double sum = 0.0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) sum += static_cast<double>(in[i]);
-    part[threadIdx.x] = sum;
-    __syncthreads();
-    for (int o = 512; o > 0; o >>= 1) {
-        if (threadIdx.x < static_cast<unsigned>(o)) part[threadIdx.x] += part[threadIdx.x + o];
-        __syncthreads();
-    }
-    if (threadIdx.x == 0) store_any(out, dtype, 0, static_cast<float>(part[0]));
-}
-
-// grad_b over an equal share of the edges a workgroup.  Every slot (a lane for each of `hp` heads) adds its edges to a
-// table of its own in LDS, one edge after another, so that no two lanes meet and the order is fixed; the tables are
-// then summed in order.  Slots beyond the `tables` that fit take no edges.  blockIdx.y: heads from hn blockIdx.y on.
+// grad_b over an equal share of the edges a workgroup.  Every slot (a lane for each of 2^lgP heads) adds its edges to a
+// table of its own in LDS, one edge after another: no two lanes meet in it, so the order is fixed although the additions
+// are LDS's own (which a lane need not wait for: read, add and write took 50 us where these take XX, 640000 edges of 8
+// heads and 100 buckets).  The tables are then summed in order.  Slots beyond the `tables` that fit take no edges.
+// blockIdx.y: heads from hn blockIdx.y on.
+template <bool WIDE>
 __global__ void __launch_bounds__(kEaBiasThreads)
 k_ea_bias(const float* __restrict__ gz, EaBias bias, int64_t E, int H, int hn, int lgP, int tables, float* __restrict__ part) {
     extern __shared__ __align__(16) float tab[];
@@ -402,39 +558,68 @@ k_ea_bias(const float* __restrict__ gz, EaBias bias, int64_t E, int H, int hn, i
     for (int i = threadIdx.x; i < tables * size; i += kEaBiasThreads) tab[i] = 0.0f;
     __syncthreads();
     const int slot = threadIdx.x >> lgP, hl = threadIdx.x & ((1 << lgP) - 1);
-    const int64_t share = (E + gridDim.x - 1) / gridDim.x;
-    const int64_t e0 = blockIdx.x * share, e1 = e0 + share < E ? e0 + share : E;
-    if (slot < tables) {
-        float* mine = tab + slot * size;
-#pragma unroll 4
-        for (int64_t e = e0 + slot; e < e1; e += tables) {
-            const int j = bucket_of(bias, e);
-            for (int h = hl; h < heads; h += 1 << lgP) {
-                const float v = gz[e * H + h0 + h];
-                if (j >= 0) mine[j * heads + h] += v;
+    const int share = static_cast<int>((E + gridDim.x - 1) / gridDim.x);      // 8 `tables` at least
+    const int64_t e0 = static_cast<int64_t>(blockIdx.x) * share;
+    const int count = static_cast<int>(e0 + share < E ? share : E > e0 ? E - e0 : 0);
+    if (slot < tables && count > 0) {
+        const float* mine = gz + e0 * H + h0;
+        for (int h = hl; h < heads; h += 1 << lgP) {
+            constexpr int AT = 8;                // edges whose loads are on their way together
+            for (int e = slot; e < count; e += AT * tables) {
+                int64_t j[AT];
+                float v[AT];
+#pragma unroll
+                for (int i = 0; i < AT; ++i) {
+                    const int at = e + i * tables < count ? e + i * tables : e;
+                    if constexpr (WIDE) j[i] = static_cast<const int64_t*>(bias.bucket)[e0 + at];
+                    else j[i] = static_cast<const int32_t*>(bias.bucket)[e0 + at];
+                    v[i] = mine[static_cast<int64_t>(at) * H + h];
+                }
+#pragma unroll
+                for (int i = 0; i < AT; ++i)
+                    if (j[i] >= 0 && j[i] < bias.count && e + i * tables < count)
+                        unsafeAtomicAdd(&tab[slot * size + static_cast<int>(j[i]) * heads + h], v[i]);
             }
         }
     }
     __syncthreads();
     for (int i = threadIdx.x; i < size; i += kEaBiasThreads) {
         float s = 0.0f;
+#pragma unroll 8
         for (int t = 0; t < tables; ++t) s += tab[t * size + i];
         const int j = i / heads, h = i % heads;
         part[(static_cast<int64_t>(blockIdx.x) * bias.count + j) * H + h0 + h] = s;
     }
 }
 
-// grad_b = the workgroups' partials summed in order: a wave for each 64 of its elements.
-__global__ void __launch_bounds__(256) k_ea_bias_sum(const float* __restrict__ part, int groups, int n, void* out, int dtype) {
-    __shared__ double sums[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = blockIdx.x * 64 + lane;
+// The last sums, in float64 and a fixed order.  grad_b = the workgroups' partials (groups, n): a workgroup for each 64
+// of its elements; grad_log_scale = the sum of ndots shares: the last workgroup.
+__global__ void __launch_bounds__(1024)
+k_ea_finish(const float* __restrict__ part, int groups, int n, void* gb, int bias_dtype, const float* __restrict__ dots, int64_t ndots,
+            void* gls, int scale_dtype) {
+    __shared__ double sums[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const bool last = gls && blockIdx.x == gridDim.x - 1;
+    const int i = blockIdx.x * 64 + lane;
     double s = 0.0;
-    if (i < n)
-#pragma unroll 8
-        for (int g = wave; g < groups; g += 4) s += static_cast<double>(part[static_cast<int64_t>(g) * n + i]);
+    if (last) {
+#pragma unroll 4
+        for (int64_t k = threadIdx.x; k < ndots; k += 1024) s += static_cast<double>(dots[k]);
+    } else if (i < n) {
+#pragma unroll 4
+        for (int g = wave; g < groups; g += 16) s += static_cast<double>(part[static_cast<int64_t>(g) * n + i]);
+    }
     sums[wave][lane] = s;
     __syncthreads();
-    if (wave == 0 && i < n) store_any(out, dtype, i, static_cast<float>(sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane]));
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < 16; ++w) s += sums[w][lane];
+    if (last) {
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_down(s, o, 64);
+        if (lane == 0) store_any(gls, scale_dtype, 0, static_cast<float>(s));
+    } else if (i < n) {
+        store_any(gb, bias_dtype, i, static_cast<float>(s));
+    }
 }
 
 // grad_r[e] = -sum over the heads of grad_z / decay.
@@ -466,6 +651,7 @@ k_buckets(const float* __restrict__ r, int64_t E, const float* __restrict__ boun
 
 struct EaShape {
     int V, NT, lgL, lgG, slices, groups;     // groups of heads
+    bool uni;                                // a wave reads one row at a time, in one slice of whole, aligned vectors within 31 bits
     EaHead head;
 };
 
@@ -486,6 +672,7 @@ EaShape ea_shape(const feq_edge_attn& a, int size) {
     s.head.len = a.head_len;
     s.head.cpd = static_cast<int>(ceil_div(a.head_len, s.V));
     s.head.vecs = s.head.cpd * a.head_runs;
+    s.head.ragged = a.head_len % s.V != 0;
     const int nt = s.V == 8 ? 2 : 4;
     int nh = std::min(1 << lg(a.heads), kEaMaxHeadLanes);
     while (nh > 1 && 64 / nh * nt < s.head.vecs) nh >>= 1;
@@ -496,6 +683,11 @@ EaShape ea_shape(const feq_edge_attn& a, int size) {
     s.slices = static_cast<int>(ceil_div(per, nt));
     s.NT = static_cast<int>(ceil_div(per, s.slices));
     s.groups = static_cast<int>(ceil_div(a.heads, nh));
+    const int64_t span = (a.heads - 1) * a.head_stride + (a.head_runs - 1) * a.run_stride + a.head_len;
+    const int64_t vec = s.V * size;          // buffer loads from multiples of a vector
+    bool whole = aligned_to(a.q, vec) && aligned_to(a.k, vec);
+    for (const int64_t stride : {a.ldq, a.ldk, a.head_stride, a.run_stride}) whole = whole && stride % s.V == 0;
+    s.uni = s.lgL == s.lgG && s.slices == 1 && !s.head.ragged && whole && span < (int64_t{1} << 31) / size - s.V;
     return s;
 }
 
@@ -630,13 +822,14 @@ extern "C" int feq_edge_attn_fwd(const feq_edge_attn* a, float* weights, void* o
             if constexpr (V * sizeof(T) > 16) {
                 return fail(FEQ_ERR_INVALID, "vectors of %d bytes", V * (int)sizeof(T));
             } else {
-                auto go = [&](auto node) -> int {
-                    auto kern = k_ea_fwd<T, V, NT, decltype(node)::value>;
+                auto go = [&](auto node, auto uni) -> int {
+                    auto kern = k_ea_fwd<T, V, NT, decltype(node)::value, decltype(uni)::value>;
                     FEQ_LAUNCH("k_ea_fwd", kern, ea_grid(a->num_nodes, s.groups), dim3(64 * kEaWaves), 0, stream_of(stream), args,
                                weights, static_cast<T*>(out));
                     return FEQ_OK;
                 };
-                return a->k_idx ? go(std::true_type{}) : go(std::false_type{});
+                if (s.uni) return a->k_idx ? go(std::true_type{}, std::true_type{}) : go(std::false_type{}, std::true_type{});
+                return a->k_idx ? go(std::true_type{}, std::false_type{}) : go(std::false_type{}, std::false_type{});
             }
         });
     });
@@ -682,7 +875,7 @@ extern "C" int feq_edge_attn_bwd(const feq_edge_attn* a, const int32_t* perm_k, 
             } else {
                 const dim3 grid = ea_grid(a->num_nodes, s.groups), block(64 * kEaWaves);
                 if (!gq || !a->k_idx) {
-                    auto kern = k_ea_bwd<T, V, NT, true, false>;
+                    auto kern = k_ea_bwd<T, V, NT, true, false, false>;
                     FEQ_LAUNCH("k_ea_bwd_z", kern, grid, block, 0, st, args, weights, g, grad_logits, static_cast<T*>(nullptr),
                                int64_t{0}, static_cast<float*>(nullptr));
                     if (!gq) return FEQ_OK;
@@ -690,19 +883,22 @@ extern "C" int feq_edge_attn_bwd(const feq_edge_attn* a, const int32_t* perm_k, 
                     FEQ_LAUNCH("k_ea_edge_rows", rows, dim3(kEaEdgeBlocks), dim3(256), 0, st, args, grad_logits, gq, ldgq, gk, ldgk, dots);
                     return FEQ_OK;
                 }
-                auto dst = k_ea_bwd<T, V, NT, true, true>;
-                FEQ_LAUNCH("k_ea_bwd_dst", dst, grid, block, 0, st, args, weights, g, grad_logits, gq, ldgq, dots);
-                args.perm = perm_k;
-                args.offsets = offsets_k;
-                args.k = args.q;
-                args.ldk = args.ldq;
-                args.kidx = a->q_idx;
-                args.nk = a->num_nodes;
-                args.N = a->num_k;
-                auto src = k_ea_bwd<T, V, NT, false, true>;
-                FEQ_LAUNCH("k_ea_bwd_src", src, ea_grid(a->num_k, s.groups), block, 0, st, args, static_cast<const float*>(nullptr),
-                           static_cast<const T*>(nullptr), grad_logits, gk, ldgk, static_cast<float*>(nullptr));
-                return FEQ_OK;
+                auto go = [&](auto uni) -> int {
+                    auto dst = k_ea_bwd<T, V, NT, true, true, decltype(uni)::value>;
+                    FEQ_LAUNCH("k_ea_bwd_dst", dst, grid, block, 0, st, args, weights, g, grad_logits, gq, ldgq, dots);
+                    args.perm = perm_k;
+                    args.offsets = offsets_k;
+                    args.k = args.q;
+                    args.ldk = args.ldq;
+                    args.kidx = a->q_idx;
+                    args.nk = a->num_nodes;
+                    args.N = a->num_k;
+                    auto src = k_ea_bwd<T, V, NT, false, true, decltype(uni)::value>;
+                    FEQ_LAUNCH("k_ea_bwd_src", src, ea_grid(a->num_k, s.groups), block, 0, st, args, static_cast<const float*>(nullptr),
+                               static_cast<const T*>(nullptr), grad_logits, gk, ldgk, static_cast<float*>(nullptr));
+                    return FEQ_OK;
+                };
+                return s.uni ? go(std::true_type{}) : go(std::false_type{});
             }
         });
     });
@@ -710,16 +906,21 @@ extern "C" int feq_edge_attn_bwd(const feq_edge_attn* a, const int32_t* perm_k, 
     if (grad_bias) {
         const EaBiasPlan p = ea_bias_plan(a->num_edges, a->heads, a->num_buckets);
         const EaBias b{a->bias, a->buckets, a->bias_dtype, a->num_buckets, a->wide_buckets};
-        const int n = a->num_buckets * a->heads;
-        auto kern = k_ea_bias;
-        FEQ_LAUNCH("k_ea_bias", kern, dim3(p.blocks, p.parts), dim3(kEaBiasThreads), static_cast<size_t>(p.tables) * a->num_buckets * p.hn * 4,
-                   st, grad_logits, b, a->num_edges, a->heads, p.hn, p.lgP, p.tables, part);
-        auto sum = k_ea_bias_sum;
-        FEQ_LAUNCH("k_ea_bias_sum", sum, dim3(ceil_div(n, 64)), dim3(256), 0, st, part, p.blocks, n, grad_bias, a->bias_dtype);
+        auto go = [&](auto wide) -> int {
+            auto kern = k_ea_bias<decltype(wide)::value>;
+            FEQ_LAUNCH("k_ea_bias", kern, dim3(p.blocks, p.parts), dim3(kEaBiasThreads),
+                       static_cast<size_t>(p.tables) * a->num_buckets * p.hn * 4, st, grad_logits, b, a->num_edges, a->heads, p.hn, p.lgP,
+                       p.tables, part);
+            return FEQ_OK;
+        };
+        if (int err = b.wide ? go(std::true_type{}) : go(std::false_type{})) return err;
     }
-    if (grad_log_scale) {
-        auto kern = k_ea_total;
-        FEQ_LAUNCH("k_ea_total", kern, dim3(1), dim3(1024), 0, st, dots, ndots, grad_log_scale, a->scale_dtype);
+    if (grad_bias || grad_log_scale) {
+        const int n = grad_bias ? a->num_buckets * a->heads : 0;
+        const int groups = grad_bias ? ea_bias_plan(a->num_edges, a->heads, a->num_buckets).blocks : 0;
+        auto kern = k_ea_finish;
+        FEQ_LAUNCH("k_ea_finish", kern, dim3(ceil_div(n, 64) + (grad_log_scale ? 1 : 0)), dim3(1024), 0, st, part, groups, n, grad_bias,
+                   a->bias_dtype, dots, ndots, grad_log_scale, a->scale_dtype);
     }
     if (grad_dist) {
         auto kern = k_ea_dist;
