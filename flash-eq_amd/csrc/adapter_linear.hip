@@ -17,106 +17,22 @@
 // 0 to 3 the rounded values, 4 to 7 what is left), with up's elements twice: 2^-16 (bfloat16) or 2^-21 of the value is lost,
 // where one number would lose 2^-8 or 2^-11 of a sum that the result rounds only once.  float16's narrow range: every row is
 // multiplied by a power of two that brings its largest reduced value to 2^13 .. 2^14, and so is its accumulator meanwhile.
-#include "expert_tiles.h"
+#include "adapter_tiles.h"
 
 namespace feq {
 namespace {
 
-constexpr int kAdMaxRank = 64;
-
-struct AdArgs {
-    const void *in, *W, *F, *G, *bias;
-    const int32_t *offsets, *order;
-    void* out;
-    float* low;                  // NULL: not kept
-    int X, S, K, N, R, nreps, nbias, dim;
-    int rt;                      // rank tiles of 16
-    float scale;
-};
-
-// The vector of elements k .. of the row at `row`, of which n exist (n <= 0: none); `safe`: any 16 bytes of the table.
-template <class T, int HOW>
-__device__ __forceinline__ uint4 load_row(const T* row, int k, int n, const T* safe) {
-    constexpr int V = 16 / sizeof(T);
-    if constexpr (HOW == kWhole) {
-        return *reinterpret_cast<const uint4*>(n > 0 ? row + k : safe);
-    } else if constexpr (HOW == kRagged) {
-        const T* p = n < V ? row + k - (V - n) : row + k;
-        const typename VecOf<T, V>::type v = *reinterpret_cast<const typename VecOf<T, V>::any*>(n > 0 ? p : safe);
-        return __builtin_bit_cast(uint4, v);
-    } else {
-        typename VecOf<T, V>::type v;
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const T e = n > j ? row[k + j] : *safe;
-            v[j] = n > j ? e : static_cast<T>(0.0f);
-        }
-        return __builtin_bit_cast(uint4, v);
-    }
-}
-// What load_row returned with its elements in place and zeros for those that do not exist.
-template <class T, int HOW>
-__device__ __forceinline__ uint4 placed_row(uint4 v, int n, int length, const T* safe) {
-    if constexpr (HOW == kWhole) return n > 0 ? v : uint4{0, 0, 0, 0};
-    else return arrived16<T, HOW>(rows_at(safe, safe, length), v, n);
-}
-
-// Largest of a row's values over the lanes (c, 0 .. 3).
-__device__ __forceinline__ float row_max(float v) {
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-
-// The second product's operand of four reduced values.
-__device__ __forceinline__ v4f low_frag(v4f t, float) { return t; }
-__device__ __forceinline__ b8 low_frag(v4f t, __bf16) {
-    b8 f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        f[j] = static_cast<__bf16>(t[j]);
-        f[j + 4] = static_cast<__bf16>(t[j] - static_cast<float>(f[j]));
-    }
-    return f;
-}
-__device__ __forceinline__ h8 low_frag(v4f t, _Float16) {
-    h8 f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        f[j] = static_cast<_Float16>(t[j]);
-        f[j + 4] = static_cast<_Float16>(t[j] - static_cast<float>(f[j]));
-    }
-    return f;
-}
-// G's operand: four elements of a row, in 16-bit types twice.
-template <class T>
-__device__ __forceinline__ typename Mma<T>::frag twice(const T (&e)[4]) {
-    typename Mma<T>::frag f;
-#pragma unroll
-    for (int j = 0; j < Mma<T>::FE; ++j) f[j] = e[j & 3];
-    return f;
-}
-
-// The power of two that a row of reduced values is multiplied by (float16), its exponent; 0 for a row of zeros, or one
-// that is not finite.
-__device__ __forceinline__ int low_exponent(float most) {
-    const int e = static_cast<int>(__float_as_uint(most) >> 23 & 255u);
-    return e == 0 || e == 255 ? 0 : 127 + 13 - e;
-}
-__device__ __forceinline__ float times_power(float v, int e) { return __builtin_amdgcn_ldexpf(v, e); }
-
 // A reduction of at most 128 columns: the shared map and the maps of one adapter stay in LDS, the rows stream (see
 // k_xl_stream, whose division of the work this is).
-template <class T, int HOW, bool TRANS, int NB, int NS>
-__global__ void __launch_bounds__(kXlThreads)
+template <class T, int HOW, bool TRANS, int NB, int NS, int RT>
+__global__ void __launch_bounds__(kXlThreads, NB * NS * Mma<T>::KS * sizeof(T) > 40000 || RT > 1 ? 2 : 3)
 k_ad_stream(AdArgs a, XlMap map) {
     using M = Mma<T>;
     typedef typename M::frag frag;
     constexpr int V = 16 / sizeof(T), KM = NS * M::KS;
     constexpr int NT = NB / 16, NA = NT < 4 ? NT : 4;
     constexpr int LD = KM + V, LDT = NB + M::PAD;
-    const int rp = 16 * a.rt, K = a.K, N = a.N, X = a.X, S = a.S, R = a.R, nreps = a.nreps;
+    const int rt = RT == 1 ? 1 : a.rt, rp = 16 * rt, K = a.K, N = a.N, X = a.X, S = a.S, R = a.R, nreps = a.nreps;
     const int LDF = TRANS ? rp + M::PAD : LD, LDG = TRANS ? LDT : rp + 4;
     extern __shared__ __align__(16) char smem[];
     T* sW = reinterpret_cast<T*>(smem);
@@ -212,7 +128,7 @@ k_ad_stream(AdArgs a, XlMap map) {
             const int after = number(blk + 8);
             load(next, b1);
             asm volatile("" ::: "memory");           // the maps are read from LDS for every block (k_xl_stream)
-            v4f acc[NT], low[kAdMaxRank / 16];
+            v4f acc[NT], low[RT];
 #pragma unroll
             for (int i = 0; i < NT; ++i)
                 acc[i] = *reinterpret_cast<const v4f*>(sBias + 16 * (i - i % kDealt<T>) + V * g + 4 * (i % kDealt<T>));
@@ -232,8 +148,8 @@ k_ad_stream(AdArgs a, XlMap map) {
             if (own) {
                 float most = 0.0f;
 #pragma unroll
-                for (int q = 0; q < kAdMaxRank / 16; ++q) {
-                    if (q >= a.rt) break;
+                for (int q = 0; q < RT; ++q) {
+                    if (q >= rt) break;
                     low[q] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int ks = 0; ks < NS; ++ks) {
@@ -258,8 +174,8 @@ k_ad_stream(AdArgs a, XlMap map) {
                         for (int j = 0; j < 4; ++j) acc[i][j] = times_power(acc[i][j], power);
                 }
 #pragma unroll
-                for (int q = 0; q < kAdMaxRank / 16; ++q) {
-                    if (q >= a.rt) break;
+                for (int q = 0; q < RT; ++q) {
+                    if (q >= rt) break;
                     v4f v = low[q];
                     if constexpr (std::is_same<T, _Float16>::value)
 #pragma unroll
@@ -518,15 +434,7 @@ k_ad_mm(AdArgs a, XlMap map) {
                 // the column that row 16 i + c of the dealt tile is
                 const int m = 16 * i + c, p = m & 31;
                 const int n = n0 + 64 * wr + (kDealt<T> == 1 ? m : (m - p) + 8 * (p >> 2 & 3) + 4 * (p >> 4) + (p & 3));
-                T el[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = 16 * q + 4 * g + j;
-                    const bool has = n < N && r < R;
-                    const T v = ge[has ? (TRANS ? static_cast<int64_t>(r) * N + n : static_cast<int64_t>(n) * R + r) : 0];
-                    el[j] = has ? v : static_cast<T>(0.0f);
-                }
-                f[i] = twice<T>(el);
+                f[i] = second_frag<T, TRANS>(ge, n, 16 * q + 4 * g, N, R);
             }
 #pragma unroll
             for (int j = 0; j < PT; ++j) {
@@ -571,6 +479,137 @@ k_ad_mm(AdArgs a, XlMap map) {
             const int n = nw + 16 * i;
             store_tiles<T, HOW, PT>(o + n, N - n, &acc[i][j]);
         }
+    }
+}
+
+// The same product for few rows, whose 128-row blocks would leave the chip idle: a wave takes 16 rows and 32 columns, all
+// operands straight from memory in the matrix cores' layout, the reduction in steps of four loads each.
+template <class T, int HOW, bool TRANS>
+__global__ void __launch_bounds__(64)
+k_ad_few(AdArgs a, XlMap map) {
+    using M = Mma<T>;
+    typedef typename M::frag frag;
+    constexpr int V = 16 / sizeof(T), CT = 2, NU = 4;            // column tiles; reduction steps on their way together
+    const int d = blockIdx.z, K = a.K, N = a.N, X = a.X, S = a.S, R = a.R;
+    const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
+    const int row0 = blockIdx.y * 16, n0 = blockIdx.x * 16 * CT, rows = S - row0 < 16 ? S - row0 : 16;
+    const int rep = __builtin_amdgcn_readfirstlane(map.rep[d]);
+    const T *in = static_cast<const T*>(a.in), *we = static_cast<const T*>(a.W) + static_cast<int64_t>(rep) * K * N;
+    const int mine = a.order[row0 + (c < rows ? c : 0)];
+    const T* row = in + (static_cast<int64_t>(d) * S + mine) * K;
+    // the column that row c of tile i is: as stored, 16 bytes of a row of the result are a lane's
+    int col[CT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i) col[i] = n0 + (kDealt<T> == 1 ? 16 * i + c : 8 * (c >> 2) + 4 * i + (c & 3));
+    const int bc = __builtin_amdgcn_readfirstlane(map.bcol[d]);
+    const bool biased = !TRANS && a.bias && bc >= 0;
+    const Table be = table(a.bias, biased);
+    v4f acc[CT];
+#pragma unroll
+    for (int i = 0; i < CT; ++i)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const int n = n0 + V * g + 16 * (i - i % kDealt<T>) + 4 * (i % kDealt<T>) + m;
+            acc[i][m] = load1<T>(be, (n * a.nbias + bc) * sizeof(T), n < N);
+        }
+    const int steps = (K + M::KS - 1) / M::KS;
+    for (int s0 = 0; s0 < steps; s0 += NU) {
+        uint4 vb[NU];
+        frag fw[NU][CT];
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int k = (s0 + u) * M::KS + M::FE * g;
+            vb[u] = load_row<T, HOW>(row, k, K - k, in);
+#pragma unroll
+            for (int i = 0; i < CT; ++i) {
+                if constexpr (!TRANS) {
+                    const int n = col[i] < N ? K - k : 0;
+                    fw[u][i] = __builtin_bit_cast(frag, placed_row<T, HOW>(load_row<T, HOW>(we + static_cast<int64_t>(col[i] < N ? col[i] : 0) * K, k, n, we), n, K, we));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < M::FE; ++j) {
+                        const bool has = col[i] < N && k + j < K;
+                        const T v = we[has ? static_cast<int64_t>(k + j) * N + col[i] : 0];
+                        fw[u][i][j] = has ? v : static_cast<T>(0.0f);
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+            const int k = (s0 + u) * M::KS + M::FE * g;
+            const frag b = __builtin_bit_cast(frag, placed_row<T, HOW>(vb[u], K - k, K, in));
+#pragma unroll
+            for (int i = 0; i < CT; ++i) acc[i] = M::mul(fw[u][i], b, acc[i]);
+        }
+    }
+    const int placed = a.offsets[X];
+    int power = 0;
+    const float* lo = a.low + (static_cast<int64_t>(d) * S + row0 + c) * 16 * a.rt + 4 * g;
+    const bool own = c < rows && row0 + c < placed;
+    if constexpr (std::is_same<T, _Float16>::value) {
+        float most = 0.0f;
+        if (own)
+            for (int q = 0; q < a.rt; ++q)
+#pragma unroll
+                for (int m = 0; m < 4; ++m) most = fmaxf(most, fabsf(lo[16 * q + m]));
+        power = low_exponent(row_max(most));
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) acc[i][m] = times_power(acc[i][m], power);
+    }
+    // the row's adapter: the last whose rows begin at or before it
+    int lo_e = 0, hi_e = X;
+    while (hi_e - lo_e > 1) {
+        const int mid = (lo_e + hi_e) >> 1;
+        if (a.offsets[mid] <= row0 + (c < rows ? c : 0)) lo_e = mid;
+        else hi_e = mid;
+    }
+    const int adapter = own ? lo_e : -1;
+    for (int q = 0; q < a.rt; ++q) {
+        v4f v = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        if (own) v = *reinterpret_cast<const v4f*>(lo + 16 * q);
+        if constexpr (std::is_same<T, _Float16>::value)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) v[m] = times_power(v[m], power);
+        const frag b = low_frag(v, T{});
+        // the adapters of the rows, four at a time; a row takes the sums of its own
+        for (int p0 = 0; p0 < rows; p0 += 4) {
+            frag f[4][CT];
+            int e[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                e[u] = p0 + u < rows ? __builtin_amdgcn_readlane(adapter, p0 + u) : -1;
+                const int before = p0 + u > 0 ? __builtin_amdgcn_readlane(adapter, (p0 + u - 1) & 15) : -1;
+                if (e[u] == before) e[u] = -1;                   // uniform: rows of an adapter are neighbours
+                const T* ge = static_cast<const T*>(a.G) + (static_cast<int64_t>(e[u] < 0 ? 0 : e[u]) * a.nreps + rep) * R * N;
+#pragma unroll
+                for (int i = 0; i < CT; ++i) f[u][i] = second_frag<T, TRANS>(ge, e[u] < 0 ? N : col[i], 16 * q + 4 * g, N, R);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (e[u] < 0) continue;
+#pragma unroll
+                for (int i = 0; i < CT; ++i) {
+                    const v4f sum = M::mul(f[u][i], b, v4f{0.0f, 0.0f, 0.0f, 0.0f});
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) acc[i][m] += adapter == e[u] ? sum[m] : 0.0f;
+                }
+            }
+        }
+    }
+    if constexpr (std::is_same<T, _Float16>::value)
+#pragma unroll
+        for (int i = 0; i < CT; ++i)
+#pragma unroll
+            for (int m = 0; m < 4; ++m) acc[i][m] = times_power(acc[i][m], -power);
+    if (c >= rows) return;
+    T* o = static_cast<T*>(a.out) + (static_cast<int64_t>(d) * S + mine) * N;
+#pragma unroll
+    for (int i = 0; i < CT; i += kDealt<T>) {
+        const int n = n0 + 16 * i + V * g;
+        store_tiles<T, HOW, 1>(o + n, N - n, &acc[i]);
     }
 }
 
@@ -687,14 +726,6 @@ __global__ void k_ad_all(int32_t* offsets, int S) {
     if (threadIdx.x < 2) offsets[threadIdx.x] = threadIdx.x ? S : 0;
 }
 
-struct AdShape {
-    const int32_t* lvals;
-    int32_t nreps;
-    int32_t X;
-    int64_t S;
-    int32_t ci, co, R, dtype;
-};
-
 int ad_check(const AdShape& p, const int32_t* bias_cols, int32_t nbias, float scale, XlMap* map) {
     if (p.R < 1) return fail(FEQ_ERR_INVALID, "adapters of rank %d", p.R);
     if (p.R > kAdMaxRank) return fail(FEQ_ERR_UNSUPPORTED, "adapters of a rank above %d", kAdMaxRank);
@@ -723,6 +754,12 @@ int ad_run(const AdShape& p, const XlMap& map, AdArgs a, std::initializer_list<c
             if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
             auto low = k_ad_low<T, HOW, TRANS>;
             FEQ_LAUNCH(TRANS ? "k_ad_low_t" : "k_ad_low", low, dim3(blocks, dim), dim3(kXlThreads), 0, s, a, map);
+            // blocks of 128 rows for fewer than half of the CUs: 9 us against 80 for 64 bfloat16 rows, 512 to 1024 columns
+            if (ceil_div(p.S, kXlBM) * ceil_div(N, 128) * dim < 128) {
+                auto few = k_ad_few<T, HOW, TRANS>;
+                FEQ_LAUNCH(TRANS ? "k_ad_few_t" : "k_ad_few", few, dim3(ceil_div(N, 32), ceil_div(p.S, 16), dim), dim3(64), 0, s, a, map);
+                return FEQ_OK;
+            }
             auto tile = [&](auto wr) -> int {
                 constexpr int WR = decltype(wr)::value;
                 const int64_t tiles = xcd_grid(ceil_div(p.S, kXlBM), ceil_div(N, 64 * WR));
@@ -735,20 +772,24 @@ int ad_run(const AdShape& p, const XlMap& map, AdArgs a, std::initializer_list<c
             if constexpr (HOW == kNarrow) return FEQ_ERR_INVALID;              // N is narrow
             else return tile(std::integral_constant<int, 2>{});
         }
-        auto stream = [&](auto nn, auto ns) -> int {
+        auto stream_rt = [&](auto nn, auto ns, auto rts) -> int {
             constexpr int NB = decltype(nn)::value, NS = decltype(ns)::value;
             using M = Mma<T>;
             constexpr int V = 16 / sizeof(T), KM = NS * M::KS, LD = KM + V, LDT = NB + M::PAD;
             const int rp = 16 * a.rt;
             const size_t lds = sizeof(T) * ((TRANS ? KM * LDT : NB * LD) + (TRANS ? KM * (rp + M::PAD) : rp * LD) +
                                             (TRANS ? rp * LDT : NB * (rp + 4))) + sizeof(float) * NB;
-            auto kern = k_ad_stream<T, HOW, TRANS, NB, NS>;
+            auto kern = k_ad_stream<T, HOW, TRANS, NB, NS, decltype(rts)::value>;
             const int fit = static_cast<int>(std::min<size_t>(163840 / lds, 4));
             const int64_t blocks = std::min<int64_t>(256 * fit, tile_bound(p.S, p.X, 16) * dim * ceil_div(N, NB));
             if (lds > 65536)
                 FEQ_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
             FEQ_LAUNCH(TRANS ? "k_ad_stream_t" : "k_ad_stream", kern, dim3(blocks), dim3(kXlThreads), lds, s, a, map);
             return FEQ_OK;
+        };
+        auto stream = [&](auto nn, auto ns) -> int {
+            if (a.rt == 1) return stream_rt(nn, ns, std::integral_constant<int, 1>{});
+            return stream_rt(nn, ns, std::integral_constant<int, kAdMaxRank / 16>{});
         };
         constexpr int H = 64 / Mma<T>::KS;
         auto with_ns = [&](auto nn) -> int {
@@ -810,10 +851,15 @@ struct AdScratch {
 // Of a backward: the reduced gradient rows, the partial sums, the shared map's.
 size_t ad_scratch(const AdShape& p, int dim, bool shared, int nbias, void* base, AdScratch* out) {
     Carver c(base);
-    out->low = c.take<float>(static_cast<size_t>(dim) * p.S * 16 * ad_tiles(p.R));
     XlChunks ch;
-    out->parts_down = c.take<float>(static_cast<size_t>(wgrad_chunks(p.S, p.X, p.lvals, p.nreps, p.ci, p.R, &ch)) * p.ci * p.R);
-    out->parts_up = c.take<float>(static_cast<size_t>(wgrad_chunks(p.S, p.X, p.lvals, p.nreps, p.co, p.R, &ch)) * p.co * p.R);
+    if (adapter_fused(p.ci, p.co, p.R)) {
+        out->low = out->parts_up = nullptr;
+        out->parts_down = c.take<float>(static_cast<size_t>(wgrad_chunks(p.S, p.X, p.lvals, p.nreps, p.ci, p.co, &ch)) * p.R * (p.ci + p.co));
+    } else {
+        out->low = c.take<float>(static_cast<size_t>(dim) * p.S * 16 * ad_tiles(p.R));
+        out->parts_down = c.take<float>(static_cast<size_t>(wgrad_chunks(p.S, p.X, p.lvals, p.nreps, p.ci, p.R, &ch)) * p.ci * p.R);
+        out->parts_up = c.take<float>(static_cast<size_t>(wgrad_chunks(p.S, p.X, p.lvals, p.nreps, p.co, p.R, &ch)) * p.co * p.R);
+    }
     out->all = c.take<int32_t>(2);
     out->shared_bytes = shared ? feq_expert_linear_bwd_workspace(p.lvals, p.nreps, 1, p.S, p.ci, p.co, nbias) : 0;
     out->shared = c.take<char>(out->shared_bytes);
@@ -844,13 +890,15 @@ extern "C" int feq_adapter_linear_fwd(const int32_t* lvals, int32_t nreps, int32
     });
 }
 
-extern "C" size_t feq_adapter_linear_low_floats(const int32_t* lvals, int32_t nreps, int64_t rows, int32_t rank) {
-    if (!lvals || nreps < 1 || nreps > kXlMaxReps || rows < 1 || rank < 1 || rank > kAdMaxRank) return 0;
+extern "C" size_t feq_adapter_linear_low_floats(const int32_t* lvals, int32_t nreps, int64_t rows, int32_t cin, int32_t cout, int32_t rank,
+                                                int32_t train) {
+    if (!lvals || nreps < 1 || nreps > kXlMaxReps || rows < 1 || cin < 1 || cout < 1 || rank < 1 || rank > kAdMaxRank) return 0;
     int64_t dim = 0;
     for (int r = 0; r < nreps; ++r) {
         if (lvals[r] < 0 || lvals[r] > kXlMaxPlanes) return 0;
         dim += 2 * lvals[r] + 1;
     }
+    if (cin <= kXlStreamK && (!train || adapter_fused(cin, cout, rank))) return 0;
     return static_cast<size_t>(dim) * rows * 16 * ad_tiles(rank);
 }
 
@@ -874,8 +922,9 @@ extern "C" int feq_adapter_linear_bwd(const int32_t* lvals, int32_t nreps, int32
     if (int rc = ad_check(p, grad_bias ? bias_cols : nullptr, nbias, scale, &map)) return rc;
     if (rows == 0) return fail(FEQ_ERR_INVALID, "no rows");
     if (!grad_y || !x || !weight || !down || !up || !order || !offsets) return fail(FEQ_ERR_INVALID, "NULL pointer");
-    if (grad_up && !low) return fail(FEQ_ERR_INVALID, "the gradient of up needs the forward's reduced rows");
-    if (grad_down && !grad_x) return fail(FEQ_ERR_INVALID, "the gradient of down comes with that of x");
+    const bool fused = adapter_fused(cin, cout, rank);
+    if (grad_up && !low && !fused) return fail(FEQ_ERR_INVALID, "the gradient of up needs the forward's reduced rows");
+    if ((grad_down || grad_up) && !grad_x) return fail(FEQ_ERR_INVALID, "the adapters' gradients come with that of x");
     if (grad_bias && (!grad_weight || !bias_cols || nbias < 1)) return fail(FEQ_ERR_INVALID, "a bias gradient needs bias columns and comes with the weight's");
     AdScratch w;
     const size_t need = ad_scratch(p, map.first[nreps], grad_weight, grad_bias ? nbias : 0, workspace, &w);
@@ -887,6 +936,7 @@ extern "C" int feq_adapter_linear_bwd(const int32_t* lvals, int32_t nreps, int32
         if (grad_x) {
             AdArgs a{grad_y, weight, up, down, nullptr, offsets, order, grad_x, w.low};
             a.scale = scale;
+            if (fused && (grad_down || grad_up)) return adapter_bwd_fused(lvals, nreps, adapters, rows, cin, cout, rank, dtype, a, x, grad_down, grad_up, w.parts_down, s);
             if (int err = ad_run<T, true>(p, map, a, {grad_y, weight, down, grad_x}, s)) return err;
         }
         if (grad_down)

@@ -547,7 +547,7 @@ k_ea_edge_rows(EaArgs<T> a, const float* __restrict__ gz, T* __restrict__ gq, in
 
 // grad_b over an equal share of the edges a workgroup.  Every slot (a lane for each of 2^lgP heads) adds its edges to a
 // table of its own in LDS, one edge after another: no two lanes meet in it, so the order is fixed although the additions
-// are LDS's own (which a lane need not wait for: read, add and write took 50 us where these take XX, 640000 edges of 8
+// are LDS's own (which a lane need not wait for: read, add and write took 45 us where these take 29, 640000 edges of 8
 // heads and 100 buckets).  The tables are then summed in order.  Slots beyond the `tables` that fit take no edges.
 // blockIdx.y: heads from hn blockIdx.y on.
 template <bool WIDE>

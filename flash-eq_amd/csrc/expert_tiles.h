@@ -312,6 +312,32 @@ __device__ __forceinline__ int xcd_tile(int block, int subs, int tiles, int& sub
 }
 inline int64_t xcd_grid(int64_t bound, int64_t subs) { return 8 * ceil_div(bound, 8) * subs; }
 
+// Of the experts with several chunks of rc rows, the one of number `want` (-1: there are fewer): its chunks and those of such
+// experts before it.  Asked by whole waves; results are uniform.
+__device__ __forceinline__ XlTile several_chunks(const int32_t* __restrict__ offsets, int X, int rc, int want) {
+    const int lane = threadIdx.x & 63;
+    XlTile t{-1, 0, 0, 0, 0, 0};
+    int carry = 0, slots = 0;
+    for (int e0 = 0; e0 < X; e0 += 64) {
+        const int e = e0 + lane;
+        const int n = e < X ? (offsets[e + 1] - offsets[e] + rc - 1) / rc : 0;
+        const int m = n > 1 ? n : 0;
+        const uint64_t many = __ballot(n > 1);
+        const int incl = inclusive_sum(m);
+        const uint64_t hit = __ballot(n > 1 && carry + static_cast<int>(__popcll(many & ((1ull << lane) - 1ull))) == want);
+        if (hit) {
+            const int f = __ffsll(static_cast<unsigned long long>(hit)) - 1;
+            t.expert = e0 + f;
+            t.before = slots + __builtin_amdgcn_readlane(incl - m, f);
+            t.count = __builtin_amdgcn_readlane(n, f);
+            break;
+        }
+        carry += static_cast<int>(__popcll(many));
+        slots += __builtin_amdgcn_readlane(incl, 63);
+    }
+    return t;
+}
+
 // The gradients of the experts of several chunks: the sum of their partials, in an order that no launch changes.
 // blockIdx.y: the expert's number among these, blockIdx.z: the irrep, and behind the irreps the bias columns.
 // SPLIT: the four waves of a workgroup take a quarter of the partials each, for experts of many (111 of 34 x 51
@@ -324,24 +350,8 @@ k_xl_wsum(const float* __restrict__ pw, const float* __restrict__ pb, const int3
     __shared__ __align__(16) float part[SPLIT ? 3 : 1][64 * V];
     const int z = blockIdx.z, lane = threadIdx.x & 63, want = blockIdx.y;
     const int rep = z < nreps ? z : ch.brep[z - nreps], rc = ch.rows[rep];
-    int expert = -1, first = 0, count = 0, carry = 0, slots = 0;
-    for (int e0 = 0; e0 < X; e0 += 64) {
-        const int e = e0 + lane;
-        const int n = e < X ? (offsets[e + 1] - offsets[e] + rc - 1) / rc : 0;
-        const int m = n > 1 ? n : 0;
-        const uint64_t many = __ballot(n > 1);
-        const int incl = inclusive_sum(m);
-        const uint64_t hit = __ballot(n > 1 && carry + static_cast<int>(__popcll(many & ((1ull << lane) - 1ull))) == want);
-        if (hit) {
-            const int f = __ffsll(static_cast<unsigned long long>(hit)) - 1;
-            expert = e0 + f;
-            first = slots + __builtin_amdgcn_readlane(incl - m, f);
-            count = __builtin_amdgcn_readlane(n, f);
-            break;
-        }
-        carry += static_cast<int>(__popcll(many));
-        slots += __builtin_amdgcn_readlane(incl, 63);
-    }
+    const XlTile t = several_chunks(offsets, X, rc, want);
+    const int expert = t.expert, first = t.before, count = t.count;
     if (expert < 0) return;
     constexpr int EACH = (SPLIT ? 64 : 256) * V;
     const int wave = SPLIT ? threadIdx.x >> 6 : 0;

@@ -965,7 +965,7 @@ struct AdapterLinearNode final : TuneNode {
         const bool shared = need(1) || need(4);
         const int32_t nb = need(4) ? static_cast<int32_t>(nbias) : 0;
         Tensor gx, gw, gd, gu, gb;
-        if (need(0) || need(2)) gx = make(xs.sizes(), xs, xs.scalar_type());
+        if (need(0) || need(2) || need(3)) gx = make(xs.sizes(), xs, xs.scalar_type());
         if (shared) gw = make(w.sizes(), w, w.scalar_type());
         if (need(2)) gd = make(dn.sizes(), dn, dn.scalar_type());
         if (need(3)) gu = make(u.sizes(), u, u.scalar_type());
@@ -1037,8 +1037,8 @@ Tensor adapter_linear(const Tensor& x, const Tensor& weight, const Tensor& down,
         shape.back() = co;
         y = make(shape, x, x.scalar_type());
         Tensor low;
-        if (rows && (ci > 128 || (node && wants_grad(up))))
-            low = make({static_cast<int64_t>(feq_adapter_linear_low_floats(irreps.lvals.data(), irreps.n(), rows, rank))}, x, at::kFloat);
+        const size_t floats = feq_adapter_linear_low_floats(irreps.lvals.data(), irreps.n(), rows, ci, co, rank, node && wants_grad(up));
+        if (floats) low = make({static_cast<int64_t>(floats)}, x, at::kFloat);
         On on(x);
         done(feq_adapter_linear_fwd(irreps.lvals.data(), irreps.n(), adapters, rows, ci, co, rank, code, ptr(xc), ptr(wc), ptr(dc), ptr(uc),
                                     static_cast<float>(scale), ptr_as<int32_t>(order), ptr_as<int32_t>(offsets), ptr(bc),

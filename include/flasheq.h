@@ -889,15 +889,15 @@ int feq_edge_attn_bwd(const feq_edge_attn* a, const int32_t* perm_k, const int32
  * cout, rank), bias (cout, nbias) or NULL, all of dtype; order and offsets of feq_expert_plan over the rows (top_k 1).
  *   y[d, i] = weight[r] x[d, i] + scale up[a, r] (down[a, r] x[d, i])  (+ bias column bias_cols[r])
  * for the plane d of a component of irrep r and the adapter a of row i; rows without one get the shared map alone.
- * low: feq_adapter_linear_low_floats floats, the reduced rows scale down x in the plan's order, which the backward needs for
- * grad_up and the forward itself where cin > 128 (else it may be NULL).  rank <= 64; the others as feq_expert_linear_fwd. */
-size_t feq_adapter_linear_low_floats(const int32_t* lvals, int32_t nreps, int64_t rows, int32_t rank);
+ * low: feq_adapter_linear_low_floats floats (0: NULL will do), the reduced rows scale down x in the plan's order, for the
+ * forward itself and, where train is set, for the backward's grad_up.  rank <= 64; the others as feq_expert_linear_fwd. */
+size_t feq_adapter_linear_low_floats(const int32_t* lvals, int32_t nreps, int64_t rows, int32_t cin, int32_t cout,
+                                     int32_t rank, int32_t train);
 int feq_adapter_linear_fwd(const int32_t* lvals, int32_t nreps, int32_t adapters, int64_t rows, int32_t cin, int32_t cout,
                            int32_t rank, int32_t dtype, const void* x, const void* weight, const void* down, const void* up,
                            float scale, const int32_t* order, const int32_t* offsets, const void* bias, int32_t nbias,
                            const int32_t* bias_cols, void* y, float* low, feq_stream_t stream);
-/* From grad_y: grad_x, grad_down (with grad_x), grad_up (with low), grad_weight, grad_bias (with grad_weight), any of them
- * NULL; sums in a fixed order, zeros for an adapter without rows.  rows > 0.  Workspace
+/* From grad_y: grad_x, grad_down and grad_up (with grad_x), grad_weight, grad_bias (with grad_weight), any of them NULL; sums in a fixed order, zeros for an adapter without rows.  rows > 0.  Workspace
  * feq_adapter_linear_bwd_workspace bytes (shared: whether grad_weight is wanted; nbias 0 without grad_bias). */
 size_t feq_adapter_linear_bwd_workspace(const int32_t* lvals, int32_t nreps, int32_t adapters, int64_t rows, int32_t cin,
                                         int32_t cout, int32_t rank, int32_t shared, int32_t nbias);
