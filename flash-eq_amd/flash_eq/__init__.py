@@ -30,6 +30,10 @@ from .layers import (
     GraphPooling,
     EquivariantTransformerBlock,
     EquivariantTransformer,
+    DistanceBuckets,
+    EquivariantDropout,
+    LinearAdapters,
+    add_adapters,
 )
 from ._native import CUDANotAvailableError
 
@@ -44,7 +48,7 @@ __all__ = [
     "InvariantLayerNorm", "ExpertPlan", "expert_topk", "expert_linear",
     "ExpertRouter", "EquivariantExpertLinear", "EquivariantExpertMLP",
     "dropout_seed", "feature_dropout", "distance_buckets", "edge_attention_weights", "edge_attention_weights_qk",
-    "adapter_linear",
+    "adapter_linear", "DistanceBuckets", "EquivariantDropout", "LinearAdapters", "add_adapters",
     "RadialBasisFunctions", "RadialMLP", "SeparableRadialNet",
     "CUDANotAvailableError",
 ]

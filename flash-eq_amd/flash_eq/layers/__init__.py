@@ -1,6 +1,8 @@
 """Equivariant layers of the edge hot path and their node-side neighbours."""
 from .linear import EquivariantEdgewiseLinear, EquivariantLinear
-from .attention import EquivariantEdgeAttention, EquivariantAttention
+from .adapters import LinearAdapters, add_adapters
+from .attention import DistanceBuckets, EquivariantEdgeAttention, EquivariantAttention
+from .dropout import EquivariantDropout
 from .norm import RepNorm, EquivariantLayerNorm, InvariantLayerNorm, SeparableEquivariantLayerNorm
 from .pooling import GraphPooling
 from .gating import EquivariantGating
@@ -16,4 +18,5 @@ __all__ = [
     "ExpertRouter", "EquivariantExpertLinear", "EquivariantExpertMLP",
     "EquivariantTransformerBlock", "EquivariantTransformer",
     "RadialBasisFunctions", "RadialMLP", "SeparableRadialNet",
+    "DistanceBuckets", "EquivariantDropout", "LinearAdapters", "add_adapters",
 ]

@@ -25,6 +25,7 @@ from ..ops import (_use_hl, edgewise_attention_pool, edgewise_linear, edgewise_l
                    edgewise_pool_supported, edgewise_pq_supported, edgewise_src_supported,
                    embedding_for, rows_weight_grad, BiasRowsFn, EqLinearFn)
 from ..representations import ProductRepr, Repr
+from .adapters import LinearAdapters
 from .radial import SeparableRadialNet
 from ..utils import half_precision_active
 
@@ -245,7 +246,9 @@ class EquivariantEdgewiseLinear(nn.Module):
 
 
 class EquivariantLinear(nn.Module):
-    """Per-degree channel mixing of node features; bias/activation on scalars only."""
+    """Per-degree channel mixing of node features; bias/activation on scalars only.
+
+    With adapters (``add_adapters``) a call given their plan adds every row's low-rank map."""
 
     def __init__(self, in_repr: Repr, out_repr: Repr, bias: bool = True,
                  activation: nn.Module | None = None) -> None:
@@ -272,20 +275,46 @@ class EquivariantLinear(nn.Module):
         # per irrep: the bias column of a scalar irrep, -1 otherwise
         self._bias_cols = tuple(locs.index(a) if (self.bias is not None and a in locs) else -1
                                 for a, _ in self._slices)
+        self.adapters: LinearAdapters | None = None
+
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        if "adapters" not in self._modules:      # a layer pickled before there were any
+            self.__dict__.setdefault("adapters", None)
+
+    def add_adapters(self, num_adapters: int, rank: int = 8, alpha: float | None = None) -> list[nn.Parameter]:
+        """Gives the layer ``num_adapters`` new adapters (in the place of any it had); returns their parameters."""
+        new = LinearAdapters(self.in_repr, self.out_repr, num_adapters, rank, alpha)
+        self.__dict__.pop("adapters", None)
+        self.adapters = new.to(device=self.weight.device, dtype=self.weight.dtype)
+        return list(self.adapters.parameters())
+
+    def _adapted(self, plan) -> bool:
+        """Whether a call with this plan goes through the adapters."""
+        if plan is None:
+            return False
+        if self.adapters is None:
+            raise ValueError("adapters were given to an EquivariantLinear that has none (add_adapters)")
+        return True
 
     def fused_ok(self, f: torch.Tensor) -> bool:
         """Float32 GPU features without an activation take EqLinearFn."""
         return (f.is_cuda and f.dtype == torch.float32 and self.weight.dtype == torch.float32
                 and isinstance(self.activation, nn.Identity))
 
-    def forward_layout(self, f: torch.Tensor, in_cm: bool, out_cm: bool) -> torch.Tensor:
+    def forward_layout(self, f: torch.Tensor, in_cm: bool, out_cm: bool, plan=None) -> torch.Tensor:
         """The map on node-major (rows, cin, dim) or component-major (dim, rows,
-        cin) features (in_cm), returning either layout (out_cm); fused_ok(f)."""
+        cin) features (in_cm), returning either layout (out_cm); fused_ok(f).
+        ``plan``: the rows' adapters."""
+        if self._adapted(plan):
+            y = self.adapters(f if in_cm else f.reshape(-1, *f.shape[-2:]).permute(2, 0, 1).contiguous(), self.weight, self.bias, plan)
+            return y if out_cm else y.permute(1, 2, 0).contiguous()
         return EqLinearFn.apply(f, self.weight, self.bias, self._slices, self._bias_cols,
                                 self.in_repr.mult, self.out_repr.mult, in_cm, out_cm)
 
-    def forward(self, f: torch.Tensor) -> torch.Tensor:
-        """(..., in_mult, dim) -> (..., out_mult, dim).
+    def forward(self, f: torch.Tensor, plan=None) -> torch.Tensor:
+        """(..., in_mult, dim) -> (..., out_mult, dim).  ``plan``: the ``ExpertPlan`` of
+        the adapters of the rows, all leading axes together.
 
         Computed component-major: f is copied once to (dim, rows, in_mult), each
         irrep's components are one plain (components * rows, in_mult) x
@@ -295,6 +324,11 @@ class EquivariantLinear(nn.Module):
         before summing them.)"""
         cin, cout = self.in_repr.mult, self.out_repr.mult
         lead = f.shape[:-2]
+        if self._adapted(plan):
+            y = self.forward_layout(f, False, True, plan)                # (dim, rows, cout)
+            if self.bias is not None and not isinstance(self.activation, nn.Identity):
+                y = torch.stack([self.activation(t).to(t.dtype) if a in self.scalar_locs else t for a, t in enumerate(y)])
+            return y.permute(1, 2, 0).reshape(*lead, cout, y.shape[0])
         if self.fused_ok(f):
             return self.forward_layout(f, False, False).view(*lead, cout, f.shape[-1])
         w = self.weight.view(self.in_repr.nreps(), cout, cin)

@@ -13,7 +13,9 @@ import torch.nn as nn
 from ..graph import Graph
 from ..representations import Repr, WignerDBasis
 from ..ops import FanOutFn, ResidualScaleCmFn, ResidualScaleFn, ScaleFn
-from .attention import EquivariantAttention
+from .adapters import Adapters, adapter_plan
+from .attention import DistanceBuckets, EquivariantAttention
+from .dropout import EquivariantDropout
 from .experts import EquivariantExpertMLP
 from .gating import EquivariantGating
 from .linear import EquivariantLinear
@@ -60,9 +62,9 @@ class DropPath(nn.Module):
         return x / (1 - self.drop_prob)
 
 
-def _wanted(balance: list[torch.Tensor] | None) -> dict:
-    """The keyword of a call, where there is a list: blocks and subclasses without it stay callable."""
-    return {} if balance is None else {"balance": balance}
+def _wanted(**options) -> dict:
+    """The keywords of a call that are given: blocks and subclasses without the others stay callable."""
+    return {k: v for k, v in options.items() if v is not None}
 
 
 class EquivariantTransformerBlock(nn.Module):
@@ -70,7 +72,10 @@ class EquivariantTransformerBlock(nn.Module):
 
     With ``num_experts`` > 0 the MLP is a mixture of experts (``EquivariantExpertMLP``), each node
     taking ``experts_per_node`` of them; ``forward(..., balance=terms)`` appends its balancing term to
-    the list ``terms``.  The reference has no such option."""
+    the list ``terms``.  ``bias_buckets`` and ``counter_dropout`` are the attention's (``EquivariantEdgeAttention``);
+    ``feature_dropout`` drops irreps of the attention's and the MLP's results (``EquivariantDropout``);
+    ``forward(..., adapters=ids)`` goes through the nodes' adapters (``add_adapters``).  The reference has no such
+    options."""
 
     def __init__(self, in_repr: Repr, out_repr: Repr, num_heads: int = 1, num_bins: int = 100,
                  rank: int = 4, hidden_dim: int = 64, min_dist: float = 0.0,
@@ -79,7 +84,8 @@ class EquivariantTransformerBlock(nn.Module):
                  layer_scale_init: float | None = 1e-4, use_gating: bool = True,
                  use_s2_activation: bool = False, s2_precision: int = 47,
                  distance_decay_scale: float | None = None, num_experts: int = 0,
-                 experts_per_node: int = 2) -> None:
+                 experts_per_node: int = 2, bias_buckets: int = 0, counter_dropout: bool = False,
+                 feature_dropout: float = 0.0) -> None:
         super().__init__()
         if use_s2_activation:
             raise NotImplementedError(
@@ -93,7 +99,8 @@ class EquivariantTransformerBlock(nn.Module):
         self.attn = EquivariantAttention(
             in_repr=in_repr, out_repr=out_repr, num_heads=num_heads, num_bins=num_bins, rank=rank,
             hidden_dim=hidden_dim, min_dist=min_dist, max_dist=max_dist, log_bins=log_bins,
-            dropout=dropout, reduce="sum", distance_decay_scale=distance_decay_scale)
+            dropout=dropout, reduce="sum", distance_decay_scale=distance_decay_scale,
+            bias_buckets=bias_buckets, counter_dropout=counter_dropout)
         self.norm2 = SeparableEquivariantLayerNorm(out_repr)
         self.experts: EquivariantExpertMLP | None = None
         if num_experts < 0:
@@ -112,20 +119,28 @@ class EquivariantTransformerBlock(nn.Module):
         self.layer_scale_mlp: nn.Module = (LayerScale(layer_scale_init)
                                            if layer_scale_init is not None else nn.Identity())
         self.drop_path: nn.Module = DropPath(drop_path) if drop_path > 0.0 else nn.Identity()
+        self.feature_dropout: EquivariantDropout | None = (
+            EquivariantDropout(out_repr, feature_dropout) if feature_dropout != 0.0 else None)
 
     def __setstate__(self, state: dict) -> None:
         super().__setstate__(state)
-        if "experts" not in self._modules:       # a block pickled before there were any
-            self.__dict__.setdefault("experts", None)
+        for name in ("experts", "feature_dropout"):      # a block pickled before there were any
+            if name not in self._modules:
+                self.__dict__.setdefault(name, None)
+
+    def _dropped(self, y: torch.Tensor, cm: bool = False) -> torch.Tensor:
+        return y if self.feature_dropout is None else self.feature_dropout(y, cm)
 
     def forward(self, P: torch.Tensor, Q: torch.Tensor, node_features: torch.Tensor,
                 distances: torch.Tensor, graph: Graph,
                 edge_features: torch.Tensor | None = None,
-                balance: list[torch.Tensor] | None = None) -> torch.Tensor:
+                balance: list[torch.Tensor] | None = None, buckets: torch.Tensor | None = None,
+                adapters: Adapters | None = None) -> torch.Tensor:
+        adapters = adapter_plan(self, adapters)
         half = half_dtype(node_features)
         if half is not None:
             return run_float32(self, half, (P, Q, node_features, distances, graph),
-                               dict(edge_features=edge_features, **_wanted(balance)))
+                               dict(edge_features=edge_features, **_wanted(balance=balance, buckets=buckets, adapters=adapters)))
         # With the residual connection, the norm also returns the features for
         # it (forward_pair): the residual's gradient is then added inside the
         # norm's backward kernel instead of by autograd in a separate pass.
@@ -133,14 +148,15 @@ class EquivariantTransformerBlock(nn.Module):
             h, nf = self.norm1.forward_pair(node_features)
         else:
             h, nf = self.norm1(node_features), node_features
-        attn_out = self.attn(P, Q, h, distances, graph, edge_features=edge_features)
+        attn_out = self._dropped(self.attn(P, Q, h, distances, graph, edge_features=edge_features,
+                                           **_wanted(buckets=buckets, adapters=adapters)))
         if self._use_attn_residual:
             x = _residual(nf, attn_out, self.layer_scale_attn, self.drop_path)
         else:
             x = attn_out
         if self.experts is not None:
             h, xr = self.norm2.forward_pair(x) if self.norm2.cm_ok(x) else (self.norm2(x), x)
-            return _residual(xr, self.experts(h, balance), self.layer_scale_mlp, self.drop_path)
+            return _residual(xr, self._dropped(self.experts(h, balance)), self.layer_scale_mlp, self.drop_path)
         if (isinstance(self.mlp_act, EquivariantGating) and self.mlp_act.kernels_ok(x)
                 and self.mlp_up.fused_ok(x) and self.mlp_down.fused_ok(x)):
             # the MLP runs component-major (dim, N, c) from the norm's output to
@@ -150,15 +166,15 @@ class EquivariantTransformerBlock(nn.Module):
                   and isinstance(self.drop_path, nn.Identity)
                   and self.layer_scale_mlp.gamma.dtype == torch.float32)
             h, xr = self.norm2.forward_pair(x, cm) if self.norm2.cm_ok(x) else (self.norm2(x), x)
-            t = self.mlp_act.forward_cm(self.mlp_up.forward_layout(h, cm, True))
+            t = self.mlp_act.forward_cm(self.mlp_up.forward_layout(h, cm, True, adapters))
             if cm:
-                return ResidualScaleCmFn.apply(xr, self.mlp_down.forward_layout(t, True, True),
+                return ResidualScaleCmFn.apply(xr, self._dropped(self.mlp_down.forward_layout(t, True, True, adapters), True),
                                                self.layer_scale_mlp.gamma)
-            mlp_out = self.mlp_down.forward_layout(t, True, False).view(*x.shape[:-2], self.out_repr.mult,
-                                                                       x.shape[-1])
-            return _residual(xr, mlp_out, self.layer_scale_mlp, self.drop_path)
-        mlp_out = self.mlp_down(self.mlp_act(self.mlp_up(self.norm2(x))))
-        return _residual(x, mlp_out, self.layer_scale_mlp, self.drop_path)
+            mlp_out = self.mlp_down.forward_layout(t, True, False, adapters).view(*x.shape[:-2], self.out_repr.mult,
+                                                                                 x.shape[-1])
+            return _residual(xr, self._dropped(mlp_out), self.layer_scale_mlp, self.drop_path)
+        mlp_out = self.mlp_down(self.mlp_act(self.mlp_up(self.norm2(x), adapters)), adapters)
+        return _residual(x, self._dropped(mlp_out), self.layer_scale_mlp, self.drop_path)
 
     def extra_repr(self) -> str:
         return (f"in_repr={self.in_repr}, out_repr={self.out_repr}, "
@@ -168,7 +184,10 @@ class EquivariantTransformerBlock(nn.Module):
 class EquivariantTransformer(nn.Module):
     """Stack of blocks: in -> hidden -> ... -> hidden -> out, basis computed from coordinates.
     ``num_experts`` > 0 makes every block's MLP a mixture of experts, and ``forward(..., balance=terms)``
-    appends every block's balancing term to the list ``terms``."""
+    appends every block's balancing term to the list ``terms``.  ``bias_buckets`` > 0 gives every block's attention a
+    learned bias for each head and bucket of the distances (``DistanceBuckets`` over the radial range, made once a
+    call); ``counter_dropout`` and ``feature_dropout`` are the blocks'; ``forward(..., adapters=ids)`` sends every
+    node through its adapter of each map (``add_adapters``)."""
 
     def __init__(self, in_repr: Repr, hidden_repr: Repr, out_repr: Repr, num_layers: int = 6,
                  num_heads: int = 1, num_bins: int = 100, rank: int = 4, hidden_dim: int = 64,
@@ -176,7 +195,8 @@ class EquivariantTransformer(nn.Module):
                  mlp_ratio: int = 2, dropout: float = 0.0, drop_path: float = 0.0,
                  layer_scale_init: float | None = 1e-4, use_s2_activation: bool = False,
                  s2_precision: int = 47, distance_decay_scale: float | None = None,
-                 num_experts: int = 0, experts_per_node: int = 2) -> None:
+                 num_experts: int = 0, experts_per_node: int = 2, bias_buckets: int = 0,
+                 counter_dropout: bool = False, feature_dropout: float = 0.0) -> None:
         super().__init__()
         self.in_repr = in_repr
         self.hidden_repr = hidden_repr
@@ -196,14 +216,24 @@ class EquivariantTransformer(nn.Module):
                 log_bins=log_bins, mlp_ratio=mlp_ratio, dropout=dropout, drop_path=rates[i],
                 layer_scale_init=layer_scale_init, use_s2_activation=use_s2_activation,
                 s2_precision=s2_precision, distance_decay_scale=distance_decay_scale,
-                num_experts=num_experts, experts_per_node=experts_per_node))
+                num_experts=num_experts, experts_per_node=experts_per_node, bias_buckets=bias_buckets,
+                counter_dropout=counter_dropout, feature_dropout=feature_dropout))
         self.final_norm = SeparableEquivariantLayerNorm(out_repr)
+        self.buckets: DistanceBuckets | None = (
+            DistanceBuckets(bias_buckets, min_dist, max_dist, log_bins) if bias_buckets else None)
+
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        if "buckets" not in self._modules:       # a model pickled before there were any
+            self.__dict__.setdefault("buckets", None)
 
     def forward(self, coordinates: torch.Tensor, node_features: torch.Tensor,
-                graph: Graph, balance: list[torch.Tensor] | None = None) -> torch.Tensor:
+                graph: Graph, balance: list[torch.Tensor] | None = None,
+                adapters: Adapters | None = None) -> torch.Tensor:
+        adapters = adapter_plan(self, adapters)
         half = half_dtype(node_features)
         if half is not None:
-            return run_float32(self, half, (coordinates, node_features, graph), _wanted(balance))
+            return run_float32(self, half, (coordinates, node_features, graph), _wanted(balance=balance, adapters=adapters))
         # src - dst, as transformer.py:406.  In float32 through the graph's CSR
         # gathers: their backward (the coordinate gradient) is a fixed-order
         # segmented sum, where torch's indexing backward sorts the indices
@@ -225,8 +255,10 @@ class EquivariantTransformer(nn.Module):
                 views = iter(FanOutFn.apply(m_hidden, k))
                 uses = [(next(views) if P is m_hidden else P, next(views) if Q is m_hidden else Q)
                         for P, Q in uses]
+        options = _wanted(balance=balance, adapters=adapters,
+                          buckets=None if self.buckets is None else self.buckets(distances))
         for layer, (P, Q) in zip(self.layers, uses):
-            x = layer(P, Q, x, distances, graph, **_wanted(balance))
+            x = layer(P, Q, x, distances, graph, **options)
         return self.final_norm(x)
 
     def extra_repr(self) -> str:
