@@ -6,22 +6,26 @@ namespace {
 
 // grad_x, grad_down and grad_up in one pass over grad_y and x: channels of at most 128 both ways and ranks of at most 16.  A
 // workgroup takes a chunk of rows of one adapter (or of none) and one irrep, all its planes, as k_xl_wgrad; the shared map
-// and the adapter's stay in LDS, and a wave takes RB rows at a time straight from memory in the matrix cores' layout, the next
+// and the adapter's stay in LDS, and a wave takes 16 rows at a time straight from memory in the matrix cores' layout, the next
 // ones in flight meanwhile.  Both reduced rows are formed here: u as in k_ad_stream for grad_x, and again with the operands
 // exchanged, which leaves lane (c, g) rank c of rows 4 g .. 4 g + 3, the first operand of the sums over rows; t likewise.  Their
-// second operands are columns of x and grad_y: the wave writes its rows to LDS and reads them transposed.  16-bit types
-// sum 32 rows a product: element j < 4 is row 4 g + j of the first 16, j >= 4 of the next.  The waves' sums are added at
-// the chunk's end.
+// second operands are columns of x and grad_y: the wave writes its rows to LDS, 64 columns at a time, and reads them
+// transposed.  16-bit types take a reduced row as two numbers, as in k_ad_stream, so 16 rows fill a product.  The waves' sums
+// are added at the chunk's end.
+template <class T, int NB, int KB>
+constexpr size_t kAdBwdLds =
+    sizeof(T) * (KB * (NB + Mma<T>::PAD) + KB * (16 + Mma<T>::PAD) + 16 * (NB + Mma<T>::PAD) + 16 * (NB + 16 / sizeof(T)) + 4 * 16 * (64 + Mma<T>::PAD));
+
 template <class T, int HOW, int NB, int KB>
-__global__ void __launch_bounds__(kXlThreads, 1)
+__global__ void __launch_bounds__(kXlThreads, (2 * kAdBwdLds<T, NB, KB> <= 163840 ? 2 : 1))
 k_ad_bwd(AdArgs a, const T* __restrict__ x, XlMap map, XlChunks ch, T* __restrict__ gdown, T* __restrict__ gup,
          float* __restrict__ parts) {
     using M = Mma<T>;
     typedef typename M::frag frag;
     constexpr bool F16 = std::is_same<T, _Float16>::value;
-    constexpr int V = 16 / sizeof(T), RT = sizeof(T) == 4 ? 1 : 2, RB = 16 * RT;      // row tiles and rows of a step
+    constexpr int V = 16 / sizeof(T);
     constexpr int NT = NB / 16, KT = KB / 16, NA = NT < 4 ? NT : 4, NSK = KB / M::KS, NSX = NB / M::KS;
-    constexpr int LDT = NB + M::PAD, LDF = 16 + M::PAD, LDX = NB + V, LC = (NB > KB ? NB : KB) + M::PAD;
+    constexpr int LDT = NB + M::PAD, LDF = 16 + M::PAD, LDX = NB + V, LC = 64 + M::PAD;
     const int K = a.K, N = a.N, X = a.X, S = a.S, R = a.R, nreps = a.nreps;
     extern __shared__ __align__(16) char smem[];
     T* sW = reinterpret_cast<T*>(smem);              // W as it lies (co, ci), its columns dealt
@@ -30,7 +34,7 @@ k_ad_bwd(AdArgs a, const T* __restrict__ x, XlMap map, XlChunks ch, T* __restric
     T* sD = sG + 16 * LDT;                           // down (R, ci)
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    T* buf = sD + 16 * LDX + wave * RB * LC;
+    T* buf = sD + 16 * LDX + wave * 16 * LC;
     const int xcds = ch.xcds, block = blockIdx.x / xcds;
     int rep = nreps - 1;                             // the irreps of most planes first
     while (rep > 0 && block >= ch.tile0[rep - 1]) --rep;
@@ -40,37 +44,28 @@ k_ad_bwd(AdArgs a, const T* __restrict__ x, XlMap map, XlChunks ch, T* __restric
     const bool own = t.expert < X;                   // uniform
     const int rows = t.row1 - t.row0 < rc ? t.row1 - t.row0 : rc;
     const int d0 = __builtin_amdgcn_readfirstlane(map.first[rep]), d1 = __builtin_amdgcn_readfirstlane(map.first[rep + 1]);
-    const int steps = (rows + RB - 1) / RB, total = steps * (d1 - d0);
+    const int steps = (rows + 15) / 16, total = steps * (d1 - d0);
     const T *gy = static_cast<const T*>(a.in), *W = static_cast<const T*>(a.W);
 
-    auto number = [&](int it, int r) {               // row tile r's row at this lane's place, -1: none
-        const int i = it < total ? it % steps * RB + 16 * r + c : rows;
+    auto number = [&](int it) {                      // the row at this lane's place, -1: none
+        const int i = it < total ? it % steps * 16 + c : rows;
         return i < rows ? a.order[t.row0 + i] : -1;
     };
-    uint4 vg[RT][NSK], vx[RT][NSX];                  // in flight
-    int row[RT], next[RT];
-    auto load = [&](int it, const int (&at)[RT]) {
-        const int d = it < total ? d0 + it / steps : d0;
+    uint4 vg[NSK], vx[NSX];                          // in flight
+    auto load = [&](int it, int at) {
+        const int64_t i = static_cast<int64_t>(it < total ? d0 + it / steps : d0) * S + (at < 0 ? 0 : at);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const int64_t i = static_cast<int64_t>(d) * S + (at[r] < 0 ? 0 : at[r]);
+        for (int ks = 0; ks < NSK; ++ks) {
+            const int k = ks * M::KS + M::FE * g;
+            vg[ks] = load_row<T, HOW>(gy + i * K, k, at < 0 ? 0 : K - k, gy);
+        }
 #pragma unroll
-            for (int ks = 0; ks < NSK; ++ks) {
-                const int k = ks * M::KS + M::FE * g;
-                vg[r][ks] = load_row<T, HOW>(gy + i * K, k, at[r] < 0 ? 0 : K - k, gy);
-            }
-#pragma unroll
-            for (int ks = 0; ks < NSX; ++ks) {
-                const int k = ks * M::KS + M::FE * g;
-                vx[r][ks] = load_row<T, HOW>(x + i * N, k, at[r] < 0 || !own ? 0 : N - k, x);
-            }
+        for (int ks = 0; ks < NSX; ++ks) {
+            const int k = ks * M::KS + M::FE * g;
+            vx[ks] = load_row<T, HOW>(x + i * N, k, at < 0 || !own ? 0 : N - k, x);
         }
     };
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        row[r] = number(wave, r);
-        next[r] = number(wave + 4, r);
-    }
+    int row = number(wave), next = number(wave + 4);
     load(wave, row);
     const T* wm = W + static_cast<int64_t>(rep) * K * N;
     const Rows we = rows_at(wm, W, N);
@@ -106,174 +101,130 @@ k_ad_bwd(AdArgs a, const T* __restrict__ x, XlMap map, XlChunks ch, T* __restric
     for (int i = 0; i < KT; ++i) gb[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     int pa = 0, pb = 0;                              // the powers of two that float16's sums are multiplied by
     bool have_a = false, have_b = false;
-    // columns of the wave's rows in `buf`
-    auto columns = [&](int c0) -> frag {
-        if constexpr (sizeof(T) == 4) {
-            return M::columns(buf, LC, 0, g, c, c0);
-        } else {
-            const T* p = buf + (4 * g + (c >> 2)) * LC + c0 + 4 * (c & 3);
-            const v4s u = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p));
-            const v4s w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(p + 16 * LC));
-            const v8s v = {u[0], u[1], u[2], u[3], w[0], w[1], w[2], w[3]};
-            return __builtin_bit_cast(frag, v);
+    // sums += z^T r for reduced rows z and the wave's rows r
+    auto add = [&](v4f z, const auto& r, auto& sums, int& power, bool& have) {
+        constexpr int TILES = sizeof(sums) / sizeof(v4f), PIECE = TILES < 4 ? TILES : 4;
+        if constexpr (F16) {                         // the sums' power follows the largest reduced value so far
+            float most = 0.0f;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) most = fmaxf(most, fabsf(z[m]));
+            most = group_max(most, 64);
+            const int p = low_exponent(most);
+            if (most > 0.0f && (!have || p < power)) {           // uniform
+                if (have)
+#pragma unroll
+                    for (int i = 0; i < TILES; ++i)
+#pragma unroll
+                        for (int m = 0; m < 4; ++m) sums[i][m] = times_power(sums[i][m], p - power);
+                power = p;
+                have = true;
+            }
+#pragma unroll
+            for (int m = 0; m < 4; ++m) z[m] = times_power(z[m], power);
         }
-    };
-    // sums += z^T (columns of the rows in `buf`)
-    auto add = [&](v4f (&z)[RT], auto& sums, int& power, bool& have) {
-        constexpr int TILES = sizeof(sums) / sizeof(v4f);
-        if constexpr (sizeof(T) == 4) {
+        const frag f = low_frag(z, T{});
 #pragma unroll
-            for (int i = 0; i < TILES; ++i) sums[i] = M::mul(z[0], columns(16 * i), sums[i]);
-        } else {
-            if constexpr (F16) {                     // the sums' power follows the largest reduced value so far
-                float most = 0.0f;
+        for (int i0 = 0; i0 < TILES; i0 += PIECE) {
 #pragma unroll
-                for (int r = 0; r < RT; ++r)
+            for (int k = 0; k < 16 * PIECE; k += M::KS)
+                *reinterpret_cast<frag*>(buf + c * LC + k + M::FE * g) = r[(16 * i0 + k) / M::KS];
+            wave_lds();
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) most = fmaxf(most, fabsf(z[r][m]));
-                most = group_max(most, 64);
-                const int p = low_exponent(most);
-                if (most > 0.0f && (!have || p < power)) {           // uniform
-                    if (have)
-#pragma unroll
-                        for (int i = 0; i < TILES; ++i)
-#pragma unroll
-                            for (int m = 0; m < 4; ++m) sums[i][m] = times_power(sums[i][m], p - power);
-                    power = p;
-                    have = true;
+            for (int i = 0; i < PIECE; ++i) {
+                frag b;
+                if constexpr (sizeof(T) == 4) {
+                    b = M::columns(buf, LC, 0, g, c, 16 * i);
+                } else {
+                    const v4s w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(buf + (4 * g + (c >> 2)) * LC + 16 * i + 4 * (c & 3)));
+                    const v8s v = {w[0], w[1], w[2], w[3], w[0], w[1], w[2], w[3]};
+                    b = __builtin_bit_cast(frag, v);
                 }
-#pragma unroll
-                for (int r = 0; r < RT; ++r)
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) z[r][m] = times_power(z[r][m], power);
+                sums[i0 + i] = M::mul(f, b, sums[i0 + i]);
             }
-            frag hi, lo;
-#pragma unroll
-            for (int r = 0; r < 2; ++r)
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                    const float v = z[r % RT][m];
-                    const T h = static_cast<T>(v);
-                    hi[4 * r + m] = h;
-                    lo[4 * r + m] = static_cast<T>(v - static_cast<float>(h));
-                }
-#pragma unroll
-            for (int i = 0; i < TILES; ++i) {
-                const frag b = columns(16 * i);
-                sums[i] = M::mul(hi, b, sums[i]);
-                sums[i] = M::mul(lo, b, sums[i]);
-            }
+            wave_lds();
         }
     };
     for (int it = wave; it < total; it += 4) {
-        frag gf[RT][NSK], xf[RT][NSX];
+        frag gf[NSK], xf[NSX];
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
+        for (int ks = 0; ks < NSK; ++ks)
+            gf[ks] = __builtin_bit_cast(frag, placed_row<T, HOW>(vg[ks], row < 0 ? 0 : K - ks * M::KS - M::FE * g, K, gy));
 #pragma unroll
-            for (int ks = 0; ks < NSK; ++ks)
-                gf[r][ks] = __builtin_bit_cast(frag, placed_row<T, HOW>(vg[r][ks], row[r] < 0 ? 0 : K - ks * M::KS - M::FE * g, K, gy));
-#pragma unroll
-            for (int ks = 0; ks < NSX; ++ks)
-                xf[r][ks] = __builtin_bit_cast(frag, placed_row<T, HOW>(vx[r][ks], row[r] < 0 || !own ? 0 : N - ks * M::KS - M::FE * g, N, x));
-        }
-        int after[RT];
-#pragma unroll
-        for (int r = 0; r < RT; ++r) after[r] = number(it + 8, r);
+        for (int ks = 0; ks < NSX; ++ks)
+            xf[ks] = __builtin_bit_cast(frag, placed_row<T, HOW>(vx[ks], row < 0 || !own ? 0 : N - ks * M::KS - M::FE * g, N, x));
+        const int after = number(it + 8);
         load(it + 4, next);
         asm volatile("" ::: "memory");               // the maps are read from LDS for every step
-        v4f u[RT], v[RT];
-        T* od = static_cast<T*>(a.out) + static_cast<int64_t>(d0 + it / steps) * S * N;
+        v4f acc[NT], low = v4f{0.0f, 0.0f, 0.0f, 0.0f}, u = low, v = low;
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            v4f acc[NT], low = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int i = 0; i < NT; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < NT; ++i) acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int ks = 0; ks < NSK; ++ks)
 #pragma unroll
-            for (int ks = 0; ks < NSK; ++ks)
+            for (int i0 = 0; i0 < NT; i0 += NA) {
+                frag f[NA];
 #pragma unroll
-                for (int i0 = 0; i0 < NT; i0 += NA) {
-                    frag f[NA];
-#pragma unroll
-                    for (int i = 0; i < NA; ++i) f[i] = M::columns(sW, LDT, ks * M::KS, g, c, 16 * (i0 + i));
-                    M::template mul_all<NA>(f, gf[r][ks], acc + i0);
-                }
-            if (own) {
-                u[r] = v[r] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int ks = 0; ks < NSK; ++ks) {
-                    const frag f = M::columns(sF, LDF, ks * M::KS, g, c, 0);
-                    low = M::mul(f, gf[r][ks], low);
-                    u[r] = M::mul(gf[r][ks], f, u[r]);
-                }
-#pragma unroll
-                for (int ks = 0; ks < NSX; ++ks)
-                    v[r] = M::mul(xf[r][ks], *reinterpret_cast<const frag*>(sD + c * LDX + ks * M::KS + M::FE * g), v[r]);
-                low *= a.scale;
-                u[r] *= a.scale;
-                v[r] *= a.scale;
-                int power = 0;
-                if constexpr (F16) {
-                    float most = 0.0f;
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) most = fmaxf(most, fabsf(low[m]));
-                    power = low_exponent(row_max(most));
-#pragma unroll
-                    for (int m = 0; m < 4; ++m) low[m] = times_power(low[m], power);
-#pragma unroll
-                    for (int i = 0; i < NT; ++i)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) acc[i][m] = times_power(acc[i][m], power);
-                }
-                const frag b = low_frag(low, T{});
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    T e[4];
-                    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) e[j] = sG[(4 * g + j) * LDT + 16 * i + c];
-                    } else {
-                        const v4s w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(sG + (4 * g + (c >> 2)) * LDT + 16 * i + 4 * (c & 3)));
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) e[j] = __builtin_bit_cast(T, static_cast<short>(w[j]));
-                    }
-                    acc[i] = M::mul(twice<T>(e), b, acc[i]);
-                }
-                if constexpr (F16)
-#pragma unroll
-                    for (int i = 0; i < NT; ++i)
-#pragma unroll
-                        for (int m = 0; m < 4; ++m) acc[i][m] = times_power(acc[i][m], -power);
+                for (int i = 0; i < NA; ++i) f[i] = M::columns(sW, LDT, ks * M::KS, g, c, 16 * (i0 + i));
+                M::template mul_all<NA>(f, gf[ks], acc + i0);
             }
-            if (row[r] >= 0) {
-                T* o = od + static_cast<int64_t>(row[r]) * N;
+        if (own) {
 #pragma unroll
-                for (int i = 0; i < NT; i += kDealt<T>) {
-                    const int n = 16 * i + V * g;
-                    store_tiles<T, HOW, 1>(o + n, N - n, &acc[i]);
+            for (int ks = 0; ks < NSK; ++ks) {
+                const frag f = M::columns(sF, LDF, ks * M::KS, g, c, 0);
+                low = M::mul(f, gf[ks], low);
+                u = M::mul(gf[ks], f, u);
+            }
+#pragma unroll
+            for (int ks = 0; ks < NSX; ++ks)
+                v = M::mul(xf[ks], *reinterpret_cast<const frag*>(sD + c * LDX + ks * M::KS + M::FE * g), v);
+            low *= a.scale;
+            int power = 0;
+            if constexpr (F16) {
+                float most = 0.0f;
+#pragma unroll
+                for (int m = 0; m < 4; ++m) most = fmaxf(most, fabsf(low[m]));
+                power = low_exponent(row_max(most));
+#pragma unroll
+                for (int m = 0; m < 4; ++m) low[m] = times_power(low[m], power);
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) acc[i][m] = times_power(acc[i][m], power);
+            }
+            const frag b = low_frag(low, T{});
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                T e[4];
+                if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) e[j] = sG[(4 * g + j) * LDT + 16 * i + c];
+                } else {
+                    const v4s w = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s*)(sG + (4 * g + (c >> 2)) * LDT + 16 * i + 4 * (c & 3)));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) e[j] = __builtin_bit_cast(T, static_cast<short>(w[j]));
                 }
+                acc[i] = M::mul(twice<T>(e), b, acc[i]);
+            }
+            if constexpr (F16)
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int m = 0; m < 4; ++m) acc[i][m] = times_power(acc[i][m], -power);
+        }
+        if (row >= 0) {
+            T* o = static_cast<T*>(a.out) + (static_cast<int64_t>(d0 + it / steps) * S + row) * N;
+#pragma unroll
+            for (int i = 0; i < NT; i += kDealt<T>) {
+                const int n = 16 * i + V * g;
+                store_tiles<T, HOW, 1>(o + n, N - n, &acc[i]);
             }
         }
         if (own) {
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int ks = 0; ks < NSX; ++ks) *reinterpret_cast<frag*>(buf + (16 * r + c) * LC + ks * M::KS + M::FE * g) = xf[r][ks];
-            wave_lds();
-            add(u, ga, pa, have_a);
-            wave_lds();
-#pragma unroll
-            for (int r = 0; r < RT; ++r)
-#pragma unroll
-                for (int ks = 0; ks < NSK; ++ks) *reinterpret_cast<frag*>(buf + (16 * r + c) * LC + ks * M::KS + M::FE * g) = gf[r][ks];
-            wave_lds();
-            add(v, gb, pb, have_b);
-            wave_lds();
+            add(u * a.scale, xf, ga, pa, have_a);
+            add(v * a.scale, gf, gb, pb, have_b);
         }
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            row[r] = next[r];
-            next[r] = after[r];
-        }
+        row = next;
+        next = after;
     }
     if (!own) return;
     __syncthreads();                                 // the maps have been read
@@ -281,9 +232,9 @@ k_ad_bwd(AdArgs a, const T* __restrict__ x, XlMap map, XlChunks ch, T* __restric
     float* sum = reinterpret_cast<float*>(smem) + wave * 16 * LP;
 #pragma unroll
     for (int i = 0; i < NT + KT; ++i) {
-        const v4f v = i < NT ? ga[i < NT ? i : 0] : gb[i < NT ? 0 : i - NT];
+        const v4f s = i < NT ? ga[i < NT ? i : 0] : gb[i < NT ? 0 : i - NT];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) sum[(4 * g + m) * LP + 16 * i + c] = F16 ? times_power(v[m], -(i < NT ? pa : pb)) : v[m];
+        for (int m = 0; m < 4; ++m) sum[(4 * g + m) * LP + 16 * i + c] = F16 ? times_power(s[m], -(i < NT ? pa : pb)) : s[m];
     }
     __syncthreads();
     const float* sums = reinterpret_cast<const float*>(smem);
@@ -293,10 +244,10 @@ k_ad_bwd(AdArgs a, const T* __restrict__ x, XlMap map, XlChunks ch, T* __restric
         const bool up = i >= R * N;                  // grad_down (R, ci), then grad_up (co, R)
         const int j = up ? i - R * N : i, q = up ? j % R : j / N, k = up ? j / R : j % N;
         const float* p = sums + q * LP + (up ? NB + k : k);
-        const float v = p[0] + p[16 * LP] + p[32 * LP] + p[48 * LP];
-        if (!direct) parts[slot * R * (N + K) + i] = v;
-        else if (up && gup) gup[one * R * K + j] = static_cast<T>(v);
-        else if (!up && gdown) gdown[one * R * N + j] = static_cast<T>(v);
+        const float s = p[0] + p[16 * LP] + p[32 * LP] + p[48 * LP];
+        if (!direct) parts[slot * R * (N + K) + i] = s;
+        else if (up && gup) gup[one * R * K + j] = static_cast<T>(s);
+        else if (!up && gdown) gdown[one * R * N + j] = static_cast<T>(s);
     }
 }
 
@@ -345,16 +296,14 @@ int run_bwd(const AdShape& p, const XlMap& map, AdArgs a, const void* x, void* g
     a.dim = map.first[p.nreps];
     a.rt = 1;
     XlChunks ch;
-    const int64_t nslots = wgrad_chunks(p.S, p.X, p.lvals, p.nreps, p.ci, p.co, &ch);
+    const int64_t nslots = fused_chunks(p, &ch);
     const int64_t blocks = ch.xcds * static_cast<int64_t>(ch.tile0[p.nreps]);
     if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
     return with_rows<T>(p.ci, p.co, {a.in, x, a.W, a.G, a.out}, [&](auto how) -> int {
         constexpr int HOW = decltype(how)::value;
         auto run = [&](auto nn, auto kk) -> int {
-            using M = Mma<T>;
-            constexpr int NB = decltype(nn)::value, KB = decltype(kk)::value, V = 16 / sizeof(T), RB = sizeof(T) == 4 ? 16 : 32;
-            constexpr size_t maps = KB * (NB + M::PAD) + KB * (16 + M::PAD) + 16 * (NB + M::PAD) + 16 * (NB + V);
-            constexpr size_t lds = std::max(sizeof(T) * (maps + 4 * RB * (std::max(NB, KB) + M::PAD)), sizeof(float) * 64 * (NB + KB));
+            constexpr int NB = decltype(nn)::value, KB = decltype(kk)::value;
+            constexpr size_t lds = std::max(kAdBwdLds<T, NB, KB>, sizeof(float) * 64 * (NB + KB));       // the maps and rows, or the sums
             auto kern = k_ad_bwd<T, HOW, NB, KB>;
             if (lds > 65536)
                 FEQ_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(kern), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));

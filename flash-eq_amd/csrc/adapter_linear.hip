@@ -854,7 +854,7 @@ size_t ad_scratch(const AdShape& p, int dim, bool shared, int nbias, void* base,
     XlChunks ch;
     if (adapter_fused(p.ci, p.co, p.R)) {
         out->low = out->parts_up = nullptr;
-        out->parts_down = c.take<float>(static_cast<size_t>(wgrad_chunks(p.S, p.X, p.lvals, p.nreps, p.ci, p.co, &ch)) * p.R * (p.ci + p.co));
+        out->parts_down = c.take<float>(static_cast<size_t>(fused_chunks(p, &ch)) * p.R * (p.ci + p.co));
     } else {
         out->low = c.take<float>(static_cast<size_t>(dim) * p.S * 16 * ad_tiles(p.R));
         out->parts_down = c.take<float>(static_cast<size_t>(wgrad_chunks(p.S, p.X, p.lvals, p.nreps, p.ci, p.R, &ch)) * p.ci * p.R);
@@ -903,9 +903,9 @@ extern "C" size_t feq_adapter_linear_low_floats(const int32_t* lvals, int32_t nr
 }
 
 extern "C" size_t feq_adapter_linear_bwd_workspace(const int32_t* lvals, int32_t nreps, int32_t adapters, int64_t rows, int32_t cin,
-                                                   int32_t cout, int32_t rank, int32_t shared, int32_t nbias) {
+                                                   int32_t cout, int32_t rank, int32_t dtype, int32_t shared, int32_t nbias) {
     XlMap map;
-    const AdShape p{lvals, nreps, adapters, rows, cin, cout, rank, FEQ_F32};
+    const AdShape p{lvals, nreps, adapters, rows, cin, cout, rank, dtype};
     if (ad_check(p, nullptr, 0, 1.0f, &map) || rows == 0 || nbias < 0) return 0;
     AdScratch s;
     return ad_scratch(p, map.first[nreps], shared, nbias, nullptr, &s);

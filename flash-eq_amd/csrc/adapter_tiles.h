@@ -135,5 +135,29 @@ struct AdShape {
     int32_t ci, co, R, dtype;
 };
 
+// Row chunks of a sum over rows, all of about as many row-planes, so that `want` workgroups and the adapters' last, shorter
+// chunks run at once; rows are rounded up to `unit`.  Returns the number of partials.
+inline int64_t adapter_chunks(const AdShape& p, int want, int unit, XlChunks* ch) {
+    int64_t dim = 0;
+    for (int r = 0; r < p.nreps; ++r) dim += 2 * p.lvals[r] + 1;
+    const int64_t full = std::max<int64_t>(want - static_cast<int64_t>(p.X + 1) * p.nreps, want / 2);
+    const int64_t share = ceil_div(std::max<int64_t>(p.S, 1) * dim, full);
+    int64_t tiles = 0, slots = 0;
+    ch->xcds = 8;
+    for (int r = p.nreps - 1; r >= 0; --r) {
+        const int64_t rows = std::min<int64_t>(ceil_div(ceil_div(share, 2 * p.lvals[r] + 1), unit) * unit, 1 << 20);
+        ch->rows[r] = static_cast<int32_t>(rows);
+        ch->tile0[r] = static_cast<int32_t>(tiles);
+        ch->slot0[r] = static_cast<int32_t>(slots);
+        tiles += ceil_div(p.S / rows + p.X + 1, ch->xcds);
+        slots += p.S > rows ? 2 * p.S / rows : 0;
+    }
+    ch->tile0[p.nreps] = static_cast<int32_t>(tiles);
+    ch->slot0[p.nreps] = static_cast<int32_t>(slots);
+    return slots;
+}
+// Of the kernel that adapter_fused names, and of the other sums.
+inline int64_t fused_chunks(const AdShape& p, XlChunks* ch) { return adapter_chunks(p, p.dtype == FEQ_F32 && p.ci > 64 && p.co > 64 ? 256 : 512, 16, ch); }
+
 }  // namespace
 }  // namespace feq

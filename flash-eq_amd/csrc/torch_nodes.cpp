@@ -974,7 +974,7 @@ struct AdapterLinearNode final : TuneNode {
             for (Tensor* t : {&gx, &gw, &gd, &gu, &gb})
                 if (t->defined()) t->zero_();
         } else {
-            const Tensor ws = scratch(feq_adapter_linear_bwd_workspace(lv, n, adapters, rows, ci, co, rank, shared, nb), xs);
+            const Tensor ws = scratch(feq_adapter_linear_bwd_workspace(lv, n, adapters, rows, ci, co, rank, code_of(xs, "x"), shared, nb), xs);
             On on(xs);
             done(feq_adapter_linear_bwd(lv, n, adapters, rows, ci, co, rank, code_of(xs, "x"), ptr(g), ptr(xs), ptr(w), ptr(dn), ptr(u),
                                         scale, ptr_as<int32_t>(order), ptr_as<int32_t>(offsets), ptr_as<float>(lo), nb,

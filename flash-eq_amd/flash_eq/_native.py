@@ -229,7 +229,7 @@ _SIGS = {
     "feq_adapter_linear_low_floats": ([_P, _I32, _I64, _I32, _I32, _I32, _I32], _SZ),
     "feq_adapter_linear_fwd": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _F, _P, _P, _P, _I32, _P, _P, _P, _P],
                                ctypes.c_int),
-    "feq_adapter_linear_bwd_workspace": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _I32, _I32], _SZ),
+    "feq_adapter_linear_bwd_workspace": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _I32, _I32, _I32], _SZ),
     "feq_adapter_linear_bwd": ([_P, _I32, _I32, _I64, _I32, _I32, _I32, _I32, _P, _P, _P, _P, _P, _F, _P, _P, _P, _I32, _P, _P, _P,
                                 _P, _P, _P, _P, _SZ, _P], ctypes.c_int),
 }

@@ -900,7 +900,7 @@ int feq_adapter_linear_fwd(const int32_t* lvals, int32_t nreps, int32_t adapters
 /* From grad_y: grad_x, grad_down and grad_up (with grad_x), grad_weight, grad_bias (with grad_weight), any of them NULL; sums in a fixed order, zeros for an adapter without rows.  rows > 0.  Workspace
  * feq_adapter_linear_bwd_workspace bytes (shared: whether grad_weight is wanted; nbias 0 without grad_bias). */
 size_t feq_adapter_linear_bwd_workspace(const int32_t* lvals, int32_t nreps, int32_t adapters, int64_t rows, int32_t cin,
-                                        int32_t cout, int32_t rank, int32_t shared, int32_t nbias);
+                                        int32_t cout, int32_t rank, int32_t dtype, int32_t shared, int32_t nbias);
 int feq_adapter_linear_bwd(const int32_t* lvals, int32_t nreps, int32_t adapters, int64_t rows, int32_t cin, int32_t cout,
                            int32_t rank, int32_t dtype, const void* grad_y, const void* x, const void* weight,
                            const void* down, const void* up, float scale, const int32_t* order, const int32_t* offsets,

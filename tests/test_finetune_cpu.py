@@ -138,7 +138,7 @@ def test_adapter_abi_refusals():
     low = lambda ci, co, r, train: lib.feq_adapter_linear_low_floats(lv, 2, 7, ci, co, r, train)
     assert low(64, 64, 16, 1) == low(128, 300, 64, 0) == 0
     assert low(129, 8, 1, 0) == 4 * 7 * 16 and low(64, 129, 17, 1) == low(64, 64, 17, 1) == 4 * 7 * 32
-    need = lib.feq_adapter_linear_bwd_workspace(lv, 2, 3, 7, 8, 200, 4, 1, 1)
+    need = lib.feq_adapter_linear_bwd_workspace(lv, 2, 3, 7, 8, 200, 4, 0, 1, 1)
     assert need > 0
 
     def bwd(co=200, gx=FAKE, gd=FAKE, gu=FAKE, gw=FAKE, gb=FAKE, low=FAKE, ws=FAKE, size=need, rows=7):
