@@ -14,6 +14,9 @@
 // weight and gradient, so exponentials, random numbers and stores are work of all lanes.  Rows are read by subgroups of G
 // lanes, lane j holding vectors j, j + G, ... (NT of them) of the head; subgroup s serves the edges whose place is
 // s modulo L / G, so short segments still keep all subgroups busy.  Heads too long for NT G vectors take several slices.
+// Where a head's runs are shorter than its lanes (component-major tables), the lanes of a run of all heads are neighbours:
+// a load then touches memory in pieces of 64 bytes and more (neighbouring lanes on different runs: 50000 x 24 edges,
+// eight heads of 8 channels, 212 us against XX).
 // Sums run in the CSR's order: no atomics, the same bits on every run.
 #include <algorithm>
 
@@ -55,7 +58,7 @@ struct EaArgs {
     const int32_t *perm, *offsets;
     int64_t N, E;
     int H;
-    int lgL, lgG, slices;      // lanes of a head, of a row; slices of a row
+    int lgL, lgG, lgC, slices;      // lanes of a head, of a row, of a row's run where these are neighbours; slices of a row
     EaHead head;
     const void* log_scale;
     int scale_dtype;
@@ -79,17 +82,77 @@ __device__ __forceinline__ int64_t ea_block(int64_t blocks) {
     return i < chunk ? blockIdx.x % 8 * chunk + i : blocks;
 }
 
-// The lane's place: head, position in a chunk, subgroup and place in it.
+// The lane's place: head, position in a chunk, subgroup and place in it.  UNI (one subgroup): the lowest lgC bits of j are the
+// lane's lowest, the others its highest, the head between them.
 struct EaLane {
-    int h, pos, j, base;       // base: first lane of the subgroup
+    int h, pos, j, hg;
     bool hv;
-    __device__ __forceinline__ EaLane(int H, int lgL, int lgG) {
-        const int lane = threadIdx.x & 63, L = 1 << lgL, G = 1 << lgG, p = lane & (L - 1);
-        h = static_cast<int>(blockIdx.y) * (64 >> lgL) + (lane >> lgL);
+    __device__ __forceinline__ EaLane(int H, int lgL, int lgG, int lgC, bool uni) {
+        const int lane = threadIdx.x & 63, L = 1 << lgL, G = 1 << lgG, lgH = 6 - lgL;
+        if (uni) {
+            hg = (lane >> lgC) & ((1 << lgH) - 1);
+            j = (lane >> (lgC + lgH) << lgC) | (lane & ((1 << lgC) - 1));
+            pos = j;
+        } else {
+            const int p = lane & (L - 1);
+            hg = lane >> lgL;
+            j = p & (G - 1);
+            pos = (j << (lgL - lgG)) + (p >> lgG);
+        }
+        h = static_cast<int>(blockIdx.y) * (1 << lgH) + hg;
         hv = h < H;
-        j = p & (G - 1);
-        pos = (j << (lgL - lgG)) + (p >> lgG);
-        base = lane & ~(G - 1);
+    }
+};
+
+// Sums and maxima over lanes that differ in their `low` lowest and `high` highest bits (uniform), of N values at once; the
+// moves of a level are the same instruction for all.  Neighbours within 16 lanes by data-parallel moves: exchanges for the
+// low bits, rotations (of values that are equal in the bits above) for the high ones.
+struct EaReduce {
+    int low, high;
+    template <int N, class Op>
+    __device__ __forceinline__ void run(float (&v)[N], Op op) const {
+        auto move = [&](auto c) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = op(v[i], __uint_as_float(dpp_u<decltype(c)::value>(__float_as_uint(v[i]))));
+        };
+        auto swap16 = [&] {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+                v[i] = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+            }
+        };
+        auto swap32 = [&] {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i]), false, false);
+                v[i] = op(__uint_as_float(p[0]), __uint_as_float(p[1]));
+            }
+        };
+        if (low > 0) move(std::integral_constant<int, 0xB1>{});      // quad_perm [1, 0, 3, 2]
+        if (low > 1) move(std::integral_constant<int, 0x4E>{});      // quad_perm [2, 3, 0, 1]
+        if (low > 2) move(std::integral_constant<int, 0x141>{});     // row_half_mirror
+        if (low > 3) move(std::integral_constant<int, 0x140>{});     // row_mirror
+        if (low > 4) swap16();
+        if (low > 5) swap32();
+        if (high > 0) swap32();
+        if (high > 1) swap16();
+        if (high > 2) move(std::integral_constant<int, 0x128>{});    // row_ror 8
+        if (high > 3) move(std::integral_constant<int, 0x124>{});    // 4
+        if (high > 4) move(std::integral_constant<int, 0x122>{});    // 2
+        if (high > 5) move(std::integral_constant<int, 0x121>{});    // 1
+    }
+    template <int N>
+    __device__ __forceinline__ void sums(float (&v)[N]) const { run(v, [](float a, float b) { return a + b; }); }
+    __device__ __forceinline__ float sum(float v) const {
+        float a[1] = {v};
+        sums(a);
+        return a[0];
+    }
+    __device__ __forceinline__ float most(float v) const {
+        float a[1] = {v};
+        run(a, [](float x, float y) { return fmaxf(x, y); });
+        return a[0];
     }
 };
 
@@ -186,26 +249,6 @@ __device__ __forceinline__ bool ea_segment(const int32_t* __restrict__ offsets, 
     return true;
 }
 
-// The sums of N values over their lane groups of g lanes (uniform), as group_sum.
-template <int N>
-__device__ __forceinline__ void group_sums(float (&v)[N], int g) {
-    auto step = [&](auto move) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] += move(v[i]);
-    };
-    auto dpp = [](float x, auto c) { return __uint_as_float(dpp_u<decltype(c)::value>(__float_as_uint(x))); };
-    if (g > 1) step([&](float x) { return dpp(x, std::integral_constant<int, 0xB1>{}); });
-    if (g > 2) step([&](float x) { return dpp(x, std::integral_constant<int, 0x4E>{}); });
-    if (g > 4) step([&](float x) { return dpp(x, std::integral_constant<int, 0x141>{}); });
-    if (g > 8) step([&](float x) { return dpp(x, std::integral_constant<int, 0x140>{}); });
-    if (g > 16)
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = group_sum16(v[i]);
-    if (g > 32)
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = group_sum32(v[i]);
-}
-
 // The edges of 64 places of a segment, one a lane: number, row (-1: outside the table) and bucket (-1: none).
 template <class T>
 struct EaEdges {
@@ -237,7 +280,8 @@ k_ea_fwd(EaArgs<T> a, float* __restrict__ w, T* __restrict__ out) {
     int b, cnt;
     if (!ea_segment(a.offsets, a.N, a.E, n, b, cnt)) return;
     const int H = a.H, lgL = a.lgL, L = 1 << lgL, G = 1 << a.lgG, lgE = lgL - a.lgG, lane = threadIdx.x & 63;
-    const EaLane me(H, lgL, a.lgG);
+    const EaLane me(H, lgL, a.lgG, a.lgC, UNI);
+    const EaReduce all{UNI ? a.lgC : lgL, UNI ? lgL - a.lgC : 0}, row{UNI ? a.lgC : a.lgG, UNI ? lgL - a.lgC : 0};
     const int64_t h = me.hv ? me.h : 0;
     if (n == a.N) {                              // destinations outside the graph
         for (int i = me.pos; i < cnt; i += L) {
@@ -285,14 +329,14 @@ k_ea_fwd(EaArgs<T> a, float* __restrict__ w, T* __restrict__ out) {
             z = 0.0f;
         };
         auto finish = [&](int c0) {
-            const int row = __shfl(ed.row, (c0 + me.pos) & 63, 64);
-            z = row < 0 ? 0.0f : z * scale;      // an edge from outside the graph: a row of zeros
+            const int from = __shfl(ed.row, (c0 + me.pos) & 63, 64);
+            z = from < 0 ? 0.0f : z * scale;      // an edge from outside the graph: a row of zeros
             z = !there || bias == -INFINITY ? -INFINITY : z + bias;
             if (cnt <= 64) zs[(c0 >> lgL) * 64 + lane] = z;
             else if (there && me.hv) w[e * H + h] = z;
-            const float most = group_max(fmaxf(z, top), L);
+            const float most = all.most(fmaxf(z, top));
             const float base = most == -INFINITY ? 0.0f : most;
-            sum = sum * expf(top - base) + group_sum(expf(z - base), L);
+            sum = sum * expf(top - base) + all.sum(expf(z - base));
             top = most;
         };
         auto row_at = [&](int i) {               // of the edge at place i of the 64
@@ -313,7 +357,7 @@ k_ea_fwd(EaArgs<T> a, float* __restrict__ w, T* __restrict__ out) {
                 }
                 d[u] = ea_dot<UNI>(q, k[u], vecs, a.head.ragged);
             }
-            group_sums<UE>(d, G);
+            row.sums(d);
             const int u0 = t * UE & (G - 1);
 #pragma unroll
             for (int u = 0; u < UE; ++u)
@@ -381,7 +425,14 @@ k_ea_bwd(EaArgs<T> a, const float* __restrict__ w, const T* __restrict__ g, floa
     int b, cnt;
     if (!ea_segment(a.offsets, a.N, a.E, n, b, cnt)) return;
     const int H = a.H, L = 1 << a.lgL, G = 1 << a.lgG, lgE = a.lgL - a.lgG, lane = threadIdx.x & 63;
-    const EaLane me(H, a.lgL, a.lgG);
+    const EaLane me(H, a.lgL, a.lgG, a.lgC, UNI);
+    const EaReduce all{UNI ? a.lgC : a.lgL, UNI ? a.lgL - a.lgC : 0};
+    // the lane that holds the edge of row step j
+    const int lgH = 6 - a.lgL;
+    auto holder = [&](int j) {
+        if constexpr (UNI) return (j >> a.lgC << (a.lgC + lgH)) | (me.hg << a.lgC) | (j & ((1 << a.lgC) - 1));
+        else return (lane & ~(G - 1)) | j;
+    };
     const int64_t h = me.hv ? me.h : 0;
     if (n == a.N) {
         if (DST)
@@ -405,7 +456,7 @@ k_ea_bwd(EaArgs<T> a, const float* __restrict__ w, const T* __restrict__ g, floa
                 if (v != 0.0f) total += v * ea_grad(g, at, a.drop, key);
             }
         }
-        total = group_sum(total, L);
+        total = all.sum(total);
     }
     constexpr int UE = kEaRows<V, NT>;
     const int per = UE << lgE, lg_per = lgE + (UE == 4 ? 2 : 1), su = G >> (UE == 4 ? 2 : 1), sub = UNI ? 0 : (lane & (L - 1)) >> a.lgG;
@@ -453,7 +504,7 @@ k_ea_bwd(EaArgs<T> a, const float* __restrict__ w, const T* __restrict__ g, floa
                     const int u0 = t * UE & (G - 1);
                     float cu[UE];
 #pragma unroll
-                    for (int u = 0; u < UE; ++u) cu[u] = __shfl(c, me.base | (u0 + u), 64);
+                    for (int u = 0; u < UE; ++u) cu[u] = __shfl(c, holder(u0 + u), 64);
 #pragma unroll
                     for (int u = 0; u < UE; ++u) {
                         if (__any(cu[u] == 0.0f)) {      // 0 times what an absent or forbidden edge's row holds may be NaN
@@ -480,12 +531,13 @@ k_ea_bwd(EaArgs<T> a, const float* __restrict__ w, const T* __restrict__ g, floa
             }
         }
         if constexpr (ROWS) {
+            if constexpr (!UNI)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int v = 0; v < V; ++v)
-                    for (int o = G; o < L; o <<= 1) acc[t][v] += __shfl_xor(acc[t][v], o, 64);
-            if (me.hv && (me.pos & ((1 << lgE) - 1)) == 0) {      // the first subgroup
+                    for (int v = 0; v < V; ++v)
+                        for (int o = G; o < L; o <<= 1) acc[t][v] += __shfl_xor(acc[t][v], o, 64);
+            if (me.hv && (UNI || (me.pos & ((1 << lgE) - 1)) == 0)) {      // the first subgroup
                 T* o = out + n * ldo;
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
@@ -650,7 +702,7 @@ k_buckets(const float* __restrict__ r, int64_t E, const float* __restrict__ boun
 // ---- host ------------------------------------------------------------------------------
 
 struct EaShape {
-    int V, NT, lgL, lgG, slices, groups;     // groups of heads
+    int V, NT, lgL, lgG, lgC, slices, groups;     // groups of heads
     bool uni;                                // a wave reads one row at a time, in one slice of whole, aligned vectors within 31 bits
     EaHead head;
 };
@@ -687,6 +739,9 @@ EaShape ea_shape(const feq_edge_attn& a, int size) {
     const int64_t vec = s.V * size;          // buffer loads from multiples of a vector
     bool whole = aligned_to(a.q, vec) && aligned_to(a.k, vec);
     for (const int64_t stride : {a.ldq, a.ldk, a.head_stride, a.run_stride}) whole = whole && stride % s.V == 0;
+    // short runs of neighbouring heads: their lanes lie together (EaLane)
+    const bool together = s.head.cpd == 1 << lg(s.head.cpd) && lg(s.head.cpd) < s.lgL && a.head_stride == a.head_len;
+    s.lgC = a.head_runs > 1 && together ? lg(s.head.cpd) : s.lgL;
     s.uni = s.lgL == s.lgG && s.slices == 1 && !s.head.ragged && whole && span < (int64_t{1} << 31) / size - s.V;
     return s;
 }
@@ -752,6 +807,7 @@ EaArgs<T> ea_args(const feq_edge_attn& a, const EaShape& s) {
     r.H = a.heads;
     r.lgL = s.lgL;
     r.lgG = s.lgG;
+    r.lgC = s.lgC;
     r.slices = s.slices;
     r.head = s.head;
     r.log_scale = a.log_scale;

@@ -38,15 +38,6 @@ __device__ __forceinline__ float group_sum(float v, int g) {
         return __float_as_uint(__uint_as_float(a) + __uint_as_float(b));
     }));
 }
-// The last two steps of group_sum alone.
-__device__ __forceinline__ float group_sum16(float v) {
-    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
-}
-__device__ __forceinline__ float group_sum32(float v) {
-    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(p[0]) + __uint_as_float(p[1]);
-}
 __device__ __forceinline__ float group_max(float v, int g) {
     return __uint_as_float(group_op(__float_as_uint(v), g, [](uint32_t a, uint32_t b) {
         return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
