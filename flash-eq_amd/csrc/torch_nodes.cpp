@@ -873,6 +873,7 @@ Tensor edge_attention(const Tensor& q, const OptTensor& k_, const OptTensor& src
     same_device(q, perm);
     if (!(decay >= 0.0)) value_error("distance decay must not be negative, got ", decay);
     if (decay > 0.0) {
+        if (static_cast<float>(decay) == 0.0f) value_error("a distance decay of ", decay, " is 0 in float32");
         if (!dist.defined()) value_error("distance decay needs distances");
         code_of(dist, "distances");
         if (dist.dim() != 1 || dist.size(0) != edges) value_error("distances must be (", edges, ",), got shape ", dist.sizes());

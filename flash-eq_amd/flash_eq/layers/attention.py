@@ -53,8 +53,9 @@ class DistanceBuckets(nn.Module):
         self.register_buffer("boundaries", torch.tensor(self._values, dtype=torch.float32), persistent=False)
 
     def _apply(self, fn, recurse: bool = True):
+        unset = self.boundaries.is_meta              # to_empty leaves what the memory held
         super()._apply(fn, recurse)
-        if self.boundaries.dtype != torch.float32:
+        if unset or self.boundaries.dtype != torch.float32:
             self.boundaries = torch.tensor(self._values, dtype=torch.float32, device=self.boundaries.device)
         return self
 

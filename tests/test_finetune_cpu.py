@@ -238,3 +238,11 @@ def test_options_change_nothing_where_they_are_off():
     assert attention.bias is None and attention.counter_dropout == 0.0 and old.buckets is None
     assert old.layers[0].feature_dropout is None and old.layers[0].mlp_up.adapters is None
     assert fe.EquivariantDropout(fe.Repr([0], 4), 0.5).eval()(torch.ones(2, 4, 1)).eq(1).all()
+
+
+def test_bucket_boundaries_of_a_model_built_without_memory():
+    want = fe.DistanceBuckets(9, 0.5, 8.0, True).boundaries
+    with torch.device("meta"):
+        b = fe.DistanceBuckets(9, 0.5, 8.0, True)
+    assert b.boundaries.is_meta
+    assert torch.equal(b.to_empty(device="cpu").boundaries, want)

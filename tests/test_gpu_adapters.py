@@ -301,3 +301,35 @@ def test_captured_step(dev, ci, co):
             assert torch.equal(a, b)
         with torch.no_grad():
             t[0].mul_(0.5)
+
+
+@pytest.mark.parametrize("rows,lvals,ci,co,rank", [(1_050_005, [0], 2048, 16, 12), (350_003, list(range(7)), 128, 128, 8)])
+def test_offsets_past_32_bits(dev, rows, lvals, ci, co, rank):
+    """The ends of tables of more than 4 GB.  All values are 0 and +-1 (a reduced row's sums are below 2^16: two bfloat16 numbers
+    hold them), and gradients reach 30 rows at either end, so sums are of whole numbers below 2^24 and exact."""
+    g = gen(5)
+    rep, n, ends = OF.irreps(lvals).tolist(), len(lvals), 30
+    dim = len(rep)
+
+    def signs(*s):
+        return torch.randint(-1, 2, s, generator=g).to(torch.bfloat16)
+    w, down, up = signs(n, co, ci), signs(2, n, rank, ci), signs(2, n, co, rank)
+    x_at, gy_at = signs(dim, 2 * ends, ci), signs(dim, 2 * ends, co)
+    ids = torch.randint(0, 2, (rows,), generator=g)
+    x, gy = (torch.zeros(dim, rows, c, dtype=torch.bfloat16, device=dev) for c in (ci, co))
+    for full, part in ((x, x_at), (gy, gy_at)):
+        full[:, :ends], full[:, -ends:] = part[:, :ends].to(dev), part[:, ends:].to(dev)
+    f = [t.double().requires_grad_() for t in (x_at, w, down, up)]
+    y64 = OF.adapter_linear(*f, torch.cat([ids[:ends], ids[-ends:]]), lvals, None, 1.0)
+    want = torch.autograd.grad(y64, f, gy_at.double())
+    leaves = [x.requires_grad_(), *(t.to(dev).requires_grad_() for t in (w, down, up))]
+    y = fe.adapter_linear(*leaves, fe.ExpertPlan(ids.to(dev), 2), lvals)
+    grads = torch.autograd.grad(y, leaves, gy)
+    both = torch.cat([y.detach()[:, :ends], y.detach()[:, -ends:]], 1)
+    assert torch.equal(both.cpu(), y64.detach().to(torch.bfloat16)) and not y.detach()[:, ends:-ends].any()
+    gx = torch.cat([grads[0][:, :ends], grads[0][:, -ends:]], 1)
+    assert torch.equal(gx.cpu(), want[0].to(torch.bfloat16)) and not grads[0][:, ends:-ends].any()
+    for a, b in zip(grads[1:], want[1:]):
+        assert torch.equal(a.cpu().view(b.shape), b.to(torch.bfloat16))
+    del x, gy, y, grads, leaves, both, gx
+    torch.cuda.empty_cache()

@@ -555,3 +555,122 @@ def test_captured_step_draws_new_masks(dev):
         for a, b in zip(got, (ww.detach(), *torch.autograd.grad(loss, [q2, b2], torch.ones_like(loss)))):
             assert torch.equal(a, b)
     assert len(set(seeds)) == 4
+
+
+# ---- large tables, several threads ---------------------------------------------------------
+
+@pytest.mark.parametrize("cm", [False, True])
+def test_attention_offsets_past_32_bits(dev, cm):
+    """The last nodes of a table of more than 4 GB (float32, 9 components, 64 channels).  Queries and keys are 0 and +-1
+    and a node has two edges either way, so every sum is one of whole numbers or of two terms and has the same bits
+    in a small table of these nodes alone."""
+    n, far, heads = 2_000_003, 500, 4
+    first = n - far
+    i = torch.arange(far)
+    src, dst = torch.cat([i, i]), torch.cat([(i + 1) % far, (i + 2) % far])
+    g = gen(21)
+    small = torch.randint(-1, 2, (far, 64, 9), generator=g).float()
+    bias = torch.randn(5, heads, generator=g)
+    bucket = torch.randint(0, 5, (2 * far,), generator=g).int().to(dev)
+    gw = torch.randn(2 * far, heads, generator=g).to(dev)
+    ls = torch.tensor(0.125).log().to(dev)
+
+    def run(qk, s, d, nodes):
+        qk.requires_grad_()
+        b = bias.to(dev).requires_grad_()
+        graph = fe.Graph(s.to(dev), d.to(dev), nodes)
+        w = fe.edge_attention_weights(qk, graph, heads, ls, component_major=cm, bias=b, buckets=bucket, dropout=0.25, seed=seed_of(dev, 4))
+        return w.detach(), *torch.autograd.grad(w, [qk, b], gw)
+
+    at = small.to(dev)
+    big = torch.zeros((9, n, 64) if cm else (n, 64, 9), device=dev)
+    if cm:
+        big[:, first:] = at.permute(2, 0, 1)
+    else:
+        big[first:] = at
+    w, gq, gb = run(big, src + first, dst + first, n)
+    w1, gq1, gb1 = run(at.permute(2, 0, 1).contiguous() if cm else at, src, dst, far)
+    near, rest = (gq[:, first:], gq[:, :first]) if cm else (gq[first:], gq[:first])
+    assert torch.equal(w, w1) and torch.equal(near, gq1) and torch.equal(gb, gb1)
+    assert not rest.any() and gq1.any()
+    del big, gq, near, rest
+    torch.cuda.empty_cache()
+
+
+def test_calls_of_several_threads(dev):
+    """Threads with streams of their own at once: each gets what it gets alone."""
+    import threading
+    src, dst = random_graph(15, 300, 4000)
+    g = gen(15)
+    qk0, bias = torch.randn(300, 32, 9, generator=g).to(dev), torch.randn(8, 4, generator=g).to(dev)
+    bucket = torch.randint(0, 8, (4000,), generator=g).to(dev)
+    graph = fe.Graph(src.to(dev), dst.to(dev), 300)
+    graph.csr(), graph.csr_src()
+    ls = torch.zeros((), device=dev)
+    plan = fe.ExpertPlan(torch.randint(0, 3, (300,), generator=g).to(dev), 3)
+    maps = [torch.randn(*s, generator=g).to(dev) for s in ((3, 32, 32), (3, 3, 4, 32), (3, 3, 32, 4))]
+
+    def step(n):
+        leaves = [t.clone().requires_grad_() for t in (qk0, bias, *maps)]
+        x = fe.feature_dropout(leaves[0], 0.2, seed_of(dev, n), [0, 1, 2])
+        y = fe.adapter_linear(x.permute(2, 0, 1), *leaves[2:], plan, [0, 1, 2])
+        w = fe.edge_attention_weights(y, graph, 4, ls, component_major=True, bias=leaves[1], buckets=bucket, dropout=0.1, seed=seed_of(dev, n + 9))
+        return torch.autograd.grad(w.square().sum(), leaves)
+
+    want = [step(n) for n in range(4)]
+    torch.cuda.synchronize()
+    got, errors = [None] * 4, []
+
+    def work(n):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(5):
+                    got[n] = step(n)
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:      # for the test's own thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(got, want):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_two_captured_steps_replayed_in_turn(dev):
+    """Two captured steps, replayed in turn and one after the other, each with the eager result."""
+    from flash_eq.capture import capture_step
+    g = gen(16)
+    ls = torch.zeros((), device=dev)
+    steps = []
+    for nodes, edges in ((100, 900), (250, 4000)):
+        src, dst = random_graph(nodes, nodes, edges)
+        qk, bias = torch.randn(nodes, 32, 9, generator=g).to(dev).requires_grad_(), torch.randn(8, 4, generator=g).to(dev).requires_grad_()
+        bucket = torch.randint(0, 8, (edges,), generator=g).to(dev)
+        graph = fe.Graph(src.to(dev), dst.to(dev), nodes)
+        graph.csr(), graph.csr_src()
+        seed = seed_of(dev, nodes)
+
+        def step(qk=qk, bias=bias, bucket=bucket, graph=graph, seed=seed):
+            w = fe.edge_attention_weights(qk, graph, 4, ls, bias=bias, buckets=bucket, dropout=0.1, seed=seed)
+            loss = w.square().sum(1)
+            loss.backward(torch.ones_like(loss))
+            return w
+
+        q2, b2 = qk.detach().clone().requires_grad_(), bias.detach().clone().requires_grad_()
+        w = fe.edge_attention_weights(q2, graph, 4, ls, bias=b2, buckets=bucket, dropout=0.1, seed=seed)
+        loss = w.square().sum(1)
+        want = [w.detach().clone(), *torch.autograd.grad(loss, [q2, b2], torch.ones_like(loss))]
+        del w, loss, q2, b2
+        cuda_graph, out = capture_step(step, [qk, bias])
+        steps.append((cuda_graph, out, qk, bias, want, step))       # the graph reads the step's tensors
+    for order in ((0, 1), (1, 0), (0, 0, 1), (1, 1)):
+        for i in order:
+            steps[i][0].replay()
+        torch.cuda.synchronize()
+        for i in set(order):
+            _, out, qk, bias, want, _ = steps[i]
+            assert all(torch.equal(a.detach(), b) for a, b in zip((out, qk.grad, bias.grad), want))

@@ -435,3 +435,10 @@ def test_refusals_of_the_adapters(dev):
         call(lv=())
     with pytest.raises(fe.CUDANotAvailableError):
         call(w=w.cpu())
+
+
+def test_a_decay_that_is_zero_in_float32_is_refused(dev):
+    src = torch.zeros(6, dtype=torch.int64, device=dev)
+    graph, qk = fe.Graph(src, src, 3), torch.randn(3, 8, 4, device=dev)
+    with pytest.raises(ValueError, match="is 0 in float32"):
+        fe.edge_attention_weights(qk, graph, 2, torch.zeros((), device=dev), decay=1e-60, distances=torch.rand(6, device=dev))
