@@ -70,3 +70,9 @@ def adapter_plan(module: nn.Module, adapters: Optional[Adapters]) -> Optional[Ex
     if count is None:
         raise ValueError("adapters were given to a module that has none (add_adapters)")
     return ExpertPlan(adapters, count)
+
+
+def wanted(**options) -> dict:
+    """The keywords of a call that are given: modules and subclasses without the others stay callable, and a hook that
+    returns a new input leaves them alone."""
+    return {k: v for k, v in options.items() if v is not None}

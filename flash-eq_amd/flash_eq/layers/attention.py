@@ -26,7 +26,7 @@ from ..graph import Graph
 from ..ops import AttnPoolFn, EdgeSoftmaxFn, NodeSoftmaxFn
 from ..representations import Repr
 from ..experts import ExpertPlan
-from .adapters import adapter_plan
+from .adapters import adapter_plan, wanted
 from .linear import EquivariantEdgewiseLinear, EquivariantLinear
 from .norm import EquivariantLayerNorm
 from .pooling import GraphPooling
@@ -148,7 +148,7 @@ class EquivariantEdgeAttention(nn.Module):
     def forward(self, Q: torch.Tensor, K: torch.Tensor, V: torch.Tensor, graph: Graph,
                 distances: torch.Tensor | None = None, buckets: torch.Tensor | None = None) -> torch.Tensor:
         """Q, K (E, H, qk_dim); V (E, mult, dim) -> attention-weighted V (E, mult, dim)."""
-        attn = self.attention_weights(Q, K, graph, distances, buckets)
+        attn = self.attention_weights(Q, K, graph, distances, **wanted(buckets=buckets))
         return self._apply_attention(V, attn)
 
     def _apply_attention(self, V: torch.Tensor, attn: torch.Tensor) -> torch.Tensor:
@@ -203,7 +203,7 @@ class EquivariantAttention(nn.Module):
         half = half_dtype(node_features)
         if half is not None:
             return run_float32(self, half, (P, Q_basis, node_features, distances, graph),
-                               dict(edge_features=edge_features, buckets=buckets, adapters=adapters))
+                               dict(edge_features=edge_features, **wanted(buckets=buckets, adapters=adapters)))
         if (node_features.dim() == 3 and self.norm_qk.cm_ok(node_features)
                 and self.linear_qk.fused_ok(node_features)):
             # the norm writes the component-major layout the projection reads;
@@ -212,14 +212,14 @@ class EquivariantAttention(nn.Module):
             # the attention kernels read the projection's component-major
             # (dim, N, 2 mult) table as it is written
             q_in, node_features = self.norm_qk.forward_pair(node_features, cm=True)
-            qk, qk_cm = self.linear_qk.forward_layout(q_in, True, True, adapters), True
+            qk, qk_cm = self.linear_qk.forward_layout(q_in, True, True, **wanted(plan=adapters)), True
         else:
-            qk, qk_cm = self.linear_qk(self.norm_qk(node_features), adapters), False   # (N, 2 mult, dim)
+            qk, qk_cm = self.linear_qk(self.norm_qk(node_features), **wanted(plan=adapters)), False   # (N, 2 mult, dim)
         if edge_features is None and self.pool.reduce == "sum":
             # V projection, head weighting and sum pooling in one pass over the
             # edges where the fused kernels cover the layer (neither attn * V
             # nor its gradient is formed)
-            attn = self.attention.node_attention_weights(qk, graph, distances, qk_cm, buckets)
+            attn = self.attention.node_attention_weights(qk, graph, distances, qk_cm, **wanted(buckets=buckets))
             out = self.linear_v.attention_pool(P, Q_basis, node_features.contiguous(), distances, graph,
                                                attn, self.num_heads)
             if out is not None:
@@ -233,7 +233,7 @@ class EquivariantAttention(nn.Module):
         else:
             # x[src] gathered inside the fused layer (message-passing form)
             V = self.linear_v(P, Q_basis, node_features.contiguous(), distances, graph=graph)
-        attn = self.attention.node_attention_weights(qk, graph, distances, qk_cm, buckets)
+        attn = self.attention.node_attention_weights(qk, graph, distances, qk_cm, **wanted(buckets=buckets))
         if self.pool.reduce == "sum":
             perm, offsets = graph.csr()
             return AttnPoolFn.apply(V, attn, graph.dst, perm, offsets, graph.num_nodes,

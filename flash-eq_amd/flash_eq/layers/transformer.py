@@ -13,7 +13,7 @@ import torch.nn as nn
 from ..graph import Graph
 from ..representations import Repr, WignerDBasis
 from ..ops import FanOutFn, ResidualScaleCmFn, ResidualScaleFn, ScaleFn
-from .adapters import Adapters, adapter_plan
+from .adapters import Adapters, adapter_plan, wanted
 from .attention import DistanceBuckets, EquivariantAttention
 from .dropout import EquivariantDropout
 from .experts import EquivariantExpertMLP
@@ -60,11 +60,6 @@ class DropPath(nn.Module):
         if torch.rand(1, device=x.device).item() < self.drop_prob:
             return torch.zeros_like(x)
         return x / (1 - self.drop_prob)
-
-
-def _wanted(**options) -> dict:
-    """The keywords of a call that are given: blocks and subclasses without the others stay callable."""
-    return {k: v for k, v in options.items() if v is not None}
 
 
 class EquivariantTransformerBlock(nn.Module):
@@ -140,7 +135,7 @@ class EquivariantTransformerBlock(nn.Module):
         half = half_dtype(node_features)
         if half is not None:
             return run_float32(self, half, (P, Q, node_features, distances, graph),
-                               dict(edge_features=edge_features, **_wanted(balance=balance, buckets=buckets, adapters=adapters)))
+                               dict(edge_features=edge_features, **wanted(balance=balance, buckets=buckets, adapters=adapters)))
         # With the residual connection, the norm also returns the features for
         # it (forward_pair): the residual's gradient is then added inside the
         # norm's backward kernel instead of by autograd in a separate pass.
@@ -149,7 +144,7 @@ class EquivariantTransformerBlock(nn.Module):
         else:
             h, nf = self.norm1(node_features), node_features
         attn_out = self._dropped(self.attn(P, Q, h, distances, graph, edge_features=edge_features,
-                                           **_wanted(buckets=buckets, adapters=adapters)))
+                                           **wanted(buckets=buckets, adapters=adapters)))
         if self._use_attn_residual:
             x = _residual(nf, attn_out, self.layer_scale_attn, self.drop_path)
         else:
@@ -157,6 +152,7 @@ class EquivariantTransformerBlock(nn.Module):
         if self.experts is not None:
             h, xr = self.norm2.forward_pair(x) if self.norm2.cm_ok(x) else (self.norm2(x), x)
             return _residual(xr, self._dropped(self.experts(h, balance)), self.layer_scale_mlp, self.drop_path)
+        plan = wanted(plan=adapters)
         if (isinstance(self.mlp_act, EquivariantGating) and self.mlp_act.kernels_ok(x)
                 and self.mlp_up.fused_ok(x) and self.mlp_down.fused_ok(x)):
             # the MLP runs component-major (dim, N, c) from the norm's output to
@@ -166,14 +162,14 @@ class EquivariantTransformerBlock(nn.Module):
                   and isinstance(self.drop_path, nn.Identity)
                   and self.layer_scale_mlp.gamma.dtype == torch.float32)
             h, xr = self.norm2.forward_pair(x, cm) if self.norm2.cm_ok(x) else (self.norm2(x), x)
-            t = self.mlp_act.forward_cm(self.mlp_up.forward_layout(h, cm, True, adapters))
+            t = self.mlp_act.forward_cm(self.mlp_up.forward_layout(h, cm, True, **plan))
             if cm:
-                return ResidualScaleCmFn.apply(xr, self._dropped(self.mlp_down.forward_layout(t, True, True, adapters), True),
+                return ResidualScaleCmFn.apply(xr, self._dropped(self.mlp_down.forward_layout(t, True, True, **plan), True),
                                                self.layer_scale_mlp.gamma)
-            mlp_out = self.mlp_down.forward_layout(t, True, False, adapters).view(*x.shape[:-2], self.out_repr.mult,
-                                                                                 x.shape[-1])
+            mlp_out = self.mlp_down.forward_layout(t, True, False, **plan).view(*x.shape[:-2], self.out_repr.mult,
+                                                                               x.shape[-1])
             return _residual(xr, self._dropped(mlp_out), self.layer_scale_mlp, self.drop_path)
-        mlp_out = self.mlp_down(self.mlp_act(self.mlp_up(self.norm2(x), adapters)), adapters)
+        mlp_out = self.mlp_down(self.mlp_act(self.mlp_up(self.norm2(x), **plan)), **plan)
         return _residual(x, self._dropped(mlp_out), self.layer_scale_mlp, self.drop_path)
 
     def extra_repr(self) -> str:
@@ -233,7 +229,7 @@ class EquivariantTransformer(nn.Module):
         adapters = adapter_plan(self, adapters)
         half = half_dtype(node_features)
         if half is not None:
-            return run_float32(self, half, (coordinates, node_features, graph), _wanted(balance=balance, adapters=adapters))
+            return run_float32(self, half, (coordinates, node_features, graph), wanted(balance=balance, adapters=adapters))
         # src - dst, as transformer.py:406.  In float32 through the graph's CSR
         # gathers: their backward (the coordinate gradient) is a fixed-order
         # segmented sum, where torch's indexing backward sorts the indices
@@ -255,8 +251,8 @@ class EquivariantTransformer(nn.Module):
                 views = iter(FanOutFn.apply(m_hidden, k))
                 uses = [(next(views) if P is m_hidden else P, next(views) if Q is m_hidden else Q)
                         for P, Q in uses]
-        options = _wanted(balance=balance, adapters=adapters,
-                          buckets=None if self.buckets is None else self.buckets(distances))
+        options = wanted(balance=balance, adapters=adapters,
+                         buckets=None if self.buckets is None else self.buckets(distances))
         for layer, (P, Q) in zip(self.layers, uses):
             x = layer(P, Q, x, distances, graph, **options)
         return self.final_norm(x)
