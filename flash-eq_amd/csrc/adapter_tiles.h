@@ -119,10 +119,14 @@ __device__ __forceinline__ typename Mma<T>::frag second_frag(const T* ge, int n,
 }
 
 // The power of two that a row of reduced values is multiplied by (float16), its exponent; 0 for a row of zeros, or one
-// that is not finite.
+// that is not finite.  64 at most: the shared map's sum of up to 65536 products of float16 numbers, below 2^48, is multiplied
+// too and stays in float32's range.  Rows that would need more lose what is below 2^-14 after the product, so 2^-78 of a reduced
+// value: 2^-32 in a sum over 2^30 rows of float16 numbers, where half a step of the smallest result is 2^-25.
+constexpr int kAdMaxPower = 64;
 __device__ __forceinline__ int low_exponent(float most) {
     const int e = static_cast<int>(__float_as_uint(most) >> 23 & 255u);
-    return e == 0 || e == 255 ? 0 : 127 + 13 - e;
+    const int p = 127 + 13 - e;
+    return e == 0 || e == 255 ? 0 : p < kAdMaxPower ? p : kAdMaxPower;
 }
 __device__ __forceinline__ float times_power(float v, int e) { return __builtin_amdgcn_ldexpf(v, e); }
 
