@@ -40,6 +40,7 @@ constexpr int kEaMaxBuckets = 4096;
 constexpr int64_t kEaMaxNodes = int64_t{1} << 25;     // a grid of 2^32 threads and more loses its last workgroups
 constexpr int kEaBiasLds = 65536;      // bytes of the bias gradient's tables in LDS
 constexpr int kEaBiasThreads = 256;
+constexpr int kEaBiasRun = 2048;        // edges of a slot between two sums of the tables
 
 // A head of a row is `segs` runs of `len` elements, `cs` apart, the runs in vectors of V elements (the last one of a run
 // begins V before its end).
@@ -620,48 +621,57 @@ k_ea_edge_rows(EaArgs<T> a, const float* __restrict__ gz, T* __restrict__ gq, in
 // grad_b over an equal share of the edges a workgroup.  Every slot (a lane for each of 2^lgP heads) adds its edges to a
 // table of its own in LDS, one edge after another: no two lanes meet in it, so the order is fixed although the additions
 // are LDS's own (which a lane need not wait for: read, add and write took 45 us where these take 32, 640000 edges of 8
-// heads and 100 buckets).  The tables are then summed in order.  Slots beyond the `tables` that fit take no edges.
+// heads and 100 buckets).  After at most kEaBiasRun edges of a slot the tables are summed in order and added to the workgroup's
+// partial: a sum of n numbers one after another may be off by n 2^-24 of them, and the largest tables leave a slot a quarter
+// million of two million edges.  Slots beyond the `tables` that fit take no edges.
 // blockIdx.y: heads from hn blockIdx.y on.
 template <bool WIDE>
 __global__ void __launch_bounds__(kEaBiasThreads)
 k_ea_bias(const float* __restrict__ gz, EaBias bias, int64_t E, int H, int hn, int lgP, int tables, float* __restrict__ part) {
     extern __shared__ __align__(16) float tab[];
     const int h0 = blockIdx.y * hn, heads = H - h0 < hn ? H - h0 : hn, size = bias.count * heads;
-    for (int i = threadIdx.x; i < tables * size; i += kEaBiasThreads) tab[i] = 0.0f;
-    __syncthreads();
     const int slot = threadIdx.x >> lgP, hl = threadIdx.x & ((1 << lgP) - 1);
-    const int share = static_cast<int>((E + gridDim.x - 1) / gridDim.x);      // 8 `tables` at least
+    const int share = static_cast<int>((E + gridDim.x - 1) / gridDim.x);      // below 2^31 / 8 where there are so many
     const int64_t e0 = static_cast<int64_t>(blockIdx.x) * share;
     const int count = static_cast<int>(e0 + share < E ? share : E > e0 ? E - e0 : 0);
-    if (slot < tables && count > 0) {
-        const float* mine = gz + e0 * H + h0;
-        for (int h = hl; h < heads; h += 1 << lgP) {
-            constexpr int AT = 8;                // edges whose loads are on their way together
-            for (int e = slot; e < count; e += AT * tables) {
-                int64_t j[AT];
-                float v[AT];
+    const float* mine = gz + e0 * H + h0;
+    int from = 0;
+    do {
+        const int upto = count - from < kEaBiasRun * tables ? count : from + kEaBiasRun * tables;
+        for (int i = threadIdx.x; i < tables * size; i += kEaBiasThreads) tab[i] = 0.0f;
+        __syncthreads();
+        if (slot < tables) {
+            for (int h = hl; h < heads; h += 1 << lgP) {
+                constexpr int AT = 8;            // edges whose loads are on their way together
+                for (int e = from + slot; e < upto; e += AT * tables) {
+                    int64_t j[AT];
+                    float v[AT];
 #pragma unroll
-                for (int i = 0; i < AT; ++i) {
-                    const int at = e + i * tables < count ? e + i * tables : e;
-                    if constexpr (WIDE) j[i] = static_cast<const int64_t*>(bias.bucket)[e0 + at];
-                    else j[i] = static_cast<const int32_t*>(bias.bucket)[e0 + at];
-                    v[i] = mine[static_cast<int64_t>(at) * H + h];
+                    for (int i = 0; i < AT; ++i) {
+                        const int at = e + i * tables < upto ? e + i * tables : e;
+                        if constexpr (WIDE) j[i] = static_cast<const int64_t*>(bias.bucket)[e0 + at];
+                        else j[i] = static_cast<const int32_t*>(bias.bucket)[e0 + at];
+                        v[i] = mine[static_cast<int64_t>(at) * H + h];
+                    }
+#pragma unroll
+                    for (int i = 0; i < AT; ++i)
+                        if (j[i] >= 0 && j[i] < bias.count && e + i * tables < upto)
+                            unsafeAtomicAdd(&tab[slot * size + static_cast<int>(j[i]) * heads + h], v[i]);
                 }
-#pragma unroll
-                for (int i = 0; i < AT; ++i)
-                    if (j[i] >= 0 && j[i] < bias.count && e + i * tables < count)
-                        unsafeAtomicAdd(&tab[slot * size + static_cast<int>(j[i]) * heads + h], v[i]);
             }
         }
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < size; i += kEaBiasThreads) {
-        float s = 0.0f;
+        __syncthreads();
+        for (int i = threadIdx.x; i < size; i += kEaBiasThreads) {
+            float s = 0.0f;
 #pragma unroll 8
-        for (int t = 0; t < tables; ++t) s += tab[t * size + i];
-        const int j = i / heads, h = i % heads;
-        part[(static_cast<int64_t>(blockIdx.x) * bias.count + j) * H + h0 + h] = s;
-    }
+            for (int t = 0; t < tables; ++t) s += tab[t * size + i];
+            const int j = i / heads, h = i % heads;
+            float& to = part[(static_cast<int64_t>(blockIdx.x) * bias.count + j) * H + h0 + h];
+            to = from ? to + s : s;
+        }
+        from = upto;
+        __syncthreads();                         // the tables have been read
+    } while (from < count);
 }
 
 // The last sums, in float64 and a fixed order.  grad_b = the workgroups' partials (groups, n): a workgroup for each 64
