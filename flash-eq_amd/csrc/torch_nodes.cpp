@@ -1050,7 +1050,7 @@ Tensor adapter_linear(const Tensor& x, const Tensor& weight, const Tensor& down,
             node->weight.keep(wc);
             node->down.keep(dc);
             node->up.keep(uc);
-            node->low.keep(low);
+            if (wants_grad(up)) node->low.keep(low);     // for its gradient alone
             node->order = order;
             node->offsets = offsets;
             node->irreps = irreps;
