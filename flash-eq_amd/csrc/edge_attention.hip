@@ -245,8 +245,7 @@ __device__ __forceinline__ void ea_bytes(const EaVecs<V, NT>& v, uint32_t (&at)[
     for (int t = 0; t < NT; ++t) at[t] = v.shared[t] < V ? static_cast<uint32_t>(v.off[t]) * static_cast<uint32_t>(sizeof(T)) : kEaOutside;
 }
 
-template <int V, int NT>
-constexpr int kEaRows = V * NT <= 8 ? 4 : V * NT <= 16 ? 4 : 2;      // rows in flight
+constexpr int kEaLgRows = 2, kEaRows = 1 << kEaLgRows;      // rows in flight
 
 __device__ __forceinline__ bool ea_segment(const int32_t* __restrict__ offsets, int64_t N, int64_t E, int64_t& n, int& b, int& cnt) {
     n = ea_block((N + kEaWaves) / kEaWaves) * kEaWaves + __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
@@ -302,9 +301,9 @@ k_ea_fwd(EaArgs<T> a, float* __restrict__ w, T* __restrict__ out) {
     if (cnt == 0) return;
     float* const zs = kept_z[threadIdx.x >> 6];
     const float scale = expf(load_any(a.log_scale, a.scale_dtype, 0));
-    constexpr int UE = kEaRows<V, NT>;
+    constexpr int UE = kEaRows;
     const int sub = UNI ? 0 : (lane & (L - 1)) >> a.lgG, per = UE << lgE;      // subgroup; places of a step
-    const int lg_per = lgE + (UE == 4 ? 2 : 1);
+    const int lg_per = lgE + kEaLgRows;
     const bool one = UNI || a.slices == 1;
     float q[NT][V];
     const EaVecs<V, NT> first(a.head, h, me.j, G, 0);
@@ -375,7 +374,7 @@ k_ea_fwd(EaArgs<T> a, float* __restrict__ w, T* __restrict__ out) {
             for (int u = 0; u < UE; ++u)
                 if (me.j == u0 + u) z += d[u];
         };
-        const int su = G >> (UE == 4 ? 2 : 1);   // steps of a chunk
+        const int su = G >> kEaLgRows;   // steps of a chunk
         if (one) {
             if (NODE && s0 == 0) queries(first);
             for (int t = 0; t < steps; ++t) {
@@ -479,8 +478,8 @@ k_ea_bwd(EaArgs<T> a, const float* __restrict__ w, const T* __restrict__ g, floa
         }
         total = all.sum(total);
     }
-    constexpr int UE = kEaRows<V, NT>;
-    const int per = UE << lgE, lg_per = lgE + (UE == 4 ? 2 : 1), su = G >> (UE == 4 ? 2 : 1), sub = UNI ? 0 : (lane & (L - 1)) >> a.lgG;
+    constexpr int UE = kEaRows;
+    const int per = UE << lgE, lg_per = lgE + kEaLgRows, su = G >> kEaLgRows, sub = UNI ? 0 : (lane & (L - 1)) >> a.lgG;
     float dot = 0.0f;
     for (int sl = 0; sl < (ROWS && !UNI ? a.slices : 1); ++sl) {
         const EaVecs<V, NT> vecs(a.head, h, me.j, G, sl);
