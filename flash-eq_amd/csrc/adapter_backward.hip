@@ -13,8 +13,8 @@ namespace {
 // transposed.  16-bit types take a reduced row as two numbers, as in k_ad_stream, so 16 rows fill a product.  The waves' sums
 // are added at the chunk's end.
 //
-// 20011 x 49 bfloat16 rows of 128 columns both ways, 16 adapters of rank 16: 190 us, 4.0 TB/s, where grad_x and the two
-// sums in kernels of their own took 410; float32, 20000 x 9 rows of 64 to 128: 83 us, memory's 37 and the products' 41 overlapped
+// 20011 x 49 bfloat16 rows of 128 columns both ways, 16 adapters of rank 16: 195 us, 3.9 TB/s, where grad_x and the two
+// sums in kernels of their own took 410; float32, 20000 x 9 rows of 64 to 128: 88 us, memory's 37 and the products' 41 overlapped
 // in part.
 template <class T, int NB, int KB>
 constexpr size_t kAdBwdLds =

@@ -24,7 +24,7 @@ namespace {
 
 // A reduction of at most 128 columns: the shared map and the maps of one adapter stay in LDS, the rows stream (see
 // k_xl_stream, whose division of the work this is).  20011 x 49 bfloat16 rows of 128 to 128 columns, 16 adapters of rank
-// 16, take 122 us, 4.1 TB/s; 20000 x 9 float32 rows of 64 to 128 take 60, memory's 28 and the products' 27 overlapped in part.
+// 16, take 132 us, 3.8 TB/s; 20000 x 9 float32 rows of 64 to 128 take 65, memory's 28 and the products' 27 overlapped in part.
 template <class T, int HOW, bool TRANS, int NB, int NS, int RT>
 __global__ void __launch_bounds__(kXlThreads, NB * NS * Mma<T>::KS * sizeof(T) > 40000 || RT > 1 ? 2 : 3)
 k_ad_stream(AdArgs a, XlMap map) {
@@ -281,7 +281,7 @@ k_ad_low(AdArgs a, XlMap map) {
 
 // The product for a wider reduction: blocks of 128 rows in the plan's order, whatever their adapters, through LDS (k_xl_mm's
 // tiles); then, for the adapters of the block in turn, the reduced rows (k_ad_low's) times G, whose operands come from
-// memory in the matrix cores' layout.  8191 bfloat16 rows, 512 to 1024 columns, 64 adapters: 30 us, 280 TFLOP/s; 64 row blocks
+// memory in the matrix cores' layout.  8191 bfloat16 rows, 512 to 1024 columns, 64 adapters: 32 us, 270 TFLOP/s; 64 row blocks
 // by 8 column blocks are one round of the chip, of 8 steps whose LDS and barrier latency bounds it.
 template <class T, int HOW, bool TRANS, int WR>
 __global__ void __launch_bounds__(kXlThreads, 2)
@@ -759,7 +759,7 @@ int ad_run(const AdShape& p, const XlMap& map, AdArgs a, std::initializer_list<c
             if (blocks > INT32_MAX / kXlThreads) return fail(FEQ_ERR_UNSUPPORTED, "%lld blocks", (long long)blocks);
             auto low = k_ad_low<T, HOW, TRANS>;
             FEQ_LAUNCH(TRANS ? "k_ad_low_t" : "k_ad_low", low, dim3(blocks, dim), dim3(kXlThreads), 0, s, a, map);
-            // blocks of 128 rows for fewer than half of the CUs: 9 us against 80 for 64 bfloat16 rows, 512 to 1024 columns
+            // blocks of 128 rows for fewer than half of the CUs: a call of 64 bfloat16 rows, 512 to 1024 columns, 15 us against 88
             if (ceil_div(p.S, kXlBM) * ceil_div(N, 128) * dim < 128) {
                 auto few = k_ad_few<T, HOW, TRANS>;
                 FEQ_LAUNCH(TRANS ? "k_ad_few_t" : "k_ad_few", few, dim3(ceil_div(N, 32), ceil_div(p.S, 16), dim), dim3(64), 0, s, a, map);

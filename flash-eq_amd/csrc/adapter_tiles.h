@@ -160,7 +160,7 @@ inline int64_t adapter_chunks(const AdShape& p, int want, int unit, XlChunks* ch
     ch->slot0[p.nreps] = static_cast<int32_t>(slots);
     return slots;
 }
-// Of the kernel that adapter_fused names, and of the other sums.
+// Those of the kernel that adapter_fused names.
 inline int64_t fused_chunks(const AdShape& p, XlChunks* ch) { return adapter_chunks(p, p.dtype == FEQ_F32 && p.ci > 64 && p.co > 64 ? 256 : 512, 16, ch); }
 
 }  // namespace

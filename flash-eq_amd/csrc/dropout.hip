@@ -11,7 +11,7 @@
 // element; component-major: a byte for eight neighbours of a plane, for each irrep), and the elements stream past
 // them, eight a thread.  Elementwise dropout (scalars alone) takes the first step's bits as they are.
 //
-// Memory bounds it: 50000 x 64 x 9 float32 in 50 us, 4.6 TB/s read and written; 160000 x 896 bfloat16 in 93, 6.1 TB/s (the
+// Memory bounds it: 50000 x 64 x 9 float32 in 51 us, 4.5 TB/s read and written; 160000 x 896 bfloat16 in 112, 5.1 TB/s (the
 // 256 MB cache behind the L2s keeps a part).  Numbers have 16 bits, so a block of the generator, ten rounds of four products,
 // serves eight units: 32 bits would double its work for the same bytes.
 #include <algorithm>

@@ -17,12 +17,15 @@
 // Where a head's runs are shorter than its lanes (component-major tables), the lanes of a run of all heads are neighbours:
 // a load then touches memory in pieces of 64 bytes and more (neighbouring lanes on different runs: 50000 x 24 edges,
 // eight heads of 8 channels, 212 us against 204 for the forward).
-// Sums run in the CSR's order: no atomics, the same bits on every run.
+// Sums run in the CSR's order, those of grad_b in the edges' (k_ea_bias: additions in LDS that no two lanes share): the same bits
+// on every run.
 //
-// What bounds a pass is the gather of a row for each edge: 640000 random edges of 2304-byte rows take 203 us forward, 213 and
-// 219 in the two backward passes (by destination, by source), 7.0 to 7.4 TB/s from behind the L2s, where a kernel that only
-// gathers reaches 8.1.  Along a chain the L2s hold the rows, and the vector units bound it: 184 us for 1.2 million edges, 116 for
-// the gather alone (dot products a third of the instructions; the rest joins lanes and makes logits and weights).
+// What bounds a pass is the gather of a row for each edge: 640000 random edges of 2304-byte rows take 203 us forward, 214 and
+// 219 in the two backward passes (by destination, by source), 6.7 to 7.3 TB/s from behind the L2s, where a kernel that only
+// gathers reaches 8.1.  Along a chain the L2s hold the rows: 186 us for 1.2 million edges, where gathers alone take 116, and no
+// unit is full (vector units 51 of 100, scalar ones 39).  Of a wave's time 47 in 100 go to waiting for loads, a segment of
+// 24 edges beginning with four that depend on each other (offsets, edge, source and bucket, rows), and 29 to waiting for a
+// place to issue from, 4.4 waves to a vector unit: latency bounds it.
 // Tried without gain: two rows in flight and the next two loading, rows' addresses formed by lanes, more waves on a unit.
 #include <algorithm>
 
@@ -620,7 +623,10 @@ k_ea_edge_rows(EaArgs<T> a, const float* __restrict__ gz, T* __restrict__ gq, in
 // grad_b over an equal share of the edges a workgroup.  Every slot (a lane for each of 2^lgP heads) adds its edges to a
 // table of its own in LDS, one edge after another: no two lanes meet in it, so the order is fixed although the additions
 // are LDS's own (which a lane need not wait for: read, add and write took 45 us where these take 32, 640000 edges of 8
-// heads and 100 buckets).  After at most kEaBiasRun edges of a slot the tables are summed in order and added to the workgroup's
+// heads and 100 buckets).  Latency bounds it: 64 KB of tables leave a vector unit two waves, of whose time half goes to waiting for
+// loads, in eight rounds a slot, and 38 in 100 to waiting for a place to issue from, with no bank conflict and every unit below a
+// tenth.  Larger tables leave fewer slots: of 16 heads and 512 buckets two fit (32 of 256 lanes), 77 us, of 8 heads and 4096
+// buckets one for each half of the heads (4 lanes), 277 us.  After at most kEaBiasRun edges of a slot the tables are summed in order and added to the workgroup's
 // partial: a sum of n numbers one after another may be off by n 2^-24 of them, and the largest tables leave a slot a quarter
 // million of two million edges.  Slots beyond the `tables` that fit take no edges.
 // blockIdx.y: heads from hn blockIdx.y on.
